@@ -584,6 +584,76 @@ QGRU_API int qgru_calibrate_from_histogram(const float *counts, int num_bins, fl
                                            float max_val, int64_t total_count, int use_pot2,
                                            int use_percentile, float percentile, qgru_op *op);
 
+/* ------------------------------------------------- sequence operators beside the GRU
+ * No counterpart in the reference.  Linear attention with a decay for each head, a recurrent layer that is
+ * linear in its state, and the root-mean-square norm with the residual's addition that such layers stand
+ * between.  These calls have no handle: they keep nothing, allocate nothing and wait for nothing; workspaces are the
+ * caller's, and calls that do not share one may run at the same time.  They run on `device`, whatever the thread's current
+ * device is.  qgru_seq_last_error: why the calling thread's last of these calls failed. */
+QGRU_API const char *qgru_seq_last_error(void);
+
+/* Element (t, b, h, d) of a tensor lies at p + t * ts + b * bs + h * hs + d (elements; decays have no d). */
+typedef struct qgru_seq_tensor {
+    void *p;
+    long long ts, bs, hs;
+} qgru_seq_tensor;
+
+/* For every sequence b and head h, with q and k of head h / (H / Hk) and the state S [Dk][Dv] in fp32:
+ *     S_t = exp(decay_t) S_{t-1} + k_t^T v_t,    out_t = scale * q_t S_t,    t < lengths[b]
+ * decay: the logarithm, at most 0 (-inf forgets everything; above 0 sums may overflow).  Tokens from lengths[b] on are not
+ * read; their outputs and gradients are written as zeros.  lengths (device) may be NULL (all T) and is clamped to 0 .. T.
+ * state0 [B][H][Dk][Dv] (NULL: zeros) and state, the last one, are dense.
+ * Backward: dout, dstate (NULL: zeros) -> dq, dk, dv (elements of the type of q), ddecay (of the type of decay), dstate0 (may
+ * be NULL).  `states`: qgru_attention_sizes bytes, written by the forward and read by the backward of the same arguments; 256-byte
+ * aligned, as `workspace`, which holds nothing between calls. */
+typedef struct qgru_attention {
+    int device, T, B, H, Hk, Dk, Dv;
+    int bf16, decay_bf16;               /* else fp32 */
+    float scale;
+    const int32_t *lengths;
+    const float *state0, *dstate;
+    float *state, *dstate0;
+    void *states, *workspace;
+    size_t states_bytes, workspace_bytes;
+    qgru_seq_tensor q, k, v, decay, out, dout, dq, dk, dv, ddecay;
+} qgru_attention;
+QGRU_API int qgru_attention_sizes(const qgru_attention *a, size_t *states_bytes, size_t *forward_workspace,
+                                  size_t *backward_workspace);
+QGRU_API int qgru_attention_forward(const qgru_attention *a, void *stream);
+QGRU_API int qgru_attention_backward(const qgru_attention *a, void *stream);
+/* One token (T = 1; ts unused; no lengths): `state` is read and written in place, element (b, h, i, j) at
+ * b * state_bs + h * state_hs + i * Dv + j. */
+QGRU_API int qgru_attention_step(const qgru_attention *a, long long state_bs, long long state_hs, void *stream);
+
+/* Rows of `cols` elements, row i of x at x + i * x_stride (elements; the other tensors likewise, 0 < stride where there is
+ * more than one row).  h = x + residual rounded to the element type (residual NULL: h = x, and h_out is not written),
+ * y = h * weight / sqrt(mean(h^2) + eps).  One of
+ *   y      element type;
+ *   q8     int8, dense rows: q = round(127 y / max|y|), scales[row] = max|y| / 127 (a row of zeros: 0, 0; one with infinities
+ *          or NaN: 0, NaN).  With q8_scale > 0: q = clamp(round(y / q8_scale) + q8_zero_point, q8_lo, q8_hi), stored in a byte (as
+ *          uint8 where q8_hi > 127; NaN gives q8_lo); scales is not written.  Halves round to even.
+ * rstd (may be NULL) [rows]: 1 / sqrt(mean(h^2) + eps), which the backward reads. */
+typedef struct qgru_norm {
+    int device, bf16, weight_bf16, cols;
+    long long rows;
+    float eps;
+    const void *x, *residual, *weight;
+    long long x_stride, residual_stride;
+    void *h_out, *y;
+    long long h_stride, y_stride;
+    void *q8;
+    float *scales, *rstd;
+    float q8_scale;
+    int q8_zero_point, q8_lo, q8_hi;
+} qgru_norm;
+QGRU_API int qgru_norm_forward(const qgru_norm *n, void *stream);
+/* h (x of the forward where it had no residual), dy and dh (the gradient of the stream, may be NULL) -> dx (of x and of the
+ * residual) and dweight (may be NULL; of the weight's type).  workspace: qgru_norm_workspace bytes, 16-byte aligned. */
+QGRU_API size_t qgru_norm_workspace(int device, long long rows, int cols);
+QGRU_API int qgru_norm_backward(const qgru_norm *n, const void *h, long long h_stride, const void *dy, long long dy_stride,
+                                const void *dh, long long dh_stride, void *dx, long long dx_stride, void *dweight,
+                                void *workspace, size_t workspace_bytes, void *stream);
+
 /* Initialise a qgru_ranges to "empty" (min=+FLT_MAX, max=-FLT_MAX), as
  * GRUQuantizationRanges::reset does (include/gru_quantization_ranges.h:75-123). */
 QGRU_API void qgru_ranges_reset(qgru_ranges *r, int hidden);

@@ -10,6 +10,8 @@ The directory name contains a hyphen, so the package is loaded under the module 
 ``gru_ops``    functions with the names and argument meaning of the reference's ``gru_ops``
                pybind module (pytorch/lib/gru_interface_binding.cc) for the integer path
 ``quant_gru``  ``QuantGRU``: the nn.GRU-compatible module of pytorch/quant_gru.py, hot path only
+``linear_attention``  linear attention with a decay for each head: whole sequences, single tokens, a layer
+``norm``       root-mean-square norm with the residual's addition, 8-bit output
 ``sharding``   batch / direction partition over several GPUs (one process per GPU)
 """
 from . import _cabi  # noqa: F401

@@ -66,6 +66,28 @@ class Ranges(C.Structure):
                 ("min_br", C.POINTER(C.c_float)), ("max_br", C.POINTER(C.c_float))]
 
 
+class SeqTensor(C.Structure):
+    """qgru_seq_tensor: address and strides (elements) of a [T, B, heads, D] tensor."""
+    _fields_ = [("p", C.c_void_p), ("ts", C.c_longlong), ("bs", C.c_longlong), ("hs", C.c_longlong)]
+
+
+class Attention(C.Structure):
+    """qgru_attention: sizes, states, workspaces and tensors of a linear attention call."""
+    _fields_ = ([(n, C.c_int) for n in ("device", "T", "B", "H", "Hk", "Dk", "Dv", "bf16", "decay_bf16")] + [("scale", C.c_float)] +
+                [(n, C.c_void_p) for n in ("lengths", "state0", "dstate", "state", "dstate0", "states", "workspace")] +
+                [("states_bytes", C.c_size_t), ("workspace_bytes", C.c_size_t)] +
+                [(n, SeqTensor) for n in ("q", "k", "v", "decay", "out", "dout", "dq", "dk", "dv", "ddecay")])
+
+
+class Norm(C.Structure):
+    """qgru_norm: sizes, tensors and 8-bit output of a root-mean-square norm call."""
+    _fields_ = ([(n, C.c_int) for n in ("device", "bf16", "weight_bf16", "cols")] + [("rows", C.c_longlong), ("eps", C.c_float)] +
+                [(n, C.c_void_p) for n in ("x", "residual", "weight")] + [("x_stride", C.c_longlong), ("residual_stride", C.c_longlong)] +
+                [("h_out", C.c_void_p), ("y", C.c_void_p), ("h_stride", C.c_longlong), ("y_stride", C.c_longlong)] +
+                [(n, C.c_void_p) for n in ("q8", "scales", "rstd")] + [("q8_scale", C.c_float)] +
+                [(n, C.c_int) for n in ("q8_zero_point", "q8_lo", "q8_hi")])
+
+
 # every symbol include/qgru.h declares: name -> (restype, argtypes)
 _P = C.c_void_p
 _F = C.POINTER(C.c_float)
@@ -139,6 +161,14 @@ SYMBOLS = {
     "qgru_calc_params_from_hist": (C.c_int, [_P, C.c_int, C.c_float, C.POINTER(Params), _F, _F, _F, _F]),
     "qgru_calibrate_from_histogram": (C.c_int, [_F, C.c_int, C.c_float, C.c_float, C.c_int64, C.c_int,
                                                 C.c_int, C.c_float, C.POINTER(Op)]),
+    "qgru_seq_last_error": (C.c_char_p, []),
+    "qgru_attention_sizes": (C.c_int, [C.POINTER(Attention)] + [C.POINTER(C.c_size_t)] * 3),
+    "qgru_attention_forward": (C.c_int, [C.POINTER(Attention), _P]),
+    "qgru_attention_backward": (C.c_int, [C.POINTER(Attention), _P]),
+    "qgru_attention_step": (C.c_int, [C.POINTER(Attention), C.c_longlong, C.c_longlong, _P]),
+    "qgru_norm_forward": (C.c_int, [C.POINTER(Norm), _P]),
+    "qgru_norm_workspace": (C.c_size_t, [C.c_int, C.c_longlong, C.c_int]),
+    "qgru_norm_backward": (C.c_int, [C.POINTER(Norm)] + [_P, C.c_longlong] * 4 + [_P, _P, C.c_size_t, _P]),
 }
 HIST_GATE0 = 17
 HIST_CHANNEL0 = 29
@@ -176,5 +206,14 @@ def check(status, where, handle=None):
     if status != QGRU_OK:
         detail = lib().qgru_last_error(handle).decode() if handle else ""
         if status in (QGRU_ERR_BAD_ARG,):
+            raise ValueError(f"{where}: {detail or 'bad argument'}")
+        raise QgruError(status, where, detail)
+
+
+def check_seq(status, where):
+    """As check, for the calls without a handle."""
+    if status != QGRU_OK:
+        detail = lib().qgru_seq_last_error().decode()
+        if status == QGRU_ERR_BAD_ARG:
             raise ValueError(f"{where}: {detail or 'bad argument'}")
         raise QgruError(status, where, detail)

@@ -1,0 +1,652 @@
+// qgru_attn.cu - linear attention: the entry points, the kernels for every size and type, and the single-token form.
+//
+// The kernels here compute in fp32 by multiply-adds, whatever the inputs' type, 64 tokens a chunk and 64 x 64 tiles; they serve
+// head sizes above 128.
+#include <algorithm>
+
+#include "qgru_attn.cuh"
+
+namespace qgru {
+namespace attn {
+namespace {
+
+constexpr int C = 64, LD = 65, THREADS = 256;
+using bf16 = __nv_bfloat16;
+
+// 64 x 64 sums of a thread grid of 16 x 16: rows ty + 16 i, columns tx + 16 j.
+struct Acc {
+    float v[4][4];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i][j] = 0.f;
+    }
+};
+// acc += sum_k A(m, k) B(k, n), element (m, k) of A at m * AM + k * AK
+template <int AM, int AK, int BK, int BN>
+__device__ __forceinline__ void multiply(Acc &c, const float *A, const float *B, int tid) {
+    const float *a = A + (tid >> 4) * AM, *b = B + (tid & 15) * BN;
+#pragma unroll 4
+    for (int k = 0; k < 64; ++k) {
+        float x[4], y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = a[16 * i * AM + k * AK];
+            y[i] = b[16 * i * BN + k * BK];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) c.v[i][j] = fmaf(x[i], y[j], c.v[i][j]);
+    }
+}
+template <class F>
+__device__ __forceinline__ void each(Acc &c, int tid, F f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f((tid >> 4) + 16 * i, (tid & 15) + 16 * j, c.v[i][j]);
+}
+
+// 64 tokens x 64 columns of a tensor, zeros outside.
+template <class T>
+__device__ __forceinline__ void load_tile(float *to, const qgru_seq_tensor &x, long long base, int t0, int tokens, int d0, int d, int tid) {
+    const T *p = static_cast<const T *>(x.p) + base;
+    for (int e = tid; e < C * 64; e += THREADS) {
+        const int r = e >> 6, c = e & 63;
+        to[r * LD + c] = r < tokens && d0 + c < d ? seq::to_f(p[(long long)(t0 + r) * x.ts + d0 + c]) : 0.f;
+    }
+}
+__device__ __forceinline__ void load_state(float *to, const float *S, int i0, int j0, const qgru_attention &a, int tid) {
+    for (int e = tid; e < 4096; e += THREADS) {
+        const int r = e >> 6, c = e & 63;
+        to[r * LD + c] = i0 + r < a.Dk && j0 + c < a.Dv ? S[(long long)(i0 + r) * a.Dv + j0 + c] : 0.f;
+    }
+}
+__device__ __forceinline__ long long at(const qgru_seq_tensor &x, int b, int h) { return b * x.bs + h * x.hs; }
+
+// The chunk's running sums G[0 .. 63] (tokens behind the sequence add nothing).
+__device__ __forceinline__ void load_decays(float2 *G, double *sums, const qgru_attention &a, int b, int h, int t0, int tokens, int tid) {
+    double g = 0.0;
+    if (tid < C) {
+        if (tid < tokens) g = decay_log2(a, at(a.decay, b, h) + (long long)(t0 + tid) * a.decay.ts);
+        g = running_sum<C>(g, sums, tid);
+    }
+    __syncthreads();
+    if (tid < C) G[tid] = two_floats(g + (tid >= 32 ? sums[0] : 0.0));
+    __syncthreads();
+}
+
+struct Pass {                      // a state pass
+    qgru_seq_tensor k, v;
+    int k_share;                   // heads that share one of k
+    const float *first;            // the state it starts from, or null
+    float *last;                   // where the last one goes, or null
+    float *states;                 // before each chunk (in the pass's order)
+    bool own_sums;                 // instead: each segment's sum, from zero
+    float *seg_state, *seg_log;    // [segments][B H][Dk][Dv], [segments][B H]
+    int segments, per, chunks;
+};
+
+// grid: (B H, tiles of the state, segments).  Order of chunks: forward, or from the last one back (Reverse), where the weight of a
+// token is scale 2^G_t instead of 2^(G_C - G_t).
+template <class T, bool Reverse>
+__global__ void __launch_bounds__(THREADS) k_states(const __grid_constant__ qgru_attention a, const Pass p) {
+    __shared__ float K[C * LD], V[C * LD];
+    __shared__ float2 G[C];
+    __shared__ double sums[2];
+    const int tid = threadIdx.x, bh = blockIdx.x, b = bh / a.H, h = bh % a.H;
+    const int nj = (a.Dv + 63) / 64, i0 = (int)blockIdx.y / nj * 64, j0 = (int)blockIdx.y % nj * 64;
+    const int n = valid_tokens(a, b), seg = blockIdx.z;
+    const long long kb = at(p.k, b, h / p.k_share), vb = at(p.v, b, h), tile = (long long)bh * a.Dk * a.Dv;
+    const bool own_sums = p.own_sums;
+    Acc S;
+    S.zero();
+    const long long size = (long long)gridDim.x * a.Dk * a.Dv;
+    const auto inside = [&](int i, int j) { return i0 + i < a.Dk && j0 + j < a.Dv; };
+    const auto place = [&](int i, int j) { return (long long)(i0 + i) * a.Dv + j0 + j; };
+    const float *first = p.segments > 1 ? p.seg_state + seg * size : p.first;
+    if (!own_sums && first) each(S, tid, [&](int i, int j, float &s) { s = inside(i, j) ? first[tile + place(i, j)] : 0.f; });
+    double all = 0.0;
+    const int c_end = min((seg + 1) * p.per, p.chunks);
+    for (int c = seg * p.per; c < c_end; ++c) {
+        const int chunk = Reverse ? p.chunks - 1 - c : c, t0 = chunk * C, tokens = min(max(n - t0, 0), C);
+        if (!own_sums) each(S, tid, [&](int i, int j, float &s) { if (inside(i, j)) p.states[chunk * size + tile + place(i, j)] = s; });
+        if (tokens == 0) continue;
+        __syncthreads();
+        load_decays(G, sums, a, b, h, t0, tokens, tid);
+        load_tile<T>(K, p.k, kb, t0, tokens, i0, a.Dk, tid);
+        load_tile<T>(V, p.v, vb, t0, tokens, j0, a.Dv, tid);
+        __syncthreads();
+        const float2 end = G[C - 1];
+        for (int e = tid; e < C * 64; e += THREADS) K[(e >> 6) * LD + (e & 63)] *= Reverse ? a.scale * exp2_of(G[e >> 6]) : exp2_diff(end, G[e >> 6]);
+        __syncthreads();
+        const float whole = exp2_of(end);
+        all += (double)end.x + (double)end.y;
+        each(S, tid, [&](int, int, float &s) { s *= whole; });
+        multiply<1, LD, LD, 1>(S, K, V, tid);
+    }
+    if (own_sums) {
+        each(S, tid, [&](int i, int j, float &s) { if (inside(i, j)) p.seg_state[seg * size + tile + place(i, j)] = s; });
+        if (blockIdx.y == 0 && tid == 0) p.seg_log[seg * gridDim.x + bh] = (float)all;
+    } else if (p.last && seg == p.segments - 1) {
+        each(S, tid, [&](int i, int j, float &s) { if (inside(i, j)) p.last[tile + place(i, j)] = s; });
+    }
+}
+
+// The segments' own sums become the states that they start from.
+__global__ void k_scan_segments(float *seg_state, const float *seg_log, const float *first, int segments, long long size, int per_head) {
+    const long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (e >= size) return;
+    const int heads = (int)(size / per_head), bh = (int)(e / per_head);
+    float s = first ? first[e] : 0.f;
+    for (int g = 0; g < segments; ++g) {
+        const float own = seg_state[g * size + e], keep = exp2f(seg_log[g * heads + bh]);
+        seg_state[g * size + e] = s;
+        s = fmaf(keep, s, own);
+    }
+}
+
+// grid: chunks x B H, the heads of one chunk beside each other (their tokens lie together)
+template <class T>
+__global__ void __launch_bounds__(THREADS) k_outputs(const __grid_constant__ qgru_attention a, const float *states) {
+    extern __shared__ float smem[];
+    float *X = smem, *Y = X + C * LD, *P = Y + C * LD;
+    __shared__ float2 G[C];
+    __shared__ double sums[2];
+    const int tid = threadIdx.x, heads = a.B * a.H, chunk = blockIdx.x / heads, bh = blockIdx.x % heads, b = bh / a.H, h = bh % a.H, t0 = chunk * C;
+    const int all = min(a.T - t0, C), tokens = min(max(valid_tokens(a, b) - t0, 0), C);
+    T *out = static_cast<T *>(a.out.p) + at(a.out, b, h) + t0 * a.out.ts;
+    if (tokens == 0) {
+        for (int e = tid; e < all * a.Dv; e += THREADS) out[(e / a.Dv) * a.out.ts + e % a.Dv] = seq::from_f<T>(0.f);
+        return;
+    }
+    const int hk = h / (a.H / a.Hk);
+    const long long qb = at(a.q, b, hk), kb = at(a.k, b, hk), vb = at(a.v, b, h);
+    const float *S = states + chunk * (long long)heads * a.Dk * a.Dv + (long long)bh * a.Dk * a.Dv;
+    load_decays(G, sums, a, b, h, t0, tokens, tid);
+    Acc c;
+    c.zero();
+    for (int d = 0; d < a.Dk; d += 64) {
+        load_tile<T>(X, a.q, qb, t0, tokens, d, a.Dk, tid);
+        load_tile<T>(Y, a.k, kb, t0, tokens, d, a.Dk, tid);
+        __syncthreads();
+        multiply<LD, 1, 1, LD>(c, X, Y, tid);
+        __syncthreads();
+    }
+    each(c, tid, [&](int t, int s, float &x) { P[t * LD + s] = s <= t ? a.scale * exp2_diff(G[t], G[s]) * x : 0.f; });
+    for (int j = 0; j < a.Dv; j += 64) {
+        c.zero();
+        for (int d = 0; d < a.Dk; d += 64) {
+            load_tile<T>(X, a.q, qb, t0, tokens, d, a.Dk, tid);
+            load_state(Y, S, d, j, a, tid);
+            __syncthreads();
+            multiply<LD, 1, LD, 1>(c, X, Y, tid);
+            __syncthreads();
+        }
+        each(c, tid, [&](int t, int, float &x) { x *= a.scale * exp2_of(G[t]); });
+        load_tile<T>(Y, a.v, vb, t0, tokens, j, a.Dv, tid);
+        // A later token's infinity or NaN is none of an earlier one's business, and zero times it is NaN.
+        int odd = 0;
+        for (int e = tid; e < C * 64; e += THREADS) odd |= !isfinite(Y[(e >> 6) * LD + (e & 63)]);
+        if (__syncthreads_or(odd)) {
+            each(c, tid, [&](int t, int n, float &x) {
+                for (int s = 0; s <= t; ++s) x = fmaf(P[t * LD + s], Y[s * LD + n], x);
+            });
+        } else {
+            multiply<LD, 1, LD, 1>(c, P, Y, tid);
+        }
+        __syncthreads();
+        each(c, tid, [&](int t, int n, float &x) {
+            if (t < all && j + n < a.Dv) out[t * a.out.ts + j + n] = seq::from_f<T>(t < tokens ? x : 0.f);
+        });
+    }
+}
+
+// grid: chunks x B H.  dq, dk: where the type's elements go, or fp32 sums of every head [T][B][H][Dk] (heads that share q and k).
+template <class T>
+__global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ qgru_attention a, const float *states, const float *dstates, float *dq_heads,
+                                                       float *dk_heads) {
+    extern __shared__ float smem[];
+    float *X = smem, *Y = X + C * LD, *P = Y + C * LD, *E = P + C * LD;
+    __shared__ float2 G[C];
+    __shared__ double sums[2];
+    __shared__ float dG[C + 1], kE[C];       // what a change of the decays' sum up to token t brings; k_s's share behind the chunk
+    const int tid = threadIdx.x, heads = a.B * a.H, chunk = blockIdx.x / heads, bh = blockIdx.x % heads, b = bh / a.H, h = bh % a.H, t0 = chunk * C;
+    const int all = min(a.T - t0, C), tokens = min(max(valid_tokens(a, b) - t0, 0), C);
+    const int hk = h / (a.H / a.Hk);
+    const long long qb = at(a.q, b, hk), kb = at(a.k, b, hk), vb = at(a.v, b, h), ob = at(a.dout, b, h);
+    const auto put_qk = [&](const qgru_seq_tensor &x, float *heads, int t, int d, float v) {
+        if (heads)
+            heads[(((long long)(t0 + t) * a.B + b) * a.H + h) * a.Dk + d] = v;
+        else
+            static_cast<T *>(x.p)[at(x, b, h) + (t0 + t) * x.ts + d] = seq::from_f<T>(v);
+    };
+    T *dv = static_cast<T *>(a.dv.p) + at(a.dv, b, h) + t0 * a.dv.ts;
+    const long long gb = at(a.ddecay, b, h) + t0 * a.ddecay.ts;
+    if (tokens == 0) {
+        for (int e = tid; e < all * a.Dk; e += THREADS) {
+            put_qk(a.dq, dq_heads, e / a.Dk, e % a.Dk, 0.f);
+            put_qk(a.dk, dk_heads, e / a.Dk, e % a.Dk, 0.f);
+        }
+        for (int e = tid; e < all * a.Dv; e += THREADS) dv[(e / a.Dv) * a.dv.ts + e % a.Dv] = seq::from_f<T>(0.f);
+        if (tid < all) seq::store_f(a.ddecay.p, gb + tid * a.ddecay.ts, a.decay_bf16, 0.f);
+        return;
+    }
+    const long long tile = chunk * (long long)heads * a.Dk * a.Dv + (long long)bh * a.Dk * a.Dv;
+    const float *S = states + tile, *dS = dstates + tile;
+    load_decays(G, sums, a, b, h, t0, tokens, tid);
+    if (tid < C) kE[tid] = 0.f;
+    if (tid <= C) dG[tid] = 0.f;
+    Acc c, e2;
+    c.zero();
+    e2.zero();
+    for (int d = 0; d < a.Dk; d += 64) {
+        load_tile<T>(X, a.q, qb, t0, tokens, d, a.Dk, tid);
+        load_tile<T>(Y, a.k, kb, t0, tokens, d, a.Dk, tid);
+        __syncthreads();
+        multiply<LD, 1, 1, LD>(c, X, Y, tid);
+        __syncthreads();
+    }
+    for (int d = 0; d < a.Dv; d += 64) {
+        load_tile<T>(X, a.dout, ob, t0, tokens, d, a.Dv, tid);
+        load_tile<T>(Y, a.v, vb, t0, tokens, d, a.Dv, tid);
+        __syncthreads();
+        multiply<LD, 1, 1, LD>(e2, X, Y, tid);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int t = (tid >> 4) + 16 * i, s = (tid & 15) + 16 * j;
+            const float w = s <= t ? a.scale * exp2_diff(G[t], G[s]) : 0.f;
+            const float p = s <= t ? w * c.v[i][j] : 0.f, e = s <= t ? w * e2.v[i][j] : 0.f;
+            P[t * LD + s] = p;
+            E[t * LD + s] = e;
+            X[t * LD + s] = s < t ? p * e2.v[i][j] : 0.f;
+        }
+    __syncthreads();
+    // every pair (t, s), s < t: a change of G_t adds, one of G_s takes away
+    if (tid < C) {
+        double r = 0.0;
+        for (int s = 0; s < C; ++s) r += (double)X[tid * LD + s] - (double)X[s * LD + tid];
+        dG[tid] = (float)r;
+    }
+    __syncthreads();
+    const float2 end = G[C - 1];
+    for (int i = 0; i < a.Dk; i += 64) {
+        // dq = E k + scale 2^G_t dout S^T
+        c.zero();
+        for (int j = 0; j < a.Dv; j += 64) {
+            load_tile<T>(X, a.dout, ob, t0, tokens, j, a.Dv, tid);
+            load_state(Y, S, i, j, a, tid);
+            __syncthreads();
+            multiply<LD, 1, 1, LD>(c, X, Y, tid);
+            __syncthreads();
+        }
+        load_tile<T>(X, a.q, qb, t0, tokens, i, a.Dk, tid);
+        load_tile<T>(Y, a.k, kb, t0, tokens, i, a.Dk, tid);
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int t = (tid >> 4) + 16 * r;
+            const float w = a.scale * exp2_of(G[t]);
+            float x = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                c.v[r][j] *= w;
+                x = fmaf(c.v[r][j], X[t * LD + (tid & 15) + 16 * j], x);
+            }
+            for (int o = 8; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+            if ((tid & 15) == 0) dG[t] += x;
+        }
+        multiply<LD, 1, LD, 1>(c, E, Y, tid);
+        each(c, tid, [&](int t, int d, float &x) { if (t < all && i + d < a.Dk) put_qk(a.dq, dq_heads, t, i + d, t < tokens ? x : 0.f); });
+        __syncthreads();
+        // dk = E^T q + 2^(G_C - G_s) v dS^T
+        c.zero();
+        for (int j = 0; j < a.Dv; j += 64) {
+            load_tile<T>(X, a.v, vb, t0, tokens, j, a.Dv, tid);
+            load_state(Y, dS, i, j, a, tid);
+            __syncthreads();
+            multiply<LD, 1, 1, LD>(c, X, Y, tid);
+            __syncthreads();
+        }
+        load_tile<T>(X, a.q, qb, t0, tokens, i, a.Dk, tid);
+        load_tile<T>(Y, a.k, kb, t0, tokens, i, a.Dk, tid);
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int s = (tid >> 4) + 16 * r;
+            const float w = exp2_diff(end, G[s]);
+            float x = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                c.v[r][j] *= w;
+                x = fmaf(c.v[r][j], Y[s * LD + (tid & 15) + 16 * j], x);
+            }
+            for (int o = 8; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+            if ((tid & 15) == 0) kE[s] += x;
+        }
+        multiply<1, LD, LD, 1>(c, E, X, tid);
+        each(c, tid, [&](int s, int d, float &x) { if (s < all && i + d < a.Dk) put_qk(a.dk, dk_heads, s, i + d, s < tokens ? x : 0.f); });
+        __syncthreads();
+    }
+    for (int j = 0; j < a.Dv; j += 64) {
+        // dv = P^T dout + 2^(G_C - G_s) k dS
+        c.zero();
+        for (int i = 0; i < a.Dk; i += 64) {
+            load_tile<T>(X, a.k, kb, t0, tokens, i, a.Dk, tid);
+            load_state(Y, dS, i, j, a, tid);
+            __syncthreads();
+            multiply<LD, 1, LD, 1>(c, X, Y, tid);
+            __syncthreads();
+        }
+        each(c, tid, [&](int s, int, float &x) { x *= exp2_diff(end, G[s]); });
+        load_tile<T>(X, a.dout, ob, t0, tokens, j, a.Dv, tid);
+        __syncthreads();
+        multiply<1, LD, LD, 1>(c, P, X, tid);
+        each(c, tid, [&](int s, int d, float &x) { if (s < all && j + d < a.Dv) dv[s * a.dv.ts + j + d] = seq::from_f<T>(s < tokens ? x : 0.f); });
+        __syncthreads();
+    }
+    // The state before the chunk reaches everything behind it through all of the chunk's decays.
+    double through = 0.0;
+    for (int e = tid; e < a.Dk * a.Dv; e += THREADS) through += (double)S[e] * (double)dS[e];
+    for (int o = 16; o; o >>= 1) through += __shfl_xor_sync(0xffffffffu, through, o);
+    double *part = reinterpret_cast<double *>(smem);
+    if ((tid & 31) == 0) part[tid >> 5] = through;
+    __syncthreads();
+    if (tid == 0) {
+        through = 0.0;
+        for (int w = 0; w < THREADS / 32; ++w) through += part[w];
+        through *= (double)exp2_of(end);
+        for (int s = 0; s < tokens; ++s) through += (double)kE[s];
+        // from the end: sum over u >= t of dG_u, the shares of k_s for s < t, and what passes through
+        double acc = 0.0;
+        for (int t = tokens - 1; t >= 0; --t) {
+            acc += (double)dG[t];
+            through -= (double)kE[t];
+            X[64 + t] = (float)(acc + through);
+        }
+    }
+    __syncthreads();
+    if (tid < all) seq::store_f(a.ddecay.p, gb + tid * a.ddecay.ts, a.decay_bf16, tid < tokens ? X[64 + tid] : 0.f);
+}
+
+// dq and dk of heads that share q and k: the sum over each group, one rounding.
+template <class T>
+__global__ void k_sum_groups(const __grid_constant__ qgru_attention a, const float *dq, const float *dk) {
+    const int g = a.H / a.Hk;
+    const long long n = (long long)a.T * a.B * a.Hk * a.Dk;
+    const qgru_seq_tensor to = blockIdx.y ? a.dk : a.dq;
+    const float *from = blockIdx.y ? dk : dq;
+    for (long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (long long)gridDim.x * blockDim.x) {
+        const int d = (int)(e % a.Dk), hk = (int)(e / a.Dk % a.Hk);
+        const long long tb = e / a.Dk / a.Hk;
+        const float *p = from + (tb * a.H + (long long)hk * g) * a.Dk + d;
+        float s = 0.f;
+        for (int i = 0; i < g; ++i) s += p[(long long)i * a.Dk];
+        static_cast<T *>(to.p)[tb / a.B * to.ts + tb % a.B * to.bs + hk * to.hs + d] = seq::from_f<T>(s);
+    }
+}
+
+template <class F>
+int with_smem(F *kernel, size_t bytes) {
+    SEQ_CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    return QGRU_OK;
+}
+
+template <class T, bool Reverse>
+int run_states(const qgru_attention &a, const Cut &c, float *states, char *seg, cudaStream_t st) {
+    Pass p{};
+    p.k = Reverse ? a.q : a.k;
+    p.v = Reverse ? a.dout : a.v;
+    p.k_share = a.H / a.Hk;
+    p.first = Reverse ? a.dstate : a.state0;
+    p.last = Reverse ? a.dstate0 : a.state;
+    p.segments = c.segments;
+    p.per = c.per;
+    p.chunks = c.chunks;
+    const dim3 grid(a.B * a.H, (unsigned)((a.Dk + 63) / 64 * ((a.Dv + 63) / 64)), c.segments);
+    if (c.segments > 1) {
+        p.seg_state = reinterpret_cast<float *>(seg);
+        p.seg_log = p.seg_state + c.segments * state_elems(a);
+        p.own_sums = true;
+        k_states<T, Reverse><<<grid, THREADS, 0, st>>>(a, p);
+        SEQ_CK(cudaGetLastError());
+        if (const int rc = scan_segments(a, c, Reverse, seg, st)) return rc;
+    }
+    p.states = states;
+    p.own_sums = false;
+    k_states<T, Reverse><<<grid, THREADS, 0, st>>>(a, p);
+    SEQ_CK(cudaGetLastError());
+    return QGRU_OK;
+}
+
+template <class T>
+int forward(const qgru_attention &a, const Cut &c, cudaStream_t st) {
+    float *states = static_cast<float *>(a.states);
+    if (const int rc = run_states<T, false>(a, c, states, static_cast<char *>(a.workspace), st)) return rc;
+    if (c.chunks == 0) return QGRU_OK;
+    constexpr size_t bytes = 3 * C * LD * sizeof(float);
+    if (const int rc = with_smem(k_outputs<T>, bytes)) return rc;
+    k_outputs<T><<<c.chunks * a.B * a.H, THREADS, bytes, st>>>(a, states);
+    SEQ_CK(cudaGetLastError());
+    return QGRU_OK;
+}
+
+template <class T>
+int backward(const qgru_attention &a, const Cut &c, cudaStream_t st) {
+    char *ws = static_cast<char *>(a.workspace);
+    float *dstates = reinterpret_cast<float *>(ws);
+    ws += a256(c.states);
+    char *seg = ws;
+    ws += a256(c.seg);
+    if (const int rc = run_states<T, true>(a, c, dstates, seg, st)) return rc;
+    if (c.chunks == 0) return QGRU_OK;
+    float *dq = nullptr, *dk = nullptr;
+    if (a.H != a.Hk) {
+        dq = reinterpret_cast<float *>(ws);
+        dk = dq + group_bytes(a) / 8;
+    }
+    constexpr size_t bytes = 4 * C * LD * sizeof(float);
+    if (const int rc = with_smem(k_gradients<T>, bytes)) return rc;
+    k_gradients<T><<<c.chunks * a.B * a.H, THREADS, bytes, st>>>(a, static_cast<const float *>(a.states), dstates, dq, dk);
+    SEQ_CK(cudaGetLastError());
+    return dq ? sum_groups(a, dq, dk, st) : QGRU_OK;
+}
+
+// ------------------------------------------------------------------------------------ single tokens
+// One CTA per (row, head, 128 columns of the state): a lane has V neighbouring columns of a state row, W lanes a row and 256 / W rows at
+// a time, U of them in flight.  Bytes bound it: the state, read and written once.
+template <class T, int V>
+__global__ void __launch_bounds__(256) k_step(const __grid_constant__ qgru_attention a, long long state_bs, long long state_hs, int W) {
+    constexpr int U = 8;
+    __shared__ float qs[MAX_D], ks[MAX_D], part[256 * V];
+    const int tid = threadIdx.x, b = blockIdx.x / a.H, h = blockIdx.x % a.H, hk = h / (a.H / a.Hk);
+    const int lane = tid % W, group = tid / W, groups = 256 / W, j = blockIdx.y * 32 * V + lane * V;
+    const bool on = j < a.Dv;
+    float *S = a.state + b * state_bs + h * state_hs + j;
+    float s[U][V];
+    const auto fetch = [&](int r0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * groups;
+            if (!on || r >= a.Dk) continue;
+            if constexpr (V == 4)
+                *reinterpret_cast<float4 *>(s[u]) = *reinterpret_cast<const float4 *>(S + (long long)r * a.Dv);
+            else
+                s[u][0] = S[(long long)r * a.Dv];
+        }
+    };
+    fetch(group);
+    const T *q = static_cast<const T *>(a.q.p) + at(a.q, b, hk), *k = static_cast<const T *>(a.k.p) + at(a.k, b, hk);
+    for (int d = tid; d < a.Dk; d += 256) {
+        qs[d] = seq::to_f(q[d]);
+        ks[d] = seq::to_f(k[d]);
+    }
+    const float g = seq::load_f(a.decay.p, at(a.decay, b, h), a.decay_bf16), keep = expf(g);
+    float v[V], o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        v[i] = on ? seq::to_f(static_cast<const T *>(a.v.p)[at(a.v, b, h) + j + i]) : 0.f;
+        o[i] = 0.f;
+    }
+    __syncthreads();
+    for (int r0 = group; r0 < a.Dk; r0 += U * groups) {
+        if (r0 != group) fetch(r0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * groups;
+            if (!on || r >= a.Dk) continue;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                s[u][i] = fmaf(ks[r], v[i], keep * s[u][i]);
+                o[i] = fmaf(qs[r], s[u][i], o[i]);
+            }
+            if constexpr (V == 4)
+                *reinterpret_cast<float4 *>(S + (long long)r * a.Dv) = *reinterpret_cast<const float4 *>(s[u]);
+            else
+                S[(long long)r * a.Dv] = s[u][0];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) part[tid * V + i] = o[i];
+    __syncthreads();
+    for (int c = tid; c < W * V; c += 256) {
+        float x = 0.f;
+        for (int g2 = 0; g2 < groups; ++g2) x += part[g2 * W * V + c];
+        const int col = blockIdx.y * 32 * V + c;
+        if (col < a.Dv) static_cast<T *>(a.out.p)[at(a.out, b, h) + col] = seq::from_f<T>(a.scale * x);
+    }
+}
+
+template <class T>
+int step(const qgru_attention &a, long long bs, long long hs, cudaStream_t st) {
+    const bool wide = a.Dv % 4 == 0 && bs % 4 == 0 && hs % 4 == 0 && reinterpret_cast<uintptr_t>(a.state) % 16 == 0;
+    const int V = wide ? 4 : 1, vectors = (a.Dv + V - 1) / V;
+    int W = 1;
+    while (W < vectors && W < 32) W *= 2;
+    const dim3 grid(a.B * a.H, (a.Dv + 32 * V - 1) / (32 * V));
+    if (wide)
+        k_step<T, 4><<<grid, 256, 0, st>>>(a, bs, hs, W);
+    else
+        k_step<T, 1><<<grid, 256, 0, st>>>(a, bs, hs, W);
+    SEQ_CK(cudaGetLastError());
+    return QGRU_OK;
+}
+
+}  // namespace
+
+size_t group_bytes(const qgru_attention &a) { return a.H == a.Hk ? 0 : 2 * sizeof(float) * (size_t)a.T * a.B * a.H * a.Dk; }
+
+int sum_groups(const qgru_attention &a, const float *dq, const float *dk, cudaStream_t st) {
+    const long long n = (long long)a.T * a.B * a.Hk * a.Dk;
+    const dim3 grid((unsigned)std::min<long long>((n + 255) / 256, 4096), 2);
+    if (a.bf16)
+        k_sum_groups<bf16><<<grid, 256, 0, st>>>(a, dq, dk);
+    else
+        k_sum_groups<float><<<grid, 256, 0, st>>>(a, dq, dk);
+    SEQ_CK(cudaGetLastError());
+    return QGRU_OK;
+}
+
+int scan_segments(const qgru_attention &a, const Cut &c, bool reverse, char *seg, cudaStream_t st) {
+    float *s = reinterpret_cast<float *>(seg);
+    const long long n = (long long)state_elems(a);
+    k_scan_segments<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(s, s + c.segments * n, reverse ? a.dstate : a.state0, c.segments, n, a.Dk * a.Dv);
+    SEQ_CK(cudaGetLastError());
+    return QGRU_OK;
+}
+
+// Segments: as many as fill the SMs twice where the heads alone do not, of two chunks at the least (each token's k and v are read
+// once more for it).
+Cut generic_cut(const qgru_attention &a, int sms) {
+    Cut c;
+    c.chunk = C;
+    c.chunks = (a.T + C - 1) / C;
+    const long long units = (long long)a.B * a.H * ((a.Dk + 63) / 64) * ((a.Dv + 63) / 64);
+    c.segments = (int)std::max<long long>(1, std::min<long long>(c.chunks / 2, (2 * sms + units - 1) / std::max<long long>(units, 1)));
+    c.per = std::max(1, (c.chunks + c.segments - 1) / c.segments);
+    c.segments = std::max(1, (c.chunks + c.per - 1) / c.per);
+    c.states = sizeof(float) * c.chunks * state_elems(a);
+    c.seg = c.segments > 1 ? sizeof(float) * c.segments * (state_elems(a) + (size_t)a.B * a.H) : 0;
+    return c;
+}
+int generic_forward(const qgru_attention &a, const Cut &c, cudaStream_t st) { return a.bf16 ? forward<bf16>(a, c, st) : forward<float>(a, c, st); }
+int generic_backward(const qgru_attention &a, const Cut &c, cudaStream_t st) { return a.bf16 ? backward<bf16>(a, c, st) : backward<float>(a, c, st); }
+
+namespace {
+
+int check(const qgru_attention *a) {
+    using seq::fail;
+    if (!a) return fail(QGRU_ERR_BAD_ARG, "null argument block");
+    if (a->T < 0 || a->B < 0 || a->H < 1 || a->Hk < 1 || a->Dk < 1 || a->Dv < 1) return fail(QGRU_ERR_BAD_ARG, "sizes must be positive (T and B may be 0)");
+    if (a->H % a->Hk) return fail(QGRU_ERR_BAD_ARG, "%d heads cannot share %d heads of q and k", a->H, a->Hk);
+    if (a->Dk > MAX_D || a->Dv > MAX_D) return fail(QGRU_ERR_UNSUPPORTED, "head sizes are at most %d, got %d and %d", MAX_D, a->Dk, a->Dv);
+    if (a->T > 1 << 30 || (long long)a->B * a->H > 2147483647ll || (long long)a->B * a->H * ((a->T + 63) / 64) > 2147483647ll)
+        return fail(QGRU_ERR_UNSUPPORTED, "at most 2^30 tokens, and 2^31 chunks of 64 tokens over all sequences and heads");
+    return QGRU_OK;
+}
+
+int sm_count(int device, int *sms) {
+    SEQ_CK(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device));
+    return QGRU_OK;
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace qgru
+
+using namespace qgru;
+
+extern "C" {
+
+int qgru_attention_sizes(const qgru_attention *a, size_t *states_bytes, size_t *forward_workspace, size_t *backward_workspace) {
+    if (const int rc = attn::check(a)) return rc;
+    int sms = 0;
+    if (const int rc = attn::sm_count(a->device, &sms)) return rc;
+    const attn::Cut c = attn::generic_cut(*a, sms);
+    if (states_bytes) *states_bytes = attn::a256(c.states);
+    if (forward_workspace) *forward_workspace = attn::a256(c.seg);
+    if (backward_workspace) *backward_workspace = attn::a256(c.states) + attn::a256(c.seg) + attn::group_bytes(*a);
+    return QGRU_OK;
+}
+
+static int attention_run(const qgru_attention *a, bool backward, void *stream) {
+    if (const int rc = attn::check(a)) return rc;
+    if (a->B == 0) return QGRU_OK;
+    size_t states = 0, fwd = 0, bwd = 0;
+    if (const int rc = qgru_attention_sizes(a, &states, &fwd, &bwd)) return rc;
+    const size_t ws = backward ? bwd : fwd;
+    if (a->T > 0 && (!a->q.p || !a->k.p || !a->v.p || !a->decay.p)) return seq::fail(QGRU_ERR_BAD_ARG, "null input");
+    if (a->T > 0 && (backward ? !a->dout.p || !a->dq.p || !a->dk.p || !a->dv.p || !a->ddecay.p : !a->out.p)) return seq::fail(QGRU_ERR_BAD_ARG, "null output or gradient");
+    if ((states && !a->states) || a->states_bytes < states) return seq::fail(QGRU_ERR_BAD_ARG, "states needs %zu bytes, got %zu", states, a->states_bytes);
+    if ((ws && !a->workspace) || a->workspace_bytes < ws) return seq::fail(QGRU_ERR_BAD_ARG, "workspace needs %zu bytes, got %zu", ws, a->workspace_bytes);
+    if ((reinterpret_cast<uintptr_t>(a->states) | reinterpret_cast<uintptr_t>(a->workspace)) % 256) return seq::fail(QGRU_ERR_BAD_ARG, "states and workspace must be aligned to 256 bytes");
+    const seq::OnDevice on(a->device);
+    SEQ_CK(on.error());
+    int sms = 0;
+    if (const int rc = attn::sm_count(a->device, &sms)) return rc;
+    const attn::Cut c = attn::generic_cut(*a, sms);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return backward ? attn::generic_backward(*a, c, st) : attn::generic_forward(*a, c, st);
+}
+
+int qgru_attention_forward(const qgru_attention *a, void *stream) { return attention_run(a, false, stream); }
+int qgru_attention_backward(const qgru_attention *a, void *stream) { return attention_run(a, true, stream); }
+
+int qgru_attention_step(const qgru_attention *a, long long state_bs, long long state_hs, void *stream) {
+    if (const int rc = attn::check(a)) return rc;
+    if (a->B == 0) return QGRU_OK;
+    if (!a->q.p || !a->k.p || !a->v.p || !a->decay.p || !a->out.p || !a->state) return seq::fail(QGRU_ERR_BAD_ARG, "null tensor");
+    if (a->T != 1 || a->lengths) return seq::fail(QGRU_ERR_BAD_ARG, "a step takes one token of every sequence");
+    const seq::OnDevice on(a->device);
+    SEQ_CK(on.error());
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return a->bf16 ? attn::step<__nv_bfloat16>(*a, state_bs, state_hs, st) : attn::step<float>(*a, state_bs, state_hs, st);
+}
+
+}  // extern "C"

@@ -1,0 +1,67 @@
+// qgru_attn.cuh - linear attention with a decay for each head: what its kernels share.
+//
+// A sequence is cut into chunks of C tokens.  With G_t the running sum of the decays' logarithms from the chunk's start (base 2
+// here) and S0 the state before the chunk
+//     out_t = scale (2^G_t q_t S0 + sum_{s<=t} 2^(G_t - G_s) (q_t.k_s) v_s),    S' = 2^G_C S0 + sum_s 2^(G_C - G_s) k_s^T v_s
+// so that one pass ("state pass") walks the chunks and leaves the state before each of them, and another takes every chunk by
+// itself.  The gradient of the states obeys the same recurrence from the end, with q for k, dout for v and scale 2^G_t as
+// weight, and is left behind each chunk by the same pass.
+#pragma once
+#include "qgru_seq.cuh"
+
+namespace qgru {
+namespace attn {
+
+constexpr int MAX_D = 256;
+constexpr float LOG2E = 1.4426950408889634f;
+// A decay below 2^-256 is zero to any fp32 sum; the clamp keeps -inf out of the differences of the running sums.
+constexpr double LOWEST = -256.0;
+
+struct Cut {               // of a sequence of T tokens into chunks, and of the chunks into segments that run side by side
+    int chunk = 0, chunks = 0, segments = 0, per = 0;
+    size_t states = 0;     // bytes of the states before the chunks
+    size_t seg = 0;        // bytes of the segments' own last states and decays, 0 for one segment
+};
+
+__device__ __forceinline__ int valid_tokens(const qgru_attention &a, int b) {
+    return a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+}
+
+// One token's decay, base 2.  A running sum over a chunk reaches 2^14 at the most and is kept as two floats, so that the
+// difference of two of them is as exact as the difference itself: G_t - G_s = (hi_t - hi_s) + (lo_t - lo_s).
+__device__ __forceinline__ double decay_log2(const qgru_attention &a, long long at) {
+    const double g = (double)seq::load_f(a.decay.p, at, a.decay_bf16) * 1.4426950408889634074;
+    return g < LOWEST ? LOWEST : g;       // (NaN stays)
+}
+__device__ __forceinline__ float2 two_floats(double x) {
+    const float hi = (float)x;
+    return make_float2(hi, (float)(x - (double)hi));
+}
+__device__ __forceinline__ float exp2_diff(float2 t, float2 s) { return exp2f((t.x - s.x) + (t.y - s.y)); }
+__device__ __forceinline__ float exp2_of(float2 t) { return exp2f(t.x + t.y); }
+
+// Running sums over N tokens (N / 32 warps, thread i has token i of them): the sum up to and with the thread's own.
+template <int N>
+__device__ __forceinline__ double running_sum(double g, double *warp_sums, int tid) {
+    const int lane = tid & 31;
+    for (int o = 1; o < 32; o <<= 1) {
+        const double u = __shfl_up_sync(0xffffffffu, g, o);
+        if (lane >= o) g += u;
+    }
+    if (lane == 31) warp_sums[tid >> 5] = g;
+    return g;
+}
+
+// ---- kernels for every size and type (qgru_attn.cu): fp32 sums by multiply-adds
+Cut generic_cut(const qgru_attention &a, int sms);
+int generic_forward(const qgru_attention &a, const Cut &c, cudaStream_t st);
+int generic_backward(const qgru_attention &a, const Cut &c, cudaStream_t st);
+size_t group_bytes(const qgru_attention &a);
+int sum_groups(const qgru_attention &a, const float *dq, const float *dk, cudaStream_t st);
+int scan_segments(const qgru_attention &a, const Cut &c, bool reverse, char *seg, cudaStream_t st);
+
+inline size_t a256(size_t n) { return (n + 255) & ~size_t(255); }
+inline size_t state_elems(const qgru_attention &a) { return (size_t)a.B * a.H * a.Dk * a.Dv; }
+
+}  // namespace attn
+}  // namespace qgru
