@@ -589,7 +589,9 @@ QGRU_API int qgru_calibrate_from_histogram(const float *counts, int num_bins, fl
  * linear in its state, and the root-mean-square norm with the residual's addition that such layers stand
  * between.  These calls have no handle: they keep nothing, allocate nothing and wait for nothing; workspaces are the
  * caller's, and calls that do not share one may run at the same time.  They run on `device`, whatever the thread's current
- * device is.  qgru_seq_last_error: why the calling thread's last of these calls failed. */
+ * device is.  A wait inside a kernel that runs out (each is bounded) leaves NaN in its results and is told once, by the next of
+ * these calls that begins after the GPU got there (QGRU_ERR_TIMEOUT).
+ * qgru_seq_last_error: why the calling thread's last of these calls failed. */
 QGRU_API const char *qgru_seq_last_error(void);
 
 /* Element (t, b, h, d) of a tensor lies at p + t * ts + b * bs + h * hs + d (elements; decays have no d). */

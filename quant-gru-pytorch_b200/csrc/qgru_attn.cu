@@ -1,10 +1,11 @@
 // qgru_attn.cu - linear attention: the entry points, the kernels for every size and type, and the single-token form.
 //
 // The kernels here compute in fp32 by multiply-adds, whatever the inputs' type, 64 tokens a chunk and 64 x 64 tiles; they serve
-// head sizes above 128.
+// what the tensor-core kernels (qgru_attn_tc.cu) do not take.
 #include <algorithm>
 
 #include "qgru_attn.cuh"
+#include "qgru_attn_tc.cuh"
 
 namespace qgru {
 namespace attn {
@@ -591,8 +592,10 @@ int check(const qgru_attention *a) {
     return QGRU_OK;
 }
 
-int sm_count(int device, int *sms) {
-    SEQ_CK(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device));
+int cut(const qgru_attention &a, Cut *c) {
+    int sms = 0;
+    SEQ_CK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, a.device));
+    *c = tc_takes(a) ? tc_cut(a, sms) : generic_cut(a, sms);
     return QGRU_OK;
 }
 
@@ -606,9 +609,8 @@ extern "C" {
 
 int qgru_attention_sizes(const qgru_attention *a, size_t *states_bytes, size_t *forward_workspace, size_t *backward_workspace) {
     if (const int rc = attn::check(a)) return rc;
-    int sms = 0;
-    if (const int rc = attn::sm_count(a->device, &sms)) return rc;
-    const attn::Cut c = attn::generic_cut(*a, sms);
+    attn::Cut c;
+    if (const int rc = attn::cut(*a, &c)) return rc;
     if (states_bytes) *states_bytes = attn::a256(c.states);
     if (forward_workspace) *forward_workspace = attn::a256(c.seg);
     if (backward_workspace) *backward_workspace = attn::a256(c.states) + attn::a256(c.seg) + attn::group_bytes(*a);
@@ -628,10 +630,14 @@ static int attention_run(const qgru_attention *a, bool backward, void *stream) {
     if ((reinterpret_cast<uintptr_t>(a->states) | reinterpret_cast<uintptr_t>(a->workspace)) % 256) return seq::fail(QGRU_ERR_BAD_ARG, "states and workspace must be aligned to 256 bytes");
     const seq::OnDevice on(a->device);
     SEQ_CK(on.error());
-    int sms = 0;
-    if (const int rc = attn::sm_count(a->device, &sms)) return rc;
-    const attn::Cut c = attn::generic_cut(*a, sms);
+    attn::Cut c;
+    if (const int rc = attn::cut(*a, &c)) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (attn::tc_takes(*a)) {
+        int *flag = nullptr;
+        if (const int rc = seq::expiry_flag(a->device, &flag)) return rc;
+        return backward ? attn::tc_backward(*a, c, flag, st) : attn::tc_forward(*a, c, flag, st);
+    }
     return backward ? attn::generic_backward(*a, c, st) : attn::generic_forward(*a, c, st);
 }
 

@@ -1,0 +1,899 @@
+// qgru_attn_tc.cu - linear attention on the tensor cores: bf16 tensors, head sizes up to 128 (padded to 64 or 128), chunks of 128 tokens.
+//
+// Three kernels: the state pass (forward, and for the gradient of the states from the end), the outputs, and the gradients; in the
+// last two every chunk is a CTA's own.  All products are tcgen05.mma kind::f16 with fp32 sums in tensor memory and
+// operands in shared memory as rows of 128 bytes with the 128-byte swizzle.  Such a tile [rows][64 columns] is an operand with
+// its columns as K (K-major) and one with its rows as K (MN-major), so that no operand is transposed anywhere.
+//
+// What is rounded to bf16 on the way: the weights of the pairs of tokens (P, E), and the state before a chunk and its
+// gradient behind it where they are factors of a product.  Each is one rounding of a factor, the size of the one that the results
+// get in the end.  The states themselves are fp32: their products take k scaled by the decays as three bf16 parts (24 bits).
+#include <algorithm>
+#include <type_traits>
+
+#include "qgru_attn.cuh"
+#include "qgru_attn_tc.cuh"
+#include "qgru_tc.cuh"
+
+namespace qgru {
+namespace attn {
+namespace {
+
+constexpr int C = 128, THREADS = 256;
+constexpr int PANEL = C * 128;                          // bytes of 64 columns of a tile of 128 rows
+constexpr long long WAIT_BUDGET = 2000000000ll;         // about a second of SM clocks
+using bf16 = __nv_bfloat16;
+
+// ------------------------------------------------------------------------------------- operands and products
+constexpr uint32_t DESC_HI = (uint32_t)(1024 >> 4) | (1u << 14) | (2u << 29);     // groups of eight rows 1024 bytes apart, 128-byte swizzle
+
+struct Operand {                        // a tile, `panel` bytes from 64 columns to the next
+    uint32_t at;
+    int panel;
+};
+// Low word of the descriptor for K = 16 j .. 16 j + 15.  K in the columns: 32 bytes a step, four steps a panel.  K in the rows:
+// 2048 bytes (sixteen rows) a step, and the descriptor's leading distance is that between panels.
+template <bool KRows>
+__device__ __forceinline__ uint32_t desc_lo(const Operand &o, int j) {
+    if constexpr (KRows)
+        return (((o.at + j * 2048) & 0x3FFFFu) >> 4) | ((uint32_t)o.panel >> 4 << 16);
+    else
+        return (((o.at + (j >> 2) * o.panel + (j & 3) * 32) & 0x3FFFFu) >> 4) | (1u << 16);
+}
+// D fp32, A and B bf16, M = 128
+__host__ __device__ constexpr uint32_t idesc(int N, bool a_rows, bool b_rows) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((a_rows ? 1u : 0u) << 15) | ((b_rows ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        ".reg .b64 da, db;\n"
+        "mov.b64 da, {%1, %5};\n"
+        "mov.b64 db, {%2, %5};\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n"
+        "}\n" ::"r"(d),
+        "r"(a_lo), "r"(b_lo), "r"(id), "r"(accumulate), "n"(DESC_HI)
+        : "memory");
+}
+// A from tensor memory: lane i is row i, a column holds two neighbouring K, sixteen K are eight columns
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        ".reg .b64 db;\n"
+        "mov.b64 db, {%2, %5};\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n"
+        "}\n" ::"r"(d),
+        "r"(a), "r"(b_lo), "r"(id), "r"(accumulate), "n"(DESC_HI)
+        : "memory");
+}
+template <bool ARows, bool BRows, int N, int K>
+__device__ __forceinline__ void product(uint32_t d, const Operand &a, const Operand &b, bool add) {
+#pragma unroll
+    for (int j = 0; j < K / 16; ++j) mma(d, desc_lo<ARows>(a, j), desc_lo<BRows>(b, j), idesc(N, ARows, BRows), (add || j) ? 1u : 0u);
+}
+template <bool BRows, int N, int K>
+__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, const Operand &b, bool add) {
+#pragma unroll
+    for (int j = 0; j < K / 16; ++j) mma_ts(d, a + j * 8, desc_lo<BRows>(b, j), idesc(N, false, BRows), (add || j) ? 1u : 0u);
+}
+
+__device__ __forceinline__ uint32_t lane_base(uint32_t tmem, int warp) { return tmem + ((uint32_t)((warp & 3) * 32) << 16); }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
+                 "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+// Cols / 16 groups of sixteen columns
+template <int Cols>
+__device__ __forceinline__ void tmem_load(uint32_t taddr, float (&v)[Cols]) {
+    int32_t r[Cols / 16][16];
+#pragma unroll
+    for (int i = 0; i < Cols / 16; ++i) tc::tmem_ld16(taddr + i * 16, r[i]);
+    tc::tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < Cols; ++i) v[i] = __int_as_float(r[i / 16][i % 16]);
+}
+template <int Cols>
+__device__ __forceinline__ void tmem_store(uint32_t taddr, const uint32_t (&v)[Cols]) {
+#pragma unroll
+    for (int i = 0; i < Cols / 16; ++i) {
+        uint32_t r[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r[j] = v[i * 16 + j];
+        tmem_st16(taddr + i * 16, r);
+    }
+}
+
+// ------------------------------------------------------------------------------------- values
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float low(uint32_t x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float high(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float ex2_diff(float2 t, float2 s) { return ex2((t.x - s.x) + (t.y - s.y)); }
+
+// 16-byte chunk c (of eight columns) of row r of a panel
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
+
+__device__ __forceinline__ void cp_async(uint32_t to, const void *from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int Left>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(Left) : "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Rows t0 .. t0 + 127 of a tensor (zeros from `tokens` on and behind its columns) as a tile of D columns.  Vec: rows and strides
+// are multiples of 16 bytes; else element by element.
+template <int D, bool Vec>
+__device__ __forceinline__ void load_rows(uint32_t tile, const qgru_seq_tensor &x, long long base, int t0, int tokens, int d, int tid) {
+    const bf16 *p = static_cast<const bf16 *>(x.p) + base + (long long)t0 * x.ts;
+    constexpr int PER_ROW = D / 8;
+#pragma unroll
+    for (int i = 0; i < C * PER_ROW / THREADS; ++i) {
+        const int e = i * THREADS + tid, r = e / PER_ROW, c = e % PER_ROW;
+        const uint32_t to = tile + (c >> 3) * PANEL + chunk_at(r, c & 7);
+        if constexpr (Vec) {
+            const bool on = r < tokens && c * 8 < d;
+            cp_async(to, on ? p + r * x.ts + c * 8 : p, on ? 16 : 0);
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int d0 = c * 8 + 2 * j;
+                const uint32_t u0 = r < tokens && d0 < d ? __bfloat16_as_ushort(p[r * x.ts + d0]) : 0u;
+                const uint32_t u1 = r < tokens && d0 + 1 < d ? __bfloat16_as_ushort(p[r * x.ts + d0 + 1]) : 0u;
+                w[j] = u0 | u1 << 16;
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        }
+    }
+}
+// A state [DK][DV] as it is kept before each chunk (bf16, padded) as a tile.
+template <int DK, int DV>
+__device__ __forceinline__ void load_state(uint32_t tile, const bf16 *S, int tid) {
+#pragma unroll
+    for (int i = 0; i < DK * DV / 8 / THREADS; ++i) {
+        const int e = i * THREADS + tid, r = e / (DV / 8), c = e % (DV / 8);
+        cp_async(tile + (c >> 3) * (DK * 128) + chunk_at(r, c & 7), S + e * 8, 16);
+    }
+}
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ long long at(const qgru_seq_tensor &x, int b, int h) { return b * x.bs + h * x.hs; }
+
+// A thread's Cols neighbouring columns, from `c0` on, of a row of bf16.
+template <int Cols>
+__device__ __forceinline__ void store_row(bf16 *row, const float (&v)[Cols], int c0, int d, bool vec) {
+#pragma unroll
+    for (int i = 0; i < Cols; i += 8) {
+        if (vec) {
+            if (c0 + i < d) *reinterpret_cast<uint4 *>(row + c0 + i) = make_uint4(pack(v[i], v[i + 1]), pack(v[i + 2], v[i + 3]), pack(v[i + 4], v[i + 5]), pack(v[i + 6], v[i + 7]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c0 + i + j < d) row[c0 + i + j] = __float2bfloat16_rn(v[i + j]);
+        }
+    }
+}
+
+struct Shared {                 // behind the tiles
+    float2 G[C];                // running sums of the decays, base 2
+    float f[C];                 // factors of a token
+    double sums[4];
+    uint64_t bar[4];
+    uint32_t tmem;
+    int failed;
+};
+
+__device__ __forceinline__ double load_decay(const qgru_attention &a, int b, int h, int t0, int tokens, int tid) {
+    return tid < tokens ? decay_log2(a, at(a.decay, b, h) + (long long)(t0 + tid) * a.decay.ts) : 0.0;
+}
+// G of the chunk from the threads' decays (the first 128; two __syncthreads).
+__device__ __forceinline__ void sum_decays(Shared &s, double g, int tid) {
+    if (tid < C) g = running_sum<C>(g, s.sums, tid);
+    __syncthreads();
+    if (tid < C) {
+        for (int w = 0; w < tid >> 5; ++w) g += s.sums[w];
+        s.G[tid] = two_floats(g);
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ void begin(Shared &s, uint32_t columns, int tid) {
+    if (tid == 0) {
+        for (int i = 0; i < 4; ++i) tc::mbar_init(&s.bar[i], 1);
+        s.failed = 0;
+        tc::fence_barrier_init();
+    }
+    if (tid < 32) tc::tmem_alloc(&s.tmem, columns);
+    tc::tc_fence_before_sync();
+    __syncthreads();
+    tc::tc_fence_after_sync();
+}
+// Every warp's wait for products: false once one has run out (all warps of the CTA then leave at the next common point).
+__device__ __forceinline__ void await(Shared &s, int bar, uint32_t parity) {
+    if (!tc::mbar_wait(&s.bar[bar], parity, WAIT_BUDGET)) s.failed = 1;
+    tc::tc_fence_after_sync();
+}
+__device__ __forceinline__ void end(Shared &s, uint32_t columns, int *flag, int tid) {
+    tc::tc_fence_before_sync();
+    __syncthreads();
+    if (tid < 32) tc::tmem_dealloc(s.tmem, columns);
+    if (tid == 0 && s.failed) *flag = 1;
+}
+__device__ __forceinline__ unsigned char *tiles_of(unsigned char *raw) {
+    return reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+}
+
+// ------------------------------------------------------------------------------------- state pass
+struct Pass {
+    qgru_seq_tensor k, v;
+    int k_share;
+    const float *first;
+    float *last;
+    bf16 *states;                  // before each chunk in the pass's order, [chunks][B H][DK][DV]
+    bool own_sums;                 // instead: each segment's sum, from zero
+    float *seg_state, *seg_log;
+    int segments, per, chunks;
+    int *flag;
+};
+template <int DK, int DV>
+constexpr int STATES_TILES = DK / 64 * PANEL + 2 * (DV / 64) * PANEL + 3 * (DK / 64) * PANEL;
+
+// grid (B H, segments).  S' = 2^G_C S + (w k)^T v: lane i of tensor memory is row i of the state, whose fp32 sums stay in
+// registers, half a row a thread.  While the products of a chunk run, the next one's tokens arrive and the state before this one
+// leaves.  With DK = 64 lanes 64 .. 127 repeat the first 64 (M is 128) and are not read.
+template <int DK, int DV, bool Reverse, bool Vec>
+__global__ void __launch_bounds__(THREADS) k_states_tc(const __grid_constant__ qgru_attention a, const __grid_constant__ Pass p) {
+    extern __shared__ unsigned char raw[];
+    unsigned char *tiles = tiles_of(raw);
+    Shared &s = *reinterpret_cast<Shared *>(tiles + STATES_TILES<DK, DV>);
+    constexpr int KT = DK / 64 * PANEL, VT = DV / 64 * PANEL, HALF = DV / 2;
+    const uint32_t k_raw = tc::smem_u32(tiles), v_raw = k_raw + KT, parts = v_raw + 2 * VT;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, bh = blockIdx.x, b = bh / a.H, h = bh % a.H, seg = blockIdx.y;
+    const int n = valid_tokens(a, b), row = (warp & 3) * 32 + lane, c0 = (warp >> 2) * HALF;
+    const bool mine = (warp & 3) * 32 < DK;
+    const long long kb = at(p.k, b, h / p.k_share), vb = at(p.v, b, h), dense = (long long)bh * a.Dk * a.Dv, dense_all = (long long)gridDim.x * a.Dk * a.Dv;
+    const bool own_sums = p.own_sums;
+    float S[HALF];
+    const float *first = own_sums ? nullptr : p.segments > 1 ? p.seg_state + seg * dense_all : p.first;
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) S[i] = first && row < a.Dk && c0 + i < a.Dv ? first[dense + (long long)row * a.Dv + c0 + i] : 0.f;
+    begin(s, DV == 64 ? 64 : 128, tid);
+    const uint32_t U = lane_base(s.tmem, warp) + c0;
+    // the chunks with tokens, in the pass's order
+    int c = seg * p.per;
+    const int c_end = min((seg + 1) * p.per, p.chunks), used = (n + C - 1) / C;
+    const auto chunk_of = [&](int i) { return Reverse ? p.chunks - 1 - i : i; };
+    const auto leave = [&](int chunk) {            // the state before the chunk
+        if (own_sums || !mine) return;
+        uint4 *to = reinterpret_cast<uint4 *>(p.states + ((long long)chunk * gridDim.x + bh) * (DK * DV) + row * DV + c0);
+#pragma unroll
+        for (int i = 0; i < HALF; i += 8) to[i / 8] = make_uint4(pack(S[i], S[i + 1]), pack(S[i + 2], S[i + 3]), pack(S[i + 4], S[i + 5]), pack(S[i + 6], S[i + 7]));
+    };
+    const auto fetch = [&](int i) {
+        const int t0 = chunk_of(i) * C, tokens = min(max(n - t0, 0), C);
+        load_rows<DK, Vec>(k_raw, p.k, kb, t0, tokens, a.Dk, tid);
+        load_rows<DV, Vec>(v_raw + (i & 1) * VT, p.v, vb, t0, tokens, a.Dv, tid);
+        cp_commit();
+    };
+    if (Reverse) {                                 // those behind the sequence: nothing reads the state there
+        c = max(c, p.chunks - used);
+    }
+    const int stop = Reverse ? c_end : min(c_end, used);
+    double all = 0.0, g = 0.0;
+    uint32_t phase = 0;
+    if (c < stop) {
+        fetch(c);
+        g = load_decay(a, b, h, chunk_of(c) * C, min(n - chunk_of(c) * C, C), tid);
+    }
+    for (; c < stop; ++c) {
+        const int chunk = chunk_of(c);
+        cp_wait<0>();
+        sum_decays(s, g, tid);
+        const float2 last = s.G[C - 1];
+        if (tid < C) s.f[tid] = Reverse ? a.scale * exp2_of(s.G[tid]) : exp2_diff(last, s.G[tid]);
+        __syncthreads();
+        // w k as the sum of three bf16 values; the parts lie as k does
+#pragma unroll 2
+        for (int i = 0; i < C * DK / 8 / THREADS; ++i) {
+            const int e = i * THREADS + tid, r = e / (DK / 8), ch = e % (DK / 8);
+            const uint32_t off = (ch >> 3) * PANEL + chunk_at(r, ch & 7);
+            const uint4 q = lds16(k_raw + off);
+            const uint32_t in[4] = {q.x, q.y, q.z, q.w};
+            const float w = s.f[r];
+            uint32_t o[3][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float x0 = low(in[j]) * w, x1 = high(in[j]) * w;
+#pragma unroll
+                for (int t = 0; t < 3; ++t) {
+                    o[t][j] = pack(x0, x1);
+                    x0 -= low(o[t][j]);
+                    x1 -= high(o[t][j]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 3; ++t) sts16(parts + t * KT + off, o[t][0], o[t][1], o[t][2], o[t][3]);
+        }
+        fence_async();
+        tc::tc_fence_before_sync();
+        __syncthreads();
+        if (tid == 0) {
+            tc::tc_fence_after_sync();
+            const Operand v{v_raw + (uint32_t)(c & 1) * VT, PANEL};
+            for (int t = 2; t >= 0; --t) {
+                const Operand k{parts + (uint32_t)t * KT, DK == 64 ? 0 : PANEL};
+                product<true, true, DV, C>(s.tmem, k, v, t != 2);
+            }
+            tc::mma_commit(&s.bar[0]);
+        }
+        if (c + 1 < stop) {
+            fetch(c + 1);
+            g = load_decay(a, b, h, chunk_of(c + 1) * C, min(n - chunk_of(c + 1) * C, C), tid);
+        }
+        leave(chunk);
+        const float whole = exp2_of(last);
+        all += (double)last.x + (double)last.y;
+        await(s, 0, phase);
+        phase ^= 1;
+        if (mine) {
+            float u[HALF];
+            tmem_load(U, u);
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) S[i] = fmaf(whole, S[i], u[i]);
+        }
+        tc::tc_fence_before_sync();
+        __syncthreads();
+        if (s.failed) break;
+    }
+    cp_wait<0>();
+    float *to = own_sums ? p.seg_state + seg * dense_all : p.last && seg == p.segments - 1 ? p.last : nullptr;
+    if (to) {
+#pragma unroll
+        for (int i = 0; i < HALF; ++i)
+            if (row < a.Dk && c0 + i < a.Dv) to[dense + (long long)row * a.Dv + c0 + i] = s.failed ? NAN : S[i];
+    }
+    if (own_sums && tid == 0) p.seg_log[seg * gridDim.x + bh] = (float)all;
+    end(s, DV == 64 ? 64 : 128, p.flag, tid);
+}
+
+// ------------------------------------------------------------------------------------- outputs
+template <int DK, int DV>
+constexpr int OUTPUTS_TILES = 2 * (DK / 64) * PANEL + DV / 64 * PANEL;
+
+// grid: chunks x B H, the heads of one chunk beside each other.  Two threads a token, each half of the pairs' weights and half of the
+// output's columns.  The state lies where k was once q k^T is there.
+template <int DK, int DV, bool Vec>
+__global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant__ qgru_attention a, const bf16 *states, int *flag) {
+    extern __shared__ unsigned char raw[];
+    unsigned char *tiles = tiles_of(raw);
+    Shared &s = *reinterpret_cast<Shared *>(tiles + OUTPUTS_TILES<DK, DV>);
+    constexpr int KT = DK / 64 * PANEL, HALF = DV / 2;
+    const uint32_t q_t = tc::smem_u32(tiles), k_t = q_t + KT, v_t = k_t + KT;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, heads = a.B * a.H, chunk = blockIdx.x / heads, bh = blockIdx.x % heads, b = bh / a.H, h = bh % a.H;
+    const int t0 = chunk * C, all = min(a.T - t0, C), tokens = min(max(valid_tokens(a, b) - t0, 0), C);
+    const int block = warp & 3, row = block * 32 + lane, half = warp >> 2, c0 = half * HALF;
+    bf16 *out = static_cast<bf16 *>(a.out.p) + at(a.out, b, h) + (long long)(t0 + row) * a.out.ts;
+    const bool vec_out = a.Dv % 8 == 0 && (a.out.ts | a.out.bs | a.out.hs) % 8 == 0 && reinterpret_cast<uintptr_t>(a.out.p) % 16 == 0;
+    float o[HALF];
+    if (tokens == 0) {
+#pragma unroll
+        for (int i = 0; i < HALF; ++i) o[i] = 0.f;
+        if (row < all) store_row(out, o, c0, a.Dv, vec_out);
+        return;
+    }
+    const int hk = h / (a.H / a.Hk);
+    const bool carried = chunk > 0 || a.state0;
+    const bf16 *S = states + ((long long)chunk * heads + bh) * (DK * DV);
+    load_rows<DK, Vec>(q_t, a.q, at(a.q, b, hk), t0, tokens, a.Dk, tid);
+    load_rows<DK, Vec>(k_t, a.k, at(a.k, b, hk), t0, tokens, a.Dk, tid);
+    cp_commit();
+    load_rows<DV, Vec>(v_t, a.v, at(a.v, b, h), t0, tokens, a.Dv, tid);
+    cp_commit();
+    const double g = load_decay(a, b, h, t0, tokens, tid);
+    begin(s, 256, tid);
+    const uint32_t base = lane_base(s.tmem, warp);
+    cp_wait<1>();
+    fence_async();
+    sum_decays(s, g, tid);
+    if (tid == 0) {
+        tc::tc_fence_after_sync();
+        product<false, false, C, DK>(s.tmem, Operand{q_t, PANEL}, Operand{k_t, PANEL}, false);
+        tc::mma_commit(&s.bar[0]);
+    }
+    // Blocks of 32 x 32 pairs.  Below the diagonal 2^(G_t - G_s) is a product of two factors, both at most 1: from s to the end of
+    // its block and from there to t.
+    if (tid < C) s.f[tid] = ex2_diff(s.G[tid | 31], s.G[tid]);
+    await(s, 0, 0);
+    __syncthreads();
+    if (carried) {
+        load_state<DK, DV>(k_t, S, tid);
+        cp_commit();
+    }
+    const float2 G = s.G[row];
+    uint32_t P[32];
+    {
+        float x[64];
+        tmem_load(base + half * 64, x);
+#pragma unroll
+        for (int jb = 0; jb < 2; ++jb) {
+            const int sb = half * 2 + jb;               // block of s
+            if (sb < block) {
+                const float r = a.scale * ex2_diff(G, s.G[sb * 32 + 31]);
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) P[jb * 16 + i / 2] = pack(x[jb * 32 + i] * (r * s.f[sb * 32 + i]), x[jb * 32 + i + 1] * (r * s.f[sb * 32 + i + 1]));
+            } else if (sb == block) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float w0 = a.scale * ex2_diff(G, s.G[sb * 32 + i]), w1 = a.scale * ex2_diff(G, s.G[sb * 32 + i + 1]);
+                    P[jb * 16 + i / 2] = pack(i <= lane ? x[jb * 32 + i] * w0 : 0.f, i + 1 <= lane ? x[jb * 32 + i + 1] * w1 : 0.f);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) P[jb * 16 + i] = 0u;
+            }
+        }
+    }
+    cp_wait<0>();
+    fence_async();
+    tc::tc_fence_before_sync();
+    __syncthreads();                                    // every sum of q k^T has been read, the state is there
+    if (carried && tid == 0) {
+        tc::tc_fence_after_sync();
+        product<false, true, DV, DK>(s.tmem + 128, Operand{q_t, PANEL}, Operand{k_t, DK * 128}, false);
+        tc::mma_commit(&s.bar[1]);
+    }
+    tc::tc_fence_after_sync();
+    tmem_store(base + half * 32, P);
+    tc::tmem_st_wait();
+    if (carried) {
+        await(s, 1, 0);
+        tmem_load(base + 128 + c0, o);
+        const float r = a.scale * ex2(G.x + G.y);
+#pragma unroll
+        for (int i = 0; i < HALF; ++i) o[i] *= r;
+    } else {
+#pragma unroll
+        for (int i = 0; i < HALF; ++i) o[i] = 0.f;
+    }
+    tc::tc_fence_before_sync();
+    __syncthreads();
+    if (tid == 0) {
+        tc::tc_fence_after_sync();
+        product_ts<true, DV, C>(s.tmem + 128, s.tmem, Operand{v_t, PANEL}, false);
+        tc::mma_commit(&s.bar[2]);
+    }
+    await(s, 2, 0);
+    float x[HALF];
+    tmem_load(base + 128 + c0, x);
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) odd |= !isfinite(x[i]);
+    if (odd && row < tokens) {
+        // A later token's infinity or NaN is none of an earlier one's business, and zero times it is NaN: the sums again, over the
+        // tokens up to this one.
+        const bf16 *q = static_cast<const bf16 *>(a.q.p) + at(a.q, b, hk) + (long long)(t0 + row) * a.q.ts;
+        const bf16 *k = static_cast<const bf16 *>(a.k.p) + at(a.k, b, hk) + (long long)t0 * a.k.ts;
+        const bf16 *v = static_cast<const bf16 *>(a.v.p) + at(a.v, b, h) + (long long)t0 * a.v.ts + c0;
+#pragma unroll
+        for (int i = 0; i < HALF; ++i) x[i] = 0.f;
+        for (int t = 0; t <= row; ++t) {
+            float w = 0.f;
+            for (int d = 0; d < a.Dk; ++d) w = fmaf(seq::to_f(q[d]), seq::to_f(k[t * a.k.ts + d]), w);
+            w *= a.scale * ex2_diff(G, s.G[t]);
+#pragma unroll
+            for (int i = 0; i < HALF; ++i)
+                if (c0 + i < a.Dv) x[i] = fmaf(w, seq::to_f(v[t * a.v.ts + i]), x[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) o[i] = row < tokens ? (s.failed ? NAN : o[i] + x[i]) : 0.f;
+    if (row < all) store_row(out, o, c0, a.Dv, vec_out);
+    end(s, 256, flag, tid);
+}
+
+// ------------------------------------------------------------------------------------- gradients
+struct Gradients {
+    const bf16 *states, *dstates;
+    float *dq_heads, *dk_heads;          // [T][B][H][Dk] where heads share q and k, else null
+    int *flag;
+};
+template <int DK, int DV>
+constexpr int GRADIENTS_TILES = 2 * (DK / 64) * PANEL + 2 * (DV / 64) * PANEL + 2 * DK * DV * 2 + 2 * PANEL;
+
+// Sum over the lanes of a warp for each of 32 columns: lane i gets column i's.
+__device__ __forceinline__ float sum_columns(float (&m)[32], int lane) {
+#pragma unroll
+    for (int w = 16; w; w >>= 1) {
+        const bool up = lane & w;
+#pragma unroll
+        for (int i = 0; i < w; ++i) {
+            const float give = up ? m[i] : m[i + w], keep = up ? m[i + w] : m[i];
+            m[i] = keep + __shfl_xor_sync(0xffffffffu, give, w);
+        }
+    }
+    return m[0];
+}
+// sum of a row's Cols values, from column c0 on, times those of a tile
+template <int Cols>
+__device__ __forceinline__ float dot_row(uint32_t tile, int row, int c0, const float (&v)[Cols]) {
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < Cols; i += 8) {
+        const int c = (c0 + i) / 8;
+        const uint4 u = lds16(tile + (c >> 3) * PANEL + chunk_at(row, c & 7));
+        const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x = fmaf(v[i + 2 * j], low(in[j]), x);
+            x = fmaf(v[i + 2 * j + 1], high(in[j]), x);
+        }
+    }
+    return x;
+}
+// The sums of a row times a factor, back into tensor memory for the products that add to them; their product with the tile's row.
+template <int Cols>
+__device__ __forceinline__ float scale_sums(uint32_t taddr, float w, uint32_t tile, int row, int c0, bool dot) {
+    float v[Cols];
+    tmem_load(taddr, v);
+    uint32_t r[Cols];
+#pragma unroll
+    for (int i = 0; i < Cols; ++i) {
+        v[i] *= w;
+        r[i] = __float_as_uint(v[i]);
+    }
+    tmem_store(taddr, r);
+    return dot ? dot_row(tile, row, c0, v) : 0.f;
+}
+
+// grid: chunks x B H.  Pairs lie as [s][t] here, lane s of tensor memory.  Four blocks of 128 columns of it:
+//   0  (k q^T), then P^T in bf16     1  (v dout^T), then dv     2  dk     3  dq
+// P^T is the operand of dv from tensor memory, E^T that of dk (K in its columns) and of dq (K in its rows) from shared memory.
+template <int DK, int DV, bool Vec>
+__global__ void __launch_bounds__(THREADS) k_gradients_tc(const __grid_constant__ qgru_attention a, const __grid_constant__ Gradients p) {
+    extern __shared__ unsigned char raw[];
+    unsigned char *tiles = tiles_of(raw);
+    Shared &s = *reinterpret_cast<Shared *>(tiles + GRADIENTS_TILES<DK, DV>);
+    constexpr int KT = DK / 64 * PANEL, VT = DV / 64 * PANEL, ST = DK * DV * 2, KHALF = DK / 2, VHALF = DV / 2;
+    const uint32_t q_t = tc::smem_u32(tiles), k_t = q_t + KT, v_t = k_t + KT, o_t = v_t + VT, S_t = o_t + VT, dS_t = S_t + ST, E_t = dS_t + ST;
+    // once v has been used, its tile holds sums by token
+    float *t_sums = reinterpret_cast<float *>(tiles + 2 * KT);          // [4][128] over s of a block's lanes, for each t
+    float *s_sums = t_sums + 4 * C, *q_dots = s_sums + 2 * C, *k_dots = q_dots + 2 * C;     // [2][128] each
+    double *warp_part = reinterpret_cast<double *>(k_dots + 2 * C);     // [8]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, heads = a.B * a.H, chunk = blockIdx.x / heads, bh = blockIdx.x % heads, b = bh / a.H, h = bh % a.H;
+    const int t0 = chunk * C, all = min(a.T - t0, C), tokens = min(max(valid_tokens(a, b) - t0, 0), C);
+    const int block = warp & 3, row = block * 32 + lane, half = warp >> 2;
+    const auto put_qk = [&](const qgru_seq_tensor &x, float *heads_sums, const float (&v)[KHALF]) {
+        if (row >= all) return;
+        const int c0 = half * KHALF;
+        if (heads_sums) {
+            float *to = heads_sums + (((long long)(t0 + row) * a.B + b) * a.H + h) * a.Dk + c0;
+#pragma unroll
+            for (int i = 0; i < KHALF; ++i)
+                if (c0 + i < a.Dk) to[i] = v[i];
+        } else {
+            store_row(static_cast<bf16 *>(x.p) + at(x, b, h) + (long long)(t0 + row) * x.ts, v, c0, a.Dk,
+                      a.Dk % 8 == 0 && (x.ts | x.bs | x.hs) % 8 == 0 && reinterpret_cast<uintptr_t>(x.p) % 16 == 0);
+        }
+    };
+    const auto put_v = [&](const float (&v)[VHALF]) {
+        if (row < all)
+            store_row(static_cast<bf16 *>(a.dv.p) + at(a.dv, b, h) + (long long)(t0 + row) * a.dv.ts, v, half * VHALF, a.Dv,
+                      a.Dv % 8 == 0 && (a.dv.ts | a.dv.bs | a.dv.hs) % 8 == 0 && reinterpret_cast<uintptr_t>(a.dv.p) % 16 == 0);
+    };
+    const long long gb = at(a.ddecay, b, h) + (long long)t0 * a.ddecay.ts;
+    if (tokens == 0) {
+        float z[KHALF], y[VHALF];
+#pragma unroll
+        for (int i = 0; i < KHALF; ++i) z[i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < VHALF; ++i) y[i] = 0.f;
+        put_qk(a.dq, p.dq_heads, z);
+        put_qk(a.dk, p.dk_heads, z);
+        put_v(y);
+        if (tid < all) seq::store_f(a.ddecay.p, gb + tid * a.ddecay.ts, a.decay_bf16, 0.f);
+        return;
+    }
+    const int hk = h / (a.H / a.Hk);
+    const long long state = ((long long)chunk * heads + bh) * (DK * DV);
+    load_rows<DK, Vec>(q_t, a.q, at(a.q, b, hk), t0, tokens, a.Dk, tid);
+    load_rows<DK, Vec>(k_t, a.k, at(a.k, b, hk), t0, tokens, a.Dk, tid);
+    cp_commit();
+    load_rows<DV, Vec>(v_t, a.v, at(a.v, b, h), t0, tokens, a.Dv, tid);
+    load_rows<DV, Vec>(o_t, a.dout, at(a.dout, b, h), t0, tokens, a.Dv, tid);
+    cp_commit();
+    load_state<DK, DV>(S_t, p.states + state, tid);
+    load_state<DK, DV>(dS_t, p.dstates + state, tid);
+    cp_commit();
+    const double g = load_decay(a, b, h, t0, tokens, tid);
+    begin(s, 512, tid);
+    const uint32_t tm = s.tmem, base = lane_base(tm, warp);
+    const Operand q{q_t, PANEL}, k{k_t, PANEL}, v{v_t, PANEL}, o{o_t, PANEL}, S{S_t, DK * 128}, dS{dS_t, DK * 128}, E{E_t, PANEL};
+    cp_wait<1>();
+    fence_async();
+    sum_decays(s, g, tid);
+    if (tid == 0) {
+        tc::tc_fence_after_sync();
+        product<false, false, C, DK>(tm, k, q, false);
+        product<false, false, C, DV>(tm + 128, v, o, false);
+        tc::mma_commit(&s.bar[0]);
+    }
+    // from the start of t's block of 32 to t
+    if (tid < C) s.f[tid] = tid < 32 ? ex2(s.G[tid].x + s.G[tid].y) : ex2_diff(s.G[tid], s.G[(tid & ~31) - 1]);
+    cp_wait<0>();
+    fence_async();
+    __syncthreads();
+    if (tid == 0) {
+        tc::tc_fence_after_sync();
+        product<false, false, DK, DV>(tm + 256, v, dS, false);
+        product<false, false, DK, DV>(tm + 384, o, S, false);
+        tc::mma_commit(&s.bar[1]);
+    }
+    await(s, 0, 0);
+    await(s, 1, 0);
+    const float2 G = s.G[row], last = s.G[C - 1];
+    // the pairs: blocks of 32 x 32, t from s on
+    uint32_t P[32];
+    float s_sum = 0.f;
+#pragma unroll
+    for (int jb = 0; jb < 2; ++jb) {
+        const int tb = half * 2 + jb;
+        float m[32];
+        if (tb < block) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) P[jb * 16 + i] = 0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sts16(E_t + half * PANEL + chunk_at(row, jb * 4 + i), 0u, 0u, 0u, 0u);
+            continue;
+        }
+        const float r = a.scale * (tb > block ? ex2_diff(s.G[tb * 32 - 1], G) : 1.f);
+#pragma unroll
+        for (int i8 = 0; i8 < 32; i8 += 16) {
+            float x[16], y[16];
+            tmem_load(base + half * 64 + jb * 32 + i8, x);
+            tmem_load(base + 128 + half * 64 + jb * 32 + i8, y);
+            uint32_t e[8];
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                float pv[2], ev[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int t = i8 + i + j;
+                    const float w = tb > block ? r * s.f[tb * 32 + t] : t >= lane ? a.scale * ex2_diff(s.G[tb * 32 + t], G) : 0.f;
+                    const bool on = tb > block || t >= lane;
+                    pv[j] = on ? w * x[i + j] : 0.f;
+                    ev[j] = on ? w * y[i + j] : 0.f;
+                    m[t] = tb > block || t > lane ? pv[j] * y[i + j] : 0.f;
+                    s_sum += m[t];
+                }
+                P[jb * 16 + (i8 + i) / 2] = pack(pv[0], pv[1]);
+                e[i / 2] = pack(ev[0], ev[1]);
+            }
+            sts16(E_t + half * PANEL + chunk_at(row, jb * 4 + i8 / 8), e[0], e[1], e[2], e[3]);
+            sts16(E_t + half * PANEL + chunk_at(row, jb * 4 + i8 / 8 + 1), e[4], e[5], e[6], e[7]);
+        }
+        t_sums[block * C + tb * 32 + lane] = sum_columns(m, lane);
+    }
+    s_sums[half * C + row] = s_sum;
+    const float to_end = ex2_diff(last, G), from_start = a.scale * ex2(G.x + G.y);
+    k_dots[half * C + row] = scale_sums<KHALF>(base + 256 + half * KHALF, to_end, k_t, row, half * KHALF, true);
+    q_dots[half * C + row] = scale_sums<KHALF>(base + 384 + half * KHALF, from_start, q_t, row, half * KHALF, true);
+    {
+        double x = 0.0;
+        for (int e = tid; e < DK * DV / 8; e += THREADS) {
+            const uint4 u = lds16(S_t + e * 16), w = lds16(dS_t + e * 16);      // (the same order in both)
+            float f = low(u.x) * low(w.x);
+            f = fmaf(high(u.x), high(w.x), f);
+            f = fmaf(low(u.y), low(w.y), f);
+            f = fmaf(high(u.y), high(w.y), f);
+            f = fmaf(low(u.z), low(w.z), f);
+            f = fmaf(high(u.z), high(w.z), f);
+            f = fmaf(low(u.w), low(w.w), f);
+            f = fmaf(high(u.w), high(w.w), f);
+            x += (double)f;
+        }
+        for (int i = 16; i; i >>= 1) x += __shfl_xor_sync(0xffffffffu, x, i);
+        if (lane == 0) warp_part[warp] = x;
+    }
+    fence_async();
+    tc::tmem_st_wait();
+    tc::tc_fence_before_sync();
+    __syncthreads();                                  // the pairs' sums have been read, E^T and the scaled sums are there
+    if (tid == 0) {
+        tc::tc_fence_after_sync();
+        product<false, true, DV, DK>(tm + 128, k, dS, false);
+        tc::mma_commit(&s.bar[2]);
+        product<false, true, DK, C>(tm + 256, E, q, true);
+        product<true, true, DK, C>(tm + 384, E, k, true);
+        tc::mma_commit(&s.bar[3]);
+    }
+    tc::tc_fence_after_sync();
+    tmem_store(base + half * 32, P);
+    // the decays' gradient: from each token on, every pair across it, and what passes from the state before the chunk to that behind it
+    double d = 0.0, own = 0.0;
+    if (tid < C) {
+        float t_sum = 0.f;
+        for (int w = 0; w <= tid >> 5; ++w) t_sum += t_sums[w * C + tid];
+        own = (double)t_sum - (double)s_sums[tid] - (double)s_sums[C + tid] + (double)q_dots[tid] + (double)q_dots[C + tid];
+        const double kd = (double)k_dots[tid] + (double)k_dots[C + tid];
+        d = running_sum<C>(kd - own, s.sums, tid) - (kd - own);
+    }
+    double total = own;
+    for (int i = 16; i; i >>= 1) total += __shfl_xor_sync(0xffffffffu, total, i);
+    double *totals = warp_part + 8;
+    if (lane == 0 && tid < C) totals[warp] = total;
+    tc::tmem_st_wait();
+    await(s, 2, 0);
+    scale_sums<VHALF>(base + 128 + half * VHALF, to_end, 0, 0, 0, false);
+    tc::tmem_st_wait();
+    tc::tc_fence_before_sync();
+    __syncthreads();
+    if (tid == 0) {
+        tc::tc_fence_after_sync();
+        product_ts<true, DV, C>(tm + 128, tm, o, true);
+        tc::mma_commit(&s.bar[2]);
+    }
+    if (tid < all) {
+        double x = d;
+        for (int w = 0; w < tid >> 5; ++w) x += s.sums[w];
+        double through = 0.0;
+        for (int w = 0; w < 8; ++w) through += warp_part[w];
+        x += totals[0] + totals[1] + totals[2] + totals[3] + through * (double)exp2_of(last);
+        seq::store_f(a.ddecay.p, gb + tid * a.ddecay.ts, a.decay_bf16, tid < tokens ? (s.failed ? NAN : (float)x) : 0.f);
+    }
+    await(s, 3, 0);
+    const bool live = row < tokens, bad = s.failed;
+    {
+        float x[KHALF];
+        tmem_load(base + 384 + half * KHALF, x);
+#pragma unroll
+        for (int i = 0; i < KHALF; ++i) x[i] = live ? (bad ? NAN : x[i]) : 0.f;
+        put_qk(a.dq, p.dq_heads, x);
+        tmem_load(base + 256 + half * KHALF, x);
+#pragma unroll
+        for (int i = 0; i < KHALF; ++i) x[i] = live ? (bad ? NAN : x[i]) : 0.f;
+        put_qk(a.dk, p.dk_heads, x);
+    }
+    await(s, 2, 1);
+    {
+        float x[VHALF];
+        tmem_load(base + 128 + half * VHALF, x);
+#pragma unroll
+        for (int i = 0; i < VHALF; ++i) x[i] = live ? (s.failed ? NAN : x[i]) : 0.f;
+        put_v(x);
+    }
+    end(s, 512, p.flag, tid);
+}
+
+// ------------------------------------------------------------------------------------- launches
+bool vec_ok(const qgru_seq_tensor &x, int d) { return d % 8 == 0 && (x.ts | x.bs | x.hs) % 8 == 0 && reinterpret_cast<uintptr_t>(x.p) % 16 == 0; }
+
+template <class F>
+int with_smem(F *kernel, int tiles, int *bytes) {
+    *bytes = tiles + 1024 + (int)sizeof(Shared);
+    SEQ_CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, *bytes));
+    return QGRU_OK;
+}
+
+template <int DK, int DV, bool Reverse, bool Vec>
+int run_states(const qgru_attention &a, const Cut &c, bf16 *states, char *seg, int *flag, cudaStream_t st) {
+    Pass p{};
+    p.k = Reverse ? a.q : a.k;
+    p.v = Reverse ? a.dout : a.v;
+    p.k_share = a.H / a.Hk;
+    p.first = Reverse ? a.dstate : a.state0;
+    p.last = Reverse ? a.dstate0 : a.state;
+    p.segments = c.segments;
+    p.per = c.per;
+    p.chunks = c.chunks;
+    p.flag = flag;
+    p.states = states;
+    const auto kernel = k_states_tc<DK, DV, Reverse, Vec>;
+    int bytes = 0;
+    if (const int rc = with_smem(kernel, STATES_TILES<DK, DV>, &bytes)) return rc;
+    const dim3 grid(a.B * a.H, c.segments);
+    if (c.segments > 1) {
+        p.seg_state = reinterpret_cast<float *>(seg);
+        p.seg_log = p.seg_state + c.segments * state_elems(a);
+        p.own_sums = true;
+        kernel<<<grid, THREADS, bytes, st>>>(a, p);
+        SEQ_CK(cudaGetLastError());
+        if (const int rc = scan_segments(a, c, Reverse, seg, st)) return rc;
+        p.own_sums = false;
+    }
+    kernel<<<grid, THREADS, bytes, st>>>(a, p);
+    SEQ_CK(cudaGetLastError());
+    return QGRU_OK;
+}
+
+template <int DK, int DV, bool Vec>
+int forward(const qgru_attention &a, const Cut &c, int *flag, cudaStream_t st) {
+    bf16 *states = static_cast<bf16 *>(a.states);
+    if (const int rc = run_states<DK, DV, false, Vec>(a, c, states, static_cast<char *>(a.workspace), flag, st)) return rc;
+    if (c.chunks == 0) return QGRU_OK;
+    int bytes = 0;
+    if (const int rc = with_smem(k_outputs_tc<DK, DV, Vec>, OUTPUTS_TILES<DK, DV>, &bytes)) return rc;
+    k_outputs_tc<DK, DV, Vec><<<c.chunks * a.B * a.H, THREADS, bytes, st>>>(a, states, flag);
+    SEQ_CK(cudaGetLastError());
+    return QGRU_OK;
+}
+template <int DK, int DV, bool Vec>
+int backward(const qgru_attention &a, const Cut &c, int *flag, cudaStream_t st) {
+    char *ws = static_cast<char *>(a.workspace);
+    bf16 *dstates = reinterpret_cast<bf16 *>(ws);
+    ws += a256(c.states);
+    char *seg = ws;
+    ws += a256(c.seg);
+    if (const int rc = run_states<DK, DV, true, Vec>(a, c, dstates, seg, flag, st)) return rc;
+    if (c.chunks == 0) return QGRU_OK;
+    Gradients g{static_cast<const bf16 *>(a.states), dstates, nullptr, nullptr, flag};
+    if (a.H != a.Hk) {
+        g.dq_heads = reinterpret_cast<float *>(ws);
+        g.dk_heads = g.dq_heads + group_bytes(a) / 8;
+    }
+    int bytes = 0;
+    if (const int rc = with_smem(k_gradients_tc<DK, DV, Vec>, GRADIENTS_TILES<DK, DV>, &bytes)) return rc;
+    k_gradients_tc<DK, DV, Vec><<<c.chunks * a.B * a.H, THREADS, bytes, st>>>(a, g);
+    SEQ_CK(cudaGetLastError());
+    return g.dq_heads ? sum_groups(a, g.dq_heads, g.dk_heads, st) : QGRU_OK;
+}
+
+template <class F>
+int by_size(const qgru_attention &a, bool vec, F f) {
+    using std::integral_constant;
+    const auto with = [&](auto dk, auto dv) -> int {
+        return vec ? f(dk, dv, integral_constant<bool, true>()) : f(dk, dv, integral_constant<bool, false>());
+    };
+    const integral_constant<int, 64> small;
+    const integral_constant<int, 128> large;
+    return a.Dk <= 64 ? (a.Dv <= 64 ? with(small, small) : with(small, large)) : (a.Dv <= 64 ? with(large, small) : with(large, large));
+}
+
+}  // namespace
+
+bool tc_takes(const qgru_attention &a) { return a.bf16 && a.Dk <= 128 && a.Dv <= 128; }
+
+// Segments: one CTA of the state pass per SM (or two, with the smaller tiles) where the heads alone do not give that many; of two
+// chunks at the least.
+Cut tc_cut(const qgru_attention &a, int sms) {
+    Cut c;
+    c.chunk = C;
+    c.chunks = (a.T + C - 1) / C;
+    const long long units = std::max<long long>((long long)a.B * a.H, 1);
+    c.segments = (int)std::max<long long>(1, std::min<long long>(c.chunks / 2, sms / units));
+    c.per = std::max(1, (c.chunks + c.segments - 1) / c.segments);
+    c.segments = std::max(1, (c.chunks + c.per - 1) / c.per);
+    c.states = sizeof(bf16) * (size_t)c.chunks * a.B * a.H * (a.Dk <= 64 ? 64 : 128) * (a.Dv <= 64 ? 64 : 128);
+    c.seg = c.segments > 1 ? sizeof(float) * c.segments * (state_elems(a) + (size_t)a.B * a.H) : 0;
+    return c;
+}
+int tc_forward(const qgru_attention &a, const Cut &c, int *flag, cudaStream_t st) {
+    const bool vec = vec_ok(a.q, a.Dk) && vec_ok(a.k, a.Dk) && vec_ok(a.v, a.Dv);
+    return by_size(a, vec, [&](auto dk, auto dv, auto v) -> int { return forward<dk.value, dv.value, v.value>(a, c, flag, st); });
+}
+int tc_backward(const qgru_attention &a, const Cut &c, int *flag, cudaStream_t st) {
+    const bool vec = vec_ok(a.q, a.Dk) && vec_ok(a.k, a.Dk) && vec_ok(a.v, a.Dv) && vec_ok(a.dout, a.Dv);
+    return by_size(a, vec, [&](auto dk, auto dv, auto v) -> int { return backward<dk.value, dv.value, v.value>(a, c, flag, st); });
+}
+
+}  // namespace attn
+}  // namespace qgru
