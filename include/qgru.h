@@ -589,8 +589,8 @@ QGRU_API int qgru_calibrate_from_histogram(const float *counts, int num_bins, fl
  * linear in its state, and the root-mean-square norm with the residual's addition that such layers stand
  * between.  These calls have no handle: they keep nothing, allocate nothing and wait for nothing; workspaces are the
  * caller's, and calls that do not share one may run at the same time.  They run on `device`, whatever the thread's current
- * device is.  A wait inside a kernel that runs out (each is bounded) leaves NaN in its results and is told once, by the next of
- * these calls that begins after the GPU got there (QGRU_ERR_TIMEOUT).
+ * device is.  A wait inside a kernel that runs out (each is bounded) leaves its results unfinished and is told once, by the next
+ * of these calls that begins after the GPU got there (QGRU_ERR_TIMEOUT).
  * qgru_seq_last_error: why the calling thread's last of these calls failed. */
 QGRU_API const char *qgru_seq_last_error(void);
 
@@ -606,11 +606,13 @@ typedef struct qgru_seq_tensor {
  * read; their outputs and gradients are written as zeros.  lengths (device) may be NULL (all T) and is clamped to 0 .. T.
  * state0 [B][H][Dk][Dv] (NULL: zeros) and state, the last one, are dense.
  * Backward: dout, dstate (NULL: zeros) -> dq, dk, dv (elements of the type of q), ddecay (of the type of decay), dstate0 (may
- * be NULL).  `states`: qgru_attention_sizes bytes, written by the forward and read by the backward of the same arguments; 256-byte
- * aligned, as `workspace`, which holds nothing between calls. */
+ * be NULL).  `states` (with `keep`): written by the forward and read by the backward of the same arguments; 256-byte aligned, as
+ * `workspace`, which holds nothing between calls.  qgru_attention_sizes takes the arguments as the calls do, with the forward's tensors
+ * set but neither of the two. */
 typedef struct qgru_attention {
     int device, T, B, H, Hk, Dk, Dv;
     int bf16, decay_bf16;               /* else fp32 */
+    int keep;                           /* the forward leaves `states` for the backward */
     float scale;
     const int32_t *lengths;
     const float *state0, *dstate;

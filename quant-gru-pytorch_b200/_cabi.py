@@ -73,7 +73,7 @@ class SeqTensor(C.Structure):
 
 class Attention(C.Structure):
     """qgru_attention: sizes, states, workspaces and tensors of a linear attention call."""
-    _fields_ = ([(n, C.c_int) for n in ("device", "T", "B", "H", "Hk", "Dk", "Dv", "bf16", "decay_bf16")] + [("scale", C.c_float)] +
+    _fields_ = ([(n, C.c_int) for n in ("device", "T", "B", "H", "Hk", "Dk", "Dv", "bf16", "decay_bf16", "keep")] + [("scale", C.c_float)] +
                 [(n, C.c_void_p) for n in ("lengths", "state0", "dstate", "state", "dstate0", "states", "workspace")] +
                 [("states_bytes", C.c_size_t), ("workspace_bytes", C.c_size_t)] +
                 [(n, SeqTensor) for n in ("q", "k", "v", "decay", "out", "dout", "dq", "dk", "dv", "ddecay")])

@@ -12,7 +12,7 @@ _CSRC = os.path.join(_HERE, "csrc")
 _OBJ = os.path.join(_HERE, "build")
 SOURCES = ["qgru_api.cu", "qgru_gemm_tc.cu", "qgru_rec_mma.cu", "qgru_rec_cluster.cu", "qgru_rec_c64.cu", "qgru_rec_reg.cu",
            "qgru_rec_reg_float.cu", "qgru_float.cu", "qgru_gemm_f32.cu", "qgru_gemm_f32_tc.cu", "qgru_rec_f32.cu", "qgru_hist.cu", "qgru_backward.cu", "qgru_bwd_tc.cu", "qgru_probe.cu", "qgru_host.cc",
-           "qgru_seq.cu", "qgru_attn.cu", "qgru_attn_tc.cu", "qgru_norm.cu"]
+           "qgru_seq.cu", "qgru_attn.cu", "qgru_attn_fwd.cu", "qgru_attn_tc.cu", "qgru_norm.cu"]
 OUT = os.path.join(_HERE, "libqgru_b200.so")
 
 

@@ -428,8 +428,9 @@ int run_states(const qgru_attention &a, const Cut &c, float *states, char *seg, 
 
 template <class T>
 int forward(const qgru_attention &a, const Cut &c, cudaStream_t st) {
-    float *states = static_cast<float *>(a.states);
-    if (const int rc = run_states<T, false>(a, c, states, static_cast<char *>(a.workspace), st)) return rc;
+    float *states = static_cast<float *>(a.keep ? a.states : a.workspace);
+    char *seg = static_cast<char *>(a.workspace) + (a.keep ? 0 : a256(c.states));
+    if (const int rc = run_states<T, false>(a, c, states, seg, st)) return rc;
     if (c.chunks == 0) return QGRU_OK;
     constexpr size_t bytes = 3 * C * LD * sizeof(float);
     if (const int rc = with_smem(k_outputs<T>, bytes)) return rc;
@@ -592,10 +593,9 @@ int check(const qgru_attention *a) {
     return QGRU_OK;
 }
 
-int cut(const qgru_attention &a, Cut *c) {
-    int sms = 0;
-    SEQ_CK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, a.device));
-    *c = tc_takes(a) ? tc_cut(a, sms) : generic_cut(a, sms);
+int cut(const qgru_attention &a, Cut *c, int *sms) {
+    SEQ_CK(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, a.device));
+    *c = tc_takes(a) ? tc_cut(a, *sms) : generic_cut(a, *sms);
     return QGRU_OK;
 }
 
@@ -610,9 +610,11 @@ extern "C" {
 int qgru_attention_sizes(const qgru_attention *a, size_t *states_bytes, size_t *forward_workspace, size_t *backward_workspace) {
     if (const int rc = attn::check(a)) return rc;
     attn::Cut c;
-    if (const int rc = attn::cut(*a, &c)) return rc;
-    if (states_bytes) *states_bytes = attn::a256(c.states);
-    if (forward_workspace) *forward_workspace = attn::a256(c.seg);
+    int sms = 0;
+    if (const int rc = attn::cut(*a, &c, &sms)) return rc;
+    const bool walks = attn::tc_takes(*a) && attn::walk_takes(*a, false);
+    if (states_bytes) *states_bytes = a->keep ? attn::a256(c.states) : 0;
+    if (forward_workspace) *forward_workspace = attn::a256(c.seg) + (a->keep || walks ? 0 : attn::a256(c.states));
     if (backward_workspace) *backward_workspace = attn::a256(c.states) + attn::a256(c.seg) + attn::group_bytes(*a);
     return QGRU_OK;
 }
@@ -620,6 +622,7 @@ int qgru_attention_sizes(const qgru_attention *a, size_t *states_bytes, size_t *
 static int attention_run(const qgru_attention *a, bool backward, void *stream) {
     if (const int rc = attn::check(a)) return rc;
     if (a->B == 0) return QGRU_OK;
+    if (backward && !a->keep) return seq::fail(QGRU_ERR_BAD_ARG, "the forward has not kept its states");
     size_t states = 0, fwd = 0, bwd = 0;
     if (const int rc = qgru_attention_sizes(a, &states, &fwd, &bwd)) return rc;
     const size_t ws = backward ? bwd : fwd;
@@ -631,12 +634,13 @@ static int attention_run(const qgru_attention *a, bool backward, void *stream) {
     const seq::OnDevice on(a->device);
     SEQ_CK(on.error());
     attn::Cut c;
-    if (const int rc = attn::cut(*a, &c)) return rc;
+    int sms = 0;
+    if (const int rc = attn::cut(*a, &c, &sms)) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (attn::tc_takes(*a)) {
         int *flag = nullptr;
         if (const int rc = seq::expiry_flag(a->device, &flag)) return rc;
-        return backward ? attn::tc_backward(*a, c, flag, st) : attn::tc_forward(*a, c, flag, st);
+        return backward ? attn::tc_backward(*a, c, flag, sms, st) : attn::tc_forward(*a, c, flag, sms, st);
     }
     return backward ? attn::generic_backward(*a, c, st) : attn::generic_forward(*a, c, st);
 }

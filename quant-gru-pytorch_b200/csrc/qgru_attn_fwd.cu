@@ -1,0 +1,652 @@
+// qgru_attn_fwd.cu - linear attention over the chunks of a sequence in turn, on the tensor cores, every token read once: the outputs and
+// the state, or the states alone (also from the end, for the gradient of the states).
+//
+// A CTA per SM walks through (sequence and head, segment) after another, chunk by chunk of 128 tokens.  Five warpgroups work on
+// different chunks at the same time and hand them on through barriers in shared memory:
+//   K  takes k times the decays to the chunk's end apart into three bf16 parts (24 bits), 64 tokens at a time
+//   S  keeps the state in fp32 registers: S' = 2^G_C S + (w k)^T v, and puts it, as two bf16 parts (16 bits), beside q
+//   P  weighs the pairs of tokens: q k^T out of tensor memory, times 2^(G_t - G_s), into it again as bf16, the operand of P v
+//   O  out = 2^G_t q S + P v: out of tensor memory, into the output
+//   X  one warp each: issues the products, fetches tiles by TMA, sums the decays up
+// In the order of the products the chunk's part of the state comes first, since the next chunk's outputs wait for it.
+//
+// What is rounded to bf16 on the way: P alone, once, as the output is in the end.
+#include <algorithm>
+#include <type_traits>
+
+#include "qgru_attn_tc.cuh"
+
+namespace qgru {
+namespace attn {
+namespace {
+
+using namespace tile;
+constexpr int WG = 128, THREADS = 5 * WG;
+// 640 threads start with 96 registers each; the warpgroups share the 480 of five threads by the columns of a state that a thread has.
+constexpr int REGS = 96;
+template <int N>
+struct Regs {
+    static constexpr int S = N == 128 ? 168 : N == 64 ? 128 : 104, P = 112, O = N == 128 ? 88 : N == 64 ? 96 : 104, K = N == 128 ? 72 : N == 64 ? 80 : 88, X = N == 128 ? 40 : N == 64 ? 64 : 72;
+    static_assert(S + P + O + K + X <= 5 * REGS, "the shares add up to what the block starts with");
+};
+template <int R>
+__device__ __forceinline__ void take_registers() {
+    if constexpr (R > REGS)
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
+    else
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
+}
+constexpr int SLOTS = 4;                    // chunks whose decays are known at once
+
+struct Slot {
+    float2 G[C];                            // running sums, base 2
+    float to_block[C];                      // 2^(G at the end of s's block of 32 - G_s)
+    float weight[C];                        // of k: 2^(G_C - G_s), or from the end scale 2^G_t
+    float from_start[C];                    // scale 2^G_t
+    float whole;
+    float pad[3];
+};
+
+template <int DK, int DV, bool Outputs>
+struct Plan {
+    static constexpr int KT = DK / 64 * PANEL, VT = DV / 64 * PANEL, STAGE = (Outputs ? 2 : 1) * KT + VT;
+    static constexpr int PART = DK / 64 * PANEL / 2, PARTS = 3 * PART;            // 64 tokens
+    static constexpr int STATE = DK * DV * 2, STATES = Outputs ? 2 * STATE : 0;
+    static constexpr int NB = DK == 128 && (DV == 128 || !Outputs) ? 1 : 2;       // buffers of parts
+    static constexpr int ROOM = 213000 - NB * PARTS - STATES;
+    static constexpr int NS = ROOM / STAGE >= 3 ? 3 : ROOM / STAGE >= 2 ? 2 : 1;  // stages of tiles
+    static constexpr int NQ = DV == 64 && NS > 1 ? 2 : 1;                         // buffers of q k^T
+    static constexpr int TILES = NS * STAGE + NB * PARTS + STATES;
+    // columns of tensor memory
+    static constexpr uint32_t INTER = NQ * 128, INTRA = INTER + DV, U = Outputs ? INTRA + DV : 0, COLUMNS = Outputs ? 512 : DV;
+    static_assert(!Outputs || U + DV <= 512, "tensor memory");
+    static_assert(NS >= 1 && TILES <= 213000, "shared memory");
+};
+
+struct Ctl {
+    uint64_t k_full[3], k_empty[3], q_full[3], q_empty[3], v_full[3], v_empty[3], parts_full[2], parts_empty[2], pairs_full[2], p_full[2], g_full[SLOTS], g_empty[SLOTS];
+    uint64_t u_full, u_empty, s_full, s_empty, o_full, o_empty;
+    uint32_t tmem;
+    volatile int failed;
+};
+
+struct Args {
+    CUtensorMap q, k, v;                    // [B][heads][T][D]
+    const float *first;                     // the state it starts from, or null
+    float *last;                            // where the last one goes, or null
+    bf16 *states;                           // before each chunk in the pass's order, [chunks][B H][DK][DV], or null
+    float *seg_state, *seg_log;
+    int own_sums;                           // states alone: each segment's sum, from zero, and nothing else
+    int segments, per, chunks, items, share;
+    int *flag;
+};
+
+// A (sequence, head, segment) and its chunks with tokens, in the pass's order.
+template <bool Reverse>
+struct Item {
+    int bh, b, h, seg, n, begin, stop, end;
+    __device__ __forceinline__ Item(const qgru_attention &a, const Args &p, int item) {
+        const int heads = a.B * a.H;
+        seg = item / heads;
+        bh = item % heads;
+        b = bh / a.H;
+        h = bh % a.H;
+        n = valid_tokens(a, b);
+        const int used = (n + C - 1) / C;
+        begin = seg * p.per;
+        end = min(begin + p.per, p.chunks);
+        if (Reverse) begin = min(max(begin, p.chunks - used), end);
+        stop = Reverse ? end : max(begin, min(end, used));
+    }
+    static __device__ __forceinline__ int chunk(const Args &p, int c) { return Reverse ? p.chunks - 1 - c : c; }
+    __device__ __forceinline__ int tokens(int chunk) const { return min(n - chunk * C, C); }
+};
+
+__device__ __forceinline__ bool wait(Ctl &s, uint64_t &bar, uint32_t parity) {
+    if (tc::mbar_try_wait(&bar, parity)) return true;
+    const long long t0 = clock64();
+    while (!tc::mbar_try_wait(&bar, parity)) {
+        if (s.failed) return false;
+        if (clock64() - t0 > WAIT_BUDGET) {
+            s.failed = 1;
+            return false;
+        }
+    }
+    return true;
+}
+// for a whole warp: all its lanes or none go on
+__device__ __forceinline__ bool wait_warp(Ctl &s, uint64_t &bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(s, bar, parity)); }
+// A ring of N: the buffer and the parity of step i; `free`: of the wait for it to be empty.
+template <int N>
+struct At {
+    int buf;
+    uint32_t full, free;
+    __device__ __forceinline__ explicit At(int i) : buf(i % N), full((uint32_t)(i / N) & 1u), free(full ^ 1u) {}
+};
+__device__ __forceinline__ void tma_load_4d(uint32_t to, const CUtensorMap *map, uint64_t *bar, int x, int t, int h, int b) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(to),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(tc::smem_u32(bar)), "r"(x), "r"(t), "r"(h), "r"(b)
+                 : "memory");
+}
+
+template <int DK, int DV, bool Outputs, bool Reverse>
+struct Roles {
+    using L = Plan<DK, DV, Outputs>;
+    const qgru_attention &a;
+    const Args &p;
+    Ctl &s;
+    Slot *slots;
+    uint32_t tiles;                         // stages, then the parts, then the state
+    int tid;                                // in the warpgroup
+
+    __device__ __forceinline__ uint32_t k_tile(int st) const { return tiles + st * L::STAGE; }
+    __device__ __forceinline__ uint32_t v_tile(int st) const { return tiles + st * L::STAGE + L::KT; }
+    __device__ __forceinline__ uint32_t q_tile(int st) const { return tiles + st * L::STAGE + L::KT + L::VT; }
+    __device__ __forceinline__ uint32_t parts(int b) const { return tiles + L::NS * L::STAGE + b * L::PARTS; }
+    __device__ __forceinline__ uint32_t state(int part) const { return tiles + L::NS * L::STAGE + L::NB * L::PARTS + part * L::STATE; }
+    // f(item, its chunk in the pass's order, running number of the chunk) until it says that a wait has run out
+    template <class F>
+    __device__ __forceinline__ bool each(F f) const {
+        int i = 0;
+        for (int it = blockIdx.x; it < p.items; it += gridDim.x) {
+            const Item<Reverse> w(a, p, it);
+            for (int c = w.begin; c < w.stop; ++c, ++i)
+                if (!f(w, Item<Reverse>::chunk(p, c), i)) return false;
+        }
+        return true;
+    }
+
+    // ---- X, warp 0: products
+    __device__ __forceinline__ bool pairs(int i) const {
+        const At<L::NS> st(i);
+        if (!wait(s, s.k_full[st.buf], st.full) || !wait(s, s.q_full[st.buf], st.full)) return false;
+        tc::tc_fence_after_sync();
+        product<false, false, C, DK>(s.tmem + (i % L::NQ) * 128, Operand{q_tile(st.buf), PANEL}, Operand{k_tile(st.buf), PANEL}, false);
+        tc::mma_commit(&s.pairs_full[i % L::NQ]);
+        tc::mma_commit(&s.k_empty[st.buf]);
+        return true;
+    }
+    __device__ __forceinline__ void issue() const {
+        int steps = 0;
+        for (int it = blockIdx.x; it < p.items; it += gridDim.x) {
+            const Item<Reverse> w(a, p, it);
+            steps += w.stop - w.begin;
+        }
+        if (Outputs && L::NQ == 2 && steps && !pairs(0)) return;
+        for (int i = 0; i < steps; ++i) {
+            const At<L::NS> st(i);
+            const At<1> one(i);
+            if (Outputs && L::NQ == 1 && !pairs(i)) return;
+            for (int half = 0; half < 2; ++half) {
+                const At<L::NB> pb(2 * i + half);
+                if (!wait(s, s.parts_full[pb.buf], pb.full)) return;
+                if (half == 0 && (!wait(s, s.v_full[st.buf], st.full) || !wait(s, s.u_empty, one.free))) return;
+                tc::tc_fence_after_sync();
+                const Operand v{v_tile(st.buf) + half * (PANEL / 2), PANEL};
+                // the small parts first
+                for (int t = 2; t >= 0; --t) {
+                    const Operand k{parts(pb.buf) + t * L::PART, DK == 64 ? 0 : PANEL / 2};      // (64 lanes: the rest repeats them)
+                    product<true, true, DV, 64>(s.tmem + L::U, k, v, half || t != 2);
+                }
+                tc::mma_commit(&s.parts_empty[pb.buf]);
+            }
+            tc::mma_commit(&s.u_full);
+            if constexpr (Outputs) {
+                if (!wait(s, s.s_full, one.full) || !wait(s, s.o_empty, one.free)) return;
+                tc::tc_fence_after_sync();
+                const Operand q{q_tile(st.buf), PANEL};
+                product<false, true, DV, DK>(s.tmem + L::INTER, q, Operand{state(1), DK * 128}, false);
+                product<false, true, DV, DK>(s.tmem + L::INTER, q, Operand{state(0), DK * 128}, true);
+                tc::mma_commit(&s.q_empty[st.buf]);
+                tc::mma_commit(&s.s_empty);
+                if (L::NQ == 2 && i + 1 < steps && !pairs(i + 1)) return;
+                const At<L::NQ> qb(i);
+                if (!wait(s, s.p_full[qb.buf], qb.full)) return;
+                tc::tc_fence_after_sync();
+                product_ts<true, DV, C>(s.tmem + L::INTRA, s.tmem + qb.buf * 128, Operand{v_tile(st.buf), PANEL}, false);
+                tc::mma_commit(&s.o_full);
+            }
+            tc::mma_commit(&s.v_empty[st.buf]);
+        }
+    }
+    // ---- X, warp 1: tiles
+    __device__ __forceinline__ void fetch() const {
+        const auto load = [&](uint32_t to, const CUtensorMap *map, uint64_t *bar, int panels, int t, int h, int b) {
+            tc::mbar_expect_tx(bar, panels * PANEL);
+            for (int i = 0; i < panels; ++i) tma_load_4d(to + i * PANEL, map, bar, i * 64, t, h, b);
+        };
+        each([&](const Item<Reverse> &w, int chunk, int i) {
+            const At<L::NS> st(i);
+            if (!wait(s, s.k_empty[st.buf], st.free)) return false;
+            load(k_tile(st.buf), &p.k, &s.k_full[st.buf], DK / 64, chunk * C, w.h / p.share, w.b);
+            if constexpr (Outputs) {
+                if (!wait(s, s.q_empty[st.buf], st.free)) return false;
+                load(q_tile(st.buf), &p.q, &s.q_full[st.buf], DK / 64, chunk * C, w.h / p.share, w.b);
+            }
+            if (!wait(s, s.v_empty[st.buf], st.free)) return false;
+            load(v_tile(st.buf), &p.v, &s.v_full[st.buf], DV / 64, chunk * C, w.h, w.b);
+            return true;
+        });
+    }
+    // ---- X, warp 2: decays, four neighbouring tokens a lane
+    __device__ __forceinline__ void decays() const {
+        const int lane = tid & 31;
+        each([&](const Item<Reverse> &w, int chunk, int i) {
+            const At<SLOTS> at(i);
+            const int tokens = w.tokens(chunk);
+            const long long base = w.b * a.decay.bs + w.h * a.decay.hs + (long long)chunk * C * a.decay.ts;
+            double g[4], sum = 0.0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) g[j] = 4 * lane + j < tokens ? decay_log2(a, base + (4 * lane + j) * a.decay.ts) : 0.0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) g[j] = sum += g[j];
+            double before = sum;
+            for (int o = 1; o < 32; o <<= 1) {
+                const double u = __shfl_up_sync(0xffffffffu, before, o);
+                if (lane >= o) before += u;
+            }
+            before = __shfl_up_sync(0xffffffffu, before, 1);
+            if (lane == 0) before = 0.0;
+            float2 G[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) G[j] = two_floats(before + g[j]);
+            const float2 block_end = make_float2(__shfl_sync(0xffffffffu, G[3].x, lane | 7), __shfl_sync(0xffffffffu, G[3].y, lane | 7));
+            const float2 end = make_float2(__shfl_sync(0xffffffffu, G[3].x, 31), __shfl_sync(0xffffffffu, G[3].y, 31));
+            if (!wait_warp(s, s.g_empty[at.buf], at.free)) return false;
+            Slot &to = slots[at.buf];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float start = a.scale * exp2_of(G[j]);
+                to.G[4 * lane + j] = G[j];
+                to.to_block[4 * lane + j] = ex2_diff(block_end, G[j]);
+                to.weight[4 * lane + j] = Reverse ? start : exp2_diff(end, G[j]);
+                to.from_start[4 * lane + j] = start;
+            }
+            if (lane == 0) to.whole = exp2_of(end);
+            tc::mbar_arrive(&s.g_full[at.buf]);
+            return true;
+        });
+    }
+    // ---- K
+    __device__ __forceinline__ void split() const {
+        each([&](const Item<Reverse> &w, int chunk, int i) {
+            const At<L::NS> st(i);
+            const At<SLOTS> at(i);
+            const int tokens = w.tokens(chunk);
+            if (!wait_warp(s, s.g_full[at.buf], at.full) || !wait_warp(s, s.k_full[st.buf], st.full)) return false;
+            if (tokens < C) {              // what lies behind the sequence was fetched too: v must not bring infinities or NaN into the sums
+                if (!wait_warp(s, s.v_full[st.buf], st.full)) return false;
+                for (int e = tid; e < (C - tokens) * (DV / 8); e += WG) {
+                    const int r = tokens + e / (DV / 8), c = e % (DV / 8);
+                    sts16(v_tile(st.buf) + (c >> 3) * PANEL + r * 128 + (c & 7) * 16, 0u, 0u, 0u, 0u);
+                }
+            }
+            for (int half = 0; half < 2; ++half) {
+                const At<L::NB> pb(2 * i + half);
+                if (!wait_warp(s, s.parts_empty[pb.buf], pb.free)) return false;
+                const uint32_t from = k_tile(st.buf) + half * (PANEL / 2), to = parts(pb.buf);
+#pragma unroll 2
+                for (int j = 0; j < 64 * DK / 8 / WG; ++j) {
+                    const int e = j * WG + tid, r = e / (DK / 8), ch = e % (DK / 8);
+                    const uint32_t off = chunk_at(r, ch & 7);
+                    const uint4 u = lds16(from + (ch >> 3) * PANEL + off);
+                    const bool on = half * 64 + r < tokens;
+                    const uint32_t in[4] = {on ? u.x : 0u, on ? u.y : 0u, on ? u.z : 0u, on ? u.w : 0u};
+                    const float f = slots[at.buf].weight[half * 64 + r];
+                    uint32_t o[3][4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        float x0 = low(in[q]) * f, x1 = high(in[q]) * f;
+#pragma unroll
+                        for (int t = 0; t < 3; ++t) {
+                            o[t][q] = pack(x0, x1);
+                            x0 -= low(o[t][q]);
+                            x1 -= high(o[t][q]);
+                        }
+                    }
+#pragma unroll
+                    for (int t = 0; t < 3; ++t) sts16(to + t * L::PART + (ch >> 3) * (PANEL / 2) + off, o[t][0], o[t][1], o[t][2], o[t][3]);
+                }
+                fence_async();
+                tc::mbar_arrive(&s.parts_full[pb.buf]);
+            }
+            tc::mbar_arrive(&s.k_empty[st.buf]);
+            tc::mbar_arrive(&s.g_empty[at.buf]);
+            return true;
+        });
+    }
+    // ---- S.  Lane i of tensor memory is row i; with 64 rows the upper lanes repeat them and take the second half of the columns.
+    __device__ __forceinline__ void states() const {
+        constexpr int N = DK == 64 ? DV / 2 : DV;
+        const int row = DK == 64 ? tid & 63 : tid, c0 = DK == 64 ? (tid >> 6) * N : 0;
+        const uint32_t U = lane_base(s.tmem, tid >> 5) + L::U + c0;
+        const long long dense_all = (long long)a.B * a.H * a.Dk * a.Dv;
+        float S[N];
+        int i = 0;
+        for (int it = blockIdx.x; it < p.items; it += gridDim.x) {
+            const Item<Reverse> w(a, p, it);
+            const long long dense = (long long)w.bh * a.Dk * a.Dv + (long long)row * a.Dv + c0;
+            const float *first = p.own_sums ? nullptr : p.segments > 1 ? p.seg_state + w.seg * dense_all : p.first;
+#pragma unroll
+            for (int j = 0; j < N; ++j) S[j] = first && row < a.Dk && c0 + j < a.Dv ? first[dense + j] : 0.f;
+            double all = 0.0;
+            for (int c = w.begin; c < w.stop; ++c, ++i) {
+                const At<1> one(i);
+                const At<SLOTS> at(i);
+                if (p.states && !p.own_sums) {
+                    uint4 *to = reinterpret_cast<uint4 *>(p.states + ((long long)Item<Reverse>::chunk(p, c) * a.B * a.H + w.bh) * (DK * DV) + row * DV + c0);
+#pragma unroll
+                    for (int j = 0; j < N; j += 8) to[j / 8] = make_uint4(pack(S[j], S[j + 1]), pack(S[j + 2], S[j + 3]), pack(S[j + 4], S[j + 5]), pack(S[j + 6], S[j + 7]));
+                }
+                if constexpr (Outputs) {
+                    if (!wait_warp(s, s.s_empty, one.free)) return;
+#pragma unroll
+                    for (int j = 0; j < N; j += 8) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float x0 = S[j + 2 * e], x1 = S[j + 2 * e + 1];
+                            hi[e] = pack(x0, x1);
+                            lo[e] = pack(x0 - low(hi[e]), x1 - high(hi[e]));
+                        }
+                        const uint32_t off = (uint32_t)((c0 + j) >> 6) * (DK * 128) + chunk_at(row, ((c0 + j) >> 3) & 7);
+                        sts16(state(0) + off, hi[0], hi[1], hi[2], hi[3]);
+                        sts16(state(1) + off, lo[0], lo[1], lo[2], lo[3]);
+                    }
+                    fence_async();
+                    tc::mbar_arrive(&s.s_full);
+                }
+                if (!wait_warp(s, s.g_full[at.buf], at.full)) return;
+                const float whole = slots[at.buf].whole;
+                const float2 end = slots[at.buf].G[C - 1];
+                tc::mbar_arrive(&s.g_empty[at.buf]);
+                all += (double)end.x + (double)end.y;
+                if (!wait_warp(s, s.u_full, one.full)) return;
+                tc::tc_fence_after_sync();
+#pragma unroll
+                for (int j = 0; j < N; j += 32) {
+                    float u[32];
+                    tmem_load(U + j, u);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) S[j + e] = fmaf(whole, S[j + e], u[e]);
+                }
+                tc::tc_fence_before_sync();
+                tc::mbar_arrive(&s.u_empty);
+            }
+            float *to = p.own_sums ? p.seg_state + w.seg * dense_all : p.last && w.seg == p.segments - 1 ? p.last : nullptr;
+            if (to) {
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (row < a.Dk && c0 + j < a.Dv) to[dense + j] = S[j];
+            }
+            if (p.own_sums && tid == 0) p.seg_log[w.seg * (a.B * a.H) + w.bh] = (float)all;
+        }
+    }
+    // ---- P.  Blocks of 32 x 32 pairs; below the diagonal 2^(G_t - G_s) is a product of two factors, both at most 1: from s to the end
+    // of its block and from there to t.
+    __device__ __forceinline__ void weights() const {
+        const int warp = tid >> 5, lane = tid & 31;
+        each([&](const Item<Reverse> &, int, int i) {
+            const At<SLOTS> at(i);
+            const At<L::NQ> qb(i);
+            if (!wait_warp(s, s.g_full[at.buf], at.full)) return false;
+            const Slot &g = slots[at.buf];
+            const float2 G = g.G[tid];
+            const uint32_t from = lane_base(s.tmem, warp) + qb.buf * 128;
+            if (!wait_warp(s, s.pairs_full[qb.buf], qb.full)) return false;
+            tc::tc_fence_after_sync();
+#pragma unroll 1
+            for (int sb = 0; sb < 4; ++sb) {
+                uint32_t P[16];
+                if (sb > warp) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) P[j] = 0u;
+                } else {
+                    float x[32];
+                    tmem_load(from + sb * 32, x);
+                    if (sb < warp) {
+                        const float r = a.scale * ex2_diff(G, g.G[sb * 32 + 31]);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 f = *reinterpret_cast<const float4 *>(&g.to_block[sb * 32 + j]);
+                            P[j / 2] = pack(x[j] * (r * f.x), x[j + 1] * (r * f.y));
+                            P[j / 2 + 1] = pack(x[j + 2] * (r * f.z), x[j + 3] * (r * f.w));
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            const float w0 = a.scale * ex2_diff(G, g.G[sb * 32 + j]), w1 = a.scale * ex2_diff(G, g.G[sb * 32 + j + 1]);
+                            P[j / 2] = pack(j <= lane ? x[j] * w0 : 0.f, j + 1 <= lane ? x[j + 1] * w1 : 0.f);
+                        }
+                    }
+                }
+                tmem_st16(from + sb * 16, P);       // columns that this warp has read already
+            }
+            tc::tmem_st_wait();
+            tc::tc_fence_before_sync();
+            tc::mbar_arrive(&s.p_full[qb.buf]);
+            tc::mbar_arrive(&s.g_empty[at.buf]);
+            return true;
+        });
+    }
+    // ---- O
+    __device__ __forceinline__ void outputs() const {
+        const int warp = tid >> 5, row = tid;
+        const uint32_t from = lane_base(s.tmem, warp);
+        const bool vec = a.Dv % 8 == 0 && (a.out.ts | a.out.bs | a.out.hs) % 8 == 0 && reinterpret_cast<uintptr_t>(a.out.p) % 16 == 0;
+        int i = 0;
+        for (int it = blockIdx.x; it < p.items; it += gridDim.x) {
+            const Item<Reverse> w(a, p, it);
+            bf16 *out = static_cast<bf16 *>(a.out.p) + at(a.out, w.b, w.h) + (long long)row * a.out.ts;
+            for (int c = w.begin; c < w.stop; ++c, ++i) {
+                const At<1> one(i);
+                const At<SLOTS> g(i);
+                const int t0 = c * C, all = min(a.T - t0, C), tokens = w.tokens(c);
+                if (!wait_warp(s, s.g_full[g.buf], g.full) || !wait_warp(s, s.o_full, one.full)) return;
+                tc::tc_fence_after_sync();
+                const float r = slots[g.buf].from_start[row];
+                bf16 *to = out + (long long)t0 * a.out.ts;
+#pragma unroll 1
+                for (int j = 0; j < DV; j += 32) {
+                    float x[32], y[32];
+                    tmem_load(from + L::INTRA + j, x);
+                    tmem_load(from + L::INTER + j, y);
+                    bool odd = false;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        odd |= !isfinite(x[e]);
+                        y[e] *= r;
+                    }
+                    if (odd && row < tokens) {
+                        float z[32];
+                        again(z, w.b, w.h, t0, row, j, slots[g.buf]);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x[e] = z[e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) x[e] = row < tokens ? x[e] + y[e] : 0.f;
+                    if (row < all) store_row(to, x, j, a.Dv, vec);
+                    __syncwarp();
+                }
+                tc::tc_fence_before_sync();
+                tc::mbar_arrive(&s.o_empty);
+                tc::mbar_arrive(&s.g_empty[g.buf]);
+            }
+            for (int c = w.stop; c < w.end; ++c)               // behind the sequence
+                if (c * C + row < a.T)
+                    for (int j = 0; j < a.Dv; ++j) out[(long long)c * C * a.out.ts + j] = __float2bfloat16_rn(0.f);
+        }
+    }
+    // A later token's infinity or NaN is none of an earlier one's business, and zero times it is NaN: the sums again, over the tokens up
+    // to this one.
+    __device__ __noinline__ void again(float *x, int b, int h, int t0, int row, int j, const Slot &g) const {
+        const bf16 *q = static_cast<const bf16 *>(a.q.p) + at(a.q, b, h / p.share) + (long long)(t0 + row) * a.q.ts;
+        const bf16 *k = static_cast<const bf16 *>(a.k.p) + at(a.k, b, h / p.share) + (long long)t0 * a.k.ts;
+        const bf16 *v = static_cast<const bf16 *>(a.v.p) + at(a.v, b, h) + (long long)t0 * a.v.ts + j;
+        for (int e = 0; e < 32; ++e) x[e] = 0.f;
+        for (int t = 0; t <= row; ++t) {
+            float f = 0.f;
+            for (int d = 0; d < a.Dk; ++d) f = fmaf(seq::to_f(q[d]), seq::to_f(k[t * a.k.ts + d]), f);
+            f *= a.scale * ex2_diff(g.G[row], g.G[t]);
+            for (int e = 0; e < 32; ++e)
+                if (j + e < a.Dv) x[e] = fmaf(f, seq::to_f(v[t * a.v.ts + e]), x[e]);
+        }
+    }
+};
+
+template <int DK, int DV, bool Outputs, bool Reverse>
+__global__ void __launch_bounds__(THREADS, 1) k_walk(const __grid_constant__ qgru_attention a, const __grid_constant__ Args p) {
+    using L = Plan<DK, DV, Outputs>;
+    extern __shared__ unsigned char raw[];
+    unsigned char *tiles = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    Slot *slots = reinterpret_cast<Slot *>(tiles + L::TILES);
+    Ctl &s = *reinterpret_cast<Ctl *>(slots + SLOTS);
+    using G = Regs<DK == 64 ? DV / 2 : DV>;
+    const int tid = threadIdx.x, wg = tid / WG;
+    if (tid == 0) {
+        constexpr int readers = (Outputs ? 4 : 2) * WG;
+        for (int i = 0; i < 3; ++i) {
+            tc::mbar_init(&s.k_full[i], 1);
+            tc::mbar_init(&s.k_empty[i], WG + (Outputs ? 1 : 0));
+            tc::mbar_init(&s.q_full[i], 1);
+            tc::mbar_init(&s.q_empty[i], 1);
+            tc::mbar_init(&s.v_full[i], 1);
+            tc::mbar_init(&s.v_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&s.parts_full[i], WG);
+            tc::mbar_init(&s.parts_empty[i], 1);
+            tc::mbar_init(&s.pairs_full[i], 1);
+            tc::mbar_init(&s.p_full[i], WG);
+        }
+        for (int i = 0; i < SLOTS; ++i) {
+            tc::mbar_init(&s.g_full[i], 32);
+            tc::mbar_init(&s.g_empty[i], readers);
+        }
+        tc::mbar_init(&s.u_full, 1);
+        tc::mbar_init(&s.u_empty, WG);
+        tc::mbar_init(&s.s_full, WG);
+        tc::mbar_init(&s.s_empty, 1);
+        tc::mbar_init(&s.o_full, 1);
+        tc::mbar_init(&s.o_empty, WG);
+        s.failed = 0;
+        tc::fence_barrier_init();
+        tc::tma_prefetch_desc(&p.k);
+        tc::tma_prefetch_desc(&p.v);
+        if (Outputs) tc::tma_prefetch_desc(&p.q);
+    }
+    if (tid < 32) tc::tmem_alloc(&s.tmem, L::COLUMNS);
+    tc::tc_fence_before_sync();
+    __syncthreads();
+    tc::tc_fence_after_sync();
+    const Roles<DK, DV, Outputs, Reverse> r{a, p, s, slots, tc::smem_u32(tiles), tid % WG};
+    if (wg == 0) {
+        take_registers<G::X>();
+        const int warp = tid >> 5;
+        if (warp == 0) {
+            if (tid == 0) r.issue();
+        } else if (warp == 1) {
+            if (tid == 32) r.fetch();
+        } else if (warp == 2) {
+            r.decays();
+        }
+        __syncwarp();
+    } else if (wg == 1) {
+        take_registers<G::K>();
+        r.split();
+    } else if (wg == 2) {
+        take_registers<G::S>();
+        r.states();
+    } else if (wg == 3) {
+        take_registers<G::P>();
+        if constexpr (Outputs) r.weights();
+    } else {
+        take_registers<G::O>();
+        if constexpr (Outputs) r.outputs();
+    }
+    tc::tc_fence_before_sync();
+    __syncthreads();
+    if (s.failed) {            // copies and products may be under way: a millisecond is far more than they take
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000ll) {
+        }
+        if (tid == 0) *p.flag = 1;
+    }
+    if (tid < 32) tc::tmem_dealloc(s.tmem, L::COLUMNS);
+}
+
+// ------------------------------------------------------------------------------------- launches
+bool make_map(CUtensorMap *map, const qgru_seq_tensor &x, int T, int B, int heads, int d) {
+    const EncodeTiledFn enc = get_encode_tiled();
+    if (!enc) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)T, (cuuint64_t)heads, (cuuint64_t)B};
+    // (the stride of a dimension of one is nobody's)
+    const auto bytes = [](long long s, int n) { return n > 1 ? (cuuint64_t)s * 2 : (cuuint64_t)256; };
+    const cuuint64_t strides[3] = {bytes(x.ts, T), bytes(x.hs, heads), bytes(x.bs, B)};
+    const cuuint32_t box[4] = {64, C, 1, 1}, step[4] = {1, 1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, x.p, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DK, int DV, bool Outputs, bool Reverse>
+int launch(const qgru_attention &a, const Args &p, int sms, cudaStream_t st) {
+    const auto kernel = k_walk<DK, DV, Outputs, Reverse>;
+    constexpr int bytes = Plan<DK, DV, Outputs>::TILES + 1024 + SLOTS * (int)sizeof(Slot) + (int)sizeof(Ctl);
+    static_assert(bytes <= 232448, "shared memory");
+    SEQ_CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    kernel<<<std::min(p.items, sms), THREADS, bytes, st>>>(a, p);
+    SEQ_CK(cudaGetLastError());
+    return QGRU_OK;
+}
+
+template <int DK, int DV, bool Reverse>
+int run(const qgru_attention &a, const Cut &c, bf16 *states, char *seg, int *flag, int sms, cudaStream_t st) {
+    Args p{};
+    const qgru_seq_tensor &k = Reverse ? a.q : a.k, &v = Reverse ? a.dout : a.v;
+    if (a.T > 0 && (!make_map(&p.k, k, a.T, a.B, a.Hk, a.Dk) || !make_map(&p.v, v, a.T, a.B, a.H, a.Dv) || !make_map(&p.q, a.q, a.T, a.B, a.Hk, a.Dk)))
+        return seq::fail(QGRU_ERR_CUDA, "cuTensorMapEncodeTiled");
+    p.first = Reverse ? a.dstate : a.state0;
+    p.last = Reverse ? a.dstate0 : a.state;
+    p.states = states;
+    p.segments = c.segments;
+    p.per = c.per;
+    p.chunks = c.chunks;
+    p.share = a.H / a.Hk;
+    p.items = a.B * a.H * c.segments;
+    p.flag = flag;
+    if (c.segments > 1) {
+        p.seg_state = reinterpret_cast<float *>(seg);
+        p.seg_log = p.seg_state + c.segments * state_elems(a);
+        p.own_sums = 1;
+        if (const int rc = launch<DK, DV, false, Reverse>(a, p, sms, st)) return rc;
+        if (const int rc = scan_segments(a, c, Reverse, seg, st)) return rc;
+        p.own_sums = 0;
+    }
+    return launch<DK, DV, !Reverse, Reverse>(a, p, sms, st);
+}
+
+bool strides_ok(const qgru_seq_tensor &x, int T, int B, int heads, int d) {
+    const auto ok = [](long long s, int n) { return n <= 1 || (s > 0 && s % 8 == 0 && s < (1ll << 38)); };
+    return reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && d % 8 == 0 && ok(x.ts, T) && ok(x.bs, B) && ok(x.hs, heads);
+}
+
+}  // namespace
+
+// Whether the tensors can be fetched by TMA: rows and strides of a multiple of 16 bytes.
+bool walk_takes(const qgru_attention &a, bool reverse) {
+    if (reverse) return strides_ok(a.q, a.T, a.B, a.Hk, a.Dk) && strides_ok(a.dout, a.T, a.B, a.H, a.Dv);
+    return strides_ok(a.q, a.T, a.B, a.Hk, a.Dk) && strides_ok(a.k, a.T, a.B, a.Hk, a.Dk) && strides_ok(a.v, a.T, a.B, a.H, a.Dv);
+}
+int walk(const qgru_attention &a, const Cut &c, bool reverse, void *states, char *seg, int *flag, int sms, cudaStream_t st) {
+    using std::integral_constant;
+    const auto with = [&](auto dk, auto dv) -> int {
+        bf16 *to = static_cast<bf16 *>(states);
+        return reverse ? run<dk.value, dv.value, true>(a, c, to, seg, flag, sms, st) : run<dk.value, dv.value, false>(a, c, to, seg, flag, sms, st);
+    };
+    const integral_constant<int, 64> small;
+    const integral_constant<int, 128> large;
+    return a.Dk <= 64 ? (a.Dv <= 64 ? with(small, small) : with(small, large)) : (a.Dv <= 64 ? with(large, small) : with(large, large));
+}
+
+}  // namespace attn
+}  // namespace qgru

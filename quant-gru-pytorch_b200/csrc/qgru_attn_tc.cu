@@ -19,121 +19,8 @@ namespace qgru {
 namespace attn {
 namespace {
 
-constexpr int C = 128, THREADS = 256;
-constexpr int PANEL = C * 128;                          // bytes of 64 columns of a tile of 128 rows
-constexpr long long WAIT_BUDGET = 2000000000ll;         // about a second of SM clocks
-using bf16 = __nv_bfloat16;
-
-// ------------------------------------------------------------------------------------- operands and products
-constexpr uint32_t DESC_HI = (uint32_t)(1024 >> 4) | (1u << 14) | (2u << 29);     // groups of eight rows 1024 bytes apart, 128-byte swizzle
-
-struct Operand {                        // a tile, `panel` bytes from 64 columns to the next
-    uint32_t at;
-    int panel;
-};
-// Low word of the descriptor for K = 16 j .. 16 j + 15.  K in the columns: 32 bytes a step, four steps a panel.  K in the rows:
-// 2048 bytes (sixteen rows) a step, and the descriptor's leading distance is that between panels.
-template <bool KRows>
-__device__ __forceinline__ uint32_t desc_lo(const Operand &o, int j) {
-    if constexpr (KRows)
-        return (((o.at + j * 2048) & 0x3FFFFu) >> 4) | ((uint32_t)o.panel >> 4 << 16);
-    else
-        return (((o.at + (j >> 2) * o.panel + (j & 3) * 32) & 0x3FFFFu) >> 4) | (1u << 16);
-}
-// D fp32, A and B bf16, M = 128
-__host__ __device__ constexpr uint32_t idesc(int N, bool a_rows, bool b_rows) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((a_rows ? 1u : 0u) << 15) | ((b_rows ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-}
-__device__ __forceinline__ void mma(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t id, uint32_t accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        ".reg .b64 da, db;\n"
-        "mov.b64 da, {%1, %5};\n"
-        "mov.b64 db, {%2, %5};\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n"
-        "}\n" ::"r"(d),
-        "r"(a_lo), "r"(b_lo), "r"(id), "r"(accumulate), "n"(DESC_HI)
-        : "memory");
-}
-// A from tensor memory: lane i is row i, a column holds two neighbouring K, sixteen K are eight columns
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t id, uint32_t accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        ".reg .b64 db;\n"
-        "mov.b64 db, {%2, %5};\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n"
-        "}\n" ::"r"(d),
-        "r"(a), "r"(b_lo), "r"(id), "r"(accumulate), "n"(DESC_HI)
-        : "memory");
-}
-template <bool ARows, bool BRows, int N, int K>
-__device__ __forceinline__ void product(uint32_t d, const Operand &a, const Operand &b, bool add) {
-#pragma unroll
-    for (int j = 0; j < K / 16; ++j) mma(d, desc_lo<ARows>(a, j), desc_lo<BRows>(b, j), idesc(N, ARows, BRows), (add || j) ? 1u : 0u);
-}
-template <bool BRows, int N, int K>
-__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, const Operand &b, bool add) {
-#pragma unroll
-    for (int j = 0; j < K / 16; ++j) mma_ts(d, a + j * 8, desc_lo<BRows>(b, j), idesc(N, false, BRows), (add || j) ? 1u : 0u);
-}
-
-__device__ __forceinline__ uint32_t lane_base(uint32_t tmem, int warp) { return tmem + ((uint32_t)((warp & 3) * 32) << 16); }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
-                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
-                 "r"(v[14]), "r"(v[15])
-                 : "memory");
-}
-// Cols / 16 groups of sixteen columns
-template <int Cols>
-__device__ __forceinline__ void tmem_load(uint32_t taddr, float (&v)[Cols]) {
-    int32_t r[Cols / 16][16];
-#pragma unroll
-    for (int i = 0; i < Cols / 16; ++i) tc::tmem_ld16(taddr + i * 16, r[i]);
-    tc::tmem_ld_wait();
-#pragma unroll
-    for (int i = 0; i < Cols; ++i) v[i] = __int_as_float(r[i / 16][i % 16]);
-}
-template <int Cols>
-__device__ __forceinline__ void tmem_store(uint32_t taddr, const uint32_t (&v)[Cols]) {
-#pragma unroll
-    for (int i = 0; i < Cols / 16; ++i) {
-        uint32_t r[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) r[j] = v[i * 16 + j];
-        tmem_st16(taddr + i * 16, r);
-    }
-}
-
-// ------------------------------------------------------------------------------------- values
-__device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-__device__ __forceinline__ float low(uint32_t x) { return __uint_as_float(x << 16); }
-__device__ __forceinline__ float high(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ float ex2_diff(float2 t, float2 s) { return ex2((t.x - s.x) + (t.y - s.y)); }
-
-// 16-byte chunk c (of eight columns) of row r of a panel
-__device__ __forceinline__ uint32_t chunk_at(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
-
-__device__ __forceinline__ void cp_async(uint32_t to, const void *from, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int Left>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(Left) : "memory"); }
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+using namespace tile;
+constexpr int THREADS = 256;
 
 // Rows t0 .. t0 + 127 of a tensor (zeros from `tokens` on and behind its columns) as a tile of D columns.  Vec: rows and strides
 // are multiples of 16 bytes; else element by element.
@@ -170,31 +57,6 @@ __device__ __forceinline__ void load_state(uint32_t tile, const bf16 *S, int tid
         cp_async(tile + (c >> 3) * (DK * 128) + chunk_at(r, c & 7), S + e * 8, 16);
     }
 }
-__device__ __forceinline__ uint4 lds16(uint32_t at) {
-    uint4 v;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-    return v;
-}
-__device__ __forceinline__ void sts16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-__device__ __forceinline__ long long at(const qgru_seq_tensor &x, int b, int h) { return b * x.bs + h * x.hs; }
-
-// A thread's Cols neighbouring columns, from `c0` on, of a row of bf16.
-template <int Cols>
-__device__ __forceinline__ void store_row(bf16 *row, const float (&v)[Cols], int c0, int d, bool vec) {
-#pragma unroll
-    for (int i = 0; i < Cols; i += 8) {
-        if (vec) {
-            if (c0 + i < d) *reinterpret_cast<uint4 *>(row + c0 + i) = make_uint4(pack(v[i], v[i + 1]), pack(v[i + 2], v[i + 3]), pack(v[i + 4], v[i + 5]), pack(v[i + 6], v[i + 7]));
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (c0 + i + j < d) row[c0 + i + j] = __float2bfloat16_rn(v[i + j]);
-        }
-    }
-}
-
 struct Shared {                 // behind the tiles
     float2 G[C];                // running sums of the decays, base 2
     float f[C];                 // factors of a token
@@ -827,8 +689,9 @@ int run_states(const qgru_attention &a, const Cut &c, bf16 *states, char *seg, i
 
 template <int DK, int DV, bool Vec>
 int forward(const qgru_attention &a, const Cut &c, int *flag, cudaStream_t st) {
-    bf16 *states = static_cast<bf16 *>(a.states);
-    if (const int rc = run_states<DK, DV, false, Vec>(a, c, states, static_cast<char *>(a.workspace), flag, st)) return rc;
+    bf16 *states = static_cast<bf16 *>(a.keep ? a.states : a.workspace);
+    char *seg = static_cast<char *>(a.workspace) + (a.keep ? 0 : a256(c.states));
+    if (const int rc = run_states<DK, DV, false, Vec>(a, c, states, seg, flag, st)) return rc;
     if (c.chunks == 0) return QGRU_OK;
     int bytes = 0;
     if (const int rc = with_smem(k_outputs_tc<DK, DV, Vec>, OUTPUTS_TILES<DK, DV>, &bytes)) return rc;
@@ -837,13 +700,13 @@ int forward(const qgru_attention &a, const Cut &c, int *flag, cudaStream_t st) {
     return QGRU_OK;
 }
 template <int DK, int DV, bool Vec>
-int backward(const qgru_attention &a, const Cut &c, int *flag, cudaStream_t st) {
+int backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStream_t st) {
     char *ws = static_cast<char *>(a.workspace);
     bf16 *dstates = reinterpret_cast<bf16 *>(ws);
     ws += a256(c.states);
     char *seg = ws;
     ws += a256(c.seg);
-    if (const int rc = run_states<DK, DV, true, Vec>(a, c, dstates, seg, flag, st)) return rc;
+    if (const int rc = walk_takes(a, true) ? walk(a, c, true, dstates, seg, flag, sms, st) : run_states<DK, DV, true, Vec>(a, c, dstates, seg, flag, st)) return rc;
     if (c.chunks == 0) return QGRU_OK;
     Gradients g{static_cast<const bf16 *>(a.states), dstates, nullptr, nullptr, flag};
     if (a.H != a.Hk) {
@@ -886,13 +749,14 @@ Cut tc_cut(const qgru_attention &a, int sms) {
     c.seg = c.segments > 1 ? sizeof(float) * c.segments * (state_elems(a) + (size_t)a.B * a.H) : 0;
     return c;
 }
-int tc_forward(const qgru_attention &a, const Cut &c, int *flag, cudaStream_t st) {
+int tc_forward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStream_t st) {
+    if (walk_takes(a, false)) return walk(a, c, false, a.keep ? a.states : nullptr, static_cast<char *>(a.workspace), flag, sms, st);
     const bool vec = vec_ok(a.q, a.Dk) && vec_ok(a.k, a.Dk) && vec_ok(a.v, a.Dv);
     return by_size(a, vec, [&](auto dk, auto dv, auto v) -> int { return forward<dk.value, dv.value, v.value>(a, c, flag, st); });
 }
-int tc_backward(const qgru_attention &a, const Cut &c, int *flag, cudaStream_t st) {
+int tc_backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStream_t st) {
     const bool vec = vec_ok(a.q, a.Dk) && vec_ok(a.k, a.Dk) && vec_ok(a.v, a.Dv) && vec_ok(a.dout, a.Dv);
-    return by_size(a, vec, [&](auto dk, auto dv, auto v) -> int { return backward<dk.value, dv.value, v.value>(a, c, flag, st); });
+    return by_size(a, vec, [&](auto dk, auto dv, auto v) -> int { return backward<dk.value, dv.value, v.value>(a, c, flag, sms, st); });
 }
 
 }  // namespace attn

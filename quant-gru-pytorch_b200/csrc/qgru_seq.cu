@@ -63,7 +63,7 @@ int expiry_flag(int device, int **flag) {
     *flag = f.device;
     pthread_mutex_unlock(&flags_lock);
     if (e != cudaSuccess) return cuda_fail(e, "cudaHostAlloc");
-    return expired ? fail(QGRU_ERR_TIMEOUT, "a wait inside a kernel of an earlier call has run out; its results are NaN") : QGRU_OK;
+    return expired ? fail(QGRU_ERR_TIMEOUT, "a wait inside a kernel of an earlier call has run out: its results are not to be used") : QGRU_OK;
 }
 
 }  // namespace seq

@@ -18,11 +18,12 @@ int cuda_fail(cudaError_t e, const char *where);
 // knows without waiting.  Returns QGRU_ERR_TIMEOUT, once, where an earlier call's has.
 int expiry_flag(int device, int **flag);
 
-// Work goes to the device that the caller names; the thread's current device is put back when the call ends.
+// Work goes to the device that the caller names; the thread's current device is put back when the call ends.  (Set even where it
+// is the current one: a thread that has not used the device yet has no context, which tensor maps are encoded in.)
 class OnDevice {
   public:
     explicit OnDevice(int device) {
-        if ((err_ = cudaGetDevice(&before_)) == cudaSuccess && before_ != device && (err_ = cudaSetDevice(device)) == cudaSuccess) moved_ = true;
+        if ((err_ = cudaGetDevice(&before_)) == cudaSuccess && (err_ = cudaSetDevice(device)) == cudaSuccess) moved_ = before_ != device;
     }
     ~OnDevice() {
         if (moved_) cudaSetDevice(before_);

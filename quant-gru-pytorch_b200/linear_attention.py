@@ -36,8 +36,15 @@ def _tensor(t, name, dtype, device, shape):
     return t
 
 
-def _last_dense(t):
-    return t if t.stride(-1) == 1 or t.numel() == 0 else t.contiguous()
+def _readable(t):
+    """t, or a dense copy where its last stride is not 1 or its rows could be fetched in 16-byte pieces but for where they lie."""
+    if t.numel() == 0:
+        return t
+    per = 16 // t.element_size()
+    s = t.stride()
+    if s[-1] == 1 and (t.shape[-1] % per or not (t.data_ptr() % 16 or any(x % per for x in s[:-1]))):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _check(q, k, v, log_decay, lead):
@@ -64,9 +71,9 @@ def _check(q, k, v, log_decay, lead):
     return log_decay
 
 
-def _head(dims, dev, q, decay, scale):
+def _head(dims, dev, q, decay, scale, keep=False):
     T, B, H, Hk, Dk, Dv = dims
-    return _cabi.Attention(dev, T, B, H, Hk, Dk, Dv, q.dtype == torch.bfloat16, decay.dtype == torch.bfloat16, scale, *_BLANK)
+    return _cabi.Attention(dev, T, B, H, Hk, Dk, Dv, q.dtype == torch.bfloat16, decay.dtype == torch.bfloat16, keep, scale, *_BLANK)
 
 
 def _place(t, batch_first):
@@ -83,14 +90,15 @@ def _block(nbytes, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
-def _forward(q, k, v, decay, state0, lengths, scale, batch_first):
-    """-> out, state, states (what the backward reads)."""
-    q, k, v = _last_dense(q), _last_dense(k), _last_dense(v)
+def _forward(q, k, v, decay, state0, lengths, scale, batch_first, keep):
+    """-> out, state, states (what the backward reads, with `keep`)."""
+    q, k, v = _readable(q), _readable(k), _readable(v)
     t_dim, b_dim = (1, 0) if batch_first else (0, 1)
     dims = (q.shape[t_dim], q.shape[b_dim], v.shape[2], q.shape[2], q.shape[3], v.shape[3])
     T, B, H, _, Dk, Dv = dims
     device, dev, L = q.device, q.device.index or 0, _cabi.lib()
-    a = _head(dims, dev, q, decay, scale)
+    a = _head(dims, dev, q, decay, scale, keep)
+    a.q, a.k, a.v, a.decay = (_place(x, batch_first) for x in (q, k, v, decay))
     sizes = [C.c_size_t() for _ in range(3)]
     _cabi.check_seq(L.qgru_attention_sizes(a, *sizes), "qgru_attention_sizes")
     states, ws = _block(sizes[0].value, device), _block(sizes[1].value, device)
@@ -98,7 +106,7 @@ def _forward(q, k, v, decay, state0, lengths, scale, batch_first):
     state = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=device)
     a.lengths, a.state0, a.state, a.states, a.workspace = _ptr(lengths), _ptr(state0), state.data_ptr(), _ptr(states), _ptr(ws)
     a.states_bytes, a.workspace_bytes = sizes[0].value, sizes[1].value
-    a.q, a.k, a.v, a.decay, a.out = (_place(x, batch_first) for x in (q, k, v, decay, out))
+    a.out = _place(out, batch_first)
     _cabi.check_seq(L.qgru_attention_forward(a, torch._C._cuda_getCurrentRawStream(dev)), "qgru_attention_forward")
     return out, state, states
 
@@ -106,7 +114,7 @@ def _forward(q, k, v, decay, state0, lengths, scale, batch_first):
 class _LinearAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, decay, state0, lengths, scale, batch_first):
-        out, state, states = _forward(q, k, v, decay, state0, lengths, scale, batch_first)
+        out, state, states = _forward(q, k, v, decay, state0, lengths, scale, batch_first, True)
         ctx.save_for_backward(q, k, v, decay, lengths, states)
         ctx.scale, ctx.batch_first, ctx.has_state = scale, batch_first, state0 is not None
         ctx.states_as = None if states is None else (states.shape, states.device)
@@ -124,12 +132,14 @@ class _LinearAttention(torch.autograd.Function):
                 states = states.clone(memory_format=torch.contiguous_format)
         batch_first = ctx.batch_first
         t_dim, b_dim = (1, 0) if batch_first else (0, 1)
-        q, k, v = _last_dense(q), _last_dense(k), _last_dense(v)
+        q, k, v = _readable(q), _readable(k), _readable(v)
         dims = (q.shape[t_dim], q.shape[b_dim], v.shape[2], q.shape[2], q.shape[3], v.shape[3])
         device, dev, L = q.device, q.device.index or 0, _cabi.lib()
-        dout = torch.zeros(v.shape, dtype=v.dtype, device=device) if dout is None else _last_dense(dout)
+        dout = torch.zeros(v.shape, dtype=v.dtype, device=device) if dout is None else _readable(dout)
         dstate = dstate.contiguous() if dstate is not None else None
-        a = _head(dims, dev, q, decay, ctx.scale)
+        a = _head(dims, dev, q, decay, ctx.scale, True)
+        for name, t in (("q", q), ("k", k), ("v", v), ("decay", decay), ("dout", dout)):
+            setattr(a, name, _place(t, batch_first))
         sizes = [C.c_size_t() for _ in range(3)]
         _cabi.check_seq(L.qgru_attention_sizes(a, *sizes), "qgru_attention_sizes")
         ws = _block(sizes[2].value, device)
@@ -137,7 +147,7 @@ class _LinearAttention(torch.autograd.Function):
         dstate0 = torch.empty((dims[1], dims[2], dims[4], dims[5]), dtype=torch.float32, device=device) if ctx.has_state and ctx.needs_input_grad[4] else None
         a.lengths, a.dstate, a.dstate0, a.states, a.workspace = _ptr(lengths), _ptr(dstate), _ptr(dstate0), _ptr(states), _ptr(ws)
         a.states_bytes, a.workspace_bytes = sizes[0].value, sizes[2].value
-        for name, t in (("q", q), ("k", k), ("v", v), ("decay", decay), ("dout", dout), ("dq", dq), ("dk", dk), ("dv", dv), ("ddecay", dg)):
+        for name, t in (("dq", dq), ("dk", dk), ("dv", dv), ("ddecay", dg)):
             setattr(a, name, _place(t, batch_first))
         _cabi.check_seq(L.qgru_attention_backward(a, torch._C._cuda_getCurrentRawStream(dev)), "qgru_attention_backward")
         return dq, dk, dv, dg, dstate0, None, None, None
@@ -158,7 +168,7 @@ def linear_attention(q, k, v, log_decay, initial_state=None, lengths=None, scale
     scale = q.shape[3] ** -0.5 if scale is None else float(scale)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, initial_state)):
         return _LinearAttention.apply(q, k, v, log_decay, initial_state, lengths, scale, batch_first)
-    return _forward(q, k, v, log_decay, initial_state, lengths, scale, batch_first)[:2]
+    return _forward(q, k, v, log_decay, initial_state, lengths, scale, batch_first, False)[:2]
 
 
 def linear_attention_step(q, k, v, log_decay, state, scale=None):
@@ -175,7 +185,7 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None):
     apart = (H == 1 or hs >= Dk * Dv) and (B == 1 or bs >= Dk * Dv) and (H == 1 or B == 1 or bs >= H * hs or hs >= B * bs)
     if B and not (dense and apart):
         raise ValueError(f"a head's state must be dense and the states must not overlap, got strides {list(state.stride())}")
-    q, k, v = _last_dense(q), _last_dense(k), _last_dense(v)
+    q, k, v = _readable(q), _readable(k), _readable(v)
     out = torch.empty((B, H, Dv), dtype=q.dtype, device=q.device)
     dev = q.device.index or 0
     a = _head((1, B, H, Hk, Dk, Dv), dev, q, log_decay, Dk ** -0.5 if scale is None else float(scale))

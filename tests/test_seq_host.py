@@ -56,7 +56,7 @@ def test_given_scale_is_a_range_of_eight_bits():
 
 def test_struct_layout():
     assert C.sizeof(_cabi.SeqTensor) == 32
-    assert C.sizeof(_cabi.Attention) == 10 * 4 + 7 * 8 + 2 * 8 + 10 * 32
+    assert C.sizeof(_cabi.Attention) == 12 * 4 + 7 * 8 + 2 * 8 + 10 * 32
     assert C.sizeof(_cabi.Norm) == 16 + 8 + 8 + 3 * 8 + 16 + 16 + 16 + 24 + 16
 
 
