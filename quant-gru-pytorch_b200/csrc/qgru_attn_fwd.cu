@@ -26,7 +26,7 @@ constexpr int WG = 128, THREADS = 5 * WG;
 constexpr int REGS = 96;
 template <int N>
 struct Regs {
-    static constexpr int S = N == 128 ? 168 : N == 64 ? 128 : 104, P = 112, O = N == 128 ? 88 : N == 64 ? 96 : 104, K = N == 128 ? 72 : N == 64 ? 80 : 88, X = N == 128 ? 40 : N == 64 ? 64 : 72;
+    static constexpr int S = N == 128 ? 168 : N == 64 ? 128 : 104, P = 96, O = N == 128 ? 112 : 120, K = N == 128 ? 64 : 80, X = N == 128 ? 40 : 56;
     static_assert(S + P + O + K + X <= 5 * REGS, "the shares add up to what the block starts with");
 };
 template <int R>
@@ -39,7 +39,7 @@ __device__ __forceinline__ void take_registers() {
 constexpr int SLOTS = 4;                    // chunks whose decays are known at once
 
 struct Slot {
-    float2 G[C];                            // running sums, base 2
+    float hi[C], lo[C];                     // running sums, base 2, each as two floats
     float to_block[C];                      // 2^(G at the end of s's block of 32 - G_s)
     float weight[C];                        // of k: 2^(G_C - G_s), or from the end scale 2^G_t
     float from_start[C];                    // scale 2^G_t
@@ -157,56 +157,59 @@ struct Roles {
     }
 
     // ---- X, warp 0: products
-    __device__ __forceinline__ bool pairs(int i) const {
+    __device__ __forceinline__ bool pairs(uint32_t leader, int i) const {
         const At<L::NS> st(i);
-        if (!wait(s, s.k_full[st.buf], st.full) || !wait(s, s.q_full[st.buf], st.full)) return false;
+        if (!wait_warp(s, s.k_full[st.buf], st.full) || !wait_warp(s, s.q_full[st.buf], st.full)) return false;
         tc::tc_fence_after_sync();
-        product<false, false, C, DK>(s.tmem + (i % L::NQ) * 128, Operand{q_tile(st.buf), PANEL}, Operand{k_tile(st.buf), PANEL}, false);
-        tc::mma_commit(&s.pairs_full[i % L::NQ]);
-        tc::mma_commit(&s.k_empty[st.buf]);
+        product<false, false, C, DK>(leader, s.tmem + (i % L::NQ) * 128, Operand{q_tile(st.buf), PANEL}, Operand{k_tile(st.buf), PANEL}, false);
+        commit(leader, &s.pairs_full[i % L::NQ]);
+        commit(leader, &s.k_empty[st.buf]);
         return true;
     }
     __device__ __forceinline__ void issue() const {
+        const uint32_t leader = elect();
         int steps = 0;
         for (int it = blockIdx.x; it < p.items; it += gridDim.x) {
             const Item<Reverse> w(a, p, it);
             steps += w.stop - w.begin;
         }
-        if (Outputs && L::NQ == 2 && steps && !pairs(0)) return;
+        if (Outputs && L::NQ == 2 && steps && !pairs(leader, 0)) return;
         for (int i = 0; i < steps; ++i) {
             const At<L::NS> st(i);
             const At<1> one(i);
-            if (Outputs && L::NQ == 1 && !pairs(i)) return;
+            if (Outputs && L::NQ == 1 && !pairs(leader, i)) return;
+#pragma unroll 1
             for (int half = 0; half < 2; ++half) {
                 const At<L::NB> pb(2 * i + half);
-                if (!wait(s, s.parts_full[pb.buf], pb.full)) return;
-                if (half == 0 && (!wait(s, s.v_full[st.buf], st.full) || !wait(s, s.u_empty, one.free))) return;
+                if (!wait_warp(s, s.parts_full[pb.buf], pb.full)) return;
+                if (half == 0 && (!wait_warp(s, s.v_full[st.buf], st.full) || !wait_warp(s, s.u_empty, one.free))) return;
                 tc::tc_fence_after_sync();
                 const Operand v{v_tile(st.buf) + half * (PANEL / 2), PANEL};
                 // the small parts first
+#pragma unroll 1
                 for (int t = 2; t >= 0; --t) {
                     const Operand k{parts(pb.buf) + t * L::PART, DK == 64 ? 0 : PANEL / 2};      // (64 lanes: the rest repeats them)
-                    product<true, true, DV, 64>(s.tmem + L::U, k, v, half || t != 2);
+                    product<true, true, DV, 64>(leader, s.tmem + L::U, k, v, half || t != 2);
                 }
-                tc::mma_commit(&s.parts_empty[pb.buf]);
+                commit(leader, &s.parts_empty[pb.buf]);
             }
-            tc::mma_commit(&s.u_full);
+            commit(leader, &s.u_full);
             if constexpr (Outputs) {
-                if (!wait(s, s.s_full, one.full) || !wait(s, s.o_empty, one.free)) return;
+                if (!wait_warp(s, s.s_full, one.full) || !wait_warp(s, s.o_empty, one.free)) return;
                 tc::tc_fence_after_sync();
                 const Operand q{q_tile(st.buf), PANEL};
-                product<false, true, DV, DK>(s.tmem + L::INTER, q, Operand{state(1), DK * 128}, false);
-                product<false, true, DV, DK>(s.tmem + L::INTER, q, Operand{state(0), DK * 128}, true);
-                tc::mma_commit(&s.q_empty[st.buf]);
-                tc::mma_commit(&s.s_empty);
-                if (L::NQ == 2 && i + 1 < steps && !pairs(i + 1)) return;
+#pragma unroll 1
+                for (int part = 1; part >= 0; --part) product<false, true, DV, DK>(leader, s.tmem + L::INTER, q, Operand{state(part), DK * 128}, part == 0);
+                commit(leader, &s.q_empty[st.buf]);
+                commit(leader, &s.s_empty);
+                if (L::NQ == 2 && i + 1 < steps && !pairs(leader, i + 1)) return;
                 const At<L::NQ> qb(i);
-                if (!wait(s, s.p_full[qb.buf], qb.full)) return;
+                if (!wait_warp(s, s.p_full[qb.buf], qb.full)) return;
                 tc::tc_fence_after_sync();
-                product_ts<true, DV, C>(s.tmem + L::INTRA, s.tmem + qb.buf * 128, Operand{v_tile(st.buf), PANEL}, false);
-                tc::mma_commit(&s.o_full);
+                product_ts<true, DV, C>(leader, s.tmem + L::INTRA, s.tmem + qb.buf * 128, Operand{v_tile(st.buf), PANEL}, false);
+                commit(leader, &s.o_full);
             }
-            tc::mma_commit(&s.v_empty[st.buf]);
+            commit(leader, &s.v_empty[st.buf]);
         }
     }
     // ---- X, warp 1: tiles
@@ -257,7 +260,8 @@ struct Roles {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float start = a.scale * exp2_of(G[j]);
-                to.G[4 * lane + j] = G[j];
+                to.hi[4 * lane + j] = G[j].x;
+                to.lo[4 * lane + j] = G[j].y;
                 to.to_block[4 * lane + j] = ex2_diff(block_end, G[j]);
                 to.weight[4 * lane + j] = Reverse ? start : exp2_diff(end, G[j]);
                 to.from_start[4 * lane + j] = start;
@@ -281,11 +285,12 @@ struct Roles {
                     sts16(v_tile(st.buf) + (c >> 3) * PANEL + r * 128 + (c & 7) * 16, 0u, 0u, 0u, 0u);
                 }
             }
+#pragma unroll 1
             for (int half = 0; half < 2; ++half) {
                 const At<L::NB> pb(2 * i + half);
                 if (!wait_warp(s, s.parts_empty[pb.buf], pb.free)) return false;
                 const uint32_t from = k_tile(st.buf) + half * (PANEL / 2), to = parts(pb.buf);
-#pragma unroll 2
+#pragma unroll 1
                 for (int j = 0; j < 64 * DK / 8 / WG; ++j) {
                     const int e = j * WG + tid, r = e / (DK / 8), ch = e % (DK / 8);
                     const uint32_t off = chunk_at(r, ch & 7);
@@ -296,12 +301,11 @@ struct Roles {
                     uint32_t o[3][4];
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        float x0 = low(in[q]) * f, x1 = high(in[q]) * f;
+                        float2 x = __fmul2_rn(unpack(in[q]), both(f));
 #pragma unroll
                         for (int t = 0; t < 3; ++t) {
-                            o[t][q] = pack(x0, x1);
-                            x0 -= low(o[t][q]);
-                            x1 -= high(o[t][q]);
+                            o[t][q] = pack(x);
+                            if (t < 2) x = rest(x, o[t][q]);
                         }
                     }
 #pragma unroll
@@ -321,63 +325,93 @@ struct Roles {
         const int row = DK == 64 ? tid & 63 : tid, c0 = DK == 64 ? (tid >> 6) * N : 0;
         const uint32_t U = lane_base(s.tmem, tid >> 5) + L::U + c0;
         const long long dense_all = (long long)a.B * a.H * a.Dk * a.Dv;
-        float S[N];
+        const bool wide = a.Dv % 4 == 0;
+        float2 S[N / 2];
         int i = 0;
         for (int it = blockIdx.x; it < p.items; it += gridDim.x) {
             const Item<Reverse> w(a, p, it);
             const long long dense = (long long)w.bh * a.Dk * a.Dv + (long long)row * a.Dv + c0;
             const float *first = p.own_sums ? nullptr : p.segments > 1 ? p.seg_state + w.seg * dense_all : p.first;
+            if (first && row >= a.Dk) first = nullptr;
 #pragma unroll
-            for (int j = 0; j < N; ++j) S[j] = first && row < a.Dk && c0 + j < a.Dv ? first[dense + j] : 0.f;
+            for (int j = 0; j < N; j += 4) {
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (first) {
+                    const float *f = first + dense + j;
+                    if (wide) {
+                        if (c0 + j < a.Dv) x = *reinterpret_cast<const float4 *>(f);
+                    } else {
+                        if (c0 + j < a.Dv) x.x = f[0];
+                        if (c0 + j + 1 < a.Dv) x.y = f[1];
+                        if (c0 + j + 2 < a.Dv) x.z = f[2];
+                        if (c0 + j + 3 < a.Dv) x.w = f[3];
+                    }
+                }
+                S[j / 2] = make_float2(x.x, x.y);
+                S[j / 2 + 1] = make_float2(x.z, x.w);
+            }
             double all = 0.0;
             for (int c = w.begin; c < w.stop; ++c, ++i) {
                 const At<1> one(i);
                 const At<SLOTS> at(i);
-                if (p.states && !p.own_sums) {
-                    uint4 *to = reinterpret_cast<uint4 *>(p.states + ((long long)Item<Reverse>::chunk(p, c) * a.B * a.H + w.bh) * (DK * DV) + row * DV + c0);
-#pragma unroll
-                    for (int j = 0; j < N; j += 8) to[j / 8] = make_uint4(pack(S[j], S[j + 1]), pack(S[j + 2], S[j + 3]), pack(S[j + 4], S[j + 5]), pack(S[j + 6], S[j + 7]));
-                }
-                if constexpr (Outputs) {
+                uint4 *keep = p.states && !p.own_sums ? reinterpret_cast<uint4 *>(p.states + ((long long)Item<Reverse>::chunk(p, c) * a.B * a.H + w.bh) * (DK * DV) + row * DV + c0) : nullptr;
+                if constexpr (Outputs)
                     if (!wait_warp(s, s.s_empty, one.free)) return;
 #pragma unroll
-                    for (int j = 0; j < N; j += 8) {
-                        uint32_t hi[4], lo[4];
+                for (int j = 0; j < N; j += 8) {
+                    uint32_t hi[4], lo[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float x0 = S[j + 2 * e], x1 = S[j + 2 * e + 1];
-                            hi[e] = pack(x0, x1);
-                            lo[e] = pack(x0 - low(hi[e]), x1 - high(hi[e]));
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        hi[e] = pack(S[j / 2 + e]);
+                        if (Outputs) lo[e] = pack(rest(S[j / 2 + e], hi[e]));
+                    }
+                    if (keep) keep[j / 8] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if constexpr (Outputs) {
                         const uint32_t off = (uint32_t)((c0 + j) >> 6) * (DK * 128) + chunk_at(row, ((c0 + j) >> 3) & 7);
                         sts16(state(0) + off, hi[0], hi[1], hi[2], hi[3]);
                         sts16(state(1) + off, lo[0], lo[1], lo[2], lo[3]);
                     }
+                }
+                if constexpr (Outputs) {
                     fence_async();
                     tc::mbar_arrive(&s.s_full);
                 }
                 if (!wait_warp(s, s.g_full[at.buf], at.full)) return;
-                const float whole = slots[at.buf].whole;
-                const float2 end = slots[at.buf].G[C - 1];
+                const float2 whole = both(slots[at.buf].whole);
+                all += (double)slots[at.buf].hi[C - 1] + (double)slots[at.buf].lo[C - 1];
                 tc::mbar_arrive(&s.g_empty[at.buf]);
-                all += (double)end.x + (double)end.y;
                 if (!wait_warp(s, s.u_full, one.full)) return;
                 tc::tc_fence_after_sync();
 #pragma unroll
                 for (int j = 0; j < N; j += 32) {
-                    float u[32];
-                    tmem_load(U + j, u);
+                    float2 u[2][8];
+                    int32_t r[2][16];
+                    tc::tmem_ld16(U + j, r[0]);
+                    tc::tmem_ld16(U + j + 16, r[1]);
+                    tc::tmem_ld_wait();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) S[j + e] = fmaf(whole, S[j + e], u[e]);
+                    for (int e = 0; e < 16; ++e) {
+                        u[e / 8][e % 8] = make_float2(__int_as_float(r[e / 8][e % 8 * 2]), __int_as_float(r[e / 8][e % 8 * 2 + 1]));
+                        S[j / 2 + e] = __ffma2_rn(whole, S[j / 2 + e], u[e / 8][e % 8]);
+                    }
                 }
                 tc::tc_fence_before_sync();
                 tc::mbar_arrive(&s.u_empty);
             }
             float *to = p.own_sums ? p.seg_state + w.seg * dense_all : p.last && w.seg == p.segments - 1 ? p.last : nullptr;
-            if (to) {
+            if (to && row < a.Dk) {
 #pragma unroll
-                for (int j = 0; j < N; ++j)
-                    if (row < a.Dk && c0 + j < a.Dv) to[dense + j] = S[j];
+                for (int j = 0; j < N; j += 4) {
+                    float *f = to + dense + j;
+                    if (wide) {
+                        if (c0 + j < a.Dv) *reinterpret_cast<float4 *>(f) = make_float4(S[j / 2].x, S[j / 2].y, S[j / 2 + 1].x, S[j / 2 + 1].y);
+                    } else {
+                        if (c0 + j < a.Dv) f[0] = S[j / 2].x;
+                        if (c0 + j + 1 < a.Dv) f[1] = S[j / 2].y;
+                        if (c0 + j + 2 < a.Dv) f[2] = S[j / 2 + 1].x;
+                        if (c0 + j + 3 < a.Dv) f[3] = S[j / 2 + 1].y;
+                    }
+                }
             }
             if (p.own_sums && tid == 0) p.seg_log[w.seg * (a.B * a.H) + w.bh] = (float)all;
         }
@@ -391,36 +425,37 @@ struct Roles {
             const At<L::NQ> qb(i);
             if (!wait_warp(s, s.g_full[at.buf], at.full)) return false;
             const Slot &g = slots[at.buf];
-            const float2 G = g.G[tid];
+            const float2 G = make_float2(g.hi[tid], g.lo[tid]);
             const uint32_t from = lane_base(s.tmem, warp) + qb.buf * 128;
             if (!wait_warp(s, s.pairs_full[qb.buf], qb.full)) return false;
             tc::tc_fence_after_sync();
 #pragma unroll 1
-            for (int sb = 0; sb < 4; ++sb) {
-                uint32_t P[16];
+            for (int s0 = 0; s0 < C; s0 += 16) {
+                const int sb = s0 >> 5;
+                uint32_t P[8];
                 if (sb > warp) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) P[j] = 0u;
+                    for (int j = 0; j < 8; ++j) P[j] = 0u;
                 } else {
-                    float x[32];
-                    tmem_load(from + sb * 32, x);
+                    float2 x[8];
+                    tmem_load(from + s0, x);
                     if (sb < warp) {
-                        const float r = a.scale * ex2_diff(G, g.G[sb * 32 + 31]);
+                        const float2 r = both(a.scale * ex2_diff(G, make_float2(g.hi[s0 | 31], g.lo[s0 | 31])));
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            const float4 f = *reinterpret_cast<const float4 *>(&g.to_block[sb * 32 + j]);
-                            P[j / 2] = pack(x[j] * (r * f.x), x[j + 1] * (r * f.y));
-                            P[j / 2 + 1] = pack(x[j + 2] * (r * f.z), x[j + 3] * (r * f.w));
-                        }
+                        for (int j = 0; j < 8; ++j) P[j] = pack(__fmul2_rn(x[j], __fmul2_rn(r, *reinterpret_cast<const float2 *>(&g.to_block[s0 + 2 * j]))));
                     } else {
+                        const int last = lane - (s0 & 31);
+                        const float2 minus = both(-1.f);
 #pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            const float w0 = a.scale * ex2_diff(G, g.G[sb * 32 + j]), w1 = a.scale * ex2_diff(G, g.G[sb * 32 + j + 1]);
-                            P[j / 2] = pack(j <= lane ? x[j] * w0 : 0.f, j + 1 <= lane ? x[j + 1] * w1 : 0.f);
+                        for (int j = 0; j < 8; ++j) {
+                            const float2 d = __fadd2_rn(__ffma2_rn(*reinterpret_cast<const float2 *>(&g.hi[s0 + 2 * j]), minus, both(G.x)),
+                                                        __ffma2_rn(*reinterpret_cast<const float2 *>(&g.lo[s0 + 2 * j]), minus, both(G.y)));
+                            const float2 v = __fmul2_rn(x[j], __fmul2_rn(both(a.scale), make_float2(ex2(d.x), ex2(d.y))));
+                            P[j] = pack(2 * j <= last ? v.x : 0.f, 2 * j + 1 <= last ? v.y : 0.f);
                         }
                     }
                 }
-                tmem_st16(from + sb * 16, P);       // columns that this warp has read already
+                tmem_st8(from + s0 / 2, P);       // columns that this warp has read already
             }
             tc::tmem_st_wait();
             tc::tc_fence_before_sync();
@@ -445,32 +480,50 @@ struct Roles {
                 if (!wait_warp(s, s.g_full[g.buf], g.full) || !wait_warp(s, s.o_full, one.full)) return;
                 tc::tc_fence_after_sync();
                 const float r = slots[g.buf].from_start[row];
-                bf16 *to = out + (long long)t0 * a.out.ts;
-#pragma unroll 1
-                for (int j = 0; j < DV; j += 32) {
-                    float x[32], y[32];
-                    tmem_load(from + L::INTRA + j, x);
-                    tmem_load(from + L::INTER + j, y);
-                    bool odd = false;
+                // out of tensor memory first, so that the next chunk's products can begin
+                uint32_t y[DV / 2];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        odd |= !isfinite(x[e]);
-                        y[e] *= r;
+                for (int j = 0; j < DV; j += 16) {
+                    float2 intra[8], inter[8];
+                    int32_t u[2][16];
+                    tc::tmem_ld16(from + L::INTRA + j, u[0]);
+                    tc::tmem_ld16(from + L::INTER + j, u[1]);
+                    tc::tmem_ld_wait();
+                    float2 odd = both(0.f);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        intra[e] = make_float2(__int_as_float(u[0][2 * e]), __int_as_float(u[0][2 * e + 1]));
+                        inter[e] = make_float2(__int_as_float(u[1][2 * e]), __int_as_float(u[1][2 * e + 1]));
+                        odd = __ffma2_rn(intra[e], both(0.f), odd);
                     }
-                    if (odd && row < tokens) {
-                        float z[32];
+                    if (!(odd.x + odd.y == 0.f) && row < tokens) {      // NaN: not all are finite
+                        float z[16];
                         again(z, w.b, w.h, t0, row, j, slots[g.buf]);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) x[e] = z[e];
+                        for (int e = 0; e < 8; ++e) intra[e] = make_float2(z[2 * e], z[2 * e + 1]);
                     }
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) x[e] = row < tokens ? x[e] + y[e] : 0.f;
-                    if (row < all) store_row(to, x, j, a.Dv, vec);
                     __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[j / 2 + e] = pack(__ffma2_rn(inter[e], both(r), intra[e]));
                 }
                 tc::tc_fence_before_sync();
                 tc::mbar_arrive(&s.o_empty);
                 tc::mbar_arrive(&s.g_empty[g.buf]);
+                bf16 *to = out + (long long)t0 * a.out.ts;
+                if (row < all) {
+#pragma unroll
+                    for (int j = 0; j < DV; j += 8) {
+                        const uint4 v = row < tokens ? make_uint4(y[j / 2], y[j / 2 + 1], y[j / 2 + 2], y[j / 2 + 3]) : make_uint4(0u, 0u, 0u, 0u);
+                        if (vec) {
+                            if (j < a.Dv) *reinterpret_cast<uint4 *>(to + j) = v;
+                        } else {
+                            const uint32_t q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (j + e < a.Dv) to[j + e] = __ushort_as_bfloat16((unsigned short)(q[e / 2] >> (e & 1) * 16));
+                        }
+                    }
+                }
             }
             for (int c = w.stop; c < w.end; ++c)               // behind the sequence
                 if (c * C + row < a.T)
@@ -483,12 +536,12 @@ struct Roles {
         const bf16 *q = static_cast<const bf16 *>(a.q.p) + at(a.q, b, h / p.share) + (long long)(t0 + row) * a.q.ts;
         const bf16 *k = static_cast<const bf16 *>(a.k.p) + at(a.k, b, h / p.share) + (long long)t0 * a.k.ts;
         const bf16 *v = static_cast<const bf16 *>(a.v.p) + at(a.v, b, h) + (long long)t0 * a.v.ts + j;
-        for (int e = 0; e < 32; ++e) x[e] = 0.f;
+        for (int e = 0; e < 16; ++e) x[e] = 0.f;
         for (int t = 0; t <= row; ++t) {
             float f = 0.f;
             for (int d = 0; d < a.Dk; ++d) f = fmaf(seq::to_f(q[d]), seq::to_f(k[t * a.k.ts + d]), f);
-            f *= a.scale * ex2_diff(g.G[row], g.G[t]);
-            for (int e = 0; e < 32; ++e)
+            f *= a.scale * ex2_diff(make_float2(g.hi[row], g.lo[row]), make_float2(g.hi[t], g.lo[t]));
+            for (int e = 0; e < 16; ++e)
                 if (j + e < a.Dv) x[e] = fmaf(f, seq::to_f(v[t * a.v.ts + e]), x[e]);
         }
     }
@@ -544,7 +597,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_walk(const __grid_constant__ qgr
         take_registers<G::X>();
         const int warp = tid >> 5;
         if (warp == 0) {
-            if (tid == 0) r.issue();
+            r.issue();
         } else if (warp == 1) {
             if (tid == 32) r.fetch();
         } else if (warp == 2) {

@@ -199,14 +199,15 @@ __global__ void __launch_bounds__(THREADS) k_states_tc(const __grid_constant__ q
         fence_async();
         tc::tc_fence_before_sync();
         __syncthreads();
-        if (tid == 0) {
+        if (tid < 32) {
+            const uint32_t leader = elect();
             tc::tc_fence_after_sync();
             const Operand v{v_raw + (uint32_t)(c & 1) * VT, PANEL};
             for (int t = 2; t >= 0; --t) {
                 const Operand k{parts + (uint32_t)t * KT, DK == 64 ? 0 : PANEL};
-                product<true, true, DV, C>(s.tmem, k, v, t != 2);
+                product<true, true, DV, C>(leader, s.tmem, k, v, t != 2);
             }
-            tc::mma_commit(&s.bar[0]);
+            commit(leader, &s.bar[0]);
         }
         if (c + 1 < stop) {
             fetch(c + 1);
@@ -277,10 +278,11 @@ __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant
     cp_wait<1>();
     fence_async();
     sum_decays(s, g, tid);
-    if (tid == 0) {
+    if (tid < 32) {
+        const uint32_t leader = elect();
         tc::tc_fence_after_sync();
-        product<false, false, C, DK>(s.tmem, Operand{q_t, PANEL}, Operand{k_t, PANEL}, false);
-        tc::mma_commit(&s.bar[0]);
+        product<false, false, C, DK>(leader, s.tmem, Operand{q_t, PANEL}, Operand{k_t, PANEL}, false);
+        commit(leader, &s.bar[0]);
     }
     // Blocks of 32 x 32 pairs.  Below the diagonal 2^(G_t - G_s) is a product of two factors, both at most 1: from s to the end of
     // its block and from there to t.
@@ -319,10 +321,11 @@ __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant
     fence_async();
     tc::tc_fence_before_sync();
     __syncthreads();                                    // every sum of q k^T has been read, the state is there
-    if (carried && tid == 0) {
+    if (carried && tid < 32) {
+        const uint32_t leader = elect();
         tc::tc_fence_after_sync();
-        product<false, true, DV, DK>(s.tmem + 128, Operand{q_t, PANEL}, Operand{k_t, DK * 128}, false);
-        tc::mma_commit(&s.bar[1]);
+        product<false, true, DV, DK>(leader, s.tmem + 128, Operand{q_t, PANEL}, Operand{k_t, DK * 128}, false);
+        commit(leader, &s.bar[1]);
     }
     tc::tc_fence_after_sync();
     tmem_store(base + half * 32, P);
@@ -339,10 +342,11 @@ __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant
     }
     tc::tc_fence_before_sync();
     __syncthreads();
-    if (tid == 0) {
+    if (tid < 32) {
+        const uint32_t leader = elect();
         tc::tc_fence_after_sync();
-        product_ts<true, DV, C>(s.tmem + 128, s.tmem, Operand{v_t, PANEL}, false);
-        tc::mma_commit(&s.bar[2]);
+        product_ts<true, DV, C>(leader, s.tmem + 128, s.tmem, Operand{v_t, PANEL}, false);
+        commit(leader, &s.bar[2]);
     }
     await(s, 2, 0);
     float x[HALF];
@@ -493,22 +497,24 @@ __global__ void __launch_bounds__(THREADS) k_gradients_tc(const __grid_constant_
     cp_wait<1>();
     fence_async();
     sum_decays(s, g, tid);
-    if (tid == 0) {
+    if (tid < 32) {
+        const uint32_t leader = elect();
         tc::tc_fence_after_sync();
-        product<false, false, C, DK>(tm, k, q, false);
-        product<false, false, C, DV>(tm + 128, v, o, false);
-        tc::mma_commit(&s.bar[0]);
+        product<false, false, C, DK>(leader, tm, k, q, false);
+        product<false, false, C, DV>(leader, tm + 128, v, o, false);
+        commit(leader, &s.bar[0]);
     }
     // from the start of t's block of 32 to t
     if (tid < C) s.f[tid] = tid < 32 ? ex2(s.G[tid].x + s.G[tid].y) : ex2_diff(s.G[tid], s.G[(tid & ~31) - 1]);
     cp_wait<0>();
     fence_async();
     __syncthreads();
-    if (tid == 0) {
+    if (tid < 32) {
+        const uint32_t leader = elect();
         tc::tc_fence_after_sync();
-        product<false, false, DK, DV>(tm + 256, v, dS, false);
-        product<false, false, DK, DV>(tm + 384, o, S, false);
-        tc::mma_commit(&s.bar[1]);
+        product<false, false, DK, DV>(leader, tm + 256, v, dS, false);
+        product<false, false, DK, DV>(leader, tm + 384, o, S, false);
+        commit(leader, &s.bar[1]);
     }
     await(s, 0, 0);
     await(s, 1, 0);
@@ -580,13 +586,14 @@ __global__ void __launch_bounds__(THREADS) k_gradients_tc(const __grid_constant_
     tc::tmem_st_wait();
     tc::tc_fence_before_sync();
     __syncthreads();                                  // the pairs' sums have been read, E^T and the scaled sums are there
-    if (tid == 0) {
+    if (tid < 32) {
+        const uint32_t leader = elect();
         tc::tc_fence_after_sync();
-        product<false, true, DV, DK>(tm + 128, k, dS, false);
-        tc::mma_commit(&s.bar[2]);
-        product<false, true, DK, C>(tm + 256, E, q, true);
-        product<true, true, DK, C>(tm + 384, E, k, true);
-        tc::mma_commit(&s.bar[3]);
+        product<false, true, DV, DK>(leader, tm + 128, k, dS, false);
+        commit(leader, &s.bar[2]);
+        product<false, true, DK, C>(leader, tm + 256, E, q, true);
+        product<true, true, DK, C>(leader, tm + 384, E, k, true);
+        commit(leader, &s.bar[3]);
     }
     tc::tc_fence_after_sync();
     tmem_store(base + half * 32, P);
@@ -609,10 +616,11 @@ __global__ void __launch_bounds__(THREADS) k_gradients_tc(const __grid_constant_
     tc::tmem_st_wait();
     tc::tc_fence_before_sync();
     __syncthreads();
-    if (tid == 0) {
+    if (tid < 32) {
+        const uint32_t leader = elect();
         tc::tc_fence_after_sync();
-        product_ts<true, DV, C>(tm + 128, tm, o, true);
-        tc::mma_commit(&s.bar[2]);
+        product_ts<true, DV, C>(leader, tm + 128, tm, o, true);
+        commit(leader, &s.bar[2]);
     }
     if (tid < all) {
         double x = d;

@@ -33,54 +33,97 @@ struct Operand {                        // a tile, `panel` bytes from 64 columns
     uint32_t at;
     int panel;
 };
-// Low word of the descriptor for K = 16 j .. 16 j + 15.  K in the columns: 32 bytes a step, four steps a panel.  K in the rows:
-// 2048 bytes (sixteen rows) a step, and the descriptor's leading distance is that between panels.
+// Low word of the descriptor, and what K = 16 j .. 16 j + 15 adds to it (16-byte units; addresses below 2^18 never carry out of the
+// field).  K in the columns: 32 bytes a step, four steps a panel.  K in the rows: 2048 bytes (sixteen rows) a step, and the
+// descriptor's leading distance is that between panels.
 template <bool KRows>
-__device__ __forceinline__ uint32_t desc_lo(const Operand &o, int j) {
-    if constexpr (KRows)
-        return (((o.at + j * 2048) & 0x3FFFFu) >> 4) | ((uint32_t)o.panel >> 4 << 16);
-    else
-        return (((o.at + (j >> 2) * o.panel + (j & 3) * 32) & 0x3FFFFu) >> 4) | (1u << 16);
+__device__ __forceinline__ uint32_t desc_lo(const Operand &o) {
+    return ((o.at & 0x3FFFFu) >> 4) | (KRows ? (uint32_t)o.panel >> 4 << 16 : 1u << 16);
+}
+template <bool KRows>
+__device__ __forceinline__ uint32_t desc_step(const Operand &o, int j) {
+    return KRows ? j * (2048 >> 4) : (j >> 2) * (o.panel >> 4) + (j & 3) * (32 >> 4);
 }
 // D fp32, A and B bf16, M = 128
 __host__ __device__ constexpr uint32_t idesc(int N, bool a_rows, bool b_rows) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((a_rows ? 1u : 0u) << 15) | ((b_rows ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-__device__ __forceinline__ void mma(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t id, uint32_t accumulate) {
+// Products and their commits are issued by one lane of a warp that stays together: operands of tcgen05.mma are warp-uniform
+// registers, and in a branch of one thread every one of them costs a move from an ordinary register (about 110 cycles an
+// instruction then, 128 x 64 x 16).
+__device__ __forceinline__ uint32_t elect() {
+    uint32_t r;
     asm volatile(
         "{\n"
         ".reg .pred p;\n"
+        "elect.sync _|p, 0xffffffff;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void mma(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p, e;\n"
         ".reg .b64 da, db;\n"
         "mov.b64 da, {%1, %5};\n"
         "mov.b64 db, {%2, %5};\n"
         "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n"
+        "setp.ne.b32 e, %6, 0;\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n"
         "}\n" ::"r"(d),
-        "r"(a_lo), "r"(b_lo), "r"(id), "r"(accumulate), "n"(DESC_HI)
+        "r"(a_lo), "r"(b_lo), "r"(id), "r"(accumulate), "n"(DESC_HI), "r"(leader)
         : "memory");
 }
 // A from tensor memory: lane i is row i, a column holds two neighbouring K, sixteen K are eight columns
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t id, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t id, uint32_t accumulate) {
     asm volatile(
         "{\n"
-        ".reg .pred p;\n"
+        ".reg .pred p, e;\n"
         ".reg .b64 db;\n"
         "mov.b64 db, {%2, %5};\n"
         "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n"
+        "setp.ne.b32 e, %6, 0;\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n"
         "}\n" ::"r"(d),
-        "r"(a), "r"(b_lo), "r"(id), "r"(accumulate), "n"(DESC_HI)
+        "r"(a), "r"(b_lo), "r"(id), "r"(accumulate), "n"(DESC_HI), "r"(leader)
         : "memory");
 }
+__device__ __forceinline__ void commit(uint32_t leader, uint64_t *bar) {
+    asm volatile(
+        "{\n"
+        ".reg .pred e;\n"
+        "setp.ne.b32 e, %1, 0;\n"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+        "}\n" ::"r"(tc::smem_u32(bar)),
+        "r"(leader)
+        : "memory");
+}
+// (Loops over 64 K, four instructions each: warps that do different things share one small instruction cache.)
 template <bool ARows, bool BRows, int N, int K>
-__device__ __forceinline__ void product(uint32_t d, const Operand &a, const Operand &b, bool add) {
+__device__ __forceinline__ void product(uint32_t leader, uint32_t d, const Operand &a, const Operand &b, bool add) {
+    uint32_t a0 = desc_lo<ARows>(a), b0 = desc_lo<BRows>(b), more = add;
+#pragma unroll 1
+    for (int p = 0; p < K / 64; ++p) {
 #pragma unroll
-    for (int j = 0; j < K / 16; ++j) mma(d, desc_lo<ARows>(a, j), desc_lo<BRows>(b, j), idesc(N, ARows, BRows), (add || j) ? 1u : 0u);
+        for (int j = 0; j < 4; ++j) mma(leader, d, a0 + desc_step<ARows>(a, j), b0 + desc_step<BRows>(b, j), idesc(N, ARows, BRows), j ? 1u : more);
+        a0 += desc_step<ARows>(a, 4);
+        b0 += desc_step<BRows>(b, 4);
+        more = 1;
+    }
 }
 template <bool BRows, int N, int K>
-__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, const Operand &b, bool add) {
+__device__ __forceinline__ void product_ts(uint32_t leader, uint32_t d, uint32_t a, const Operand &b, bool add) {
+    uint32_t b0 = desc_lo<BRows>(b), more = add;
+#pragma unroll 1
+    for (int p = 0; p < K / 64; ++p) {
 #pragma unroll
-    for (int j = 0; j < K / 16; ++j) mma_ts(d, a + j * 8, desc_lo<BRows>(b, j), idesc(N, false, BRows), (add || j) ? 1u : 0u);
+        for (int j = 0; j < 4; ++j) mma_ts(leader, d, a + j * 8, b0 + desc_step<BRows>(b, j), idesc(N, false, BRows), j ? 1u : more);
+        a += 32;
+        b0 += desc_step<BRows>(b, 4);
+        more = 1;
+    }
 }
 
 __device__ __forceinline__ uint32_t lane_base(uint32_t tmem, int warp) { return tmem + ((uint32_t)((warp & 3) * 32) << 16); }
@@ -88,6 +131,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
                  "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
                  "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                 "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
 // Cols / 16 groups of sixteen columns
@@ -99,6 +147,13 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, float (&v)[Cols]) {
     tc::tmem_ld_wait();
 #pragma unroll
     for (int i = 0; i < Cols; ++i) v[i] = __int_as_float(r[i / 16][i % 16]);
+}
+__device__ __forceinline__ void tmem_load(uint32_t taddr, float2 (&v)[8]) {
+    int32_t r[16];
+    tc::tmem_ld16(taddr, r);
+    tc::tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = make_float2(__int_as_float(r[2 * i]), __int_as_float(r[2 * i + 1]));
 }
 template <int Cols>
 __device__ __forceinline__ void tmem_store(uint32_t taddr, const uint32_t (&v)[Cols]) {
@@ -119,6 +174,11 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 }
 __device__ __forceinline__ float low(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float high(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+__device__ __forceinline__ uint32_t pack(float2 x) { return pack(x.x, x.y); }
+__device__ __forceinline__ float2 unpack(uint32_t x) { return make_float2(low(x), high(x)); }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+// x minus what its rounding to bf16 keeps (exact)
+__device__ __forceinline__ float2 rest(float2 x, uint32_t packed) { return __ffma2_rn(unpack(packed), make_float2(-1.f, -1.f), x); }
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
