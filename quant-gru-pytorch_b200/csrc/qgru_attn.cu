@@ -136,16 +136,27 @@ __global__ void __launch_bounds__(THREADS) k_states(const __grid_constant__ qgru
     }
 }
 
-// The segments' own sums become the states that they start from.
-__global__ void k_scan_segments(float *seg_state, const float *seg_log, const float *first, int segments, long long size, int per_head) {
+// The segments' own sums become the states that they start from.  A thread per element; eight segments' sums are in flight.
+__global__ void __launch_bounds__(128) k_scan_segments(float *seg_state, const float *seg_log, const float *first, int segments, long long size, int per_head) {
+    constexpr int AHEAD = 8;
     const long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x;
     if (e >= size) return;
     const int heads = (int)(size / per_head), bh = (int)(e / per_head);
     float s = first ? first[e] : 0.f;
-    for (int g = 0; g < segments; ++g) {
-        const float own = seg_state[g * size + e], keep = exp2f(seg_log[g * heads + bh]);
-        seg_state[g * size + e] = s;
-        s = fmaf(keep, s, own);
+    for (int g0 = 0; g0 < segments; g0 += AHEAD) {
+        float own[AHEAD], log[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int g = min(g0 + j, segments - 1);
+            own[j] = seg_state[g * size + e];
+            log[j] = seg_log[g * heads + bh];
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            if (g0 + j >= segments) break;
+            seg_state[(g0 + j) * size + e] = s;
+            s = fmaf(exp2f(log[j]), s, own[j]);
+        }
     }
 }
 
@@ -558,7 +569,7 @@ int sum_groups(const qgru_attention &a, const float *dq, const float *dk, cudaSt
 int scan_segments(const qgru_attention &a, const Cut &c, bool reverse, char *seg, cudaStream_t st) {
     float *s = reinterpret_cast<float *>(seg);
     const long long n = (long long)state_elems(a);
-    k_scan_segments<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(s, s + c.segments * n, reverse ? a.dstate : a.state0, c.segments, n, a.Dk * a.Dv);
+    k_scan_segments<<<(unsigned)((n + 127) / 128), 128, 0, st>>>(s, s + c.segments * n, reverse ? a.dstate : a.state0, c.segments, n, a.Dk * a.Dv);
     SEQ_CK(cudaGetLastError());
     return QGRU_OK;
 }

@@ -29,10 +29,11 @@ __device__ __forceinline__ int valid_tokens(const qgru_attention &a, int b) {
 
 // One token's decay, base 2.  A running sum over a chunk reaches 2^14 at the most and is kept as two floats, so that the
 // difference of two of them is as exact as the difference itself: G_t - G_s = (hi_t - hi_s) + (lo_t - lo_s).
-__device__ __forceinline__ double decay_log2(const qgru_attention &a, long long at) {
-    const double g = (double)seq::load_f(a.decay.p, at, a.decay_bf16) * 1.4426950408889634074;
+__device__ __forceinline__ double decay_log2(float x) {
+    const double g = (double)x * 1.4426950408889634074;
     return g < LOWEST ? LOWEST : g;       // (NaN stays)
 }
+__device__ __forceinline__ double decay_log2(const qgru_attention &a, long long at) { return decay_log2(seq::load_f(a.decay.p, at, a.decay_bf16)); }
 __device__ __forceinline__ float2 two_floats(double x) {
     const float hi = (float)x;
     return make_float2(hi, (float)(x - (double)hi));

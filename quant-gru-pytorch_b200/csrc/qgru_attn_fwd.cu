@@ -7,7 +7,7 @@
 //   S  keeps the state in fp32 registers: S' = 2^G_C S + (w k)^T v, and puts it, as two bf16 parts (16 bits), beside q
 //   P  weighs the pairs of tokens: q k^T out of tensor memory, times 2^(G_t - G_s), into it again as bf16, the operand of P v
 //   O  out = 2^G_t q S + P v: out of tensor memory, into the output
-//   X  one warp each: issues the products, fetches tiles by TMA, sums the decays up
+//   X  a warp issues the products, one fetches tiles by TMA, two sum the decays up
 // In the order of the products the chunk's part of the state comes first, since the next chunk's outputs wait for it.
 //
 // What is rounded to bf16 on the way: P alone, once, as the output is in the end.
@@ -45,6 +45,7 @@ struct Slot {
     float from_start[C];                    // scale 2^G_t
     float whole;
     float pad[3];
+    __device__ __forceinline__ float2 G(int t) const { return make_float2(hi[t], lo[t]); }
 };
 
 template <int DK, int DV, bool Outputs>
@@ -102,10 +103,26 @@ struct Item {
     __device__ __forceinline__ int tokens(int chunk) const { return min(n - chunk * C, C); }
 };
 
+// A wait is one instruction that sleeps until the phase is over, most of the time: code and instructions of twenty warps that poll would
+// cost the others more than anything else here (the SM's instruction cache holds about what one step of all of them takes).
+__device__ __forceinline__ bool over(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(100000u)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ bool wait(Ctl &s, uint64_t &bar, uint32_t parity) {
-    if (tc::mbar_try_wait(&bar, parity)) return true;
+    const uint32_t at = tc::smem_u32(&bar);
+    if (over(at, parity)) return true;
     const long long t0 = clock64();
-    while (!tc::mbar_try_wait(&bar, parity)) {
+    while (!over(at, parity)) {
         if (s.failed) return false;
         if (clock64() - t0 > WAIT_BUDGET) {
             s.failed = 1;
@@ -231,18 +248,28 @@ struct Roles {
             return true;
         });
     }
-    // ---- X, warp 2: decays, four neighbouring tokens a lane
+    // ---- X, warps 2 and 3, every second chunk each: decays, four neighbouring tokens a lane
     __device__ __forceinline__ void decays() const {
         const int lane = tid & 31;
         each([&](const Item<Reverse> &w, int chunk, int i) {
+            if ((i & 1) != ((tid >> 5) & 1)) return true;
             const At<SLOTS> at(i);
             const int tokens = w.tokens(chunk);
             const long long base = w.b * a.decay.bs + w.h * a.decay.hs + (long long)chunk * C * a.decay.ts;
+            float f[4];
             double g[4], sum = 0.0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) g[j] = 4 * lane + j < tokens ? decay_log2(a, base + (4 * lane + j) * a.decay.ts) : 0.0;
+            for (int j = 0; j < 4; ++j) {
+                f[j] = 0.f;
+                if (4 * lane + j < tokens) {
+                    if (a.decay_bf16)
+                        f[j] = seq::to_f(static_cast<const bf16 *>(a.decay.p)[base + (4 * lane + j) * a.decay.ts]);
+                    else
+                        f[j] = static_cast<const float *>(a.decay.p)[base + (4 * lane + j) * a.decay.ts];
+                }
+            }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) g[j] = sum += g[j];
+            for (int j = 0; j < 4; ++j) g[j] = sum += decay_log2(f[j]);
             double before = sum;
             for (int o = 1; o < 32; o <<= 1) {
                 const double u = __shfl_up_sync(0xffffffffu, before, o);
@@ -250,21 +277,23 @@ struct Roles {
             }
             before = __shfl_up_sync(0xffffffffu, before, 1);
             if (lane == 0) before = 0.0;
-            float2 G[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) G[j] = two_floats(before + g[j]);
-            const float2 block_end = make_float2(__shfl_sync(0xffffffffu, G[3].x, lane | 7), __shfl_sync(0xffffffffu, G[3].y, lane | 7));
-            const float2 end = make_float2(__shfl_sync(0xffffffffu, G[3].x, 31), __shfl_sync(0xffffffffu, G[3].y, 31));
             if (!wait_warp(s, s.g_empty[at.buf], at.free)) return false;
             Slot &to = slots[at.buf];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float start = a.scale * exp2_of(G[j]);
-                to.hi[4 * lane + j] = G[j].x;
-                to.lo[4 * lane + j] = G[j].y;
-                to.to_block[4 * lane + j] = ex2_diff(block_end, G[j]);
-                to.weight[4 * lane + j] = Reverse ? start : exp2_diff(end, G[j]);
-                to.from_start[4 * lane + j] = start;
+                const float2 G = two_floats(before + g[j]);
+                to.hi[4 * lane + j] = G.x;
+                to.lo[4 * lane + j] = G.y;
+            }
+            __syncwarp();
+            const float2 end = to.G(C - 1);
+#pragma unroll 1
+            for (int t = lane; t < C; t += 32) {
+                const float2 G = to.G(t);
+                const float start = a.scale * exp2_of(G);
+                to.to_block[t] = ex2_diff(to.G(t | 31), G);
+                to.weight[t] = Reverse ? start : exp2_diff(end, G);
+                to.from_start[t] = start;
             }
             if (lane == 0) to.whole = exp2_of(end);
             tc::mbar_arrive(&s.g_full[at.buf]);
@@ -295,8 +324,8 @@ struct Roles {
                     const int e = j * WG + tid, r = e / (DK / 8), ch = e % (DK / 8);
                     const uint32_t off = chunk_at(r, ch & 7);
                     const uint4 u = lds16(from + (ch >> 3) * PANEL + off);
-                    const bool on = half * 64 + r < tokens;
-                    const uint32_t in[4] = {on ? u.x : 0u, on ? u.y : 0u, on ? u.z : 0u, on ? u.w : 0u};
+                    uint32_t in[4] = {u.x, u.y, u.z, u.w};
+                    if (half * 64 + r >= tokens) in[0] = in[1] = in[2] = in[3] = 0u;
                     const float f = slots[at.buf].weight[half * 64 + r];
                     uint32_t o[3][4];
 #pragma unroll
@@ -425,7 +454,7 @@ struct Roles {
             const At<L::NQ> qb(i);
             if (!wait_warp(s, s.g_full[at.buf], at.full)) return false;
             const Slot &g = slots[at.buf];
-            const float2 G = make_float2(g.hi[tid], g.lo[tid]);
+            const float2 G = g.G(tid);
             const uint32_t from = lane_base(s.tmem, warp) + qb.buf * 128;
             if (!wait_warp(s, s.pairs_full[qb.buf], qb.full)) return false;
             tc::tc_fence_after_sync();
@@ -440,7 +469,7 @@ struct Roles {
                     float2 x[8];
                     tmem_load(from + s0, x);
                     if (sb < warp) {
-                        const float2 r = both(a.scale * ex2_diff(G, make_float2(g.hi[s0 | 31], g.lo[s0 | 31])));
+                        const float2 r = both(a.scale * ex2_diff(G, g.G(s0 | 31)));
 #pragma unroll
                         for (int j = 0; j < 8; ++j) P[j] = pack(__fmul2_rn(x[j], __fmul2_rn(r, *reinterpret_cast<const float2 *>(&g.to_block[s0 + 2 * j]))));
                     } else {
@@ -480,9 +509,8 @@ struct Roles {
                 if (!wait_warp(s, s.g_full[g.buf], g.full) || !wait_warp(s, s.o_full, one.full)) return;
                 tc::tc_fence_after_sync();
                 const float r = slots[g.buf].from_start[row];
-                // out of tensor memory first, so that the next chunk's products can begin
-                uint32_t y[DV / 2];
-#pragma unroll
+                bf16 *to = out + (long long)t0 * a.out.ts;
+#pragma unroll 1
                 for (int j = 0; j < DV; j += 16) {
                     float2 intra[8], inter[8];
                     int32_t u[2][16];
@@ -502,28 +530,24 @@ struct Roles {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) intra[e] = make_float2(z[2 * e], z[2 * e + 1]);
                     }
-                    __syncwarp();
+                    uint32_t y[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) y[j / 2 + e] = pack(__ffma2_rn(inter[e], both(r), intra[e]));
+                    for (int e = 0; e < 8; ++e) y[e] = row < tokens ? pack(__ffma2_rn(inter[e], both(r), intra[e])) : 0u;
+                    if (row < all && j < a.Dv) {
+                        if (vec) {
+                            *reinterpret_cast<uint4 *>(to + j) = make_uint4(y[0], y[1], y[2], y[3]);
+                            if (j + 8 < a.Dv) *reinterpret_cast<uint4 *>(to + j + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                if (j + e < a.Dv) to[j + e] = __ushort_as_bfloat16((unsigned short)(y[e / 2] >> (e & 1) * 16));
+                        }
+                    }
+                    __syncwarp();
                 }
                 tc::tc_fence_before_sync();
                 tc::mbar_arrive(&s.o_empty);
                 tc::mbar_arrive(&s.g_empty[g.buf]);
-                bf16 *to = out + (long long)t0 * a.out.ts;
-                if (row < all) {
-#pragma unroll
-                    for (int j = 0; j < DV; j += 8) {
-                        const uint4 v = row < tokens ? make_uint4(y[j / 2], y[j / 2 + 1], y[j / 2 + 2], y[j / 2 + 3]) : make_uint4(0u, 0u, 0u, 0u);
-                        if (vec) {
-                            if (j < a.Dv) *reinterpret_cast<uint4 *>(to + j) = v;
-                        } else {
-                            const uint32_t q[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                if (j + e < a.Dv) to[j + e] = __ushort_as_bfloat16((unsigned short)(q[e / 2] >> (e & 1) * 16));
-                        }
-                    }
-                }
             }
             for (int c = w.stop; c < w.end; ++c)               // behind the sequence
                 if (c * C + row < a.T)
@@ -540,7 +564,7 @@ struct Roles {
         for (int t = 0; t <= row; ++t) {
             float f = 0.f;
             for (int d = 0; d < a.Dk; ++d) f = fmaf(seq::to_f(q[d]), seq::to_f(k[t * a.k.ts + d]), f);
-            f *= a.scale * ex2_diff(make_float2(g.hi[row], g.lo[row]), make_float2(g.hi[t], g.lo[t]));
+            f *= a.scale * ex2_diff(g.G(row), g.G(t));
             for (int e = 0; e < 16; ++e)
                 if (j + e < a.Dv) x[e] = fmaf(f, seq::to_f(v[t * a.v.ts + e]), x[e]);
         }
@@ -600,7 +624,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_walk(const __grid_constant__ qgr
             r.issue();
         } else if (warp == 1) {
             if (tid == 32) r.fetch();
-        } else if (warp == 2) {
+        } else {
             r.decays();
         }
         __syncwarp();
