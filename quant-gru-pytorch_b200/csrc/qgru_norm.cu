@@ -4,7 +4,7 @@
 //     dh = r (dy w - n mean(dy w n)) + (gradient of the stream),  n = h r;   dw = sum over rows of dy n
 //
 // Bytes bound all of them: each tensor is read or written once, with a row in registers between its sum and its output.
-// TPR threads have a row, each N vectors of V neighbouring elements; a warp each up to 1024 columns, a CTA above.
+// TPR threads have a row, each E elements of it in vectors of V neighbours; a warp each up to 1024 columns, a CTA above.
 #include <algorithm>
 #include <type_traits>
 
@@ -16,9 +16,7 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 constexpr int MOST = 32;        // elements of a row per thread; half of it in the largest CTA, whose threads have 64 registers
-template <int TPR>
-constexpr int MOST_OF = TPR == 1024 ? MOST / 2 : MOST;
-constexpr int MAX_COLS = 1024 * MOST_OF<1024>;
+constexpr int MAX_COLS = 1024 * MOST / 2;
 constexpr int WARPS_PER_CTA = 8;
 
 enum Output { PLAIN, ROW8, GIVEN8 };
@@ -65,9 +63,9 @@ __device__ __forceinline__ void load_weights(float (&w)[V], const void *p, int a
     for (int i = 0; i < V; ++i) w[i] = seq::to_f(u.v[i]);
 }
 
-template <class T, class W, int V, int TPR, Output Out>
+template <class T, class W, int V, int TPR, int E, Output Out>
 __global__ void __launch_bounds__(TPR > 32 ? TPR : 32 * WARPS_PER_CTA) k_norm(const __grid_constant__ qgru_norm n) {
-    constexpr int N = MOST_OF<TPR> / V;
+    constexpr int N = E / V;
     __shared__ float part[TPR / 32];
     __shared__ double part_d[TPR / 32];
     const int t = TPR > 32 ? threadIdx.x : threadIdx.x & 31;
@@ -149,18 +147,19 @@ __global__ void __launch_bounds__(TPR > 32 ? TPR : 32 * WARPS_PER_CTA) k_norm(co
     } else {
         // y / max|y| is h w / max|h w|: the root mean square drops out of q.  A quotient within 1e-4 of a border between two
         // steps (its fp32 rounding is below 3e-5) is decided by 64 bits, where h w is exact.
+        constexpr bool EXACT = sizeof(T) == 2 && sizeof(W) == 2;      // two bf16 factors have an exact fp32 product
+        float hw[N][V];
         float top = 0.f, bad = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int at = (i * TPR + t) * V;
-            if (at >= n.cols) continue;
-            float w[V];
-            load_weights<V, W>(w, n.weight, at);
+            float w[V] = {};
+            if (at < n.cols) load_weights<V, W>(w, n.weight, at);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float p = fabsf(h[i][j] * w[j]);
-                top = fmaxf(top, p);
-                if (!isfinite(p)) bad = 1.f;         // (fmaxf drops NaN)
+                hw[i][j] = h[i][j] * w[j];
+                top = fmaxf(top, fabsf(hw[i][j]));
+                bad = fmaf(hw[i][j], 0.f, bad);      // (fmaxf drops NaN)
             }
         }
         top = over_row<TPR>(bad != 0.f ? INFINITY : top, part, [](float p, float q) { return fmaxf(p, q); });
@@ -171,7 +170,7 @@ __global__ void __launch_bounds__(TPR > 32 ? TPR : 32 * WARPS_PER_CTA) k_norm(co
             return;
         }
         double exact_top = (double)top;
-        if constexpr (sizeof(T) == 4 || sizeof(W) == 4) {     // two bf16 factors have an exact product
+        if constexpr (!EXACT) {
             double d = 0.0;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -181,7 +180,7 @@ __global__ void __launch_bounds__(TPR > 32 ? TPR : 32 * WARPS_PER_CTA) k_norm(co
                 load_weights<V, W>(w, n.weight, at);
 #pragma unroll
                 for (int j = 0; j < V; ++j)
-                    if (fabsf(h[i][j] * w[j]) == top) d = fmax(d, fabs((double)h[i][j] * (double)w[j]));
+                    if (fabsf(hw[i][j]) == top) d = fmax(d, fabs((double)h[i][j] * (double)w[j]));
             }
             exact_top = max_over_row<TPR>(d, part_d);
         }
@@ -192,15 +191,23 @@ __global__ void __launch_bounds__(TPR > 32 ? TPR : 32 * WARPS_PER_CTA) k_norm(co
         for (int i = 0; i < N; ++i) {
             const int at = (i * TPR + t) * V;
             if (at >= n.cols) continue;
-            float w[V];
-            load_weights<V, W>(w, n.weight, at);
+            // rounded by adding 1.5 * 2^23, which leaves the integer in the low bits
             Vec<int8_t, V> u;
+            float off = 0.f;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float p = h[i][j] * w[j] * steps;
-                float k = rintf(p);
-                if (!plain_range || 0.5f - fabsf(p - k) < 1e-4f) k = (float)rint((double)h[i][j] * (double)w[j] * 127.0 / exact_top);
-                u.v[j] = (int8_t)__float2int_rn(k);
+                const float p = hw[i][j] * steps, r = __fadd_rn(p, 12582912.f);
+                u.v[j] = (int8_t)__float_as_int(r);
+                off = fmaxf(off, fabsf(p - __fadd_rn(r, -12582912.f)));
+            }
+            if (!plain_range || off > 0.5f - 1e-4f) {
+                float w[V];
+                if constexpr (!EXACT) load_weights<V, W>(w, n.weight, at);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const double exact = EXACT ? (double)hw[i][j] : (double)h[i][j] * (double)w[j];
+                    u.v[j] = (int8_t)__double2int_rn(exact * 127.0 / exact_top);
+                }
             }
             *reinterpret_cast<Vec<int8_t, V> *>(q + at) = u;
         }
@@ -214,63 +221,110 @@ struct Backward {
     float *parts;                   // [CTAs][cols], or null
 };
 
-// Rows in turn; a thread keeps the sums of dw of its columns, which leave once a CTA.
-template <class T, class W, int V, int TPR>
+__device__ __forceinline__ void cp_async16(void *to, const void *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+
+// Rows in turn; a thread keeps the weights of its E columns and the sums of dw, which leave once a CTA.  Whole vectors of the next rows
+// (three of bf16, one of fp32) are on their way into shared memory, where each thread reads back what it has fetched itself;
+// single elements come straight from memory.  51200 x 1024 bf16 with the stream's gradient, 420 MB: 155 us with a warp a row and no row
+// ahead, 123 us with one row ahead in registers, 74 us so (5.7 TB/s).
+constexpr int AHEAD_BYTES = 192;                     // of shared memory a thread
+template <class T, class W, int V, int TPR, int E>
 __global__ void __launch_bounds__(TPR > 32 ? TPR : 32 * WARPS_PER_CTA) k_norm_backward(const __grid_constant__ qgru_norm n, const Backward g) {
-    constexpr int N = MOST_OF<TPR> / V, ROWS = TPR > 32 ? 1 : WARPS_PER_CTA;
-    __shared__ float part[TPR / 32];
-    extern __shared__ float dw_part[];               // [ROWS][cols] where a row is a warp's
+    constexpr int N = E / V, ROWS = TPR > 32 ? 1 : WARPS_PER_CTA;
+    constexpr int STAGES = V > 1 ? AHEAD_BYTES / (3 * E * (int)sizeof(T)) : 1;
+    __shared__ float part[2][TPR / 32];
+    extern __shared__ uint4 smem[];                  // [STAGES][3 N][threads], then [ROWS][cols] sums where a row is a warp's
+    float *dw_part = reinterpret_cast<float *>(smem);
     const int t = TPR > 32 ? threadIdx.x : threadIdx.x & 31, mine = TPR > 32 ? 0 : threadIdx.x >> 5;
-    float dw[N][V];
+    float dw[N][V], w[N][V];
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) dw[i][j] = 0.f;
-    for (long long row = (long long)blockIdx.x * ROWS + mine; row < n.rows; row += (long long)gridDim.x * ROWS) {
-        const T *h = static_cast<const T *>(g.h) + row * g.h_stride, *dy = static_cast<const T *>(g.dy) + row * g.dy_stride;
-        Vec<T, V> u[N], v[N], s[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int at = (i * TPR + t) * V;
-            if (at >= n.cols) continue;
-            u[i] = *reinterpret_cast<const Vec<T, V> *>(h + at);
-            v[i] = *reinterpret_cast<const Vec<T, V> *>(dy + at);
-            if (g.dh) s[i] = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(g.dh) + row * g.dh_stride + at);
+        for (int j = 0; j < V; ++j) {
+            const int at = (i * TPR + t) * V + j;
+            dw[i][j] = 0.f;
+            w[i][j] = at < n.cols ? seq::to_f(static_cast<const W *>(n.weight)[at]) : 0.f;
         }
+    const long long step = (long long)gridDim.x * ROWS;
+    const auto place = [&](int stage, int which, int i) { return smem + ((stage * 3 + which) * N + i) * blockDim.x + threadIdx.x; };
+    const auto row_of = [&](const void *p, long long row, long long stride) { return static_cast<const T *>(p) + row * stride; };
+    const auto fetch = [&](long long row, int stage) {
+        if constexpr (V > 1) {
+            if (row < n.rows) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int at = (i * TPR + t) * V;
+                    if (at >= n.cols) continue;
+                    cp_async16(place(stage, 0, i), row_of(g.h, row, g.h_stride) + at);
+                    cp_async16(place(stage, 1, i), row_of(g.dy, row, g.dy_stride) + at);
+                    if (g.dh) cp_async16(place(stage, 2, i), row_of(g.dh, row, g.dh_stride) + at);
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+    };
+    long long row = (long long)blockIdx.x * ROWS + mine;
+    for (int k = 0; k < STAGES - 1; ++k) fetch(row + k * step, k);
+    int stage = 0;
+    for (int buf = 0; row < n.rows; row += step, buf ^= 1) {
         const float rstd = n.rstd[row];
-        float sum = 0.f;
+        float x[N][V], y[N][V], d[N][V], sum = 0.f;
+        if constexpr (V > 1) {
+            fetch(row + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int at = (i * TPR + t) * V;
-            if (at >= n.cols) continue;
-            float w[V];
-            load_weights<V, W>(w, n.weight, at);
+            Vec<T, V> u, v, s;
+#pragma unroll
+            for (int j = 0; j < V; ++j) u.v[j] = v.v[j] = s.v[j] = seq::from_f<T>(0.f);
+            if (at < n.cols) {
+                if constexpr (V > 1) {
+                    u = *reinterpret_cast<const Vec<T, V> *>(place(stage, 0, i));
+                    v = *reinterpret_cast<const Vec<T, V> *>(place(stage, 1, i));
+                    if (g.dh) s = *reinterpret_cast<const Vec<T, V> *>(place(stage, 2, i));
+                } else {
+                    u.v[0] = row_of(g.h, row, g.h_stride)[at];
+                    v.v[0] = row_of(g.dy, row, g.dy_stride)[at];
+                    if (g.dh) s.v[0] = row_of(g.dh, row, g.dh_stride)[at];
+                }
+            }
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float x = seq::to_f(u[i].v[j]) * rstd, y = seq::to_f(v[i].v[j]);
-                sum = fmaf(y * w[j], x, sum);
-                dw[i][j] = fmaf(y, x, dw[i][j]);
+                x[i][j] = seq::to_f(u.v[j]) * rstd;
+                const float dy = seq::to_f(v.v[j]);
+                dw[i][j] = fmaf(dy, x[i][j], dw[i][j]);
+                y[i][j] = dy * w[i][j];
+                sum = fmaf(y[i][j], x[i][j], sum);
+                d[i][j] = seq::to_f(s.v[j]);
             }
         }
-        sum = over_row<TPR>(sum, part, [](float p, float q) { return p + q; }) / (float)n.cols;
+        if (++stage == STAGES) stage = 0;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if constexpr (TPR > 32) {
+            if ((threadIdx.x & 31) == 0) part[buf][threadIdx.x >> 5] = sum;
+            __syncthreads();
+            sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < TPR / 32; ++k) sum += part[buf][k];
+        }
+        sum /= (float)n.cols;
         T *dx = static_cast<T *>(g.dx) + row * g.dx_stride;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int at = (i * TPR + t) * V;
-            if (at >= n.cols) continue;
-            float w[V];
-            load_weights<V, W>(w, n.weight, at);
             Vec<T, V> o;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float x = seq::to_f(u[i].v[j]) * rstd;
-                float d = rstd * (seq::to_f(v[i].v[j]) * w[j] - x * sum);
-                if (g.dh) d += seq::to_f(s[i].v[j]);
-                o.v[j] = seq::from_f<T>(d);
-            }
-            *reinterpret_cast<Vec<T, V> *>(dx + at) = o;
+            for (int j = 0; j < V; ++j) o.v[j] = seq::from_f<T>(fmaf(rstd, fmaf(-sum, x[i][j], y[i][j]), d[i][j]));
+            if (at < n.cols) *reinterpret_cast<Vec<T, V> *>(dx + at) = o;
         }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
     if (!g.parts) return;
     float *to = g.parts + (long long)blockIdx.x * n.cols;
     if constexpr (TPR > 32) {
@@ -294,28 +348,34 @@ __global__ void __launch_bounds__(TPR > 32 ? TPR : 32 * WARPS_PER_CTA) k_norm_ba
     }
 }
 
-// dw: the CTAs' sums, 32 columns a CTA, eight warps that take every eighth CTA's, in a fixed order.
+// dw: the CTAs' sums, 32 columns a CTA, 32 warps that take every 32nd CTA's, in a fixed order.
 template <class W>
-__global__ void __launch_bounds__(256) k_sum_parts(const float *parts, int count, int cols, W *dw) {
-    __shared__ float part[8][33];
+__global__ void __launch_bounds__(1024) k_sum_parts(const float *parts, int count, int cols, W *dw) {
+    __shared__ float part[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float x = 0.f;
-    if (c < cols)
-        for (int p = warp; p < count; p += 8) x += parts[(long long)p * cols + c];
+    if (c < cols) {
+#pragma unroll 4
+        for (int p = warp; p < count; p += 32) x += parts[(long long)p * cols + c];
+    }
     part[warp][lane] = x;
     __syncthreads();
     if (warp == 0 && c < cols) {
-        for (int w = 1; w < 8; ++w) x += part[w][lane];
+        for (int w = 1; w < 32; ++w) x += part[w][lane];
         dw[c] = seq::from_f<W>(x);
     }
 }
 
 template <class F>
 int by_width(int cols, F f) {
-    if (cols <= 32 * MOST) return f(std::integral_constant<int, 32>());
-    if (cols <= 128 * MOST) return f(std::integral_constant<int, 128>());
-    if (cols <= 256 * MOST) return f(std::integral_constant<int, 256>());
-    return f(std::integral_constant<int, 1024>());
+    const auto with = [&](auto tpr, auto e) -> int { return f(tpr, e); };
+    using std::integral_constant;
+    if (cols <= 32 * MOST / 4) return with(integral_constant<int, 32>(), integral_constant<int, MOST / 4>());
+    if (cols <= 32 * MOST / 2) return with(integral_constant<int, 32>(), integral_constant<int, MOST / 2>());
+    if (cols <= 32 * MOST) return with(integral_constant<int, 32>(), integral_constant<int, MOST>());
+    if (cols <= 128 * MOST) return with(integral_constant<int, 128>(), integral_constant<int, MOST>());
+    if (cols <= 256 * MOST) return with(integral_constant<int, 256>(), integral_constant<int, MOST>());
+    return with(integral_constant<int, 1024>(), integral_constant<int, MOST / 2>());
 }
 // whether vectors of `v` elements of `size` bytes fit all rows of a tensor
 bool fits(const void *p, long long stride, int v, int size, long long rows) {
@@ -324,10 +384,10 @@ bool fits(const void *p, long long stride, int v, int size, long long rows) {
 
 template <class T, class W, int V, Output Out>
 int forward(const qgru_norm &n, cudaStream_t st) {
-    return by_width(n.cols, [&](auto tpr) -> int {
-        constexpr int TPR = tpr.value;
+    return by_width(n.cols, [&](auto tpr, auto e) -> int {
+        constexpr int TPR = tpr.value, E = e.value;
         constexpr int per = TPR > 32 ? 1 : WARPS_PER_CTA;
-        k_norm<T, W, V, TPR, Out><<<(unsigned)((n.rows + per - 1) / per), TPR > 32 ? TPR : 32 * per, 0, st>>>(n);
+        k_norm<T, W, V, TPR, E, Out><<<(unsigned)((n.rows + per - 1) / per), TPR > 32 ? TPR : 32 * per, 0, st>>>(n);
         SEQ_CK(cudaGetLastError());
         return QGRU_OK;
     });
@@ -345,22 +405,42 @@ int forward(const qgru_norm &n, cudaStream_t st) {
     return wide ? forward<T, W, V>(n, st) : forward<T, W, 1>(n, st);
 }
 
-// CTAs of the backward: what is resident at once, each with its sums of dw at the end.
+// Threads of a row of the backward: eight columns each, up to 1024 (sixteen each above 8192 columns), and CTAs: 1024 threads an SM, whose
+// rows and next rows in flight are what its latency takes.
+int threads_of_row(int cols) {
+    int t = 32;
+    while (t < 1024 && t * 8 < cols) t *= 2;
+    return t;
+}
 int ctas(int sms, long long rows, int cols) {
-    const bool warps = cols <= 32 * MOST;
-    const long long units = warps ? (rows + WARPS_PER_CTA - 1) / WARPS_PER_CTA : rows;
-    const int per_sm = warps ? 2 : cols <= 128 * MOST ? 4 : cols <= 256 * MOST ? 2 : 1;
+    const int t = threads_of_row(cols);
+    const long long units = t == 32 ? (rows + WARPS_PER_CTA - 1) / WARPS_PER_CTA : rows;
+    const int per_sm = 1024 / (t == 32 ? 32 * WARPS_PER_CTA : t);
     return (int)std::max<long long>(1, std::min<long long>(units, (long long)sms * per_sm));
 }
 template <class T, class W, int V>
 int backward(const qgru_norm &n, const Backward &g, int grid, cudaStream_t st) {
-    return by_width(n.cols, [&](auto tpr) -> int {
-        constexpr int TPR = tpr.value;
-        const size_t bytes = TPR == 32 && g.parts ? sizeof(float) * WARPS_PER_CTA * n.cols : 0;
-        k_norm_backward<T, W, V, TPR><<<grid, TPR > 32 ? TPR : 32 * WARPS_PER_CTA, bytes, st>>>(n, g);
+    using std::integral_constant;
+    const auto run = [&](auto tpr, auto e) -> int {
+        constexpr int TPR = tpr.value, E = e.value;
+        constexpr int threads = TPR > 32 ? TPR : 32 * WARPS_PER_CTA;
+        const size_t sums = TPR == 32 && g.parts ? sizeof(float) * WARPS_PER_CTA * n.cols : 0, ahead = V > 1 ? (size_t)AHEAD_BYTES * threads : 0;
+        const size_t bytes = std::max(sums, ahead);
+        const auto kernel = k_norm_backward<T, W, V, TPR, E>;
+        if (bytes > 40 * 1024) SEQ_CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        kernel<<<grid, threads, bytes, st>>>(n, g);
         SEQ_CK(cudaGetLastError());
         return QGRU_OK;
-    });
+    };
+    const integral_constant<int, 8> e;
+    switch (threads_of_row(n.cols)) {
+        case 32: return run(integral_constant<int, 32>(), e);
+        case 64: return run(integral_constant<int, 64>(), e);
+        case 128: return run(integral_constant<int, 128>(), e);
+        case 256: return run(integral_constant<int, 256>(), e);
+        case 512: return run(integral_constant<int, 512>(), e);
+        default: return n.cols <= 8192 ? run(integral_constant<int, 1024>(), e) : run(integral_constant<int, 1024>(), integral_constant<int, 16>());
+    }
 }
 template <class T, class W>
 int backward(const qgru_norm &n, const Backward &g, int grid, W *dw, cudaStream_t st) {
@@ -369,7 +449,7 @@ int backward(const qgru_norm &n, const Backward &g, int grid, W *dw, cudaStream_
                       fits(g.dh, g.dh_stride, V, sizeof(T), n.rows) && fits(g.dx, g.dx_stride, V, sizeof(T), n.rows) && fits(n.weight, 0, V, sizeof(W), 1);
     if (const int rc = wide ? backward<T, W, V>(n, g, grid, st) : backward<T, W, 1>(n, g, grid, st)) return rc;
     if (dw) {
-        k_sum_parts<W><<<(n.cols + 31) / 32, 256, 0, st>>>(g.parts, grid, n.cols, dw);
+        k_sum_parts<W><<<(n.cols + 31) / 32, 1024, 0, st>>>(g.parts, grid, n.cols, dw);
         SEQ_CK(cudaGetLastError());
     }
     return QGRU_OK;
