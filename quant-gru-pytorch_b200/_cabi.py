@@ -210,10 +210,17 @@ def check(status, where, handle=None):
         raise QgruError(status, where, detail)
 
 
-def check_seq(status, where):
-    """As check, for the calls without a handle."""
-    if status != QGRU_OK:
-        detail = lib().qgru_seq_last_error().decode()
-        if status == QGRU_ERR_BAD_ARG:
-            raise ValueError(f"{where}: {detail or 'bad argument'}")
-        raise QgruError(status, where, detail)
+
+_seq = None
+
+
+def seq():
+    """The torch binding of the sequence operators (csrc/qgru_seq_torch.cc), loaded once; raises if it is missing."""
+    global _seq
+    if _seq is None:
+        lib()
+        if not os.path.exists(os.path.join(_HERE, "_seq.so")):
+            raise RuntimeError(f"{os.path.join(_HERE, '_seq.so')} is missing: build it with __graft_entry__.build()")
+        from . import _seq as binding
+        _seq = binding
+    return _seq
