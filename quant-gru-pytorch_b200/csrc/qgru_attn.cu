@@ -11,35 +11,48 @@ namespace qgru {
 namespace attn {
 namespace {
 
-constexpr int C = 64, LD = 65, THREADS = 256;
+constexpr int C = 64, THREADS = 256;
+constexpr int TILE = 64 * 64;                   // floats
 using bf16 = __nv_bfloat16;
 
-// 64 x 64 sums of a thread grid of 16 x 16: rows ty + 16 i, columns tx + 16 j.
+// A 64 x 64 tile in shared memory: rows of sixteen 16-byte chunks, chunk c of row r at c ^ (r / 4), so that reading four rows' chunk
+// by each of sixteen threads, or a row's sixteen chunks, meets every bank once.
+__device__ __forceinline__ int idx(int r, int c) { return r * 64 + ((((c >> 2) ^ (r >> 2)) & 15) << 2) + (c & 3); }
+__device__ __forceinline__ float4 quad(const float *t, int r, int c4) { return *reinterpret_cast<const float4 *>(t + r * 64 + (((c4 ^ (r >> 2)) & 15) << 2)); }
+__device__ __forceinline__ float part(const float4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// 64 x 64 sums of a thread grid of 16 x 16: rows 4 ty .. + 3, columns 4 tx .. + 3, neighbouring columns as packed pairs.
 struct Acc {
-    float v[4][4];
+    float2 v[4][2];
     __device__ __forceinline__ void zero() {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[i][j] = 0.f;
+        for (int i = 0; i < 4; ++i) v[i][0] = v[i][1] = make_float2(0.f, 0.f);
     }
 };
-// acc += sum_k A(m, k) B(k, n), element (m, k) of A at m * AM + k * AK
-template <int AM, int AK, int BK, int BN>
+// acc += sum_k A(m, k) B(k, n).  ARows: A's tile has k as its rows, else m; BRows: B's tile has k as its rows, else n.  Four k at a time:
+// eight 16-byte loads for 64 multiply-adds.
+template <bool ARows, bool BRows>
 __device__ __forceinline__ void multiply(Acc &c, const float *A, const float *B, int tid) {
-    const float *a = A + (tid >> 4) * AM, *b = B + (tid & 15) * BN;
-#pragma unroll 4
-    for (int k = 0; k < 64; ++k) {
-        float x[4], y[4];
+    const int ty = tid >> 4, tx = tid & 15;
+#pragma unroll 2
+    for (int k = 0; k < 16; ++k) {
+        float4 x[4], y[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            x[i] = a[16 * i * AM + k * AK];
-            y[i] = b[16 * i * BN + k * BK];
+            x[i] = ARows ? quad(A, 4 * k + i, ty) : quad(A, 4 * ty + i, k);
+            y[i] = BRows ? quad(B, 4 * k + i, tx) : quad(B, 4 * tx + i, k);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int e = 0; e < 4; ++e) {
+            const float2 b0 = BRows ? make_float2(y[e].x, y[e].y) : make_float2(part(y[0], e), part(y[1], e));
+            const float2 b1 = BRows ? make_float2(y[e].z, y[e].w) : make_float2(part(y[2], e), part(y[3], e));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) c.v[i][j] = fmaf(x[i], y[j], c.v[i][j]);
+            for (int i = 0; i < 4; ++i) {
+                const float a = ARows ? part(x[e], i) : part(x[i], e);
+                c.v[i][0] = __ffma2_rn(make_float2(a, a), b0, c.v[i][0]);
+                c.v[i][1] = __ffma2_rn(make_float2(a, a), b1, c.v[i][1]);
+            }
+        }
     }
 }
 template <class F>
@@ -47,22 +60,61 @@ __device__ __forceinline__ void each(Acc &c, int tid, F f) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f((tid >> 4) + 16 * i, (tid & 15) + 16 * j, c.v[i][j]);
+        for (int j = 0; j < 4; ++j) f((tid >> 4) * 4 + i, (tid & 15) * 4 + j, j & 1 ? c.v[i][j / 2].y : c.v[i][j / 2].x);
 }
 
-// 64 tokens x 64 columns of a tensor, zeros outside.
+// Four sums of a row times a factor, in place; their product with four values.
+__device__ __forceinline__ float scaled_dot(float2 (&v)[2], float w, const float4 &x) {
+    v[0] = __fmul2_rn(v[0], make_float2(w, w));
+    v[1] = __fmul2_rn(v[1], make_float2(w, w));
+    return fmaf(v[1].y, x.w, fmaf(v[1].x, x.z, fmaf(v[0].y, x.y, v[0].x * x.x)));
+}
+
+// 64 tokens x 64 columns of a tensor, zeros outside; four columns at a time where rows and strides allow it.
 template <class T>
 __device__ __forceinline__ void load_tile(float *to, const qgru_seq_tensor &x, long long base, int t0, int tokens, int d0, int d, int tid) {
     const T *p = static_cast<const T *>(x.p) + base;
-    for (int e = tid; e < C * 64; e += THREADS) {
-        const int r = e >> 6, c = e & 63;
-        to[r * LD + c] = r < tokens && d0 + c < d ? seq::to_f(p[(long long)(t0 + r) * x.ts + d0 + c]) : 0.f;
+    const bool wide = ((x.ts | x.bs | x.hs | d) & 3) == 0 && reinterpret_cast<uintptr_t>(x.p) % (4 * sizeof(T)) == 0;
+#pragma unroll
+    for (int e = tid; e < TILE / 4; e += THREADS) {
+        const int r = e >> 4, c = (e & 15) * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < tokens && d0 + c < d) {
+            const T *q = p + (long long)(t0 + r) * x.ts + d0 + c;
+            if (wide) {
+                if constexpr (sizeof(T) == 4) {
+                    v = *reinterpret_cast<const float4 *>(q);
+                } else {
+                    const uint2 u = *reinterpret_cast<const uint2 *>(q);
+                    v = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+                }
+            } else {
+                v.x = seq::to_f(q[0]);
+                if (d0 + c + 1 < d) v.y = seq::to_f(q[1]);
+                if (d0 + c + 2 < d) v.z = seq::to_f(q[2]);
+                if (d0 + c + 3 < d) v.w = seq::to_f(q[3]);
+            }
+        }
+        *reinterpret_cast<float4 *>(to + idx(r, c)) = v;
     }
 }
 __device__ __forceinline__ void load_state(float *to, const float *S, int i0, int j0, const qgru_attention &a, int tid) {
-    for (int e = tid; e < 4096; e += THREADS) {
-        const int r = e >> 6, c = e & 63;
-        to[r * LD + c] = i0 + r < a.Dk && j0 + c < a.Dv ? S[(long long)(i0 + r) * a.Dv + j0 + c] : 0.f;
+#pragma unroll
+    for (int e = tid; e < TILE / 4; e += THREADS) {
+        const int r = e >> 4, c = (e & 15) * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i0 + r < a.Dk && j0 + c < a.Dv) {
+            const float *q = S + (long long)(i0 + r) * a.Dv + j0 + c;
+            if (a.Dv % 4 == 0) {
+                v = *reinterpret_cast<const float4 *>(q);
+            } else {
+                v.x = q[0];
+                if (j0 + c + 1 < a.Dv) v.y = q[1];
+                if (j0 + c + 2 < a.Dv) v.z = q[2];
+                if (j0 + c + 3 < a.Dv) v.w = q[3];
+            }
+        }
+        *reinterpret_cast<float4 *>(to + idx(r, c)) = v;
     }
 }
 __device__ __forceinline__ long long at(const qgru_seq_tensor &x, int b, int h) { return b * x.bs + h * x.hs; }
@@ -94,8 +146,9 @@ struct Pass {                      // a state pass
 // token is scale 2^G_t instead of 2^(G_C - G_t).
 template <class T, bool Reverse>
 __global__ void __launch_bounds__(THREADS) k_states(const __grid_constant__ qgru_attention a, const Pass p) {
-    __shared__ float K[C * LD], V[C * LD];
+    __shared__ alignas(16) float K[TILE], V[TILE];
     __shared__ float2 G[C];
+    __shared__ float W[C];
     __shared__ double sums[2];
     const int tid = threadIdx.x, bh = blockIdx.x, b = bh / a.H, h = bh % a.H;
     const int nj = (a.Dv + 63) / 64, i0 = (int)blockIdx.y / nj * 64, j0 = (int)blockIdx.y % nj * 64;
@@ -121,12 +174,14 @@ __global__ void __launch_bounds__(THREADS) k_states(const __grid_constant__ qgru
         load_tile<T>(V, p.v, vb, t0, tokens, j0, a.Dv, tid);
         __syncthreads();
         const float2 end = G[C - 1];
-        for (int e = tid; e < C * 64; e += THREADS) K[(e >> 6) * LD + (e & 63)] *= Reverse ? a.scale * exp2_of(G[e >> 6]) : exp2_diff(end, G[e >> 6]);
+        if (tid < C) W[tid] = Reverse ? a.scale * exp2_of(G[tid]) : exp2_diff(end, G[tid]);
+        __syncthreads();
+        for (int e = tid; e < TILE; e += THREADS) K[e] *= W[e >> 6];
         __syncthreads();
         const float whole = exp2_of(end);
         all += (double)end.x + (double)end.y;
         each(S, tid, [&](int, int, float &s) { s *= whole; });
-        multiply<1, LD, LD, 1>(S, K, V, tid);
+        multiply<true, true>(S, K, V, tid);
     }
     if (own_sums) {
         each(S, tid, [&](int i, int j, float &s) { if (inside(i, j)) p.seg_state[seg * size + tile + place(i, j)] = s; });
@@ -163,8 +218,8 @@ __global__ void __launch_bounds__(128) k_scan_segments(float *seg_state, const f
 // grid: chunks x B H, the heads of one chunk beside each other (their tokens lie together)
 template <class T>
 __global__ void __launch_bounds__(THREADS) k_outputs(const __grid_constant__ qgru_attention a, const float *states) {
-    extern __shared__ float smem[];
-    float *X = smem, *Y = X + C * LD, *P = Y + C * LD;
+    extern __shared__ float4 smem4[];
+    float *X = reinterpret_cast<float *>(smem4), *Y = X + TILE, *P = Y + TILE;
     __shared__ float2 G[C];
     __shared__ double sums[2];
     const int tid = threadIdx.x, heads = a.B * a.H, chunk = blockIdx.x / heads, bh = blockIdx.x % heads, b = bh / a.H, h = bh % a.H, t0 = chunk * C;
@@ -184,30 +239,30 @@ __global__ void __launch_bounds__(THREADS) k_outputs(const __grid_constant__ qgr
         load_tile<T>(X, a.q, qb, t0, tokens, d, a.Dk, tid);
         load_tile<T>(Y, a.k, kb, t0, tokens, d, a.Dk, tid);
         __syncthreads();
-        multiply<LD, 1, 1, LD>(c, X, Y, tid);
+        multiply<false, false>(c, X, Y, tid);
         __syncthreads();
     }
-    each(c, tid, [&](int t, int s, float &x) { P[t * LD + s] = s <= t ? a.scale * exp2_diff(G[t], G[s]) * x : 0.f; });
+    each(c, tid, [&](int t, int s, float &x) { P[idx(t, s)] = s <= t ? a.scale * exp2_diff(G[t], G[s]) * x : 0.f; });
     for (int j = 0; j < a.Dv; j += 64) {
         c.zero();
         for (int d = 0; d < a.Dk; d += 64) {
             load_tile<T>(X, a.q, qb, t0, tokens, d, a.Dk, tid);
             load_state(Y, S, d, j, a, tid);
             __syncthreads();
-            multiply<LD, 1, LD, 1>(c, X, Y, tid);
+            multiply<false, true>(c, X, Y, tid);
             __syncthreads();
         }
         each(c, tid, [&](int t, int, float &x) { x *= a.scale * exp2_of(G[t]); });
         load_tile<T>(Y, a.v, vb, t0, tokens, j, a.Dv, tid);
         // A later token's infinity or NaN is none of an earlier one's business, and zero times it is NaN.
         int odd = 0;
-        for (int e = tid; e < C * 64; e += THREADS) odd |= !isfinite(Y[(e >> 6) * LD + (e & 63)]);
+        for (int e = tid; e < TILE; e += THREADS) odd |= !isfinite(Y[e]);
         if (__syncthreads_or(odd)) {
             each(c, tid, [&](int t, int n, float &x) {
-                for (int s = 0; s <= t; ++s) x = fmaf(P[t * LD + s], Y[s * LD + n], x);
+                for (int s = 0; s <= t; ++s) x = fmaf(P[idx(t, s)], Y[idx(s, n)], x);
             });
         } else {
-            multiply<LD, 1, LD, 1>(c, P, Y, tid);
+            multiply<false, true>(c, P, Y, tid);
         }
         __syncthreads();
         each(c, tid, [&](int t, int n, float &x) {
@@ -220,8 +275,8 @@ __global__ void __launch_bounds__(THREADS) k_outputs(const __grid_constant__ qgr
 template <class T>
 __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ qgru_attention a, const float *states, const float *dstates, float *dq_heads,
                                                        float *dk_heads) {
-    extern __shared__ float smem[];
-    float *X = smem, *Y = X + C * LD, *P = Y + C * LD, *E = P + C * LD;
+    extern __shared__ float4 smem4[];
+    float *X = reinterpret_cast<float *>(smem4), *Y = X + TILE, *P = Y + TILE, *E = P + TILE;
     __shared__ float2 G[C];
     __shared__ double sums[2];
     __shared__ float dG[C + 1], kE[C];       // what a change of the decays' sum up to token t brings; k_s's share behind the chunk
@@ -258,32 +313,33 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
         load_tile<T>(X, a.q, qb, t0, tokens, d, a.Dk, tid);
         load_tile<T>(Y, a.k, kb, t0, tokens, d, a.Dk, tid);
         __syncthreads();
-        multiply<LD, 1, 1, LD>(c, X, Y, tid);
+        multiply<false, false>(c, X, Y, tid);
         __syncthreads();
     }
     for (int d = 0; d < a.Dv; d += 64) {
         load_tile<T>(X, a.dout, ob, t0, tokens, d, a.Dv, tid);
         load_tile<T>(Y, a.v, vb, t0, tokens, d, a.Dv, tid);
         __syncthreads();
-        multiply<LD, 1, 1, LD>(e2, X, Y, tid);
+        multiply<false, false>(e2, X, Y, tid);
         __syncthreads();
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int t = (tid >> 4) + 16 * i, s = (tid & 15) + 16 * j;
+            const int t = (tid >> 4) * 4 + i, s = (tid & 15) * 4 + j;
+            const float qk = j & 1 ? c.v[i][j / 2].y : c.v[i][j / 2].x, ov = j & 1 ? e2.v[i][j / 2].y : e2.v[i][j / 2].x;
             const float w = s <= t ? a.scale * exp2_diff(G[t], G[s]) : 0.f;
-            const float p = s <= t ? w * c.v[i][j] : 0.f, e = s <= t ? w * e2.v[i][j] : 0.f;
-            P[t * LD + s] = p;
-            E[t * LD + s] = e;
-            X[t * LD + s] = s < t ? p * e2.v[i][j] : 0.f;
+            const float p = s <= t ? w * qk : 0.f, e = s <= t ? w * ov : 0.f;
+            P[idx(t, s)] = p;
+            E[idx(t, s)] = e;
+            X[idx(t, s)] = s < t ? p * ov : 0.f;
         }
     __syncthreads();
     // every pair (t, s), s < t: a change of G_t adds, one of G_s takes away
     if (tid < C) {
         double r = 0.0;
-        for (int s = 0; s < C; ++s) r += (double)X[tid * LD + s] - (double)X[s * LD + tid];
+        for (int s = 0; s < C; ++s) r += (double)X[idx(tid, s)] - (double)X[idx(s, tid)];
         dG[tid] = (float)r;
     }
     __syncthreads();
@@ -295,7 +351,7 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
             load_tile<T>(X, a.dout, ob, t0, tokens, j, a.Dv, tid);
             load_state(Y, S, i, j, a, tid);
             __syncthreads();
-            multiply<LD, 1, 1, LD>(c, X, Y, tid);
+            multiply<false, false>(c, X, Y, tid);
             __syncthreads();
         }
         load_tile<T>(X, a.q, qb, t0, tokens, i, a.Dk, tid);
@@ -303,18 +359,12 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int t = (tid >> 4) + 16 * r;
-            const float w = a.scale * exp2_of(G[t]);
-            float x = 0.f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                c.v[r][j] *= w;
-                x = fmaf(c.v[r][j], X[t * LD + (tid & 15) + 16 * j], x);
-            }
+            const int t = (tid >> 4) * 4 + r;
+            float x = scaled_dot(c.v[r], a.scale * exp2_of(G[t]), quad(X, t, tid & 15));
             for (int o = 8; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
             if ((tid & 15) == 0) dG[t] += x;
         }
-        multiply<LD, 1, LD, 1>(c, E, Y, tid);
+        multiply<false, true>(c, E, Y, tid);
         each(c, tid, [&](int t, int d, float &x) { if (t < all && i + d < a.Dk) put_qk(a.dq, dq_heads, t, i + d, t < tokens ? x : 0.f); });
         __syncthreads();
         // dk = E^T q + 2^(G_C - G_s) v dS^T
@@ -323,7 +373,7 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
             load_tile<T>(X, a.v, vb, t0, tokens, j, a.Dv, tid);
             load_state(Y, dS, i, j, a, tid);
             __syncthreads();
-            multiply<LD, 1, 1, LD>(c, X, Y, tid);
+            multiply<false, false>(c, X, Y, tid);
             __syncthreads();
         }
         load_tile<T>(X, a.q, qb, t0, tokens, i, a.Dk, tid);
@@ -331,18 +381,12 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int s = (tid >> 4) + 16 * r;
-            const float w = exp2_diff(end, G[s]);
-            float x = 0.f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                c.v[r][j] *= w;
-                x = fmaf(c.v[r][j], Y[s * LD + (tid & 15) + 16 * j], x);
-            }
+            const int s = (tid >> 4) * 4 + r;
+            float x = scaled_dot(c.v[r], exp2_diff(end, G[s]), quad(Y, s, tid & 15));
             for (int o = 8; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
             if ((tid & 15) == 0) kE[s] += x;
         }
-        multiply<1, LD, LD, 1>(c, E, X, tid);
+        multiply<true, true>(c, E, X, tid);
         each(c, tid, [&](int s, int d, float &x) { if (s < all && i + d < a.Dk) put_qk(a.dk, dk_heads, s, i + d, s < tokens ? x : 0.f); });
         __syncthreads();
     }
@@ -353,13 +397,13 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
             load_tile<T>(X, a.k, kb, t0, tokens, i, a.Dk, tid);
             load_state(Y, dS, i, j, a, tid);
             __syncthreads();
-            multiply<LD, 1, LD, 1>(c, X, Y, tid);
+            multiply<false, true>(c, X, Y, tid);
             __syncthreads();
         }
         each(c, tid, [&](int s, int, float &x) { x *= exp2_diff(end, G[s]); });
         load_tile<T>(X, a.dout, ob, t0, tokens, j, a.Dv, tid);
         __syncthreads();
-        multiply<1, LD, LD, 1>(c, P, X, tid);
+        multiply<true, true>(c, P, X, tid);
         each(c, tid, [&](int s, int d, float &x) { if (s < all && j + d < a.Dv) dv[s * a.dv.ts + j + d] = seq::from_f<T>(s < tokens ? x : 0.f); });
         __syncthreads();
     }
@@ -367,12 +411,12 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
     double through = 0.0;
     for (int e = tid; e < a.Dk * a.Dv; e += THREADS) through += (double)S[e] * (double)dS[e];
     for (int o = 16; o; o >>= 1) through += __shfl_xor_sync(0xffffffffu, through, o);
-    double *part = reinterpret_cast<double *>(smem);
-    if ((tid & 31) == 0) part[tid >> 5] = through;
+    double *sum_of = reinterpret_cast<double *>(smem4);
+    if ((tid & 31) == 0) sum_of[tid >> 5] = through;
     __syncthreads();
     if (tid == 0) {
         through = 0.0;
-        for (int w = 0; w < THREADS / 32; ++w) through += part[w];
+        for (int w = 0; w < THREADS / 32; ++w) through += sum_of[w];
         through *= (double)exp2_of(end);
         for (int s = 0; s < tokens; ++s) through += (double)kE[s];
         // from the end: sum over u >= t of dG_u, the shares of k_s for s < t, and what passes through
@@ -387,20 +431,34 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
     if (tid < all) seq::store_f(a.ddecay.p, gb + tid * a.ddecay.ts, a.decay_bf16, tid < tokens ? X[64 + tid] : 0.f);
 }
 
-// dq and dk of heads that share q and k: the sum over each group, one rounding.
-template <class T>
+// dq and dk of heads that share q and k: the sum over each group, one rounding.  V neighbouring elements a thread.
+template <class T, int V>
 __global__ void k_sum_groups(const __grid_constant__ qgru_attention a, const float *dq, const float *dk) {
-    const int g = a.H / a.Hk;
-    const long long n = (long long)a.T * a.B * a.Hk * a.Dk;
+    const int g = a.H / a.Hk, per_head = a.Dk / V;
+    const long long n = (long long)a.T * a.B * a.Hk * per_head;
     const qgru_seq_tensor to = blockIdx.y ? a.dk : a.dq;
     const float *from = blockIdx.y ? dk : dq;
     for (long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (long long)gridDim.x * blockDim.x) {
-        const int d = (int)(e % a.Dk), hk = (int)(e / a.Dk % a.Hk);
-        const long long tb = e / a.Dk / a.Hk;
+        const long long head = e / per_head, tb = head / a.Hk;
+        const int d = (int)(e - head * per_head) * V, hk = (int)(head - tb * a.Hk);
         const float *p = from + (tb * a.H + (long long)hk * g) * a.Dk + d;
-        float s = 0.f;
-        for (int i = 0; i < g; ++i) s += p[(long long)i * a.Dk];
-        static_cast<T *>(to.p)[tb / a.B * to.ts + tb % a.B * to.bs + hk * to.hs + d] = seq::from_f<T>(s);
+        float s[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[j] = 0.f;
+        for (int i = 0; i < g; ++i) {
+            if constexpr (V == 4) {
+                const float4 u = *reinterpret_cast<const float4 *>(p + (long long)i * a.Dk);
+                s[0] += u.x;
+                s[1] += u.y;
+                s[2] += u.z;
+                s[3] += u.w;
+            } else {
+                s[0] += p[(long long)i * a.Dk];
+            }
+        }
+        T *q = static_cast<T *>(to.p) + tb / a.B * to.ts + tb % a.B * to.bs + hk * to.hs + d;
+#pragma unroll
+        for (int j = 0; j < V; ++j) q[j] = seq::from_f<T>(s[j]);
     }
 }
 
@@ -443,7 +501,7 @@ int forward(const qgru_attention &a, const Cut &c, cudaStream_t st) {
     char *seg = static_cast<char *>(a.workspace) + (a.keep ? 0 : a256(c.states));
     if (const int rc = run_states<T, false>(a, c, states, seg, st)) return rc;
     if (c.chunks == 0) return QGRU_OK;
-    constexpr size_t bytes = 3 * C * LD * sizeof(float);
+    constexpr size_t bytes = 3 * TILE * sizeof(float);
     if (const int rc = with_smem(k_outputs<T>, bytes)) return rc;
     k_outputs<T><<<c.chunks * a.B * a.H, THREADS, bytes, st>>>(a, states);
     SEQ_CK(cudaGetLastError());
@@ -464,7 +522,7 @@ int backward(const qgru_attention &a, const Cut &c, cudaStream_t st) {
         dq = reinterpret_cast<float *>(ws);
         dk = dq + group_bytes(a) / 8;
     }
-    constexpr size_t bytes = 4 * C * LD * sizeof(float);
+    constexpr size_t bytes = 4 * TILE * sizeof(float);
     if (const int rc = with_smem(k_gradients<T>, bytes)) return rc;
     k_gradients<T><<<c.chunks * a.B * a.H, THREADS, bytes, st>>>(a, static_cast<const float *>(a.states), dstates, dq, dk);
     SEQ_CK(cudaGetLastError());
@@ -556,12 +614,11 @@ int step(const qgru_attention &a, long long bs, long long hs, cudaStream_t st) {
 size_t group_bytes(const qgru_attention &a) { return a.H == a.Hk ? 0 : 2 * sizeof(float) * (size_t)a.T * a.B * a.H * a.Dk; }
 
 int sum_groups(const qgru_attention &a, const float *dq, const float *dk, cudaStream_t st) {
-    const long long n = (long long)a.T * a.B * a.Hk * a.Dk;
+    const bool wide = a.Dk % 4 == 0;
+    const long long n = (long long)a.T * a.B * a.Hk * a.Dk / (wide ? 4 : 1);
     const dim3 grid((unsigned)std::min<long long>((n + 255) / 256, 4096), 2);
-    if (a.bf16)
-        k_sum_groups<bf16><<<grid, 256, 0, st>>>(a, dq, dk);
-    else
-        k_sum_groups<float><<<grid, 256, 0, st>>>(a, dq, dk);
+    const auto run = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(a, dq, dk); };
+    a.bf16 ? (wide ? run(k_sum_groups<bf16, 4>) : run(k_sum_groups<bf16, 1>)) : (wide ? run(k_sum_groups<float, 4>) : run(k_sum_groups<float, 1>));
     SEQ_CK(cudaGetLastError());
     return QGRU_OK;
 }
@@ -574,14 +631,14 @@ int scan_segments(const qgru_attention &a, const Cut &c, bool reverse, char *seg
     return QGRU_OK;
 }
 
-// Segments: as many as fill the SMs twice where the heads alone do not, of two chunks at the least (each token's k and v are read
-// once more for it).
+// Segments: where the heads alone leave half of two CTAs an SM idle, of two chunks at the least (each token's k and v are read once more
+// for it).
 Cut generic_cut(const qgru_attention &a, int sms) {
     Cut c;
     c.chunk = C;
     c.chunks = (a.T + C - 1) / C;
     const long long units = (long long)a.B * a.H * ((a.Dk + 63) / 64) * ((a.Dv + 63) / 64);
-    c.segments = (int)std::max<long long>(1, std::min<long long>(c.chunks / 2, (2 * sms + units - 1) / std::max<long long>(units, 1)));
+    c.segments = (int)std::max<long long>(1, std::min<long long>(c.chunks / 2, 2 * sms / std::max<long long>(units, 1)));
     c.per = std::max(1, (c.chunks + c.segments - 1) / c.segments);
     c.segments = std::max(1, (c.chunks + c.per - 1) / c.per);
     c.states = sizeof(float) * c.chunks * state_elems(a);
