@@ -1,7 +1,8 @@
 // qgru_attn.cu - linear attention: the entry points, the kernels for every size and type, and the single-token form.
 //
-// The kernels here compute in fp32 by multiply-adds, whatever the inputs' type, 64 tokens a chunk and 64 x 64 tiles; they serve
-// what the tensor-core kernels (qgru_attn_tc.cu) do not take.
+// The kernels here compute in fp32 whatever the inputs' type, 64 tokens a chunk and 64 x 64 tiles, by warp-level tensor instructions;
+// they serve fp32 tensors and head sizes above 128, which the tcgen05 kernels (qgru_attn_fwd.cu, qgru_attn_tc.cu) do not take: fp32
+// operands as three bf16 parts would be three times the shared memory, and the gradients' six tiles fill it with one.
 #include <algorithm>
 
 #include "qgru_attn.cuh"
@@ -15,59 +16,92 @@ constexpr int C = 64, THREADS = 256;
 constexpr int TILE = 64 * 64;                   // floats
 using bf16 = __nv_bfloat16;
 
-// A 64 x 64 tile in shared memory: rows of sixteen 16-byte chunks, chunk c of row r at c ^ (r / 4), so that reading four rows' chunk
-// by each of sixteen threads, or a row's sixteen chunks, meets every bank once.
-__device__ __forceinline__ int idx(int r, int c) { return r * 64 + ((((c >> 2) ^ (r >> 2)) & 15) << 2) + (c & 3); }
-__device__ __forceinline__ float4 quad(const float *t, int r, int c4) { return *reinterpret_cast<const float4 *>(t + r * 64 + (((c4 ^ (r >> 2)) & 15) << 2)); }
-__device__ __forceinline__ float part(const float4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+// A 64 x 64 tile in shared memory: rows of sixteen 16-byte chunks, chunk c of row r at c ^ f(r), so that eight rows' neighbouring four
+// values, and four rows' neighbouring eight, lie in different banks: the operands of the products below either way.
+__device__ __forceinline__ int idx(int r, int c) { return r * 64 + ((((c >> 2) ^ (2 * r) ^ (r >> 3)) & 15) << 2) + (c & 3); }
 
-// 64 x 64 sums of a thread grid of 16 x 16: rows 4 ty .. + 3, columns 4 tx .. + 3, neighbouring columns as packed pairs.
+// 64 x 64 sums of eight warps: 16 rows and 32 columns a warp, lane (g, t) = (lane / 4, lane % 4) has rows g and g + 8 and columns 2 t and
+// 2 t + 1 of each eight.
 struct Acc {
-    float2 v[4][2];
+    float v[4][4];
     __device__ __forceinline__ void zero() {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i][0] = v[i][1] = make_float2(0.f, 0.f);
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i][j] = 0.f;
     }
 };
-// acc += sum_k A(m, k) B(k, n).  ARows: A's tile has k as its rows, else m; BRows: B's tile has k as its rows, else n.  Four k at a time:
-// eight 16-byte loads for 64 multiply-adds.
+__device__ __forceinline__ uint32_t tf32(float x) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+// acc += sum over k = 8 from .. 8 to - 1 of A(m, k) B(k, n).  ARows: A's tile has k as its rows, else m; BRows: B's tile has k as its rows,
+// else n.  fp32 by warp-level tensor instructions: each operand is the sum of two tf32 values (11 bits and 11 bits, 2^-23 of it left
+// out), and of the four products the one of the two small parts is left out (2^-22 of the product at the most, the size of the rounding
+// of an fp32 sum).  Operands below 2^-114 keep 11 bits.
 template <bool ARows, bool BRows>
-__device__ __forceinline__ void multiply(Acc &c, const float *A, const float *B, int tid) {
-    const int ty = tid >> 4, tx = tid & 15;
+__device__ __forceinline__ void multiply(Acc &c, const float *A, const float *B, int from, int to, int tid) {
+    const int lane = tid & 31, g = lane >> 2, t = lane & 3, m = (tid >> 5 & 3) * 16 + g, n = (tid >> 7) * 32 + g;
 #pragma unroll 2
-    for (int k = 0; k < 16; ++k) {
-        float4 x[4], y[4];
+    for (int k = 8 * from + t; k < 8 * to; k += 8) {
+        uint32_t ah[4], al[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            x[i] = ARows ? quad(A, 4 * k + i, ty) : quad(A, 4 * ty + i, k);
-            y[i] = BRows ? quad(B, 4 * k + i, tx) : quad(B, 4 * tx + i, k);
+            const int row = m + (i & 1) * 8, kk = k + (i >> 1) * 4;
+            const float x = A[ARows ? idx(kk, row) : idx(row, kk)];
+            ah[i] = tf32(x);
+            al[i] = tf32(x - __uint_as_float(ah[i]));
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 b0 = BRows ? make_float2(y[e].x, y[e].y) : make_float2(part(y[0], e), part(y[1], e));
-            const float2 b1 = BRows ? make_float2(y[e].z, y[e].w) : make_float2(part(y[2], e), part(y[3], e));
+        for (int j = 0; j < 4; ++j) {
+            uint32_t bh[2], bl[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float a = ARows ? part(x[e], i) : part(x[i], e);
-                c.v[i][0] = __ffma2_rn(make_float2(a, a), b0, c.v[i][0]);
-                c.v[i][1] = __ffma2_rn(make_float2(a, a), b1, c.v[i][1]);
+            for (int i = 0; i < 2; ++i) {
+                const float x = B[BRows ? idx(k + 4 * i, n + 8 * j) : idx(n + 8 * j, k + 4 * i)];
+                bh[i] = tf32(x);
+                bl[i] = tf32(x - __uint_as_float(bh[i]));
             }
+            mma(c.v[j], al, bh);
+            mma(c.v[j], ah, bl);
+            mma(c.v[j], ah, bh);
         }
     }
 }
 template <class F>
 __device__ __forceinline__ void each(Acc &c, int tid, F f) {
+    const int lane = tid & 31, m = (tid >> 5 & 3) * 16 + (lane >> 2), n = (tid >> 7) * 32 + (lane & 3) * 2;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f((tid >> 4) * 4 + i, (tid & 15) * 4 + j, j & 1 ? c.v[i][j / 2].y : c.v[i][j / 2].x);
+        for (int i = 0; i < 4; ++i) f(m + (i >> 1) * 8, n + j * 8 + (i & 1), c.v[j][i]);
 }
-
-// Four sums of a row times a factor, in place; their product with four values.
-__device__ __forceinline__ float scaled_dot(float2 (&v)[2], float w, const float4 &x) {
-    v[0] = __fmul2_rn(v[0], make_float2(w, w));
-    v[1] = __fmul2_rn(v[1], make_float2(w, w));
-    return fmaf(v[1].y, x.w, fmaf(v[1].x, x.z, fmaf(v[0].y, x.y, v[0].x * x.x)));
+__device__ __forceinline__ int eights(int n) { return (min(n, 64) + 7) >> 3; }
+// Every row of the sums times a factor, in place; the rows' products with a tile's: [2][64], a half of the columns each.
+template <class F>
+__device__ __forceinline__ void scale_rows(Acc &c, const float *X, float *dots, F factor, int tid) {
+    const int lane = tid & 31, m = (tid >> 5 & 3) * 16 + (lane >> 2), n = (tid >> 7) * 32 + (lane & 3) * 2;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int row = m + 8 * h;
+        const float w = factor(row);
+        float x = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                c.v[j][2 * h + i] *= w;
+                x = fmaf(c.v[j][2 * h + i], X[idx(row, n + j * 8 + i)], x);
+            }
+        x += __shfl_xor_sync(0xffffffffu, x, 1);
+        x += __shfl_xor_sync(0xffffffffu, x, 2);
+        if ((lane & 3) == 0) dots[(tid >> 7) * 64 + row] += x;
+    }
 }
 
 // 64 tokens x 64 columns of a tensor, zeros outside; four columns at a time where rows and strides allow it.
@@ -181,7 +215,7 @@ __global__ void __launch_bounds__(THREADS) k_states(const __grid_constant__ qgru
         const float whole = exp2_of(end);
         all += (double)end.x + (double)end.y;
         each(S, tid, [&](int, int, float &s) { s *= whole; });
-        multiply<true, true>(S, K, V, tid);
+        multiply<true, true>(S, K, V, 0, eights(tokens), tid);
     }
     if (own_sums) {
         each(S, tid, [&](int i, int j, float &s) { if (inside(i, j)) p.seg_state[seg * size + tile + place(i, j)] = s; });
@@ -233,13 +267,15 @@ __global__ void __launch_bounds__(THREADS) k_outputs(const __grid_constant__ qgr
     const long long qb = at(a.q, b, hk), kb = at(a.k, b, hk), vb = at(a.v, b, h);
     const float *S = states + chunk * (long long)heads * a.Dk * a.Dv + (long long)bh * a.Dk * a.Dv;
     load_decays(G, sums, a, b, h, t0, tokens, tid);
+    // the pairs of a warp's 16 rows end in their columns
+    const int up_to = (tid >> 5 & 3) * 2 + 2;
     Acc c;
     c.zero();
     for (int d = 0; d < a.Dk; d += 64) {
         load_tile<T>(X, a.q, qb, t0, tokens, d, a.Dk, tid);
         load_tile<T>(Y, a.k, kb, t0, tokens, d, a.Dk, tid);
         __syncthreads();
-        multiply<false, false>(c, X, Y, tid);
+        multiply<false, false>(c, X, Y, 0, eights(a.Dk - d), tid);
         __syncthreads();
     }
     each(c, tid, [&](int t, int s, float &x) { P[idx(t, s)] = s <= t ? a.scale * exp2_diff(G[t], G[s]) * x : 0.f; });
@@ -249,7 +285,7 @@ __global__ void __launch_bounds__(THREADS) k_outputs(const __grid_constant__ qgr
             load_tile<T>(X, a.q, qb, t0, tokens, d, a.Dk, tid);
             load_state(Y, S, d, j, a, tid);
             __syncthreads();
-            multiply<false, true>(c, X, Y, tid);
+            multiply<false, true>(c, X, Y, 0, eights(a.Dk - d), tid);
             __syncthreads();
         }
         each(c, tid, [&](int t, int, float &x) { x *= a.scale * exp2_of(G[t]); });
@@ -262,7 +298,7 @@ __global__ void __launch_bounds__(THREADS) k_outputs(const __grid_constant__ qgr
                 for (int s = 0; s <= t; ++s) x = fmaf(P[idx(t, s)], Y[idx(s, n)], x);
             });
         } else {
-            multiply<false, true>(c, P, Y, tid);
+            multiply<false, true>(c, P, Y, 0, min(eights(tokens), up_to), tid);
         }
         __syncthreads();
         each(c, tid, [&](int t, int n, float &x) {
@@ -279,7 +315,7 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
     float *X = reinterpret_cast<float *>(smem4), *Y = X + TILE, *P = Y + TILE, *E = P + TILE;
     __shared__ float2 G[C];
     __shared__ double sums[2];
-    __shared__ float dG[C + 1], kE[C];       // what a change of the decays' sum up to token t brings; k_s's share behind the chunk
+    __shared__ float dG[3][C], kE[2][C];     // what a change of the decays' sum up to token t brings; k_s's share behind the chunk
     const int tid = threadIdx.x, heads = a.B * a.H, chunk = blockIdx.x / heads, bh = blockIdx.x % heads, b = bh / a.H, h = bh % a.H, t0 = chunk * C;
     const int all = min(a.T - t0, C), tokens = min(max(valid_tokens(a, b) - t0, 0), C);
     const int hk = h / (a.H / a.Hk);
@@ -304,8 +340,9 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
     const long long tile = chunk * (long long)heads * a.Dk * a.Dv + (long long)bh * a.Dk * a.Dv;
     const float *S = states + tile, *dS = dstates + tile;
     load_decays(G, sums, a, b, h, t0, tokens, tid);
-    if (tid < C) kE[tid] = 0.f;
-    if (tid <= C) dG[tid] = 0.f;
+    if (tid < C) kE[0][tid] = kE[1][tid] = dG[0][tid] = dG[1][tid] = dG[2][tid] = 0.f;
+    // the pairs of a warp's 16 rows end in their columns, or begin there
+    const int diagonal = (tid >> 5 & 3) * 2, last = eights(tokens);
     Acc c, e2;
     c.zero();
     e2.zero();
@@ -313,34 +350,36 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
         load_tile<T>(X, a.q, qb, t0, tokens, d, a.Dk, tid);
         load_tile<T>(Y, a.k, kb, t0, tokens, d, a.Dk, tid);
         __syncthreads();
-        multiply<false, false>(c, X, Y, tid);
+        multiply<false, false>(c, X, Y, 0, eights(a.Dk - d), tid);
         __syncthreads();
     }
     for (int d = 0; d < a.Dv; d += 64) {
         load_tile<T>(X, a.dout, ob, t0, tokens, d, a.Dv, tid);
         load_tile<T>(Y, a.v, vb, t0, tokens, d, a.Dv, tid);
         __syncthreads();
-        multiply<false, false>(e2, X, Y, tid);
+        multiply<false, false>(e2, X, Y, 0, eights(a.Dv - d), tid);
         __syncthreads();
     }
+    {
+        const int lane = tid & 31, t0 = (tid >> 5 & 3) * 16 + (lane >> 2), s0 = (tid >> 7) * 32 + (lane & 3) * 2;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int t = (tid >> 4) * 4 + i, s = (tid & 15) * 4 + j;
-            const float qk = j & 1 ? c.v[i][j / 2].y : c.v[i][j / 2].x, ov = j & 1 ? e2.v[i][j / 2].y : e2.v[i][j / 2].x;
-            const float w = s <= t ? a.scale * exp2_diff(G[t], G[s]) : 0.f;
-            const float p = s <= t ? w * qk : 0.f, e = s <= t ? w * ov : 0.f;
-            P[idx(t, s)] = p;
-            E[idx(t, s)] = e;
-            X[idx(t, s)] = s < t ? p * ov : 0.f;
-        }
+            for (int i = 0; i < 4; ++i) {
+                const int t = t0 + (i >> 1) * 8, s = s0 + j * 8 + (i & 1);
+                const float w = s <= t ? a.scale * exp2_diff(G[t], G[s]) : 0.f, ov = e2.v[j][i];
+                const float p = s <= t ? w * c.v[j][i] : 0.f, e = s <= t ? w * ov : 0.f;
+                P[idx(t, s)] = p;
+                E[idx(t, s)] = e;
+                X[idx(t, s)] = s < t ? p * ov : 0.f;
+            }
+    }
     __syncthreads();
     // every pair (t, s), s < t: a change of G_t adds, one of G_s takes away
     if (tid < C) {
         double r = 0.0;
         for (int s = 0; s < C; ++s) r += (double)X[idx(tid, s)] - (double)X[idx(s, tid)];
-        dG[tid] = (float)r;
+        dG[2][tid] = (float)r;
     }
     __syncthreads();
     const float2 end = G[C - 1];
@@ -351,20 +390,14 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
             load_tile<T>(X, a.dout, ob, t0, tokens, j, a.Dv, tid);
             load_state(Y, S, i, j, a, tid);
             __syncthreads();
-            multiply<false, false>(c, X, Y, tid);
+            multiply<false, false>(c, X, Y, 0, eights(a.Dv - j), tid);
             __syncthreads();
         }
         load_tile<T>(X, a.q, qb, t0, tokens, i, a.Dk, tid);
         load_tile<T>(Y, a.k, kb, t0, tokens, i, a.Dk, tid);
         __syncthreads();
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int t = (tid >> 4) * 4 + r;
-            float x = scaled_dot(c.v[r], a.scale * exp2_of(G[t]), quad(X, t, tid & 15));
-            for (int o = 8; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-            if ((tid & 15) == 0) dG[t] += x;
-        }
-        multiply<false, true>(c, E, Y, tid);
+        scale_rows(c, X, dG[0], [&](int t) { return a.scale * exp2_of(G[t]); }, tid);
+        multiply<false, true>(c, E, Y, 0, min(diagonal + 2, last), tid);
         each(c, tid, [&](int t, int d, float &x) { if (t < all && i + d < a.Dk) put_qk(a.dq, dq_heads, t, i + d, t < tokens ? x : 0.f); });
         __syncthreads();
         // dk = E^T q + 2^(G_C - G_s) v dS^T
@@ -373,20 +406,14 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
             load_tile<T>(X, a.v, vb, t0, tokens, j, a.Dv, tid);
             load_state(Y, dS, i, j, a, tid);
             __syncthreads();
-            multiply<false, false>(c, X, Y, tid);
+            multiply<false, false>(c, X, Y, 0, eights(a.Dv - j), tid);
             __syncthreads();
         }
         load_tile<T>(X, a.q, qb, t0, tokens, i, a.Dk, tid);
         load_tile<T>(Y, a.k, kb, t0, tokens, i, a.Dk, tid);
         __syncthreads();
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int s = (tid >> 4) * 4 + r;
-            float x = scaled_dot(c.v[r], exp2_diff(end, G[s]), quad(Y, s, tid & 15));
-            for (int o = 8; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-            if ((tid & 15) == 0) kE[s] += x;
-        }
-        multiply<true, true>(c, E, X, tid);
+        scale_rows(c, Y, kE[0], [&](int s) { return exp2_diff(end, G[s]); }, tid);
+        multiply<true, true>(c, E, X, diagonal, last, tid);
         each(c, tid, [&](int s, int d, float &x) { if (s < all && i + d < a.Dk) put_qk(a.dk, dk_heads, s, i + d, s < tokens ? x : 0.f); });
         __syncthreads();
     }
@@ -397,13 +424,13 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
             load_tile<T>(X, a.k, kb, t0, tokens, i, a.Dk, tid);
             load_state(Y, dS, i, j, a, tid);
             __syncthreads();
-            multiply<false, true>(c, X, Y, tid);
+            multiply<false, true>(c, X, Y, 0, eights(a.Dk - i), tid);
             __syncthreads();
         }
         each(c, tid, [&](int s, int, float &x) { x *= exp2_diff(end, G[s]); });
         load_tile<T>(X, a.dout, ob, t0, tokens, j, a.Dv, tid);
         __syncthreads();
-        multiply<true, true>(c, P, X, tid);
+        multiply<true, true>(c, P, X, diagonal, last, tid);
         each(c, tid, [&](int s, int d, float &x) { if (s < all && j + d < a.Dv) dv[s * a.dv.ts + j + d] = seq::from_f<T>(s < tokens ? x : 0.f); });
         __syncthreads();
     }
@@ -418,12 +445,12 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
         through = 0.0;
         for (int w = 0; w < THREADS / 32; ++w) through += sum_of[w];
         through *= (double)exp2_of(end);
-        for (int s = 0; s < tokens; ++s) through += (double)kE[s];
+        for (int s = 0; s < tokens; ++s) through += (double)kE[0][s] + (double)kE[1][s];
         // from the end: sum over u >= t of dG_u, the shares of k_s for s < t, and what passes through
         double acc = 0.0;
         for (int t = tokens - 1; t >= 0; --t) {
-            acc += (double)dG[t];
-            through -= (double)kE[t];
+            acc += (double)dG[0][t] + (double)dG[1][t] + (double)dG[2][t];
+            through -= (double)kE[0][t] + (double)kE[1][t];
             X[64 + t] = (float)(acc + through);
         }
     }
