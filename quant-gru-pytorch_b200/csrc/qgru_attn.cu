@@ -4,6 +4,7 @@
 // they serve fp32 tensors and head sizes above 128, which the tcgen05 kernels (qgru_attn_fwd.cu, qgru_attn_tc.cu) do not take: fp32
 // operands as three bf16 parts would be three times the shared memory, and the gradients' six tiles fill it with one.
 #include <algorithm>
+#include <type_traits>
 
 #include "qgru_attn.cuh"
 #include "qgru_attn_tc.cuh"
@@ -20,17 +21,19 @@ using bf16 = __nv_bfloat16;
 // values, and four rows' neighbouring eight, lie in different banks: the operands of the products below either way.
 __device__ __forceinline__ int idx(int r, int c) { return r * 64 + ((((c >> 2) ^ (2 * r) ^ (r >> 3)) & 15) << 2) + (c & 3); }
 
-// 64 x 64 sums of eight warps: 16 rows and 32 columns a warp, lane (g, t) = (lane / 4, lane % 4) has rows g and g + 8 and columns 2 t and
-// 2 t + 1 of each eight.
-struct Acc {
-    float v[4][4];
+// 64 x 64 sums of 32 / NT warps: 16 rows and 8 NT columns a warp, lane (g, t) = (lane / 4, lane % 4) has rows g and g + 8 and columns 2 t
+// and 2 t + 1 of each eight.
+template <int NT>
+struct Sums {
+    float v[NT][4];
     __device__ __forceinline__ void zero() {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[i][j] = 0.f;
     }
 };
+using Acc = Sums<4>;
 __device__ __forceinline__ uint32_t tf32(float x) {
     uint32_t r;
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
@@ -42,12 +45,12 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], const
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 // acc += sum over k = 8 from .. 8 to - 1 of A(m, k) B(k, n).  ARows: A's tile has k as its rows, else m; BRows: B's tile has k as its rows,
-// else n.  fp32 by warp-level tensor instructions: each operand is the sum of two tf32 values (11 bits and 11 bits, 2^-23 of it left
-// out), and of the four products the one of the two small parts is left out (2^-22 of the product at the most, the size of the rounding
-// of an fp32 sum).  Operands below 2^-114 keep 11 bits.
-template <bool ARows, bool BRows>
-__device__ __forceinline__ void multiply(Acc &c, const float *A, const float *B, int from, int to, int tid) {
-    const int lane = tid & 31, g = lane >> 2, t = lane & 3, m = (tid >> 5 & 3) * 16 + g, n = (tid >> 7) * 32 + g;
+// else n.  fp32 by warp-level tensor instructions: each operand is the sum of two tf32 values of 11 bits (off by 2^-22 of it at the most,
+// 2^-25 in the mean), and of the four products the one of the two small parts is left out (2^-22 of the product at the most).  Operands
+// below 2^-114 keep 11 bits.
+template <bool ARows, bool BRows, int NT>
+__device__ __forceinline__ void multiply(Sums<NT> &c, const float *A, const float *B, int from, int to, int tid) {
+    const int lane = tid & 31, g = lane >> 2, t = lane & 3, m = (tid >> 5 & 3) * 16 + g, n = (tid >> 7) * (8 * NT) + g;
 #pragma unroll 2
     for (int k = 8 * from + t; k < 8 * to; k += 8) {
         uint32_t ah[4], al[4];
@@ -59,7 +62,7 @@ __device__ __forceinline__ void multiply(Acc &c, const float *A, const float *B,
             al[i] = tf32(x - __uint_as_float(ah[i]));
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < NT; ++j) {
             uint32_t bh[2], bl[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -73,26 +76,26 @@ __device__ __forceinline__ void multiply(Acc &c, const float *A, const float *B,
         }
     }
 }
-template <class F>
-__device__ __forceinline__ void each(Acc &c, int tid, F f) {
-    const int lane = tid & 31, m = (tid >> 5 & 3) * 16 + (lane >> 2), n = (tid >> 7) * 32 + (lane & 3) * 2;
+template <int NT, class F>
+__device__ __forceinline__ void each(Sums<NT> &c, int tid, F f) {
+    const int lane = tid & 31, m = (tid >> 5 & 3) * 16 + (lane >> 2), n = (tid >> 7) * (8 * NT) + (lane & 3) * 2;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) f(m + (i >> 1) * 8, n + j * 8 + (i & 1), c.v[j][i]);
 }
 __device__ __forceinline__ int eights(int n) { return (min(n, 64) + 7) >> 3; }
-// Every row of the sums times a factor, in place; the rows' products with a tile's: [2][64], a half of the columns each.
-template <class F>
-__device__ __forceinline__ void scale_rows(Acc &c, const float *X, float *dots, F factor, int tid) {
-    const int lane = tid & 31, m = (tid >> 5 & 3) * 16 + (lane >> 2), n = (tid >> 7) * 32 + (lane & 3) * 2;
+// Every row of the sums times a factor, in place; the rows' products with a tile's: [8 / NT][64], a warp's columns each.
+template <int NT, class F>
+__device__ __forceinline__ void scale_rows(Sums<NT> &c, const float *X, float *dots, F factor, int tid) {
+    const int lane = tid & 31, m = (tid >> 5 & 3) * 16 + (lane >> 2), n = (tid >> 7) * (8 * NT) + (lane & 3) * 2;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int row = m + 8 * h;
         const float w = factor(row);
         float x = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 c.v[j][2 * h + i] *= w;
@@ -104,33 +107,47 @@ __device__ __forceinline__ void scale_rows(Acc &c, const float *X, float *dots, 
     }
 }
 
-// 64 tokens x 64 columns of a tensor, zeros outside; four columns at a time where rows and strides allow it.
+// A thread's share of a 64 x 64 tile: four neighbouring columns at four places.  64 tokens x 64 columns of a tensor, zeros outside; four
+// columns a load where rows and strides allow it.
+struct Four {
+    float4 v[4];
+    template <class T>
+    __device__ __forceinline__ void load(const qgru_seq_tensor &x, long long base, int t0, int tokens, int d0, int d, int tid) {
+        const T *p = static_cast<const T *>(x.p) + base;
+        const bool wide = ((x.ts | x.bs | x.hs | d) & 3) == 0 && reinterpret_cast<uintptr_t>(x.p) % (4 * sizeof(T)) == 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = (tid >> 4) + 16 * i, c = (tid & 15) * 4;
+            float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < tokens && d0 + c < d) {
+                const T *q = p + (long long)(t0 + r) * x.ts + d0 + c;
+                if (wide) {
+                    if constexpr (sizeof(T) == 4) {
+                        u = *reinterpret_cast<const float4 *>(q);
+                    } else {
+                        const uint2 w = *reinterpret_cast<const uint2 *>(q);
+                        u = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+                    }
+                } else {
+                    u.x = seq::to_f(q[0]);
+                    if (d0 + c + 1 < d) u.y = seq::to_f(q[1]);
+                    if (d0 + c + 2 < d) u.z = seq::to_f(q[2]);
+                    if (d0 + c + 3 < d) u.w = seq::to_f(q[3]);
+                }
+            }
+            v[i] = u;
+        }
+    }
+    __device__ __forceinline__ void store(float *to, int tid) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<float4 *>(to + idx((tid >> 4) + 16 * i, (tid & 15) * 4)) = v[i];
+    }
+};
 template <class T>
 __device__ __forceinline__ void load_tile(float *to, const qgru_seq_tensor &x, long long base, int t0, int tokens, int d0, int d, int tid) {
-    const T *p = static_cast<const T *>(x.p) + base;
-    const bool wide = ((x.ts | x.bs | x.hs | d) & 3) == 0 && reinterpret_cast<uintptr_t>(x.p) % (4 * sizeof(T)) == 0;
-#pragma unroll
-    for (int e = tid; e < TILE / 4; e += THREADS) {
-        const int r = e >> 4, c = (e & 15) * 4;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < tokens && d0 + c < d) {
-            const T *q = p + (long long)(t0 + r) * x.ts + d0 + c;
-            if (wide) {
-                if constexpr (sizeof(T) == 4) {
-                    v = *reinterpret_cast<const float4 *>(q);
-                } else {
-                    const uint2 u = *reinterpret_cast<const uint2 *>(q);
-                    v = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
-                }
-            } else {
-                v.x = seq::to_f(q[0]);
-                if (d0 + c + 1 < d) v.y = seq::to_f(q[1]);
-                if (d0 + c + 2 < d) v.z = seq::to_f(q[2]);
-                if (d0 + c + 3 < d) v.w = seq::to_f(q[3]);
-            }
-        }
-        *reinterpret_cast<float4 *>(to + idx(r, c)) = v;
-    }
+    Four f;
+    f.load<T>(x, base, t0, tokens, d0, d, tid);
+    f.store(to, tid);
 }
 __device__ __forceinline__ void load_state(float *to, const float *S, int i0, int j0, const qgru_attention &a, int tid) {
 #pragma unroll
@@ -153,16 +170,17 @@ __device__ __forceinline__ void load_state(float *to, const float *S, int i0, in
 }
 __device__ __forceinline__ long long at(const qgru_seq_tensor &x, int b, int h) { return b * x.bs + h * x.hs; }
 
-// The chunk's running sums G[0 .. 63] (tokens behind the sequence add nothing).
-__device__ __forceinline__ void load_decays(float2 *G, double *sums, const qgru_attention &a, int b, int h, int t0, int tokens, int tid) {
-    double g = 0.0;
-    if (tid < C) {
-        if (tid < tokens) g = decay_log2(a, at(a.decay, b, h) + (long long)(t0 + tid) * a.decay.ts);
-        g = running_sum<C>(g, sums, tid);
-    }
+// G of a chunk by the first 64 threads, others pass
+__device__ __forceinline__ void sum_decays(float2 *G, double *sums, double g, int tid) {
+    if (tid < C) g = running_sum<C>(g, sums, tid);
     __syncthreads();
     if (tid < C) G[tid] = two_floats(g + (tid >= 32 ? sums[0] : 0.0));
     __syncthreads();
+}
+
+// The chunk's running sums G[0 .. 63] (tokens behind the sequence add nothing).
+__device__ __forceinline__ void load_decays(float2 *G, double *sums, const qgru_attention &a, int b, int h, int t0, int tokens, int tid) {
+    sum_decays(G, sums, tid < tokens ? decay_log2(a, at(a.decay, b, h) + (long long)(t0 + tid) * a.decay.ts) : 0.0, tid);
 }
 
 struct Pass {                      // a state pass
@@ -198,15 +216,29 @@ __global__ void __launch_bounds__(THREADS) k_states(const __grid_constant__ qgru
     if (!own_sums && first) each(S, tid, [&](int i, int j, float &s) { s = inside(i, j) ? first[tile + place(i, j)] : 0.f; });
     double all = 0.0;
     const int c_end = min((seg + 1) * p.per, p.chunks);
+    const auto chunk_of = [&](int c) { return Reverse ? p.chunks - 1 - c : c; };
+    const auto tokens_of = [&](int c) { return c < c_end ? min(max(n - chunk_of(c) * C, 0), C) : 0; };
+    // (four neighbouring columns a load; the next chunk's are on their way while one is worked on)
+    Four k4, v4;
+    double g = 0.0;
+    const auto load = [&](int c) {
+        const int tokens = tokens_of(c), t0 = chunk_of(c) * C;
+        k4.template load<T>(p.k, kb, t0, tokens, i0, a.Dk, tid);
+        v4.template load<T>(p.v, vb, t0, tokens, j0, a.Dv, tid);
+        g = tid < tokens ? decay_log2(a, at(a.decay, b, h) + (long long)(t0 + tid) * a.decay.ts) : 0.0;
+    };
+    if (seg * p.per < c_end) load(seg * p.per);
     for (int c = seg * p.per; c < c_end; ++c) {
-        const int chunk = Reverse ? p.chunks - 1 - c : c, t0 = chunk * C, tokens = min(max(n - t0, 0), C);
+        const int chunk = chunk_of(c), tokens = tokens_of(c);
         if (!own_sums) each(S, tid, [&](int i, int j, float &s) { if (inside(i, j)) p.states[chunk * size + tile + place(i, j)] = s; });
+        __syncthreads();
+        if (tokens) {
+            k4.store(K, tid);
+            v4.store(V, tid);
+        }
+        sum_decays(G, sums, g, tid);
+        if (c + 1 < c_end) load(c + 1);
         if (tokens == 0) continue;
-        __syncthreads();
-        load_decays(G, sums, a, b, h, t0, tokens, tid);
-        load_tile<T>(K, p.k, kb, t0, tokens, i0, a.Dk, tid);
-        load_tile<T>(V, p.v, vb, t0, tokens, j0, a.Dv, tid);
-        __syncthreads();
         const float2 end = G[C - 1];
         if (tid < C) W[tid] = Reverse ? a.scale * exp2_of(G[tid]) : exp2_diff(end, G[tid]);
         __syncthreads();
@@ -458,6 +490,210 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
     if (tid < all) seq::store_f(a.ddecay.p, gb + tid * a.ddecay.ts, a.decay_bf16, tid < tokens ? X[64 + tid] : 0.f);
 }
 
+// ------------------------------------------------------------------------------------- fp32, head sizes up to 64
+// Every chunk's tiles are fetched at once, asynchronously, into a tile each; then nothing waits for memory.  Sixteen warps, 16 x 16 sums a
+// warp.  32 x 200 tokens of 8 heads of 64: gradients 118 us tile after tile, with eight warps, three CTAs an SM.
+constexpr int ALL = 512, NT2 = 2;
+
+__device__ __forceinline__ void cp_float4(float *to, const float *from, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_float(float *to, const float *from, bool on) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(on ? 4 : 0) : "memory");
+}
+// `rows` rows of d floats, ld apart; zeros around them
+template <int N>
+__device__ __forceinline__ void fetch(float *to, const float *p, long long ld, int rows, int d, int tid) {
+    if (d % 4 == 0 && ld % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+        for (int e = tid; e < TILE / 4; e += N) {
+            const int r = e >> 4, c = (e & 15) * 4;
+            const bool on = r < rows && c < d;
+            cp_float4(to + idx(r, c), on ? p + r * ld + c : p, on);
+        }
+    } else {
+        for (int e = tid; e < TILE; e += N) {
+            const int r = e >> 6, c = e & 63;
+            const bool on = r < rows && c < d;
+            cp_float(to + idx(r, c), on ? p + r * ld + c : p, on);
+        }
+    }
+}
+__device__ __forceinline__ const float *token(const qgru_seq_tensor &x, long long base, int t0) { return static_cast<const float *>(x.p) + base + (long long)t0 * x.ts; }
+__device__ __forceinline__ void cp_all() {
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+__global__ void __launch_bounds__(THREADS, 2) k_outputs_small(const __grid_constant__ qgru_attention a, const float *states) {
+    extern __shared__ float4 smem4[];
+    float *Q = reinterpret_cast<float *>(smem4), *K = Q + TILE, *V = K + TILE, *S = V + TILE, *P = S + TILE;
+    __shared__ float2 G[C];
+    __shared__ double sums[2];
+    const int tid = threadIdx.x, heads = a.B * a.H, chunk = blockIdx.x / heads, bh = blockIdx.x % heads, b = bh / a.H, h = bh % a.H, t0 = chunk * C;
+    const int all = min(a.T - t0, C), tokens = min(max(valid_tokens(a, b) - t0, 0), C);
+    float *out = static_cast<float *>(a.out.p) + at(a.out, b, h) + t0 * a.out.ts;
+    if (tokens == 0) {
+        for (int e = tid; e < all * a.Dv; e += THREADS) out[(e / a.Dv) * a.out.ts + e % a.Dv] = 0.f;
+        return;
+    }
+    const int hk = h / (a.H / a.Hk);
+    const bool carried = chunk > 0 || a.state0;
+    fetch<THREADS>(Q, token(a.q, at(a.q, b, hk), t0), a.q.ts, tokens, a.Dk, tid);
+    fetch<THREADS>(K, token(a.k, at(a.k, b, hk), t0), a.k.ts, tokens, a.Dk, tid);
+    fetch<THREADS>(V, token(a.v, at(a.v, b, h), t0), a.v.ts, tokens, a.Dv, tid);
+    if (carried) fetch<THREADS>(S, states + chunk * (long long)heads * a.Dk * a.Dv + (long long)bh * a.Dk * a.Dv, a.Dv, a.Dk, a.Dv, tid);
+    const double g = tid < tokens ? decay_log2(a, at(a.decay, b, h) + (long long)(t0 + tid) * a.decay.ts) : 0.0;
+    cp_all();
+    sum_decays(G, sums, g, tid);
+    const int up_to = min((tid >> 5 & 3) * 2 + 2, eights(tokens));       // the pairs of a warp's 16 rows end in their columns
+    Acc c;
+    c.zero();
+    multiply<false, false>(c, Q, K, 0, eights(a.Dk), tid);
+    each(c, tid, [&](int t, int s, float &x) { P[idx(t, s)] = s <= t ? a.scale * exp2_diff(G[t], G[s]) * x : 0.f; });
+    // A later token's infinity or NaN is none of an earlier one's business, and zero times it is NaN.
+    int odd = 0;
+    for (int e = tid; e < TILE; e += THREADS) odd |= !isfinite(V[e]);
+    c.zero();
+    if (carried) {
+        multiply<false, true>(c, Q, S, 0, eights(a.Dk), tid);
+        each(c, tid, [&](int t, int, float &x) { x *= a.scale * exp2_of(G[t]); });
+    }
+    if (__syncthreads_or(odd)) {
+        each(c, tid, [&](int t, int n, float &x) {
+            for (int s = 0; s <= t; ++s) x = fmaf(P[idx(t, s)], V[idx(s, n)], x);
+        });
+    } else {
+        multiply<false, true>(c, P, V, 0, up_to, tid);
+    }
+    each(c, tid, [&](int t, int n, float &x) {
+        if (t < all && n < a.Dv) out[t * a.out.ts + n] = t < tokens ? x : 0.f;
+    });
+}
+
+__global__ void __launch_bounds__(ALL, 1) k_gradients_small(const __grid_constant__ qgru_attention a, const float *states, const float *dstates, float *dq_heads, float *dk_heads) {
+    extern __shared__ float4 smem4[];
+    float *Q = reinterpret_cast<float *>(smem4), *K = Q + TILE, *V = K + TILE, *O = V + TILE, *S = O + TILE, *dS = S + TILE, *P = dS + TILE, *E = P + TILE;
+    __shared__ float2 G[C];
+    __shared__ double sums[2], totals[2], through_of[ALL / 32];
+    __shared__ float rows[4][C], columns[4][C], q_dots[4][C], k_dots[4][C];
+    const int tid = threadIdx.x, lane = tid & 31, heads = a.B * a.H, chunk = blockIdx.x / heads, bh = blockIdx.x % heads, b = bh / a.H, h = bh % a.H, t0 = chunk * C;
+    const int all = min(a.T - t0, C), tokens = min(max(valid_tokens(a, b) - t0, 0), C);
+    const int hk = h / (a.H / a.Hk);
+    const auto put_qk = [&](const qgru_seq_tensor &x, float *heads_sums, int t, int d, float v) {
+        if (heads_sums)
+            heads_sums[(((long long)(t0 + t) * a.B + b) * a.H + h) * a.Dk + d] = v;
+        else
+            static_cast<float *>(x.p)[at(x, b, h) + (t0 + t) * x.ts + d] = v;
+    };
+    float *dv = static_cast<float *>(a.dv.p) + at(a.dv, b, h) + t0 * a.dv.ts;
+    const long long gb = at(a.ddecay, b, h) + t0 * a.ddecay.ts;
+    if (tokens == 0) {
+        for (int e = tid; e < all * a.Dk; e += ALL) {
+            put_qk(a.dq, dq_heads, e / a.Dk, e % a.Dk, 0.f);
+            put_qk(a.dk, dk_heads, e / a.Dk, e % a.Dk, 0.f);
+        }
+        for (int e = tid; e < all * a.Dv; e += ALL) dv[(e / a.Dv) * a.dv.ts + e % a.Dv] = 0.f;
+        if (tid < all) seq::store_f(a.ddecay.p, gb + tid * a.ddecay.ts, a.decay_bf16, 0.f);
+        return;
+    }
+    const long long tile = chunk * (long long)heads * a.Dk * a.Dv + (long long)bh * a.Dk * a.Dv;
+    fetch<ALL>(Q, token(a.q, at(a.q, b, hk), t0), a.q.ts, tokens, a.Dk, tid);
+    fetch<ALL>(K, token(a.k, at(a.k, b, hk), t0), a.k.ts, tokens, a.Dk, tid);
+    fetch<ALL>(V, token(a.v, at(a.v, b, h), t0), a.v.ts, tokens, a.Dv, tid);
+    fetch<ALL>(O, token(a.dout, at(a.dout, b, h), t0), a.dout.ts, tokens, a.Dv, tid);
+    fetch<ALL>(S, states + tile, a.Dv, a.Dk, a.Dv, tid);
+    fetch<ALL>(dS, dstates + tile, a.Dv, a.Dk, a.Dv, tid);
+    const double g = tid < tokens ? decay_log2(a, at(a.decay, b, h) + (long long)(t0 + tid) * a.decay.ts) : 0.0;
+    if (tid < 4 * C) q_dots[0][tid] = k_dots[0][tid] = 0.f;
+    cp_all();
+    sum_decays(G, sums, g, tid);
+    const float2 end = G[C - 1];
+    const int ek = eights(a.Dk), ev = eights(a.Dv), last = eights(tokens), diagonal = (tid >> 5 & 3) * 2;
+    Sums<NT2> c, e;
+    c.zero();
+    e.zero();
+    multiply<false, false>(c, Q, K, 0, ek, tid);
+    multiply<false, false>(e, O, V, 0, ev, tid);
+    {
+        const int m = (tid >> 5 & 3) * 16 + (lane >> 2), n = (tid >> 7) * (8 * NT2) + (lane & 3) * 2;
+        float row[2] = {0.f, 0.f}, column[NT2][2];
+#pragma unroll
+        for (int j = 0; j < NT2; ++j) {
+            column[j][0] = column[j][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = m + (i >> 1) * 8, s = n + j * 8 + (i & 1);
+                const bool on = s <= t;
+                const float w = on ? a.scale * exp2_diff(G[t], G[s]) : 0.f, p = on ? w * c.v[j][i] : 0.f;
+                P[idx(t, s)] = p;
+                E[idx(t, s)] = on ? w * e.v[j][i] : 0.f;
+                // every pair, s < t: a change of G_t adds, one of G_s takes away
+                const float x = s < t ? p * e.v[j][i] : 0.f;
+                row[i >> 1] += x;
+                column[j][i & 1] += x;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            row[i] += __shfl_xor_sync(0xffffffffu, row[i], 1);
+            row[i] += __shfl_xor_sync(0xffffffffu, row[i], 2);
+            if ((lane & 3) == 0) rows[tid >> 7][m + 8 * i] = row[i];
+#pragma unroll
+            for (int j = 0; j < NT2; ++j) {
+                float x = column[j][i];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                if (lane < 4) columns[tid >> 5 & 3][n + 8 * j + i] = x;
+            }
+        }
+    }
+    {
+        double x = 0.0;
+        for (int i = tid; i < TILE; i += ALL) x += (double)S[i] * (double)dS[i];       // (the same order in both)
+        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        if (lane == 0) through_of[tid >> 5] = x;
+    }
+    __syncthreads();
+    // dq = E k + scale 2^G_t dout S^T
+    c.zero();
+    multiply<false, false>(c, O, S, 0, ev, tid);
+    scale_rows(c, Q, q_dots[0], [&](int t) { return a.scale * exp2_of(G[t]); }, tid);
+    multiply<false, true>(c, E, K, 0, min(diagonal + 2, last), tid);
+    each(c, tid, [&](int t, int d, float &x) { if (t < all && d < a.Dk) put_qk(a.dq, dq_heads, t, d, t < tokens ? x : 0.f); });
+    // dk = E^T q + 2^(G_C - G_s) v dS^T
+    c.zero();
+    multiply<false, false>(c, V, dS, 0, ev, tid);
+    scale_rows(c, K, k_dots[0], [&](int s) { return exp2_diff(end, G[s]); }, tid);
+    multiply<true, true>(c, E, Q, diagonal, last, tid);
+    each(c, tid, [&](int s, int d, float &x) { if (s < all && d < a.Dk) put_qk(a.dk, dk_heads, s, d, s < tokens ? x : 0.f); });
+    // dv = P^T dout + 2^(G_C - G_s) k dS
+    c.zero();
+    multiply<false, true>(c, K, dS, 0, ek, tid);
+    each(c, tid, [&](int s, int, float &x) { x *= exp2_diff(end, G[s]); });
+    multiply<true, true>(c, P, O, diagonal, last, tid);
+    each(c, tid, [&](int s, int d, float &x) { if (s < all && d < a.Dv) dv[s * a.dv.ts + d] = s < tokens ? x : 0.f; });
+    __syncthreads();
+    // the decays' gradient: sum over u >= t of dG_u, the shares of k_s for s < t, and what passes from the state before the chunk to that behind it
+    double own = 0.0, before = 0.0;
+    if (tid < C) {
+        double kd = 0.0;
+        for (int w = 0; w < 4; ++w) {
+            own += (double)rows[w][tid] - (double)columns[w][tid] + (double)q_dots[w][tid];
+            kd += (double)k_dots[w][tid];
+        }
+        before = running_sum<C>(kd - own, sums, tid) - (kd - own);
+        for (int o = 16; o; o >>= 1) own += __shfl_xor_sync(0xffffffffu, own, o);
+        if (lane == 0) totals[tid >> 5] = own;
+    }
+    __syncthreads();
+    if (tid < all) {
+        double through = 0.0;
+        for (int w = 0; w < ALL / 32; ++w) through += through_of[w];
+        const double x = before + (tid >= 32 ? sums[0] : 0.0) + totals[0] + totals[1] + through * (double)exp2_of(end);
+        seq::store_f(a.ddecay.p, gb + tid * a.ddecay.ts, a.decay_bf16, tid < tokens ? (float)x : 0.f);
+    }
+}
+
 // dq and dk of heads that share q and k: the sum over each group, one rounding.  V neighbouring elements a thread.
 template <class T, int V>
 __global__ void k_sum_groups(const __grid_constant__ qgru_attention a, const float *dq, const float *dk) {
@@ -528,6 +764,13 @@ int forward(const qgru_attention &a, const Cut &c, cudaStream_t st) {
     char *seg = static_cast<char *>(a.workspace) + (a.keep ? 0 : a256(c.states));
     if (const int rc = run_states<T, false>(a, c, states, seg, st)) return rc;
     if (c.chunks == 0) return QGRU_OK;
+    if (std::is_same<T, float>::value && a.Dk <= 64 && a.Dv <= 64) {
+        constexpr size_t bytes = 5 * TILE * sizeof(float);
+        if (const int rc = with_smem(k_outputs_small, bytes)) return rc;
+        k_outputs_small<<<c.chunks * a.B * a.H, THREADS, bytes, st>>>(a, states);
+        SEQ_CK(cudaGetLastError());
+        return QGRU_OK;
+    }
     constexpr size_t bytes = 3 * TILE * sizeof(float);
     if (const int rc = with_smem(k_outputs<T>, bytes)) return rc;
     k_outputs<T><<<c.chunks * a.B * a.H, THREADS, bytes, st>>>(a, states);
@@ -549,9 +792,16 @@ int backward(const qgru_attention &a, const Cut &c, cudaStream_t st) {
         dq = reinterpret_cast<float *>(ws);
         dk = dq + group_bytes(a) / 8;
     }
-    constexpr size_t bytes = 4 * TILE * sizeof(float);
-    if (const int rc = with_smem(k_gradients<T>, bytes)) return rc;
-    k_gradients<T><<<c.chunks * a.B * a.H, THREADS, bytes, st>>>(a, static_cast<const float *>(a.states), dstates, dq, dk);
+    const float *states = static_cast<const float *>(a.states);
+    if (std::is_same<T, float>::value && a.Dk <= 64 && a.Dv <= 64) {
+        constexpr size_t bytes = 8 * TILE * sizeof(float);
+        if (const int rc = with_smem(k_gradients_small, bytes)) return rc;
+        k_gradients_small<<<c.chunks * a.B * a.H, ALL, bytes, st>>>(a, states, dstates, dq, dk);
+    } else {
+        constexpr size_t bytes = 4 * TILE * sizeof(float);
+        if (const int rc = with_smem(k_gradients<T>, bytes)) return rc;
+        k_gradients<T><<<c.chunks * a.B * a.H, THREADS, bytes, st>>>(a, states, dstates, dq, dk);
+    }
     SEQ_CK(cudaGetLastError());
     return dq ? sum_groups(a, dq, dk, st) : QGRU_OK;
 }
