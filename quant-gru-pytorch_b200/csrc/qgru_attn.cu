@@ -48,16 +48,31 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], const
 // else n.  fp32 by warp-level tensor instructions: each operand is the sum of two tf32 values of 11 bits (off by 2^-22 of it at the most,
 // 2^-25 in the mean), and of the four products the one of the two small parts is left out (2^-22 of the product at the most).  Operands
 // below 2^-114 keep 11 bits.
+// Where a lane's value of eight K lies in a tile for K = 0 .. 7 (bytes), and for K = 8 s .. 8 s + 7 after it: the swizzle is a change of bits
+// that both depend on.  line: the row or column that is not K; up: 0 or 4 of the eight.
+template <bool KRows>
+__device__ __forceinline__ uint32_t first_at(int line, int t, int up) { return (uint32_t)idx(KRows ? t + up : line, KRows ? line : t + up) * 4; }
+template <bool KRows>
+__device__ __forceinline__ float value_at(const float *tile, uint32_t first, int s) {
+    const uint32_t at = KRows ? (first ^ (uint32_t)(s << 4)) + (uint32_t)(s << 11) : first ^ (uint32_t)(s << 5);
+    return *reinterpret_cast<const float *>(reinterpret_cast<const char *>(tile) + at);
+}
 template <bool ARows, bool BRows, int NT>
 __device__ __forceinline__ void multiply(Sums<NT> &c, const float *A, const float *B, int from, int to, int tid) {
     const int lane = tid & 31, g = lane >> 2, t = lane & 3, m = (tid >> 5 & 3) * 16 + g, n = (tid >> 7) * (8 * NT) + g;
+    uint32_t pa[4], pb[NT][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pa[i] = first_at<ARows>(m + (i & 1) * 8, t, (i >> 1) * 4);
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) pb[j][i] = first_at<BRows>(n + 8 * j, t, 4 * i);
 #pragma unroll 2
-    for (int k = 8 * from + t; k < 8 * to; k += 8) {
+    for (int s = from; s < to; ++s) {
         uint32_t ah[4], al[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int row = m + (i & 1) * 8, kk = k + (i >> 1) * 4;
-            const float x = A[ARows ? idx(kk, row) : idx(row, kk)];
+            const float x = value_at<ARows>(A, pa[i], s);
             ah[i] = tf32(x);
             al[i] = tf32(x - __uint_as_float(ah[i]));
         }
@@ -66,7 +81,7 @@ __device__ __forceinline__ void multiply(Sums<NT> &c, const float *A, const floa
             uint32_t bh[2], bl[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float x = B[BRows ? idx(k + 4 * i, n + 8 * j) : idx(n + 8 * j, k + 4 * i)];
+                const float x = value_at<BRows>(B, pb[j][i], s);
                 bh[i] = tf32(x);
                 bl[i] = tf32(x - __uint_as_float(bh[i]));
             }
