@@ -34,10 +34,11 @@ struct Sums {
     }
 };
 using Acc = Sums<4>;
-__device__ __forceinline__ uint32_t tf32(float x) {
-    uint32_t r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-    return r;
+// x as two tf32 values (11 significant bits): the nearest one, and of the rest, which has twelve bits at the most, all but the last.  A NaN
+// whose bits run over in the first is one in the second.  (By hand: the conversion instruction is three times the work.)
+__device__ __forceinline__ void two_tf32(float x, uint32_t &hi, uint32_t &lo) {
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
     asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -45,9 +46,8 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], const
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 // acc += sum over k = 8 from .. 8 to - 1 of A(m, k) B(k, n).  ARows: A's tile has k as its rows, else m; BRows: B's tile has k as its rows,
-// else n.  fp32 by warp-level tensor instructions: each operand is the sum of two tf32 values of 11 bits (off by 2^-22 of it at the most,
-// 2^-25 in the mean), and of the four products the one of the two small parts is left out (2^-22 of the product at the most).  Operands
-// below 2^-114 keep 11 bits.
+// else n.  fp32 by warp-level tensor instructions: each operand is the sum of two tf32 values (off by 2^-23 of it at the most), and of the
+// four products the one of the two small parts is left out (2^-22 of the product at the most).  Operands below 2^-114 keep 11 bits.
 // Where a lane's value of eight K lies in a tile for K = 0 .. 7 (bytes), and for K = 8 s .. 8 s + 7 after it: the swizzle is a change of bits
 // that both depend on.  line: the row or column that is not K; up: 0 or 4 of the eight.
 template <bool KRows>
@@ -72,18 +72,14 @@ __device__ __forceinline__ void multiply(Sums<NT> &c, const float *A, const floa
         uint32_t ah[4], al[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float x = value_at<ARows>(A, pa[i], s);
-            ah[i] = tf32(x);
-            al[i] = tf32(x - __uint_as_float(ah[i]));
+            two_tf32(value_at<ARows>(A, pa[i], s), ah[i], al[i]);
         }
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             uint32_t bh[2], bl[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float x = value_at<BRows>(B, pb[j][i], s);
-                bh[i] = tf32(x);
-                bl[i] = tf32(x - __uint_as_float(bh[i]));
+                two_tf32(value_at<BRows>(B, pb[j][i], s), bh[i], bl[i]);
             }
             mma(c.v[j], al, bh);
             mma(c.v[j], ah, bl);
