@@ -24,13 +24,13 @@ constexpr int THREADS = 256;
 
 // Rows t0 .. t0 + 127 of a tensor (zeros from `tokens` on and behind its columns) as a tile of D columns.  Vec: rows and strides
 // are multiples of 16 bytes; else element by element.
-template <int D, bool Vec>
+template <int D, bool Vec, int N = THREADS>
 __device__ __forceinline__ void load_rows(uint32_t tile, const qgru_seq_tensor &x, long long base, int t0, int tokens, int d, int tid) {
     const bf16 *p = static_cast<const bf16 *>(x.p) + base + (long long)t0 * x.ts;
     constexpr int PER_ROW = D / 8;
 #pragma unroll
-    for (int i = 0; i < C * PER_ROW / THREADS; ++i) {
-        const int e = i * THREADS + tid, r = e / PER_ROW, c = e % PER_ROW;
+    for (int i = 0; i < C * PER_ROW / N; ++i) {
+        const int e = i * N + tid, r = e / PER_ROW, c = e % PER_ROW;
         const uint32_t to = tile + (c >> 3) * PANEL + chunk_at(r, c & 7);
         if constexpr (Vec) {
             const bool on = r < tokens && c * 8 < d;
@@ -49,11 +49,11 @@ __device__ __forceinline__ void load_rows(uint32_t tile, const qgru_seq_tensor &
     }
 }
 // A state [DK][DV] as it is kept before each chunk (bf16, padded) as a tile.
-template <int DK, int DV>
+template <int DK, int DV, int N = THREADS>
 __device__ __forceinline__ void load_state(uint32_t tile, const bf16 *S, int tid) {
 #pragma unroll
-    for (int i = 0; i < DK * DV / 8 / THREADS; ++i) {
-        const int e = i * THREADS + tid, r = e / (DV / 8), c = e % (DV / 8);
+    for (int i = 0; i < DK * DV / 8 / N; ++i) {
+        const int e = i * N + tid, r = e / (DV / 8), c = e % (DV / 8);
         cp_async(tile + (c >> 3) * (DK * 128) + chunk_at(r, c & 7), S + e * 8, 16);
     }
 }
@@ -378,6 +378,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant
 }
 
 // ------------------------------------------------------------------------------------- gradients
+constexpr int GRAD_THREADS = 512;
 struct Gradients {
     const bf16 *states, *dstates;
     float *dq_heads, *dk_heads;          // [T][B][H][Dk] where heads share q and k, else null
@@ -433,46 +434,46 @@ __device__ __forceinline__ float scale_sums(uint32_t taddr, float w, uint32_t ti
 
 // grid: chunks x B H.  Pairs lie as [s][t] here, lane s of tensor memory.  Four blocks of 128 columns of it:
 //   0  (k q^T), then P^T in bf16     1  (v dout^T), then dv     2  dk     3  dq
-// P^T is the operand of dv from tensor memory, E^T that of dk (K in its columns) and of dq (K in its rows) from shared memory.
+// Four threads a row, a quarter of the columns each.  P^T is the operand of dv from tensor memory, E^T that of dk (K in its columns) and of dq (K in its rows) from shared memory.
 template <int DK, int DV, bool Vec>
-__global__ void __launch_bounds__(THREADS) k_gradients_tc(const __grid_constant__ qgru_attention a, const __grid_constant__ Gradients p) {
+__global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_constant__ qgru_attention a, const __grid_constant__ Gradients p) {
     extern __shared__ unsigned char raw[];
     unsigned char *tiles = tiles_of(raw);
     Shared &s = *reinterpret_cast<Shared *>(tiles + GRADIENTS_TILES<DK, DV>);
-    constexpr int KT = DK / 64 * PANEL, VT = DV / 64 * PANEL, ST = DK * DV * 2, KHALF = DK / 2, VHALF = DV / 2;
+    constexpr int KT = DK / 64 * PANEL, VT = DV / 64 * PANEL, ST = DK * DV * 2, KQ = DK / 4, VQ = DV / 4;
     const uint32_t q_t = tc::smem_u32(tiles), k_t = q_t + KT, v_t = k_t + KT, o_t = v_t + VT, S_t = o_t + VT, dS_t = S_t + ST, E_t = dS_t + ST;
     // once v has been used, its tile holds sums by token
     float *t_sums = reinterpret_cast<float *>(tiles + 2 * KT);          // [4][128] over s of a block's lanes, for each t
-    float *s_sums = t_sums + 4 * C, *q_dots = s_sums + 2 * C, *k_dots = q_dots + 2 * C;     // [2][128] each
-    double *warp_part = reinterpret_cast<double *>(k_dots + 2 * C);     // [8]
+    float *s_sums = t_sums + 4 * C, *q_dots = s_sums + 4 * C, *k_dots = q_dots + 4 * C;     // [4][128] each
+    double *warp_part = reinterpret_cast<double *>(k_dots + 4 * C);     // [16]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, heads = a.B * a.H, chunk = blockIdx.x / heads, bh = blockIdx.x % heads, b = bh / a.H, h = bh % a.H;
     const int t0 = chunk * C, all = min(a.T - t0, C), tokens = min(max(valid_tokens(a, b) - t0, 0), C);
-    const int block = warp & 3, row = block * 32 + lane, half = warp >> 2;
-    const auto put_qk = [&](const qgru_seq_tensor &x, float *heads_sums, const float (&v)[KHALF]) {
+    const int block = warp & 3, row = block * 32 + lane, part = warp >> 2;
+    const auto put_qk = [&](const qgru_seq_tensor &x, float *heads_sums, const float (&v)[KQ]) {
         if (row >= all) return;
-        const int c0 = half * KHALF;
+        const int c0 = part * KQ;
         if (heads_sums) {
             float *to = heads_sums + (((long long)(t0 + row) * a.B + b) * a.H + h) * a.Dk + c0;
 #pragma unroll
-            for (int i = 0; i < KHALF; ++i)
+            for (int i = 0; i < KQ; ++i)
                 if (c0 + i < a.Dk) to[i] = v[i];
         } else {
             store_row(static_cast<bf16 *>(x.p) + at(x, b, h) + (long long)(t0 + row) * x.ts, v, c0, a.Dk,
                       a.Dk % 8 == 0 && (x.ts | x.bs | x.hs) % 8 == 0 && reinterpret_cast<uintptr_t>(x.p) % 16 == 0);
         }
     };
-    const auto put_v = [&](const float (&v)[VHALF]) {
+    const auto put_v = [&](const float (&v)[VQ]) {
         if (row < all)
-            store_row(static_cast<bf16 *>(a.dv.p) + at(a.dv, b, h) + (long long)(t0 + row) * a.dv.ts, v, half * VHALF, a.Dv,
+            store_row(static_cast<bf16 *>(a.dv.p) + at(a.dv, b, h) + (long long)(t0 + row) * a.dv.ts, v, part * VQ, a.Dv,
                       a.Dv % 8 == 0 && (a.dv.ts | a.dv.bs | a.dv.hs) % 8 == 0 && reinterpret_cast<uintptr_t>(a.dv.p) % 16 == 0);
     };
     const long long gb = at(a.ddecay, b, h) + (long long)t0 * a.ddecay.ts;
     if (tokens == 0) {
-        float z[KHALF], y[VHALF];
+        float z[KQ], y[VQ];
 #pragma unroll
-        for (int i = 0; i < KHALF; ++i) z[i] = 0.f;
+        for (int i = 0; i < KQ; ++i) z[i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < VHALF; ++i) y[i] = 0.f;
+        for (int i = 0; i < VQ; ++i) y[i] = 0.f;
         put_qk(a.dq, p.dq_heads, z);
         put_qk(a.dk, p.dk_heads, z);
         put_v(y);
@@ -481,14 +482,14 @@ __global__ void __launch_bounds__(THREADS) k_gradients_tc(const __grid_constant_
     }
     const int hk = h / (a.H / a.Hk);
     const long long state = ((long long)chunk * heads + bh) * (DK * DV);
-    load_rows<DK, Vec>(q_t, a.q, at(a.q, b, hk), t0, tokens, a.Dk, tid);
-    load_rows<DK, Vec>(k_t, a.k, at(a.k, b, hk), t0, tokens, a.Dk, tid);
+    load_rows<DK, Vec, GRAD_THREADS>(q_t, a.q, at(a.q, b, hk), t0, tokens, a.Dk, tid);
+    load_rows<DK, Vec, GRAD_THREADS>(k_t, a.k, at(a.k, b, hk), t0, tokens, a.Dk, tid);
     cp_commit();
-    load_rows<DV, Vec>(v_t, a.v, at(a.v, b, h), t0, tokens, a.Dv, tid);
-    load_rows<DV, Vec>(o_t, a.dout, at(a.dout, b, h), t0, tokens, a.Dv, tid);
+    load_rows<DV, Vec, GRAD_THREADS>(v_t, a.v, at(a.v, b, h), t0, tokens, a.Dv, tid);
+    load_rows<DV, Vec, GRAD_THREADS>(o_t, a.dout, at(a.dout, b, h), t0, tokens, a.Dv, tid);
     cp_commit();
-    load_state<DK, DV>(S_t, p.states + state, tid);
-    load_state<DK, DV>(dS_t, p.dstates + state, tid);
+    load_state<DK, DV, GRAD_THREADS>(S_t, p.states + state, tid);
+    load_state<DK, DV, GRAD_THREADS>(dS_t, p.dstates + state, tid);
     cp_commit();
     const double g = load_decay(a, b, h, t0, tokens, tid);
     begin(s, 512, tid);
@@ -520,25 +521,21 @@ __global__ void __launch_bounds__(THREADS) k_gradients_tc(const __grid_constant_
     await(s, 1, 0);
     const float2 G = s.G[row], last = s.G[C - 1];
     // the pairs: blocks of 32 x 32, t from s on
-    uint32_t P[32];
+    uint32_t P[16];
     float s_sum = 0.f;
+    if (part < block) {
 #pragma unroll
-    for (int jb = 0; jb < 2; ++jb) {
-        const int tb = half * 2 + jb;
+        for (int i = 0; i < 16; ++i) P[i] = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + i), 0u, 0u, 0u, 0u);
+    } else {
         float m[32];
-        if (tb < block) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) P[jb * 16 + i] = 0u;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sts16(E_t + half * PANEL + chunk_at(row, jb * 4 + i), 0u, 0u, 0u, 0u);
-            continue;
-        }
-        const float r = a.scale * (tb > block ? ex2_diff(s.G[tb * 32 - 1], G) : 1.f);
+        const float r = a.scale * (part > block ? ex2_diff(s.G[part * 32 - 1], G) : 1.f);
 #pragma unroll
         for (int i8 = 0; i8 < 32; i8 += 16) {
             float x[16], y[16];
-            tmem_load(base + half * 64 + jb * 32 + i8, x);
-            tmem_load(base + 128 + half * 64 + jb * 32 + i8, y);
+            tmem_load(base + part * 32 + i8, x);
+            tmem_load(base + 128 + part * 32 + i8, y);
             uint32_t e[8];
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
@@ -546,28 +543,28 @@ __global__ void __launch_bounds__(THREADS) k_gradients_tc(const __grid_constant_
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int t = i8 + i + j;
-                    const float w = tb > block ? r * s.f[tb * 32 + t] : t >= lane ? a.scale * ex2_diff(s.G[tb * 32 + t], G) : 0.f;
-                    const bool on = tb > block || t >= lane;
+                    const float w = part > block ? r * s.f[part * 32 + t] : t >= lane ? a.scale * ex2_diff(s.G[part * 32 + t], G) : 0.f;
+                    const bool on = part > block || t >= lane;
                     pv[j] = on ? w * x[i + j] : 0.f;
                     ev[j] = on ? w * y[i + j] : 0.f;
-                    m[t] = tb > block || t > lane ? pv[j] * y[i + j] : 0.f;
+                    m[t] = part > block || t > lane ? pv[j] * y[i + j] : 0.f;
                     s_sum += m[t];
                 }
-                P[jb * 16 + (i8 + i) / 2] = pack(pv[0], pv[1]);
+                P[(i8 + i) / 2] = pack(pv[0], pv[1]);
                 e[i / 2] = pack(ev[0], ev[1]);
             }
-            sts16(E_t + half * PANEL + chunk_at(row, jb * 4 + i8 / 8), e[0], e[1], e[2], e[3]);
-            sts16(E_t + half * PANEL + chunk_at(row, jb * 4 + i8 / 8 + 1), e[4], e[5], e[6], e[7]);
+            sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + i8 / 8), e[0], e[1], e[2], e[3]);
+            sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + i8 / 8 + 1), e[4], e[5], e[6], e[7]);
         }
-        t_sums[block * C + tb * 32 + lane] = sum_columns(m, lane);
+        t_sums[block * C + part * 32 + lane] = sum_columns(m, lane);
     }
-    s_sums[half * C + row] = s_sum;
+    s_sums[part * C + row] = s_sum;
     const float to_end = ex2_diff(last, G), from_start = a.scale * ex2(G.x + G.y);
-    k_dots[half * C + row] = scale_sums<KHALF>(base + 256 + half * KHALF, to_end, k_t, row, half * KHALF, true);
-    q_dots[half * C + row] = scale_sums<KHALF>(base + 384 + half * KHALF, from_start, q_t, row, half * KHALF, true);
+    k_dots[part * C + row] = scale_sums<KQ>(base + 256 + part * KQ, to_end, k_t, row, part * KQ, true);
+    q_dots[part * C + row] = scale_sums<KQ>(base + 384 + part * KQ, from_start, q_t, row, part * KQ, true);
     {
         double x = 0.0;
-        for (int e = tid; e < DK * DV / 8; e += THREADS) {
+        for (int e = tid; e < DK * DV / 8; e += GRAD_THREADS) {
             const uint4 u = lds16(S_t + e * 16), w = lds16(dS_t + e * 16);      // (the same order in both)
             float f = low(u.x) * low(w.x);
             f = fmaf(high(u.x), high(w.x), f);
@@ -596,23 +593,27 @@ __global__ void __launch_bounds__(THREADS) k_gradients_tc(const __grid_constant_
         commit(leader, &s.bar[3]);
     }
     tc::tc_fence_after_sync();
-    tmem_store(base + half * 32, P);
+    tmem_store(base + part * 16, P);
     // the decays' gradient: from each token on, every pair across it, and what passes from the state before the chunk to that behind it
     double d = 0.0, own = 0.0;
     if (tid < C) {
         float t_sum = 0.f;
         for (int w = 0; w <= tid >> 5; ++w) t_sum += t_sums[w * C + tid];
-        own = (double)t_sum - (double)s_sums[tid] - (double)s_sums[C + tid] + (double)q_dots[tid] + (double)q_dots[C + tid];
-        const double kd = (double)k_dots[tid] + (double)k_dots[C + tid];
+        own = (double)t_sum;
+        double kd = 0.0;
+        for (int w = 0; w < 4; ++w) {
+            own += (double)q_dots[w * C + tid] - (double)s_sums[w * C + tid];
+            kd += (double)k_dots[w * C + tid];
+        }
         d = running_sum<C>(kd - own, s.sums, tid) - (kd - own);
     }
     double total = own;
     for (int i = 16; i; i >>= 1) total += __shfl_xor_sync(0xffffffffu, total, i);
-    double *totals = warp_part + 8;
+    double *totals = warp_part + 16;
     if (lane == 0 && tid < C) totals[warp] = total;
     tc::tmem_st_wait();
     await(s, 2, 0);
-    scale_sums<VHALF>(base + 128 + half * VHALF, to_end, 0, 0, 0, false);
+    scale_sums<VQ>(base + 128 + part * VQ, to_end, 0, 0, 0, false);
     tc::tmem_st_wait();
     tc::tc_fence_before_sync();
     __syncthreads();
@@ -626,29 +627,29 @@ __global__ void __launch_bounds__(THREADS) k_gradients_tc(const __grid_constant_
         double x = d;
         for (int w = 0; w < tid >> 5; ++w) x += s.sums[w];
         double through = 0.0;
-        for (int w = 0; w < 8; ++w) through += warp_part[w];
+        for (int w = 0; w < GRAD_THREADS / 32; ++w) through += warp_part[w];
         x += totals[0] + totals[1] + totals[2] + totals[3] + through * (double)exp2_of(last);
         seq::store_f(a.ddecay.p, gb + tid * a.ddecay.ts, a.decay_bf16, tid < tokens ? (s.failed ? NAN : (float)x) : 0.f);
     }
     await(s, 3, 0);
     const bool live = row < tokens, bad = s.failed;
     {
-        float x[KHALF];
-        tmem_load(base + 384 + half * KHALF, x);
+        float x[KQ];
+        tmem_load(base + 384 + part * KQ, x);
 #pragma unroll
-        for (int i = 0; i < KHALF; ++i) x[i] = live ? (bad ? NAN : x[i]) : 0.f;
+        for (int i = 0; i < KQ; ++i) x[i] = live ? (bad ? NAN : x[i]) : 0.f;
         put_qk(a.dq, p.dq_heads, x);
-        tmem_load(base + 256 + half * KHALF, x);
+        tmem_load(base + 256 + part * KQ, x);
 #pragma unroll
-        for (int i = 0; i < KHALF; ++i) x[i] = live ? (bad ? NAN : x[i]) : 0.f;
+        for (int i = 0; i < KQ; ++i) x[i] = live ? (bad ? NAN : x[i]) : 0.f;
         put_qk(a.dk, p.dk_heads, x);
     }
     await(s, 2, 1);
     {
-        float x[VHALF];
-        tmem_load(base + 128 + half * VHALF, x);
+        float x[VQ];
+        tmem_load(base + 128 + part * VQ, x);
 #pragma unroll
-        for (int i = 0; i < VHALF; ++i) x[i] = live ? (s.failed ? NAN : x[i]) : 0.f;
+        for (int i = 0; i < VQ; ++i) x[i] = live ? (s.failed ? NAN : x[i]) : 0.f;
         put_v(x);
     }
     end(s, 512, p.flag, tid);
@@ -723,7 +724,7 @@ int backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStre
     }
     int bytes = 0;
     if (const int rc = with_smem(k_gradients_tc<DK, DV, Vec>, GRADIENTS_TILES<DK, DV>, &bytes)) return rc;
-    k_gradients_tc<DK, DV, Vec><<<c.chunks * a.B * a.H, THREADS, bytes, st>>>(a, g);
+    k_gradients_tc<DK, DV, Vec><<<c.chunks * a.B * a.H, GRAD_THREADS, bytes, st>>>(a, g);
     SEQ_CK(cudaGetLastError());
     return g.dq_heads ? sum_groups(a, g.dq_heads, g.dk_heads, st) : QGRU_OK;
 }
