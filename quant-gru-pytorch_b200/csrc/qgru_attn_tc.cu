@@ -435,6 +435,37 @@ __device__ __forceinline__ float scale_sums(uint32_t taddr, float w, uint32_t ti
 // grid: chunks x B H.  Pairs lie as [s][t] here, lane s of tensor memory.  Four blocks of 128 columns of it:
 //   0  (k q^T), then P^T in bf16     1  (v dout^T), then dv     2  dk     3  dq
 // Four threads a row, a quarter of the columns each.  P^T is the operand of dv from tensor memory, E^T that of dk (K in its columns) and of dq (K in its rows) from shared memory.
+// A row's Cols values from column c0 on, as bf16, into a tile; and the tile's rows below `rows` into a tensor, whole lines at a time.
+template <int Cols>
+__device__ __forceinline__ void put_row(uint32_t tile, int row, int c0, const float (&v)[Cols]) {
+#pragma unroll
+    for (int i = 0; i < Cols; i += 8) {
+        const int c = (c0 + i) / 8;
+        sts16(tile + (c >> 3) * PANEL + chunk_at(row, c & 7), pack(v[i], v[i + 1]), pack(v[i + 2], v[i + 3]), pack(v[i + 4], v[i + 5]), pack(v[i + 6], v[i + 7]));
+    }
+}
+template <int D>
+__device__ __forceinline__ void copy_out(uint32_t tile, const qgru_seq_tensor &x, long long base, int t0, int rows, int d, int tid) {
+    bf16 *p = static_cast<bf16 *>(x.p) + base + (long long)t0 * x.ts;
+    const bool vec = d % 8 == 0 && (x.ts | x.bs | x.hs) % 8 == 0 && reinterpret_cast<uintptr_t>(x.p) % 16 == 0;
+    constexpr int PER_ROW = D / 8;
+#pragma unroll
+    for (int i = 0; i < C * PER_ROW / GRAD_THREADS; ++i) {
+        const int e = i * GRAD_THREADS + tid, r = e / PER_ROW, c = e % PER_ROW;
+        if (r >= rows || c * 8 >= d) continue;
+        const uint4 v = lds16(tile + (c >> 3) * PANEL + chunk_at(r, c & 7));
+        bf16 *to = p + (long long)r * x.ts + c * 8;
+        if (vec) {
+            *reinterpret_cast<uint4 *>(to) = v;
+        } else {
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c * 8 + j < d) to[j] = __ushort_as_bfloat16((unsigned short)(w[j / 2] >> (j & 1) * 16));
+        }
+    }
+}
+
 template <int DK, int DV, bool Vec>
 __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_constant__ qgru_attention a, const __grid_constant__ Gradients p) {
     extern __shared__ unsigned char raw[];
@@ -449,39 +480,40 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, heads = a.B * a.H, chunk = blockIdx.x / heads, bh = blockIdx.x % heads, b = bh / a.H, h = bh % a.H;
     const int t0 = chunk * C, all = min(a.T - t0, C), tokens = min(max(valid_tokens(a, b) - t0, 0), C);
     const int block = warp & 3, row = block * 32 + lane, part = warp >> 2;
-    const auto put_qk = [&](const qgru_seq_tensor &x, float *heads_sums, const float (&v)[KQ]) {
+    const auto put_heads = [&](float *sums, const float (&v)[KQ]) {        // heads that share q and k: fp32, added up afterwards
         if (row >= all) return;
         const int c0 = part * KQ;
-        if (heads_sums) {
-            float *to = heads_sums + (((long long)(t0 + row) * a.B + b) * a.H + h) * a.Dk + c0;
+        float *to = sums + (((long long)(t0 + row) * a.B + b) * a.H + h) * a.Dk + c0;
 #pragma unroll
-            for (int i = 0; i < KQ; ++i)
-                if (c0 + i < a.Dk) to[i] = v[i];
-        } else {
-            store_row(static_cast<bf16 *>(x.p) + at(x, b, h) + (long long)(t0 + row) * x.ts, v, c0, a.Dk,
-                      a.Dk % 8 == 0 && (x.ts | x.bs | x.hs) % 8 == 0 && reinterpret_cast<uintptr_t>(x.p) % 16 == 0);
+        for (int i = 0; i < KQ; i += 4) {
+            if (a.Dk % 4 == 0) {
+                if (c0 + i < a.Dk) *reinterpret_cast<float4 *>(to + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c0 + i + e < a.Dk) to[i + e] = v[i + e];
+            }
         }
-    };
-    const auto put_v = [&](const float (&v)[VQ]) {
-        if (row < all)
-            store_row(static_cast<bf16 *>(a.dv.p) + at(a.dv, b, h) + (long long)(t0 + row) * a.dv.ts, v, part * VQ, a.Dv,
-                      a.Dv % 8 == 0 && (a.dv.ts | a.dv.bs | a.dv.hs) % 8 == 0 && reinterpret_cast<uintptr_t>(a.dv.p) % 16 == 0);
     };
     const long long gb = at(a.ddecay, b, h) + (long long)t0 * a.ddecay.ts;
     if (tokens == 0) {
-        float z[KQ], y[VQ];
-#pragma unroll
-        for (int i = 0; i < KQ; ++i) z[i] = 0.f;
-#pragma unroll
-        for (int i = 0; i < VQ; ++i) y[i] = 0.f;
-        put_qk(a.dq, p.dq_heads, z);
-        put_qk(a.dk, p.dk_heads, z);
-        put_v(y);
+        for (int e = tid; e < C * (DK + DV) / 8; e += GRAD_THREADS) sts16(q_t + e * 16, 0u, 0u, 0u, 0u);      // q's, k's and v's tiles, or more
+        __syncthreads();
+        if (p.dq_heads) {
+            const float z[KQ] = {};
+            put_heads(p.dq_heads, z);
+            put_heads(p.dk_heads, z);
+        } else {
+            copy_out<DK>(q_t, a.dq, at(a.dq, b, h), t0, all, a.Dk, tid);
+            copy_out<DK>(q_t, a.dk, at(a.dk, b, h), t0, all, a.Dk, tid);
+        }
+        copy_out<DV>(q_t, a.dv, at(a.dv, b, h), t0, all, a.Dv, tid);
         if (tid < all) seq::store_f(a.ddecay.p, gb + tid * a.ddecay.ts, a.decay_bf16, 0.f);
         return;
     }
     const int hk = h / (a.H / a.Hk);
     const long long state = ((long long)chunk * heads + bh) * (DK * DV);
+    const double g = load_decay(a, b, h, t0, tokens, tid);
     load_rows<DK, Vec, GRAD_THREADS>(q_t, a.q, at(a.q, b, hk), t0, tokens, a.Dk, tid);
     load_rows<DK, Vec, GRAD_THREADS>(k_t, a.k, at(a.k, b, hk), t0, tokens, a.Dk, tid);
     cp_commit();
@@ -491,13 +523,13 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
     load_state<DK, DV, GRAD_THREADS>(S_t, p.states + state, tid);
     load_state<DK, DV, GRAD_THREADS>(dS_t, p.dstates + state, tid);
     cp_commit();
-    const double g = load_decay(a, b, h, t0, tokens, tid);
     begin(s, 512, tid);
     const uint32_t tm = s.tmem, base = lane_base(tm, warp);
     const Operand q{q_t, PANEL}, k{k_t, PANEL}, v{v_t, PANEL}, o{o_t, PANEL}, S{S_t, DK * 128}, dS{dS_t, DK * 128}, E{E_t, PANEL};
+    sum_decays(s, g, tid);
     cp_wait<1>();
     fence_async();
-    sum_decays(s, g, tid);
+    __syncthreads();
     if (tid < 32) {
         const uint32_t leader = elect();
         tc::tc_fence_after_sync();
@@ -530,32 +562,47 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
         for (int i = 0; i < 4; ++i) sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + i), 0u, 0u, 0u, 0u);
     } else {
         float m[32];
-        const float r = a.scale * (part > block ? ex2_diff(s.G[part * 32 - 1], G) : 1.f);
+        float2 sum = both(0.f);
+        const float2 r = both(a.scale * (part > block ? ex2_diff(s.G[part * 32 - 1], G) : 1.f));
 #pragma unroll
-        for (int i8 = 0; i8 < 32; i8 += 16) {
-            float x[16], y[16];
-            tmem_load(base + part * 32 + i8, x);
-            tmem_load(base + 128 + part * 32 + i8, y);
+        for (int t0 = 0; t0 < 32; t0 += 16) {
+            float2 x[8], y[8];
+            int32_t u[2][16];
+            tc::tmem_ld16(base + part * 32 + t0, u[0]);
+            tc::tmem_ld16(base + 128 + part * 32 + t0, u[1]);
+            tc::tmem_ld_wait();
             uint32_t e[8];
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                float pv[2], ev[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int t = i8 + i + j;
-                    const float w = part > block ? r * s.f[part * 32 + t] : t >= lane ? a.scale * ex2_diff(s.G[part * 32 + t], G) : 0.f;
-                    const bool on = part > block || t >= lane;
-                    pv[j] = on ? w * x[i + j] : 0.f;
-                    ev[j] = on ? w * y[i + j] : 0.f;
-                    m[t] = part > block || t > lane ? pv[j] * y[i + j] : 0.f;
-                    s_sum += m[t];
+            for (int i = 0; i < 8; ++i) {
+                x[i] = make_float2(__int_as_float(u[0][2 * i]), __int_as_float(u[0][2 * i + 1]));
+                y[i] = make_float2(__int_as_float(u[1][2 * i]), __int_as_float(u[1][2 * i + 1]));
+                const int t = t0 + 2 * i;
+                float2 w;
+                if (part > block) {
+                    w = __fmul2_rn(r, *reinterpret_cast<const float2 *>(&s.f[part * 32 + t]));
+                } else {
+                    const float4 g2 = *reinterpret_cast<const float4 *>(&s.G[part * 32 + t]);
+                    w = __fmul2_rn(r, make_float2(ex2_diff(make_float2(g2.x, g2.y), G), ex2_diff(make_float2(g2.z, g2.w), G)));
+                    // (not by a factor of 0: what it would hide may be infinite)
+                    if (t < lane) x[i].x = y[i].x = 0.f, w.x = 0.f;
+                    if (t + 1 < lane) x[i].y = y[i].y = 0.f, w.y = 0.f;
                 }
-                P[(i8 + i) / 2] = pack(pv[0], pv[1]);
-                e[i / 2] = pack(ev[0], ev[1]);
+                const float2 pv = __fmul2_rn(w, x[i]);
+                float2 mv = __fmul2_rn(pv, y[i]);
+                if (part == block) {            // a pair of a token with itself moves with no decay
+                    if (t == lane) mv.x = 0.f;
+                    if (t + 1 == lane) mv.y = 0.f;
+                }
+                sum = __fadd2_rn(sum, mv);
+                m[t] = mv.x;
+                m[t + 1] = mv.y;
+                P[t / 2] = pack(pv);
+                e[i] = pack(__fmul2_rn(w, y[i]));
             }
-            sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + i8 / 8), e[0], e[1], e[2], e[3]);
-            sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + i8 / 8 + 1), e[4], e[5], e[6], e[7]);
+            sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + t0 / 8), e[0], e[1], e[2], e[3]);
+            sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + t0 / 8 + 1), e[4], e[5], e[6], e[7]);
         }
+        s_sum = sum.x + sum.y;
         t_sums[block * C + part * 32 + lane] = sum_columns(m, lane);
     }
     s_sums[part * C + row] = s_sum;
@@ -629,29 +676,37 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
         double through = 0.0;
         for (int w = 0; w < GRAD_THREADS / 32; ++w) through += warp_part[w];
         x += totals[0] + totals[1] + totals[2] + totals[3] + through * (double)exp2_of(last);
-        seq::store_f(a.ddecay.p, gb + tid * a.ddecay.ts, a.decay_bf16, tid < tokens ? (s.failed ? NAN : (float)x) : 0.f);
+        seq::store_f(a.ddecay.p, gb + tid * a.ddecay.ts, a.decay_bf16, tid < tokens ? (float)x : 0.f);
     }
+    // Out by way of the tiles of q, k and E, which nothing reads any more: a thread's part of a row on its own would be a store of 16 bytes
+    // in each of 32 lines.
+    const bool live = row < tokens;
     await(s, 3, 0);
-    const bool live = row < tokens, bad = s.failed;
     {
         float x[KQ];
         tmem_load(base + 384 + part * KQ, x);
 #pragma unroll
-        for (int i = 0; i < KQ; ++i) x[i] = live ? (bad ? NAN : x[i]) : 0.f;
-        put_qk(a.dq, p.dq_heads, x);
+        for (int i = 0; i < KQ; ++i) x[i] = live ? x[i] : 0.f;
+        p.dq_heads ? put_heads(p.dq_heads, x) : put_row(q_t, row, part * KQ, x);
         tmem_load(base + 256 + part * KQ, x);
 #pragma unroll
-        for (int i = 0; i < KQ; ++i) x[i] = live ? (bad ? NAN : x[i]) : 0.f;
-        put_qk(a.dk, p.dk_heads, x);
+        for (int i = 0; i < KQ; ++i) x[i] = live ? x[i] : 0.f;
+        p.dk_heads ? put_heads(p.dk_heads, x) : put_row(k_t, row, part * KQ, x);
     }
     await(s, 2, 1);
     {
         float x[VQ];
         tmem_load(base + 128 + part * VQ, x);
 #pragma unroll
-        for (int i = 0; i < VQ; ++i) x[i] = live ? (s.failed ? NAN : x[i]) : 0.f;
-        put_v(x);
+        for (int i = 0; i < VQ; ++i) x[i] = live ? x[i] : 0.f;
+        put_row(E_t, row, part * VQ, x);
     }
+    __syncthreads();
+    if (!p.dq_heads) {
+        copy_out<DK>(q_t, a.dq, at(a.dq, b, h), t0, all, a.Dk, tid);
+        copy_out<DK>(k_t, a.dk, at(a.dk, b, h), t0, all, a.Dk, tid);
+    }
+    copy_out<DV>(E_t, a.dv, at(a.dv, b, h), t0, all, a.Dv, tid);
     end(s, 512, p.flag, tid);
 }
 
