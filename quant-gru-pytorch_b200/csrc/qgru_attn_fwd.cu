@@ -66,7 +66,7 @@ struct Plan {
 
 struct Ctl {
     uint64_t k_full[3], k_empty[3], q_full[3], q_empty[3], v_full[3], v_empty[3], parts_full[2], parts_empty[2], pairs_full[2], p_full[2], g_full[SLOTS], g_empty[SLOTS];
-    uint64_t u_full, u_empty, s_full, s_empty, o_full, o_empty;
+    uint64_t u_full, u_empty, s_full, o_empty;
     uint32_t tmem;
     volatile int failed;
 };
@@ -176,7 +176,7 @@ struct Roles {
     // ---- X, warp 0: products
     __device__ __forceinline__ bool pairs(uint32_t leader, int i) const {
         const At<L::NS> st(i);
-        if (!wait_warp(s, s.k_full[st.buf], st.full) || !wait_warp(s, s.q_full[st.buf], st.full)) return false;
+        if (!wait(s, s.k_full[st.buf], st.full) || !wait(s, s.q_full[st.buf], st.full)) return false;
         tc::tc_fence_after_sync();
         product<false, false, C, DK>(leader, s.tmem + (i % L::NQ) * 128, Operand{q_tile(st.buf), PANEL}, Operand{k_tile(st.buf), PANEL}, false);
         commit(leader, &s.pairs_full[i % L::NQ]);
@@ -198,8 +198,8 @@ struct Roles {
 #pragma unroll 1
             for (int half = 0; half < 2; ++half) {
                 const At<L::NB> pb(2 * i + half);
-                if (!wait_warp(s, s.parts_full[pb.buf], pb.full)) return;
-                if (half == 0 && (!wait_warp(s, s.v_full[st.buf], st.full) || !wait_warp(s, s.u_empty, one.free))) return;
+                if (!wait(s, s.parts_full[pb.buf], pb.full)) return;
+                if (half == 0 && (!wait(s, s.v_full[st.buf], st.full) || !wait(s, s.u_empty, one.free))) return;
                 tc::tc_fence_after_sync();
                 const Operand v{v_tile(st.buf) + half * (PANEL / 2), PANEL};
                 // the small parts first
@@ -210,21 +210,19 @@ struct Roles {
                 }
                 commit(leader, &s.parts_empty[pb.buf]);
             }
-            commit(leader, &s.u_full);
+            if (L::NB == 1) commit(leader, &s.u_full);
             if constexpr (Outputs) {
-                if (!wait_warp(s, s.s_full, one.full) || !wait_warp(s, s.o_empty, one.free)) return;
+                if (!wait(s, s.s_full, one.full) || !wait(s, s.o_empty, one.free)) return;
                 tc::tc_fence_after_sync();
                 const Operand q{q_tile(st.buf), PANEL};
 #pragma unroll 1
                 for (int part = 1; part >= 0; --part) product<false, true, DV, DK>(leader, s.tmem + L::INTER, q, Operand{state(part), DK * 128}, part == 0);
                 commit(leader, &s.q_empty[st.buf]);
-                commit(leader, &s.s_empty);
                 if (L::NQ == 2 && i + 1 < steps && !pairs(leader, i + 1)) return;
                 const At<L::NQ> qb(i);
-                if (!wait_warp(s, s.p_full[qb.buf], qb.full)) return;
+                if (!wait(s, s.p_full[qb.buf], qb.full)) return;
                 tc::tc_fence_after_sync();
                 product_ts<true, DV, C>(leader, s.tmem + L::INTRA, s.tmem + qb.buf * 128, Operand{v_tile(st.buf), PANEL}, false);
-                commit(leader, &s.o_full);
             }
             commit(leader, &s.v_empty[st.buf]);
         }
@@ -381,11 +379,10 @@ struct Roles {
             }
             double all = 0.0;
             for (int c = w.begin; c < w.stop; ++c, ++i) {
-                const At<1> one(i);
                 const At<SLOTS> at(i);
                 uint4 *keep = p.states && !p.own_sums ? reinterpret_cast<uint4 *>(p.states + ((long long)Item<Reverse>::chunk(p, c) * a.B * a.H + w.bh) * (DK * DV) + row * DV + c0) : nullptr;
                 if constexpr (Outputs)
-                    if (!wait_warp(s, s.s_empty, one.free)) return;
+                    if (i && !wait_warp(s, s.q_empty[At<L::NS>(i - 1).buf], At<L::NS>(i - 1).full)) return;      // q S of the chunk before is done
 #pragma unroll
                 for (int j = 0; j < N; j += 8) {
                     uint32_t hi[4], lo[4];
@@ -409,7 +406,8 @@ struct Roles {
                 const float2 whole = both(slots[at.buf].whole);
                 all += (double)slots[at.buf].hi[C - 1] + (double)slots[at.buf].lo[C - 1];
                 tc::mbar_arrive(&s.g_empty[at.buf]);
-                if (!wait_warp(s, s.u_full, one.full)) return;
+                // the products with the second half of k are done, and so all: of two buffers that half's says it
+                if (!wait_warp(s, L::NB == 1 ? s.u_full : s.parts_empty[1], (uint32_t)i & 1u)) return;
                 tc::tc_fence_after_sync();
 #pragma unroll
                 for (int j = 0; j < N; j += 32) {
@@ -503,10 +501,10 @@ struct Roles {
             const Item<Reverse> w(a, p, it);
             bf16 *out = static_cast<bf16 *>(a.out.p) + at(a.out, w.b, w.h) + (long long)row * a.out.ts;
             for (int c = w.begin; c < w.stop; ++c, ++i) {
-                const At<1> one(i);
+                const At<L::NS> done(i);
                 const At<SLOTS> g(i);
                 const int t0 = c * C, all = min(a.T - t0, C), tokens = w.tokens(c);
-                if (!wait_warp(s, s.g_full[g.buf], g.full) || !wait_warp(s, s.o_full, one.full)) return;
+                if (!wait_warp(s, s.g_full[g.buf], g.full) || !wait_warp(s, s.v_empty[done.buf], done.full)) return;      // P v, the last with v, is done
                 tc::tc_fence_after_sync();
                 const float r = slots[g.buf].from_start[row];
                 bf16 *to = out + (long long)t0 * a.out.ts;
@@ -603,8 +601,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_walk(const __grid_constant__ qgr
         tc::mbar_init(&s.u_full, 1);
         tc::mbar_init(&s.u_empty, WG);
         tc::mbar_init(&s.s_full, WG);
-        tc::mbar_init(&s.s_empty, 1);
-        tc::mbar_init(&s.o_full, 1);
         tc::mbar_init(&s.o_empty, WG);
         s.failed = 0;
         tc::fence_barrier_init();
