@@ -607,8 +607,8 @@ typedef struct qgru_seq_tensor {
  * state0 [B][H][Dk][Dv] (NULL: zeros) and state, the last one, are dense.
  * Backward: dout, dstate (NULL: zeros) -> dq, dk, dv (elements of the type of q), ddecay (of the type of decay), dstate0 (may
  * be NULL).  `states` (with `keep`): written by the forward and read by the backward of the same arguments; 256-byte aligned, as
- * `workspace`, which holds nothing between calls.  qgru_attention_sizes takes the arguments as the calls do, with the forward's tensors
- * set but neither of the two. */
+ * `workspace`, which holds nothing between calls.  qgru_attention_sizes takes the arguments as the calls do, with all
+ * tensors set but neither of the two. */
 typedef struct qgru_attention {
     int device, T, B, H, Hk, Dk, Dv;
     int bf16, decay_bf16;               /* else fp32 */

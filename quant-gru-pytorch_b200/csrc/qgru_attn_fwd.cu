@@ -352,7 +352,6 @@ struct Roles {
         const int row = DK == 64 ? tid & 63 : tid, c0 = DK == 64 ? (tid >> 6) * N : 0;
         const uint32_t U = lane_base(s.tmem, tid >> 5) + L::U + c0;
         const long long dense_all = (long long)a.B * a.H * a.Dk * a.Dv;
-        const bool wide = a.Dv % 4 == 0;
         float2 S[N / 2];
         int i = 0;
         for (int it = blockIdx.x; it < p.items; it += gridDim.x) {
@@ -363,17 +362,7 @@ struct Roles {
 #pragma unroll
             for (int j = 0; j < N; j += 4) {
                 float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (first) {
-                    const float *f = first + dense + j;
-                    if (wide) {
-                        if (c0 + j < a.Dv) x = *reinterpret_cast<const float4 *>(f);
-                    } else {
-                        if (c0 + j < a.Dv) x.x = f[0];
-                        if (c0 + j + 1 < a.Dv) x.y = f[1];
-                        if (c0 + j + 2 < a.Dv) x.z = f[2];
-                        if (c0 + j + 3 < a.Dv) x.w = f[3];
-                    }
-                }
+                if (first && c0 + j < a.Dv) x = *reinterpret_cast<const float4 *>(first + dense + j);      // (head sizes here are multiples of 8)
                 S[j / 2] = make_float2(x.x, x.y);
                 S[j / 2 + 1] = make_float2(x.z, x.w);
             }
@@ -429,15 +418,7 @@ struct Roles {
             if (to && row < a.Dk) {
 #pragma unroll
                 for (int j = 0; j < N; j += 4) {
-                    float *f = to + dense + j;
-                    if (wide) {
-                        if (c0 + j < a.Dv) *reinterpret_cast<float4 *>(f) = make_float4(S[j / 2].x, S[j / 2].y, S[j / 2 + 1].x, S[j / 2 + 1].y);
-                    } else {
-                        if (c0 + j < a.Dv) f[0] = S[j / 2].x;
-                        if (c0 + j + 1 < a.Dv) f[1] = S[j / 2].y;
-                        if (c0 + j + 2 < a.Dv) f[2] = S[j / 2 + 1].x;
-                        if (c0 + j + 3 < a.Dv) f[3] = S[j / 2 + 1].y;
-                    }
+                    if (c0 + j < a.Dv) *reinterpret_cast<float4 *>(to + dense + j) = make_float4(S[j / 2].x, S[j / 2].y, S[j / 2 + 1].x, S[j / 2 + 1].y);
                 }
             }
             if (p.own_sums && tid == 0) p.seg_log[w.seg * (a.B * a.H) + w.bh] = (float)all;
@@ -495,7 +476,6 @@ struct Roles {
     __device__ __forceinline__ void outputs() const {
         const int warp = tid >> 5, row = tid;
         const uint32_t from = lane_base(s.tmem, warp);
-        const bool vec = a.Dv % 8 == 0 && (a.out.ts | a.out.bs | a.out.hs) % 8 == 0 && reinterpret_cast<uintptr_t>(a.out.p) % 16 == 0;
         int i = 0;
         for (int it = blockIdx.x; it < p.items; it += gridDim.x) {
             const Item<Reverse> w(a, p, it);
@@ -508,63 +488,64 @@ struct Roles {
                 tc::tc_fence_after_sync();
                 const float r = slots[g.buf].from_start[row];
                 bf16 *to = out + (long long)t0 * a.out.ts;
+                uint32_t odd_groups = 0;
 #pragma unroll 1
                 for (int j = 0; j < DV; j += 16) {
-                    float2 intra[8], inter[8];
                     int32_t u[2][16];
                     tc::tmem_ld16(from + L::INTRA + j, u[0]);
                     tc::tmem_ld16(from + L::INTER + j, u[1]);
                     tc::tmem_ld_wait();
                     float2 odd = both(0.f);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        intra[e] = make_float2(__int_as_float(u[0][2 * e]), __int_as_float(u[0][2 * e + 1]));
-                        inter[e] = make_float2(__int_as_float(u[1][2 * e]), __int_as_float(u[1][2 * e + 1]));
-                        odd = __ffma2_rn(intra[e], both(0.f), odd);
-                    }
-                    if (!(odd.x + odd.y == 0.f) && row < tokens) {      // NaN: not all are finite
-                        float z[16];
-                        again(z, w.b, w.h, t0, row, j, slots[g.buf]);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) intra[e] = make_float2(z[2 * e], z[2 * e + 1]);
-                    }
                     uint32_t y[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = row < tokens ? pack(__ffma2_rn(inter[e], both(r), intra[e])) : 0u;
-                    if (row < all && j < a.Dv) {
-                        if (vec) {
-                            *reinterpret_cast<uint4 *>(to + j) = make_uint4(y[0], y[1], y[2], y[3]);
-                            if (j + 8 < a.Dv) *reinterpret_cast<uint4 *>(to + j + 8) = make_uint4(y[4], y[5], y[6], y[7]);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                if (j + e < a.Dv) to[j + e] = __ushort_as_bfloat16((unsigned short)(y[e / 2] >> (e & 1) * 16));
-                        }
+                    for (int e = 0; e < 8; ++e) {
+                        const float2 intra = make_float2(__int_as_float(u[0][2 * e]), __int_as_float(u[0][2 * e + 1]));
+                        odd = __ffma2_rn(intra, both(0.f), odd);
+                        y[e] = pack(__ffma2_rn(make_float2(__int_as_float(u[1][2 * e]), __int_as_float(u[1][2 * e + 1])), both(r), intra));
                     }
-                    __syncwarp();
+                    if (row < tokens) {
+                        if (!(odd.x + odd.y == 0.f)) odd_groups |= 1u << (j / 16);      // NaN: not all of P v are finite
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] = 0u;
+                    }
+                    if (row < all) {
+                        if (j < a.Dv) *reinterpret_cast<uint4 *>(to + j) = make_uint4(y[0], y[1], y[2], y[3]);
+                        if (j + 8 < a.Dv) *reinterpret_cast<uint4 *>(to + j + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+                    }
                 }
+                if (__any_sync(0xffffffffu, odd_groups)) again(odd_groups, from + L::INTER, r, w.b, w.h, t0, row, to, slots[g.buf]);
                 tc::tc_fence_before_sync();
                 tc::mbar_arrive(&s.o_empty);
                 tc::mbar_arrive(&s.g_empty[g.buf]);
             }
             for (int c = w.stop; c < w.end; ++c)               // behind the sequence
                 if (c * C + row < a.T)
-                    for (int j = 0; j < a.Dv; ++j) out[(long long)c * C * a.out.ts + j] = __float2bfloat16_rn(0.f);
+                    for (int j = 0; j < a.Dv; j += 8) *reinterpret_cast<uint4 *>(out + (long long)c * C * a.out.ts + j) = make_uint4(0u, 0u, 0u, 0u);
         }
     }
     // A later token's infinity or NaN is none of an earlier one's business, and zero times it is NaN: the sums again, over the tokens up
-    // to this one.
-    __device__ __noinline__ void again(float *x, int b, int h, int t0, int row, int j, const Slot &g) const {
+    // to this one, for the groups of sixteen columns that a lane has found odd.
+    __device__ __noinline__ void again(uint32_t groups, uint32_t inter, float r, int b, int h, int t0, int row, bf16 *to, const Slot &g) const {
         const bf16 *q = static_cast<const bf16 *>(a.q.p) + at(a.q, b, h / p.share) + (long long)(t0 + row) * a.q.ts;
         const bf16 *k = static_cast<const bf16 *>(a.k.p) + at(a.k, b, h / p.share) + (long long)t0 * a.k.ts;
-        const bf16 *v = static_cast<const bf16 *>(a.v.p) + at(a.v, b, h) + (long long)t0 * a.v.ts + j;
-        for (int e = 0; e < 16; ++e) x[e] = 0.f;
-        for (int t = 0; t <= row; ++t) {
-            float f = 0.f;
-            for (int d = 0; d < a.Dk; ++d) f = fmaf(seq::to_f(q[d]), seq::to_f(k[t * a.k.ts + d]), f);
-            f *= a.scale * ex2_diff(g.G(row), g.G(t));
-            for (int e = 0; e < 16; ++e)
-                if (j + e < a.Dv) x[e] = fmaf(f, seq::to_f(v[t * a.v.ts + e]), x[e]);
+        const bf16 *v = static_cast<const bf16 *>(a.v.p) + at(a.v, b, h) + (long long)t0 * a.v.ts;
+        for (int j = 0; j < DV; j += 16) {
+            float x[16];
+            tmem_load(inter + j, x);
+            if (groups >> (j / 16) & 1) {
+                for (int e = 0; e < 16; ++e) x[e] *= r;
+                for (int t = 0; t <= row; ++t) {
+                    float f = 0.f;
+                    for (int d = 0; d < a.Dk; ++d) f = fmaf(seq::to_f(q[d]), seq::to_f(k[t * a.k.ts + d]), f);
+                    f *= a.scale * ex2_diff(g.G(row), g.G(t));
+                    for (int e = 0; e < 16; ++e)
+                        if (j + e < a.Dv) x[e] = fmaf(f, seq::to_f(v[t * a.v.ts + j + e]), x[e]);
+                }
+                for (int e = 0; e < 16; ++e)
+                    if (j + e < a.Dv) to[j + e] = __float2bfloat16_rn(x[e]);
+            }
+            __syncwarp();
         }
     }
 };
@@ -699,16 +680,18 @@ int run(const qgru_attention &a, const Cut &c, bf16 *states, char *seg, int *fla
 }
 
 bool strides_ok(const qgru_seq_tensor &x, int T, int B, int heads, int d) {
-    const auto ok = [](long long s, int n) { return n <= 1 || (s > 0 && s % 8 == 0 && s < (1ll << 38)); };
+    const auto ok = [](long long s, int n) { return n <= 1 || (s > 0 && s % 8 == 0 && s < (1ll << 38)); };       // (a stride of 0 is not for TMA)
     return reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && d % 8 == 0 && ok(x.ts, T) && ok(x.bs, B) && ok(x.hs, heads);
 }
 
 }  // namespace
 
-// Whether the tensors can be fetched by TMA: rows and strides of a multiple of 16 bytes.
+// Whether the tensors can be fetched by TMA and written in vectors: rows and strides of a multiple of 16 bytes.
 bool walk_takes(const qgru_attention &a, bool reverse) {
-    if (reverse) return strides_ok(a.q, a.T, a.B, a.Hk, a.Dk) && strides_ok(a.dout, a.T, a.B, a.H, a.Dv);
-    return strides_ok(a.q, a.T, a.B, a.Hk, a.Dk) && strides_ok(a.k, a.T, a.B, a.Hk, a.Dk) && strides_ok(a.v, a.T, a.B, a.H, a.Dv);
+    const auto dense = [](const float *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    if (reverse) return strides_ok(a.q, a.T, a.B, a.Hk, a.Dk) && strides_ok(a.dout, a.T, a.B, a.H, a.Dv) && dense(a.dstate) && dense(a.dstate0);
+    return strides_ok(a.q, a.T, a.B, a.Hk, a.Dk) && strides_ok(a.k, a.T, a.B, a.Hk, a.Dk) && strides_ok(a.v, a.T, a.B, a.H, a.Dv) &&
+           strides_ok(a.out, a.T, a.B, a.H, a.Dv) && dense(a.state0) && dense(a.state);
 }
 int walk(const qgru_attention &a, const Cut &c, bool reverse, void *states, char *seg, int *flag, int sms, cudaStream_t st) {
     using std::integral_constant;

@@ -1,13 +1,10 @@
-// qgru_attn_tc.cu - linear attention on the tensor cores: bf16 tensors, head sizes up to 128 (padded to 64 or 128), chunks of 128 tokens.
+// qgru_attn_tc.cu - linear attention on the tensor cores: the gradients, and the state pass and outputs of tensors that TMA does not take
+// (rows or strides that are no multiple of 16 bytes, strides of 0).  bf16, head sizes up to 128 (padded to 64 or 128), chunks of 128 tokens.
 //
-// Three kernels: the state pass (forward, and for the gradient of the states from the end), the outputs, and the gradients; in the
-// last two every chunk is a CTA's own.  All products are tcgen05.mma kind::f16 with fp32 sums in tensor memory and
-// operands in shared memory as rows of 128 bytes with the 128-byte swizzle.  Such a tile [rows][64 columns] is an operand with
-// its columns as K (K-major) and one with its rows as K (MN-major), so that no operand is transposed anywhere.
-//
-// What is rounded to bf16 on the way: the weights of the pairs of tokens (P, E), and the state before a chunk and its
-// gradient behind it where they are factors of a product.  Each is one rounding of a factor, the size of the one that the results
-// get in the end.  The states themselves are fp32: their products take k scaled by the decays as three bf16 parts (24 bits).
+// Outputs and gradients take every chunk by itself, from the states that a pass over the chunks has left.  Rounded to bf16 on the way
+// are the weights of the pairs of tokens (P, E), and the state before a chunk and its gradient behind it where they are factors of a
+// product.  Each is one rounding of a factor, the size of the one that the results get in the end.  The states themselves are fp32:
+// their products take k scaled by the decays as three bf16 parts (24 bits).
 #include <algorithm>
 #include <type_traits>
 
@@ -121,9 +118,9 @@ template <int DK, int DV>
 constexpr int STATES_TILES = DK / 64 * PANEL + 2 * (DV / 64) * PANEL + 3 * (DK / 64) * PANEL;
 
 // grid (B H, segments).  S' = 2^G_C S + (w k)^T v: lane i of tensor memory is row i of the state, whose fp32 sums stay in
-// registers, half a row a thread.  While the products of a chunk run, the next one's tokens arrive and the state before this one
+// registers, half a row a thread.  While the products of a chunk run, the next one's tokens are read and the state before this one
 // leaves.  With DK = 64 lanes 64 .. 127 repeat the first 64 (M is 128) and are not read.
-template <int DK, int DV, bool Reverse, bool Vec>
+template <int DK, int DV, bool Reverse>
 __global__ void __launch_bounds__(THREADS) k_states_tc(const __grid_constant__ qgru_attention a, const __grid_constant__ Pass p) {
     extern __shared__ unsigned char raw[];
     unsigned char *tiles = tiles_of(raw);
@@ -153,9 +150,8 @@ __global__ void __launch_bounds__(THREADS) k_states_tc(const __grid_constant__ q
     };
     const auto fetch = [&](int i) {
         const int t0 = chunk_of(i) * C, tokens = min(max(n - t0, 0), C);
-        load_rows<DK, Vec>(k_raw, p.k, kb, t0, tokens, a.Dk, tid);
-        load_rows<DV, Vec>(v_raw + (i & 1) * VT, p.v, vb, t0, tokens, a.Dv, tid);
-        cp_commit();
+        load_rows<DK, false>(k_raw, p.k, kb, t0, tokens, a.Dk, tid);
+        load_rows<DV, false>(v_raw + (i & 1) * VT, p.v, vb, t0, tokens, a.Dv, tid);
     };
     if (Reverse) {                                 // those behind the sequence: nothing reads the state there
         c = max(c, p.chunks - used);
@@ -169,7 +165,6 @@ __global__ void __launch_bounds__(THREADS) k_states_tc(const __grid_constant__ q
     }
     for (; c < stop; ++c) {
         const int chunk = chunk_of(c);
-        cp_wait<0>();
         sum_decays(s, g, tid);
         const float2 last = s.G[C - 1];
         if (tid < C) s.f[tid] = Reverse ? a.scale * exp2_of(s.G[tid]) : exp2_diff(last, s.G[tid]);
@@ -228,12 +223,11 @@ __global__ void __launch_bounds__(THREADS) k_states_tc(const __grid_constant__ q
         __syncthreads();
         if (s.failed) break;
     }
-    cp_wait<0>();
     float *to = own_sums ? p.seg_state + seg * dense_all : p.last && seg == p.segments - 1 ? p.last : nullptr;
     if (to) {
 #pragma unroll
         for (int i = 0; i < HALF; ++i)
-            if (row < a.Dk && c0 + i < a.Dv) to[dense + (long long)row * a.Dv + c0 + i] = s.failed ? NAN : S[i];
+            if (row < a.Dk && c0 + i < a.Dv) to[dense + (long long)row * a.Dv + c0 + i] = S[i];
     }
     if (own_sums && tid == 0) p.seg_log[seg * gridDim.x + bh] = (float)all;
     end(s, DV == 64 ? 64 : 128, p.flag, tid);
@@ -245,7 +239,7 @@ constexpr int OUTPUTS_TILES = 2 * (DK / 64) * PANEL + DV / 64 * PANEL;
 
 // grid: chunks x B H, the heads of one chunk beside each other.  Two threads a token, each half of the pairs' weights and half of the
 // output's columns.  The state lies where k was once q k^T is there.
-template <int DK, int DV, bool Vec>
+template <int DK, int DV>
 __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant__ qgru_attention a, const bf16 *states, int *flag) {
     extern __shared__ unsigned char raw[];
     unsigned char *tiles = tiles_of(raw);
@@ -267,15 +261,12 @@ __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant
     const int hk = h / (a.H / a.Hk);
     const bool carried = chunk > 0 || a.state0;
     const bf16 *S = states + ((long long)chunk * heads + bh) * (DK * DV);
-    load_rows<DK, Vec>(q_t, a.q, at(a.q, b, hk), t0, tokens, a.Dk, tid);
-    load_rows<DK, Vec>(k_t, a.k, at(a.k, b, hk), t0, tokens, a.Dk, tid);
-    cp_commit();
-    load_rows<DV, Vec>(v_t, a.v, at(a.v, b, h), t0, tokens, a.Dv, tid);
-    cp_commit();
+    load_rows<DK, false>(q_t, a.q, at(a.q, b, hk), t0, tokens, a.Dk, tid);
+    load_rows<DK, false>(k_t, a.k, at(a.k, b, hk), t0, tokens, a.Dk, tid);
+    load_rows<DV, false>(v_t, a.v, at(a.v, b, h), t0, tokens, a.Dv, tid);
     const double g = load_decay(a, b, h, t0, tokens, tid);
     begin(s, 256, tid);
     const uint32_t base = lane_base(s.tmem, warp);
-    cp_wait<1>();
     fence_async();
     sum_decays(s, g, tid);
     if (tid < 32) {
@@ -372,7 +363,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant
         }
     }
 #pragma unroll
-    for (int i = 0; i < HALF; ++i) o[i] = row < tokens ? (s.failed ? NAN : o[i] + x[i]) : 0.f;
+    for (int i = 0; i < HALF; ++i) o[i] = row < tokens ? o[i] + x[i] : 0.f;
     if (row < all) store_row(out, o, c0, a.Dv, vec_out);
     end(s, 256, flag, tid);
 }
@@ -720,7 +711,7 @@ int with_smem(F *kernel, int tiles, int *bytes) {
     return QGRU_OK;
 }
 
-template <int DK, int DV, bool Reverse, bool Vec>
+template <int DK, int DV, bool Reverse>
 int run_states(const qgru_attention &a, const Cut &c, bf16 *states, char *seg, int *flag, cudaStream_t st) {
     Pass p{};
     p.k = Reverse ? a.q : a.k;
@@ -733,7 +724,7 @@ int run_states(const qgru_attention &a, const Cut &c, bf16 *states, char *seg, i
     p.chunks = c.chunks;
     p.flag = flag;
     p.states = states;
-    const auto kernel = k_states_tc<DK, DV, Reverse, Vec>;
+    const auto kernel = k_states_tc<DK, DV, Reverse>;
     int bytes = 0;
     if (const int rc = with_smem(kernel, STATES_TILES<DK, DV>, &bytes)) return rc;
     const dim3 grid(a.B * a.H, c.segments);
@@ -751,15 +742,15 @@ int run_states(const qgru_attention &a, const Cut &c, bf16 *states, char *seg, i
     return QGRU_OK;
 }
 
-template <int DK, int DV, bool Vec>
+template <int DK, int DV>
 int forward(const qgru_attention &a, const Cut &c, int *flag, cudaStream_t st) {
     bf16 *states = static_cast<bf16 *>(a.keep ? a.states : a.workspace);
     char *seg = static_cast<char *>(a.workspace) + (a.keep ? 0 : a256(c.states));
-    if (const int rc = run_states<DK, DV, false, Vec>(a, c, states, seg, flag, st)) return rc;
+    if (const int rc = run_states<DK, DV, false>(a, c, states, seg, flag, st)) return rc;
     if (c.chunks == 0) return QGRU_OK;
     int bytes = 0;
-    if (const int rc = with_smem(k_outputs_tc<DK, DV, Vec>, OUTPUTS_TILES<DK, DV>, &bytes)) return rc;
-    k_outputs_tc<DK, DV, Vec><<<c.chunks * a.B * a.H, THREADS, bytes, st>>>(a, states, flag);
+    if (const int rc = with_smem(k_outputs_tc<DK, DV>, OUTPUTS_TILES<DK, DV>, &bytes)) return rc;
+    k_outputs_tc<DK, DV><<<c.chunks * a.B * a.H, THREADS, bytes, st>>>(a, states, flag);
     SEQ_CK(cudaGetLastError());
     return QGRU_OK;
 }
@@ -770,7 +761,7 @@ int backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStre
     ws += a256(c.states);
     char *seg = ws;
     ws += a256(c.seg);
-    if (const int rc = walk_takes(a, true) ? walk(a, c, true, dstates, seg, flag, sms, st) : run_states<DK, DV, true, Vec>(a, c, dstates, seg, flag, st)) return rc;
+    if (const int rc = walk_takes(a, true) ? walk(a, c, true, dstates, seg, flag, sms, st) : run_states<DK, DV, true>(a, c, dstates, seg, flag, st)) return rc;
     if (c.chunks == 0) return QGRU_OK;
     Gradients g{static_cast<const bf16 *>(a.states), dstates, nullptr, nullptr, flag};
     if (a.H != a.Hk) {
@@ -785,14 +776,10 @@ int backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStre
 }
 
 template <class F>
-int by_size(const qgru_attention &a, bool vec, F f) {
-    using std::integral_constant;
-    const auto with = [&](auto dk, auto dv) -> int {
-        return vec ? f(dk, dv, integral_constant<bool, true>()) : f(dk, dv, integral_constant<bool, false>());
-    };
-    const integral_constant<int, 64> small;
-    const integral_constant<int, 128> large;
-    return a.Dk <= 64 ? (a.Dv <= 64 ? with(small, small) : with(small, large)) : (a.Dv <= 64 ? with(large, small) : with(large, large));
+int by_size(const qgru_attention &a, F f) {
+    const std::integral_constant<int, 64> small;
+    const std::integral_constant<int, 128> large;
+    return a.Dk <= 64 ? (a.Dv <= 64 ? f(small, small) : f(small, large)) : (a.Dv <= 64 ? f(large, small) : f(large, large));
 }
 
 }  // namespace
@@ -815,12 +802,13 @@ Cut tc_cut(const qgru_attention &a, int sms) {
 }
 int tc_forward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStream_t st) {
     if (walk_takes(a, false)) return walk(a, c, false, a.keep ? a.states : nullptr, static_cast<char *>(a.workspace), flag, sms, st);
-    const bool vec = vec_ok(a.q, a.Dk) && vec_ok(a.k, a.Dk) && vec_ok(a.v, a.Dv);
-    return by_size(a, vec, [&](auto dk, auto dv, auto v) -> int { return forward<dk.value, dv.value, v.value>(a, c, flag, st); });
+    return by_size(a, [&](auto dk, auto dv) -> int { return forward<dk.value, dv.value>(a, c, flag, st); });
 }
 int tc_backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStream_t st) {
     const bool vec = vec_ok(a.q, a.Dk) && vec_ok(a.k, a.Dk) && vec_ok(a.v, a.Dv) && vec_ok(a.dout, a.Dv);
-    return by_size(a, vec, [&](auto dk, auto dv, auto v) -> int { return backward<dk.value, dv.value, v.value>(a, c, flag, sms, st); });
+    return by_size(a, [&](auto dk, auto dv) -> int {
+        return vec ? backward<dk.value, dv.value, true>(a, c, flag, sms, st) : backward<dk.value, dv.value, false>(a, c, flag, sms, st);
+    });
 }
 
 }  // namespace attn

@@ -53,6 +53,8 @@ Tensor readable(const Tensor &t) {
 // What a backward computes has no gradient of its own: whoever differentiates it is told.
 variable_list once(variable_list grads) {
     if (!at::GradMode::is_enabled()) return grads;
+    for (Tensor &g : grads)
+        if (g.defined()) g = g.detach().requires_grad_();
     return (*std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", (int)grads.size()))(std::move(grads));
 }
 
@@ -117,18 +119,18 @@ std::tuple<Tensor, Tensor, Tensor> attention_forward(const Tensor &q0, const Ten
     a.k = place(k, batch_first);
     a.v = place(v, batch_first);
     a.decay = place(decay, batch_first);
-    size_t states_bytes = 0, ws_bytes = 0;
-    check(qgru_attention_sizes(&a, &states_bytes, &ws_bytes, nullptr), "qgru_attention_sizes");
-    Tensor states = block(states_bytes, q), ws = block(ws_bytes, q), out = at::empty(v.sizes(), v.options());
-    Tensor state = at::empty({n.B, n.H, n.Dk, n.Dv}, q.options().dtype(at::kFloat));
+    Tensor out = at::empty(v.sizes(), v.options()), state = at::empty({n.B, n.H, n.Dk, n.Dv}, q.options().dtype(at::kFloat));
     a.lengths = static_cast<const int32_t *>(ptr(lengths));
     a.state0 = static_cast<const float *>(ptr(state0));
     a.state = static_cast<float *>(ptr(state));
+    a.out = place(out, batch_first);
+    size_t states_bytes = 0, ws_bytes = 0;
+    check(qgru_attention_sizes(&a, &states_bytes, &ws_bytes, nullptr), "qgru_attention_sizes");
+    Tensor states = block(states_bytes, q), ws = block(ws_bytes, q);
     a.states = ptr(states);
     a.workspace = ptr(ws);
     a.states_bytes = states_bytes;
     a.workspace_bytes = ws_bytes;
-    a.out = place(out, batch_first);
     check(qgru_attention_forward(&a, stream_of(q)), "qgru_attention_forward");
     return {out, state, states};
 }

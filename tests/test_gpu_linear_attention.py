@@ -371,3 +371,108 @@ def test_layers_as_they_are_used(dtype, batch_first, cuda_device):
     for layer in layers:
         for name, p in layer.named_parameters():
             assert p.grad is not None and torch.isfinite(p.grad).all() and p.grad.float().abs().max() > 0, name
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_broadcast_inputs_and_states_off_alignment(dtype, cuda_device):
+    """One sequence of keys for all of the batch (a stride of 0), and a state that begins 4 bytes off."""
+    q, k, v, g, state, _ = make(cuda_device, 140, 3, 2, 64, 64, dtype, decay=dtype)
+    one = k[:, :1].clone().requires_grad_()
+    off = torch.empty(state.numel() + 1, device=cuda_device)[1:].view(state.shape).copy_(state)
+    leaves = [q.requires_grad_(), one, v.requires_grad_(), g.requires_grad_(), off.requires_grad_()]
+    out, last = la.linear_attention(q, one.expand_as(q), v, g, off)
+    dout, dstate = torch.randn_like(out), torch.randn_like(last)
+    grads = torch.autograd.grad((out, last), leaves, (dout, dstate))
+    want, bound = want_of(q.detach(), one.detach().expand_as(q), v.detach(), g.detach(), state, None, dout=dout, dstate=dstate)
+    got = dict(zip(("dq", "dk", "dv", "dg", "dstate0"), grads))
+    dk = got.pop("dk")
+    hold({"out": out.detach(), "state": last.detach(), **got}, want, bound)
+    # three results of the type, added in it: a rounding of the sum each
+    size = want["dk"].abs().sum(1, keepdim=True)
+    assert ((dk.double() - want["dk"].sum(1, keepdim=True)).abs() <= bound["dk"].sum(1, keepdim=True) + 3 * ref.U[dtype] * size).all()
+
+
+def test_a_second_derivative_is_refused(cuda_device):
+    q, k, v, g, state, _ = make(cuda_device, 20, 1, 1, 64, 64, F32)
+    q.requires_grad_()
+    dq, = torch.autograd.grad(la.linear_attention(q, k, v, g)[0].square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        dq.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_a_captured_training_step(dtype, cuda_device):
+    q, k, v, g, state, _ = make(cuda_device, 300, 2, 4, 64, 64, dtype, Hk=2, decay=dtype)
+    leaves = [t.requires_grad_() for t in (q, k, v, g, state)]
+    w = torch.randn(300, 2, 4, 64, device=cuda_device).to(dtype)
+
+    def run():
+        out, last = la.linear_attention(*leaves)
+        return [out.detach(), *torch.autograd.grad((out, last), leaves, (w, torch.ones_like(last)))]
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = run()
+    for _ in range(2):
+        with torch.no_grad():
+            q.mul_(-0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(run(), got))
+
+
+def test_threads(cuda_device):
+    """Two threads, a stream and inputs each: nothing is shared."""
+    import threading
+    results, errors = {}, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                leaves = [t.requires_grad_() for t in make(cuda_device, 400, 2, 4, 64, 64, BF, decay=BF, seed=i)[:5]]
+                for _ in range(20):
+                    out, last = la.linear_attention(*leaves)
+                    grads = torch.autograd.grad((out, last), leaves, (torch.ones_like(out), torch.ones_like(last)))
+                torch.cuda.current_stream().synchronize()
+                results[i] = [out.detach(), *grads]
+        except Exception as e:       # (told below, in the test's own thread)
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    again = results.copy()
+    for i in range(2):
+        work(i)
+        assert all(torch.equal(a, b) for a, b in zip(again[i], results[i]))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_offsets_beyond_32_bits(dtype, cuda_device):
+    """2.2e9 elements a tensor: the last sequences against the same in 64 bits."""
+    T, B, H, D = (130, 8400, 16, 128) if dtype == BF else (130, 16500, 16, 64)
+
+    def big():
+        return torch.empty(T, B, H, D, dtype=dtype, device=cuda_device).normal_()
+
+    q, k, v = big(), big(), big()
+    g = torch.full((T, B, H), -0.1, device=cuda_device)
+    out, last = la.linear_attention(q, k, v, g)
+    part = [t[:, -2:].contiguous() for t in (q, k, v, g)]
+    want, bound = want_of(*part, None, None)
+    hold({"out": out[:, -2:], "state": last[-2:]}, want, bound)
+    del q, k, v, g, out
+    # a step of all of them, the last two with tokens of their own
+    tokens = [torch.zeros(B, *t.shape[2:], dtype=t.dtype, device=cuda_device) for t in part]
+    for t, x in zip(tokens, part):
+        t[-2:] = x[0]
+    want, bound = want_of(*[t[-2:][None] for t in tokens], last[-2:].clone(), None)
+    out = la.linear_attention_step(*tokens, last)
+    hold({"out": out[-2:][None], "state": last[-2:]}, want, bound)

@@ -170,6 +170,51 @@ def test_captured_and_on_other_streams(cuda_device):
     assert all(torch.equal(a, b) for a, b in zip(norm.rms_norm_q8(x, w, r), got))
 
 
+def test_offsets_beyond_32_bits(cuda_device):
+    """2.2e9 elements: the last rows as they are alone."""
+    x = torch.empty(270000, 8192, dtype=BF, device=cuda_device).normal_().requires_grad_()
+    w = torch.ones(8192, dtype=BF, device=cuda_device)
+    y = norm.rms_norm(x, w)
+    dx, = torch.autograd.grad(y, x, x.detach())
+    q, s = norm.rms_norm_q8(x.detach(), w)
+    part = x.detach()[-3:].contiguous().requires_grad_()
+    y1 = norm.rms_norm(part, w)
+    dx1, = torch.autograd.grad(y1, part, part.detach())
+    q1, s1 = norm.rms_norm_q8(part.detach(), w)
+    assert torch.equal(y[-3:], y1) and torch.equal(dx[-3:], dx1) and torch.equal(q[-3:], q1) and torch.equal(s[-3:], s1)
+
+
+def test_a_captured_training_step(cuda_device):
+    x, r, w = make(cuda_device, 300, 512, BF)
+    leaves = [t.requires_grad_() for t in (x, w, r)]
+    dy, dh = torch.randn_like(x), torch.randn_like(x)
+
+    def run():
+        y, h = norm.rms_norm(x, w, r)
+        return [y.detach(), *torch.autograd.grad((y, h), leaves, (dy, dh))]
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = run()
+    with torch.no_grad():
+        x.mul_(-0.5)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(run(), got))
+
+
+def test_a_second_derivative_is_refused(cuda_device):
+    x, r, w = make(cuda_device, 3, 40, F32)
+    x.requires_grad_()
+    dx, = torch.autograd.grad(norm.rms_norm(x, w).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        dx.sum().backward()
+
+
 def test_before_a_quantized_layer(cuda_device):
     """The norm's output in the integers that a calibrated QuantGRU takes, with the scale of its own input operator."""
     import numpy as np
