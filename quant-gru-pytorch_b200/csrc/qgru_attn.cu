@@ -71,19 +71,19 @@ __device__ __forceinline__ void multiply(Sums<NT> &c, const float *A, const floa
     for (int s = from; s < to; ++s) {
         uint32_t ah[4], al[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            two_tf32(value_at<ARows>(A, pa[i], s), ah[i], al[i]);
-        }
+        for (int i = 0; i < 4; ++i) two_tf32(value_at<ARows>(A, pa[i], s), ah[i], al[i]);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             uint32_t bh[2], bl[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                two_tf32(value_at<BRows>(B, pb[j][i], s), bh[i], bl[i]);
-            }
-            mma(c.v[j], al, bh);
-            mma(c.v[j], ah, bl);
-            mma(c.v[j], ah, bh);
+            for (int i = 0; i < 2; ++i) two_tf32(value_at<BRows>(B, pb[j][i], s), bh[i], bl[i]);
+            // (the tensor cores cut off what a sum cannot hold: eight K stay there, longer sums are rounded to nearest)
+            float t[4] = {0.f, 0.f, 0.f, 0.f};
+            mma(t, al, bh);
+            mma(t, ah, bl);
+            mma(t, ah, bh);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c.v[j][i] += t[i];
         }
     }
 }
@@ -182,16 +182,16 @@ __device__ __forceinline__ void load_state(float *to, const float *S, int i0, in
 __device__ __forceinline__ long long at(const qgru_seq_tensor &x, int b, int h) { return b * x.bs + h * x.hs; }
 
 // G of a chunk by the first 64 threads, others pass
-__device__ __forceinline__ void sum_decays(float2 *G, double *sums, double g, int tid) {
+__device__ __forceinline__ void sum_decays(float2 *G, long long *sums, long long g, int tid) {
     if (tid < C) g = running_sum<C>(g, sums, tid);
     __syncthreads();
-    if (tid < C) G[tid] = two_floats(g + (tid >= 32 ? sums[0] : 0.0));
+    if (tid < C) G[tid] = two_floats(g + (tid >= 32 ? sums[0] : 0));
     __syncthreads();
 }
 
 // The chunk's running sums G[0 .. 63] (tokens behind the sequence add nothing).
-__device__ __forceinline__ void load_decays(float2 *G, double *sums, const qgru_attention &a, int b, int h, int t0, int tokens, int tid) {
-    sum_decays(G, sums, tid < tokens ? decay_log2(a, at(a.decay, b, h) + (long long)(t0 + tid) * a.decay.ts) : 0.0, tid);
+__device__ __forceinline__ void load_decays(float2 *G, long long *sums, const qgru_attention &a, int b, int h, int t0, int tokens, int tid) {
+    sum_decays(G, sums, tid < tokens ? decay_units(a, at(a.decay, b, h) + (long long)(t0 + tid) * a.decay.ts) : 0, tid);
 }
 
 struct Pass {                      // a state pass
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(THREADS) k_states(const __grid_constant__ qgru
     __shared__ alignas(16) float K[TILE], V[TILE];
     __shared__ float2 G[C];
     __shared__ float W[C];
-    __shared__ double sums[2];
+    __shared__ long long g_sums[2];
     const int tid = threadIdx.x, bh = blockIdx.x, b = bh / a.H, h = bh % a.H;
     const int nj = (a.Dv + 63) / 64, i0 = (int)blockIdx.y / nj * 64, j0 = (int)blockIdx.y % nj * 64;
     const int n = valid_tokens(a, b), seg = blockIdx.z;
@@ -231,12 +231,12 @@ __global__ void __launch_bounds__(THREADS) k_states(const __grid_constant__ qgru
     const auto tokens_of = [&](int c) { return c < c_end ? min(max(n - chunk_of(c) * C, 0), C) : 0; };
     // (four neighbouring columns a load; the next chunk's are on their way while one is worked on)
     Four k4, v4;
-    double g = 0.0;
+    long long g = 0;
     const auto load = [&](int c) {
         const int tokens = tokens_of(c), t0 = chunk_of(c) * C;
         k4.template load<T>(p.k, kb, t0, tokens, i0, a.Dk, tid);
         v4.template load<T>(p.v, vb, t0, tokens, j0, a.Dv, tid);
-        g = tid < tokens ? decay_log2(a, at(a.decay, b, h) + (long long)(t0 + tid) * a.decay.ts) : 0.0;
+        g = tid < tokens ? decay_units(a, at(a.decay, b, h) + (long long)(t0 + tid) * a.decay.ts) : 0;
     };
     if (seg * p.per < c_end) load(seg * p.per);
     for (int c = seg * p.per; c < c_end; ++c) {
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(THREADS) k_states(const __grid_constant__ qgru
             k4.store(K, tid);
             v4.store(V, tid);
         }
-        sum_decays(G, sums, g, tid);
+        sum_decays(G, g_sums, g, tid);
         if (c + 1 < c_end) load(c + 1);
         if (tokens == 0) continue;
         const float2 end = G[C - 1];
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(THREADS) k_outputs(const __grid_constant__ qgr
     extern __shared__ float4 smem4[];
     float *X = reinterpret_cast<float *>(smem4), *Y = X + TILE, *P = Y + TILE;
     __shared__ float2 G[C];
-    __shared__ double sums[2];
+    __shared__ long long g_sums[2];
     const int tid = threadIdx.x, heads = a.B * a.H, chunk = blockIdx.x / heads, bh = blockIdx.x % heads, b = bh / a.H, h = bh % a.H, t0 = chunk * C;
     const int all = min(a.T - t0, C), tokens = min(max(valid_tokens(a, b) - t0, 0), C);
     T *out = static_cast<T *>(a.out.p) + at(a.out, b, h) + t0 * a.out.ts;
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(THREADS) k_outputs(const __grid_constant__ qgr
     const int hk = h / (a.H / a.Hk);
     const long long qb = at(a.q, b, hk), kb = at(a.k, b, hk), vb = at(a.v, b, h);
     const float *S = states + chunk * (long long)heads * a.Dk * a.Dv + (long long)bh * a.Dk * a.Dv;
-    load_decays(G, sums, a, b, h, t0, tokens, tid);
+    load_decays(G, g_sums, a, b, h, t0, tokens, tid);
     // the pairs of a warp's 16 rows end in their columns
     const int up_to = (tid >> 5 & 3) * 2 + 2;
     Acc c;
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
     extern __shared__ float4 smem4[];
     float *X = reinterpret_cast<float *>(smem4), *Y = X + TILE, *P = Y + TILE, *E = P + TILE;
     __shared__ float2 G[C];
-    __shared__ double sums[2];
+    __shared__ long long g_sums[2];
     __shared__ float dG[3][C], kE[2][C];     // what a change of the decays' sum up to token t brings; k_s's share behind the chunk
     const int tid = threadIdx.x, heads = a.B * a.H, chunk = blockIdx.x / heads, bh = blockIdx.x % heads, b = bh / a.H, h = bh % a.H, t0 = chunk * C;
     const int all = min(a.T - t0, C), tokens = min(max(valid_tokens(a, b) - t0, 0), C);
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
     }
     const long long tile = chunk * (long long)heads * a.Dk * a.Dv + (long long)bh * a.Dk * a.Dv;
     const float *S = states + tile, *dS = dstates + tile;
-    load_decays(G, sums, a, b, h, t0, tokens, tid);
+    load_decays(G, g_sums, a, b, h, t0, tokens, tid);
     if (tid < C) kE[0][tid] = kE[1][tid] = dG[0][tid] = dG[1][tid] = dG[2][tid] = 0.f;
     // the pairs of a warp's 16 rows end in their columns, or begin there
     const int diagonal = (tid >> 5 & 3) * 2, last = eights(tokens);
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_outputs_small(const __grid_const
     extern __shared__ float4 smem4[];
     float *Q = reinterpret_cast<float *>(smem4), *K = Q + TILE, *V = K + TILE, *S = V + TILE, *P = S + TILE;
     __shared__ float2 G[C];
-    __shared__ double sums[2];
+    __shared__ long long g_sums[2];
     const int tid = threadIdx.x, heads = a.B * a.H, chunk = blockIdx.x / heads, bh = blockIdx.x % heads, b = bh / a.H, h = bh % a.H, t0 = chunk * C;
     const int all = min(a.T - t0, C), tokens = min(max(valid_tokens(a, b) - t0, 0), C);
     float *out = static_cast<float *>(a.out.p) + at(a.out, b, h) + t0 * a.out.ts;
@@ -552,9 +552,9 @@ __global__ void __launch_bounds__(THREADS, 2) k_outputs_small(const __grid_const
     fetch<THREADS>(K, token(a.k, at(a.k, b, hk), t0), a.k.ts, tokens, a.Dk, tid);
     fetch<THREADS>(V, token(a.v, at(a.v, b, h), t0), a.v.ts, tokens, a.Dv, tid);
     if (carried) fetch<THREADS>(S, states + chunk * (long long)heads * a.Dk * a.Dv + (long long)bh * a.Dk * a.Dv, a.Dv, a.Dk, a.Dv, tid);
-    const double g = tid < tokens ? decay_log2(a, at(a.decay, b, h) + (long long)(t0 + tid) * a.decay.ts) : 0.0;
+    const long long g = tid < tokens ? decay_units(a, at(a.decay, b, h) + (long long)(t0 + tid) * a.decay.ts) : 0;
     cp_all();
-    sum_decays(G, sums, g, tid);
+    sum_decays(G, g_sums, g, tid);
     const int up_to = min((tid >> 5 & 3) * 2 + 2, eights(tokens));       // the pairs of a warp's 16 rows end in their columns
     Acc c;
     c.zero();
@@ -584,6 +584,7 @@ __global__ void __launch_bounds__(ALL, 1) k_gradients_small(const __grid_constan
     extern __shared__ float4 smem4[];
     float *Q = reinterpret_cast<float *>(smem4), *K = Q + TILE, *V = K + TILE, *O = V + TILE, *S = O + TILE, *dS = S + TILE, *P = dS + TILE, *E = P + TILE;
     __shared__ float2 G[C];
+    __shared__ long long g_sums[2];
     __shared__ double sums[2], totals[2], through_of[ALL / 32];
     __shared__ float rows[4][C], columns[4][C], q_dots[4][C], k_dots[4][C];
     const int tid = threadIdx.x, lane = tid & 31, heads = a.B * a.H, chunk = blockIdx.x / heads, bh = blockIdx.x % heads, b = bh / a.H, h = bh % a.H, t0 = chunk * C;
@@ -613,10 +614,10 @@ __global__ void __launch_bounds__(ALL, 1) k_gradients_small(const __grid_constan
     fetch<ALL>(O, token(a.dout, at(a.dout, b, h), t0), a.dout.ts, tokens, a.Dv, tid);
     fetch<ALL>(S, states + tile, a.Dv, a.Dk, a.Dv, tid);
     fetch<ALL>(dS, dstates + tile, a.Dv, a.Dk, a.Dv, tid);
-    const double g = tid < tokens ? decay_log2(a, at(a.decay, b, h) + (long long)(t0 + tid) * a.decay.ts) : 0.0;
+    const long long g = tid < tokens ? decay_units(a, at(a.decay, b, h) + (long long)(t0 + tid) * a.decay.ts) : 0;
     if (tid < 4 * C) q_dots[0][tid] = k_dots[0][tid] = 0.f;
     cp_all();
-    sum_decays(G, sums, g, tid);
+    sum_decays(G, g_sums, g, tid);
     const float2 end = G[C - 1];
     const int ek = eights(a.Dk), ev = eights(a.Dv), last = eights(tokens), diagonal = (tid >> 5 & 3) * 2;
     Sums<NT2> c, e;

@@ -255,7 +255,7 @@ struct Roles {
             const int tokens = w.tokens(chunk);
             const long long base = w.b * a.decay.bs + w.h * a.decay.hs + (long long)chunk * C * a.decay.ts;
             float f[4];
-            double g[4], sum = 0.0;
+            long long g[4], sum = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 f[j] = 0.f;
@@ -267,14 +267,14 @@ struct Roles {
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) g[j] = sum += decay_log2(f[j]);
-            double before = sum;
+            for (int j = 0; j < 4; ++j) g[j] = sum += decay_units(f[j]);
+            long long before = sum;
             for (int o = 1; o < 32; o <<= 1) {
-                const double u = __shfl_up_sync(0xffffffffu, before, o);
+                const long long u = __shfl_up_sync(0xffffffffu, before, o);
                 if (lane >= o) before += u;
             }
             before = __shfl_up_sync(0xffffffffu, before, 1);
-            if (lane == 0) before = 0.0;
+            if (lane == 0) before = 0;
             if (!wait_warp(s, s.g_empty[at.buf], at.free)) return false;
             Slot &to = slots[at.buf];
 #pragma unroll

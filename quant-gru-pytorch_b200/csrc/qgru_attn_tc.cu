@@ -57,21 +57,22 @@ __device__ __forceinline__ void load_state(uint32_t tile, const bf16 *S, int tid
 struct Shared {                 // behind the tiles
     float2 G[C];                // running sums of the decays, base 2
     float f[C];                 // factors of a token
+    long long g_sums[4];
     double sums[4];
     uint64_t bar[4];
     uint32_t tmem;
     int failed;
 };
 
-__device__ __forceinline__ double load_decay(const qgru_attention &a, int b, int h, int t0, int tokens, int tid) {
-    return tid < tokens ? decay_log2(a, at(a.decay, b, h) + (long long)(t0 + tid) * a.decay.ts) : 0.0;
+__device__ __forceinline__ long long load_decay(const qgru_attention &a, int b, int h, int t0, int tokens, int tid) {
+    return tid < tokens ? decay_units(a, at(a.decay, b, h) + (long long)(t0 + tid) * a.decay.ts) : 0;
 }
 // G of the chunk from the threads' decays (the first 128; two __syncthreads).
-__device__ __forceinline__ void sum_decays(Shared &s, double g, int tid) {
-    if (tid < C) g = running_sum<C>(g, s.sums, tid);
+__device__ __forceinline__ void sum_decays(Shared &s, long long g, int tid) {
+    if (tid < C) g = running_sum<C>(g, s.g_sums, tid);
     __syncthreads();
     if (tid < C) {
-        for (int w = 0; w < tid >> 5; ++w) g += s.sums[w];
+        for (int w = 0; w < tid >> 5; ++w) g += s.g_sums[w];
         s.G[tid] = two_floats(g);
     }
     __syncthreads();
@@ -157,7 +158,8 @@ __global__ void __launch_bounds__(THREADS) k_states_tc(const __grid_constant__ q
         c = max(c, p.chunks - used);
     }
     const int stop = Reverse ? c_end : min(c_end, used);
-    double all = 0.0, g = 0.0;
+    double all = 0.0;
+    long long g = 0;
     uint32_t phase = 0;
     if (c < stop) {
         fetch(c);
@@ -264,7 +266,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant
     load_rows<DK, false>(q_t, a.q, at(a.q, b, hk), t0, tokens, a.Dk, tid);
     load_rows<DK, false>(k_t, a.k, at(a.k, b, hk), t0, tokens, a.Dk, tid);
     load_rows<DV, false>(v_t, a.v, at(a.v, b, h), t0, tokens, a.Dv, tid);
-    const double g = load_decay(a, b, h, t0, tokens, tid);
+    const long long g = load_decay(a, b, h, t0, tokens, tid);
     begin(s, 256, tid);
     const uint32_t base = lane_base(s.tmem, warp);
     fence_async();
@@ -504,7 +506,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
     }
     const int hk = h / (a.H / a.Hk);
     const long long state = ((long long)chunk * heads + bh) * (DK * DV);
-    const double g = load_decay(a, b, h, t0, tokens, tid);
+    const long long g = load_decay(a, b, h, t0, tokens, tid);
     load_rows<DK, Vec, GRAD_THREADS>(q_t, a.q, at(a.q, b, hk), t0, tokens, a.Dk, tid);
     load_rows<DK, Vec, GRAD_THREADS>(k_t, a.k, at(a.k, b, hk), t0, tokens, a.Dk, tid);
     cp_commit();
