@@ -972,7 +972,7 @@ int qgru_attention_sizes(const qgru_attention *a, size_t *states_bytes, size_t *
     const bool walks = attn::tc_takes(*a) && attn::walk_takes(*a, false);
     if (states_bytes) *states_bytes = a->keep ? attn::a256(c.states) : 0;
     if (forward_workspace) *forward_workspace = attn::a256(c.seg) + (a->keep || walks ? 0 : attn::a256(c.states));
-    if (backward_workspace) *backward_workspace = attn::a256(c.states) + attn::a256(c.seg) + attn::group_bytes(*a);
+    if (backward_workspace) *backward_workspace = attn::a256(c.states) + attn::a256(c.seg) + attn::a256(c.through) + attn::group_bytes(*a);
     return QGRU_OK;
 }
 

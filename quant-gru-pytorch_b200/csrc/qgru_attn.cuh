@@ -18,6 +18,7 @@ struct Cut {               // of a sequence of T tokens into chunks, and of the 
     int chunk = 0, chunks = 0, segments = 0, per = 0;
     size_t states = 0;     // bytes of the states before the chunks
     size_t seg = 0;        // bytes of the segments' own last states and decays, 0 for one segment
+    size_t through = 0;    // bytes of the products of the states before the chunks with their gradients, where a pass leaves them
 };
 
 __device__ __forceinline__ int valid_tokens(const qgru_attention &a, int b) {
@@ -25,9 +26,9 @@ __device__ __forceinline__ int valid_tokens(const qgru_attention &a, int b) {
 }
 
 // Decays are summed up in 64-bit integers, base 2, in units of 2^-38: exact sums (a token's own rounding is 2^-38, 128 of them make
-// 3e-10 of the decay), in a tenth of the time that the chain of fp64 additions takes.  A decay below 2^-160 is zero to any fp32 sum and one
-// above 2^128 infinite, so the clamps keep -inf, +inf and a chunk's sum in range (128 * 160 < 2^14.4, 2^52.4 units); a NaN is a
-// value beyond all sums, which makes every sum from it on NaN.
+// 3e-10 of the decay) that depend on no order.  A decay below 2^-160 is zero to any fp32 sum and one above 2^128 infinite, so the
+// clamps keep -inf, +inf and a chunk's sum in range (128 * 160 < 2^14.4, 2^52.4 units); a NaN is a value beyond all sums, which makes
+// every sum from it on NaN.
 constexpr float UNITS = 0x1p38f;
 constexpr long long NAN_UNITS = 1ll << 54;
 __device__ __forceinline__ long long decay_units(float x) {

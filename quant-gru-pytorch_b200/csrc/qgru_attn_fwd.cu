@@ -76,6 +76,8 @@ struct Args {
     const float *first;                     // the state it starts from, or null
     float *last;                            // where the last one goes, or null
     bf16 *states;                           // before each chunk in the pass's order, [chunks][B H][DK][DV], or null
+    const bf16 *other;                      // from the end: the forward's states, and where their products with these go
+    float *through;
     float *seg_state, *seg_log;
     int own_sums;                           // states alone: each segment's sum, from zero, and nothing else
     int segments, per, chunks, items, share;
@@ -370,6 +372,19 @@ struct Roles {
             for (int c = w.begin; c < w.stop; ++c, ++i) {
                 const At<SLOTS> at(i);
                 uint4 *keep = p.states && !p.own_sums ? reinterpret_cast<uint4 *>(p.states + ((long long)Item<Reverse>::chunk(p, c) * a.B * a.H + w.bh) * (DK * DV) + row * DV + c0) : nullptr;
+                if (Reverse && !p.own_sums) {
+                    const long long head = (long long)Item<Reverse>::chunk(p, c) * a.B * a.H + w.bh;
+                    const uint4 *o = reinterpret_cast<const uint4 *>(p.other + head * (DK * DV) + row * DV + c0);
+                    float2 x = both(0.f);
+#pragma unroll
+                    for (int j = 0; j < N; j += 8) x = dot8(o[j / 8], &S[j / 2], x);
+                    float sum = x.x + x.y;
+                    for (int e = 16; e; e >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, e);
+                    if ((tid & 31) == 0) {
+                        p.through[head * THROUGH + (tid >> 5)] = sum;
+                        p.through[head * THROUGH + 4 + (tid >> 5)] = 0.f;
+                    }
+                }
                 if constexpr (Outputs)
                     if (i && !wait_warp(s, s.q_empty[At<L::NS>(i - 1).buf], At<L::NS>(i - 1).full)) return;      // q S of the chunk before is done
 #pragma unroll
@@ -654,8 +669,10 @@ int launch(const qgru_attention &a, const Args &p, int sms, cudaStream_t st) {
 }
 
 template <int DK, int DV, bool Reverse>
-int run(const qgru_attention &a, const Cut &c, bf16 *states, char *seg, int *flag, int sms, cudaStream_t st) {
+int run(const qgru_attention &a, const Cut &c, bf16 *states, char *seg, float *through, int *flag, int sms, cudaStream_t st) {
     Args p{};
+    p.other = static_cast<const bf16 *>(a.states);
+    p.through = through;
     const qgru_seq_tensor &k = Reverse ? a.q : a.k, &v = Reverse ? a.dout : a.v;
     if (a.T > 0 && (!make_map(&p.k, k, a.T, a.B, a.Hk, a.Dk) || !make_map(&p.v, v, a.T, a.B, a.H, a.Dv) || !make_map(&p.q, a.q, a.T, a.B, a.Hk, a.Dk)))
         return seq::fail(QGRU_ERR_CUDA, "cuTensorMapEncodeTiled");
@@ -693,11 +710,11 @@ bool walk_takes(const qgru_attention &a, bool reverse) {
     return strides_ok(a.q, a.T, a.B, a.Hk, a.Dk) && strides_ok(a.k, a.T, a.B, a.Hk, a.Dk) && strides_ok(a.v, a.T, a.B, a.H, a.Dv) &&
            strides_ok(a.out, a.T, a.B, a.H, a.Dv) && dense(a.state0) && dense(a.state);
 }
-int walk(const qgru_attention &a, const Cut &c, bool reverse, void *states, char *seg, int *flag, int sms, cudaStream_t st) {
+int walk(const qgru_attention &a, const Cut &c, bool reverse, void *states, char *seg, float *through, int *flag, int sms, cudaStream_t st) {
     using std::integral_constant;
     const auto with = [&](auto dk, auto dv) -> int {
         bf16 *to = static_cast<bf16 *>(states);
-        return reverse ? run<dk.value, dv.value, true>(a, c, to, seg, flag, sms, st) : run<dk.value, dv.value, false>(a, c, to, seg, flag, sms, st);
+        return reverse ? run<dk.value, dv.value, true>(a, c, to, seg, through, flag, sms, st) : run<dk.value, dv.value, false>(a, c, to, seg, through, flag, sms, st);
     };
     const integral_constant<int, 64> small;
     const integral_constant<int, 128> large;

@@ -111,6 +111,8 @@ struct Pass {
     float *last;
     bf16 *states;                  // before each chunk in the pass's order, [chunks][B H][DK][DV]
     bool own_sums;                 // instead: each segment's sum, from zero
+    const bf16 *other;             // from the end: the forward's states, and where their products with these go
+    float *through;
     float *seg_state, *seg_log;
     int segments, per, chunks;
     int *flag;
@@ -211,6 +213,22 @@ __global__ void __launch_bounds__(THREADS) k_states_tc(const __grid_constant__ q
             g = load_decay(a, b, h, chunk_of(c + 1) * C, min(n - chunk_of(c + 1) * C, C), tid);
         }
         leave(chunk);
+        if (Reverse && !own_sums) {
+            const long long head = (long long)chunk * gridDim.x + bh;
+            float sum = 0.f;
+            if (mine) {
+                const uint4 *o = reinterpret_cast<const uint4 *>(p.other + head * (DK * DV) + row * DV + c0);
+                float2 x = both(0.f);
+#pragma unroll
+                for (int i = 0; i < HALF; i += 8) {
+                    const float2 u[4] = {make_float2(S[i], S[i + 1]), make_float2(S[i + 2], S[i + 3]), make_float2(S[i + 4], S[i + 5]), make_float2(S[i + 6], S[i + 7])};
+                    x = dot8(o[i / 8], u, x);
+                }
+                sum = x.x + x.y;
+            }
+            for (int i = 16; i; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+            if (lane == 0) p.through[head * THROUGH + warp] = sum;
+        }
         const float whole = exp2_of(last);
         all += (double)last.x + (double)last.y;
         await(s, 0, phase);
@@ -374,6 +392,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant
 constexpr int GRAD_THREADS = 512;
 struct Gradients {
     const bf16 *states, *dstates;
+    const float *through;                // products of the two, THROUGH parts each
     float *dq_heads, *dk_heads;          // [T][B][H][Dk] where heads share q and k, else null
     int *flag;
 };
@@ -469,7 +488,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
     // once v has been used, its tile holds sums by token
     float *t_sums = reinterpret_cast<float *>(tiles + 2 * KT);          // [4][128] over s of a block's lanes, for each t
     float *s_sums = t_sums + 4 * C, *q_dots = s_sums + 4 * C, *k_dots = q_dots + 4 * C;     // [4][128] each
-    double *warp_part = reinterpret_cast<double *>(k_dots + 4 * C);     // [16]
+    double *totals = reinterpret_cast<double *>(k_dots + 4 * C);        // [4]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, heads = a.B * a.H, chunk = blockIdx.x / heads, bh = blockIdx.x % heads, b = bh / a.H, h = bh % a.H;
     const int t0 = chunk * C, all = min(a.T - t0, C), tokens = min(max(valid_tokens(a, b) - t0, 0), C);
     const int block = warp & 3, row = block * 32 + lane, part = warp >> 2;
@@ -602,23 +621,6 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
     const float to_end = ex2_diff(last, G), from_start = a.scale * ex2(G.x + G.y);
     k_dots[part * C + row] = scale_sums<KQ>(base + 256 + part * KQ, to_end, k_t, row, part * KQ, true);
     q_dots[part * C + row] = scale_sums<KQ>(base + 384 + part * KQ, from_start, q_t, row, part * KQ, true);
-    {
-        double x = 0.0;
-        for (int e = tid; e < DK * DV / 8; e += GRAD_THREADS) {
-            const uint4 u = lds16(S_t + e * 16), w = lds16(dS_t + e * 16);      // (the same order in both)
-            float f = low(u.x) * low(w.x);
-            f = fmaf(high(u.x), high(w.x), f);
-            f = fmaf(low(u.y), low(w.y), f);
-            f = fmaf(high(u.y), high(w.y), f);
-            f = fmaf(low(u.z), low(w.z), f);
-            f = fmaf(high(u.z), high(w.z), f);
-            f = fmaf(low(u.w), low(w.w), f);
-            f = fmaf(high(u.w), high(w.w), f);
-            x += (double)f;
-        }
-        for (int i = 16; i; i >>= 1) x += __shfl_xor_sync(0xffffffffu, x, i);
-        if (lane == 0) warp_part[warp] = x;
-    }
     fence_async();
     tc::tmem_st_wait();
     tc::tc_fence_before_sync();
@@ -649,7 +651,6 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
     }
     double total = own;
     for (int i = 16; i; i >>= 1) total += __shfl_xor_sync(0xffffffffu, total, i);
-    double *totals = warp_part + 16;
     if (lane == 0 && tid < C) totals[warp] = total;
     tc::tmem_st_wait();
     await(s, 2, 0);
@@ -667,7 +668,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
         double x = d;
         for (int w = 0; w < tid >> 5; ++w) x += s.sums[w];
         double through = 0.0;
-        for (int w = 0; w < GRAD_THREADS / 32; ++w) through += warp_part[w];
+        for (int w = 0; w < THROUGH; ++w) through += (double)p.through[((long long)chunk * heads + bh) * THROUGH + w];
         x += totals[0] + totals[1] + totals[2] + totals[3] + through * (double)exp2_of(last);
         seq::store_f(a.ddecay.p, gb + tid * a.ddecay.ts, a.decay_bf16, tid < tokens ? (float)x : 0.f);
     }
@@ -714,8 +715,10 @@ int with_smem(F *kernel, int tiles, int *bytes) {
 }
 
 template <int DK, int DV, bool Reverse>
-int run_states(const qgru_attention &a, const Cut &c, bf16 *states, char *seg, int *flag, cudaStream_t st) {
+int run_states(const qgru_attention &a, const Cut &c, bf16 *states, char *seg, float *through, int *flag, cudaStream_t st) {
     Pass p{};
+    p.other = static_cast<const bf16 *>(a.states);
+    p.through = through;
     p.k = Reverse ? a.q : a.k;
     p.v = Reverse ? a.dout : a.v;
     p.k_share = a.H / a.Hk;
@@ -748,7 +751,7 @@ template <int DK, int DV>
 int forward(const qgru_attention &a, const Cut &c, int *flag, cudaStream_t st) {
     bf16 *states = static_cast<bf16 *>(a.keep ? a.states : a.workspace);
     char *seg = static_cast<char *>(a.workspace) + (a.keep ? 0 : a256(c.states));
-    if (const int rc = run_states<DK, DV, false>(a, c, states, seg, flag, st)) return rc;
+    if (const int rc = run_states<DK, DV, false>(a, c, states, seg, nullptr, flag, st)) return rc;
     if (c.chunks == 0) return QGRU_OK;
     int bytes = 0;
     if (const int rc = with_smem(k_outputs_tc<DK, DV>, OUTPUTS_TILES<DK, DV>, &bytes)) return rc;
@@ -763,9 +766,11 @@ int backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStre
     ws += a256(c.states);
     char *seg = ws;
     ws += a256(c.seg);
-    if (const int rc = walk_takes(a, true) ? walk(a, c, true, dstates, seg, flag, sms, st) : run_states<DK, DV, true>(a, c, dstates, seg, flag, st)) return rc;
+    float *through = reinterpret_cast<float *>(ws);
+    ws += a256(c.through);
+    if (const int rc = walk_takes(a, true) ? walk(a, c, true, dstates, seg, through, flag, sms, st) : run_states<DK, DV, true>(a, c, dstates, seg, through, flag, st)) return rc;
     if (c.chunks == 0) return QGRU_OK;
-    Gradients g{static_cast<const bf16 *>(a.states), dstates, nullptr, nullptr, flag};
+    Gradients g{static_cast<const bf16 *>(a.states), dstates, through, nullptr, nullptr, flag};
     if (a.H != a.Hk) {
         g.dq_heads = reinterpret_cast<float *>(ws);
         g.dk_heads = g.dq_heads + group_bytes(a) / 8;
@@ -800,10 +805,11 @@ Cut tc_cut(const qgru_attention &a, int sms) {
     c.segments = std::max(1, (c.chunks + c.per - 1) / c.per);
     c.states = sizeof(bf16) * (size_t)c.chunks * a.B * a.H * (a.Dk <= 64 ? 64 : 128) * (a.Dv <= 64 ? 64 : 128);
     c.seg = c.segments > 1 ? sizeof(float) * c.segments * (state_elems(a) + (size_t)a.B * a.H) : 0;
+    c.through = sizeof(float) * THROUGH * c.chunks * (size_t)a.B * a.H;
     return c;
 }
 int tc_forward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStream_t st) {
-    if (walk_takes(a, false)) return walk(a, c, false, a.keep ? a.states : nullptr, static_cast<char *>(a.workspace), flag, sms, st);
+    if (walk_takes(a, false)) return walk(a, c, false, a.keep ? a.states : nullptr, static_cast<char *>(a.workspace), nullptr, flag, sms, st);
     return by_size(a, [&](auto dk, auto dv) -> int { return forward<dk.value, dv.value>(a, c, flag, st); });
 }
 int tc_backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStream_t st) {

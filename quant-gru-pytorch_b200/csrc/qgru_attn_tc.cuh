@@ -17,7 +17,10 @@ int tc_forward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaSt
 int tc_backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStream_t st);
 // A walk through the chunks (qgru_attn_fwd.cu): forward with the outputs, or from the end with the gradient of the states alone
 bool walk_takes(const qgru_attention &a, bool reverse);
-int walk(const qgru_attention &a, const Cut &c, bool reverse, void *states, char *seg, int *flag, int sms, cudaStream_t st);
+int walk(const qgru_attention &a, const Cut &c, bool reverse, void *states, char *seg, float *through, int *flag, int sms, cudaStream_t st);
+// The pass from the end meets every state's gradient in fp32: it multiplies it with the state, as bf16 as it was kept, and leaves the sum in
+// THROUGH parts a chunk and head (the sums of its warps).
+constexpr int THROUGH = 8;
 
 namespace tile {
 
@@ -177,6 +180,13 @@ __device__ __forceinline__ float high(uint32_t x) { return __uint_as_float(x & 0
 __device__ __forceinline__ uint32_t pack(float2 x) { return pack(x.x, x.y); }
 __device__ __forceinline__ float2 unpack(uint32_t x) { return make_float2(low(x), high(x)); }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+// Eight values, packed, times eight of a state's
+__device__ __forceinline__ float2 dot8(const uint4 &u, const float2 *s, float2 sum) {
+    sum = __ffma2_rn(unpack(u.x), s[0], sum);
+    sum = __ffma2_rn(unpack(u.y), s[1], sum);
+    sum = __ffma2_rn(unpack(u.z), s[2], sum);
+    return __ffma2_rn(unpack(u.w), s[3], sum);
+}
 // x minus what its rounding to bf16 keeps (exact)
 __device__ __forceinline__ float2 rest(float2 x, uint32_t packed) { return __ffma2_rn(unpack(packed), make_float2(-1.f, -1.f), x); }
 __device__ __forceinline__ float ex2(float x) {

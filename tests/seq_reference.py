@@ -42,7 +42,7 @@ def attention(q, k, v, g, state=None, lengths=None, scale=None, dout=None, dstat
 def attention_bounds(want, q, k, v, g, state=None, lengths=None, scale=None, dout=None, dstate=None):
     """How far each result may be off.  The type's own rounding of the result, and inside: a factor of a sum that goes to
     the tensor cores is rounded to the type (pairs' weights, the state before a chunk, its gradient: one of them in a
-    product, two in the product of the state with its gradient), everything else is fp32, whose sums have at most n terms
+    product, at most two in what a decay moves), everything else is fp32, whose sums have at most n terms
     one after the other.  A factor of an fp32 product is held as two tf32 values of 11 bits: the first is off by 2^-11 at the
     most, and the rest has a bit more than the second can hold, so the factor is off by 2^-23 <= 2^-22; the product of the two small
     halves, 2^-22 of the whole, is left out: 3 * 2^-22 = 12 f a product.  Every result is a sum of products at most two deep (q k, then v): 24 f."""
