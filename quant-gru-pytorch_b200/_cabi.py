@@ -218,6 +218,7 @@ def seq():
     """The torch binding of the sequence operators (csrc/qgru_seq_torch.cc), loaded once; raises if it is missing."""
     global _seq
     if _seq is None:
+        import torch  # noqa: F401  (its libraries come first)
         lib()
         if not os.path.exists(os.path.join(_HERE, "_seq.so")):
             raise RuntimeError(f"{os.path.join(_HERE, '_seq.so')} is missing: build it with __graft_entry__.build()")

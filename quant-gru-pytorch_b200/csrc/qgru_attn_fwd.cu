@@ -142,12 +142,6 @@ struct At {
     uint32_t full, free;
     __device__ __forceinline__ explicit At(int i) : buf(i % N), full((uint32_t)(i / N) & 1u), free(full ^ 1u) {}
 };
-__device__ __forceinline__ void tma_load_4d(uint32_t to, const CUtensorMap *map, uint64_t *bar, int x, int t, int h, int b) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(to),
-                 "l"(reinterpret_cast<uint64_t>(map)), "r"(tc::smem_u32(bar)), "r"(x), "r"(t), "r"(h), "r"(b)
-                 : "memory");
-}
-
 template <int DK, int DV, bool Outputs, bool Reverse>
 struct Roles {
     using L = Plan<DK, DV, Outputs>;
@@ -645,18 +639,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_walk(const __grid_constant__ qgr
 }
 
 // ------------------------------------------------------------------------------------- launches
-bool make_map(CUtensorMap *map, const qgru_seq_tensor &x, int T, int B, int heads, int d) {
-    const EncodeTiledFn enc = get_encode_tiled();
-    if (!enc) return false;
-    const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)T, (cuuint64_t)heads, (cuuint64_t)B};
-    // (the stride of a dimension of one is nobody's)
-    const auto bytes = [](long long s, int n) { return n > 1 ? (cuuint64_t)s * 2 : (cuuint64_t)256; };
-    const cuuint64_t strides[3] = {bytes(x.ts, T), bytes(x.hs, heads), bytes(x.bs, B)};
-    const cuuint32_t box[4] = {64, C, 1, 1}, step[4] = {1, 1, 1, 1};
-    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, x.p, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int DK, int DV, bool Outputs, bool Reverse>
 int launch(const qgru_attention &a, const Args &p, int sms, cudaStream_t st) {
     const auto kernel = k_walk<DK, DV, Outputs, Reverse>;
@@ -674,7 +656,7 @@ int run(const qgru_attention &a, const Cut &c, bf16 *states, char *seg, float *t
     p.other = static_cast<const bf16 *>(a.states);
     p.through = through;
     const qgru_seq_tensor &k = Reverse ? a.q : a.k, &v = Reverse ? a.dout : a.v;
-    if (a.T > 0 && (!make_map(&p.k, k, a.T, a.B, a.Hk, a.Dk) || !make_map(&p.v, v, a.T, a.B, a.H, a.Dv) || !make_map(&p.q, a.q, a.T, a.B, a.Hk, a.Dk)))
+    if (a.T > 0 && (!head_map(&p.k, k, a.T, a.B, a.Hk, a.Dk) || !head_map(&p.v, v, a.T, a.B, a.H, a.Dv) || !head_map(&p.q, a.q, a.T, a.B, a.Hk, a.Dk)))
         return seq::fail(QGRU_ERR_CUDA, "cuTensorMapEncodeTiled");
     p.first = Reverse ? a.dstate : a.state0;
     p.last = Reverse ? a.dstate0 : a.state;
@@ -696,19 +678,40 @@ int run(const qgru_attention &a, const Cut &c, bf16 *states, char *seg, float *t
     return launch<DK, DV, !Reverse, Reverse>(a, p, sms, st);
 }
 
-bool strides_ok(const qgru_seq_tensor &x, int T, int B, int heads, int d) {
+}  // namespace
+
+bool head_map(CUtensorMap *map, const qgru_seq_tensor &x, int T, int B, int heads, int d) {
+    const EncodeTiledFn enc = get_encode_tiled();
+    if (!enc) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)T, (cuuint64_t)heads, (cuuint64_t)B};
+    // (the stride of a dimension of one is nobody's)
+    const auto bytes = [](long long s, int n) { return n > 1 ? (cuuint64_t)s * 2 : (cuuint64_t)256; };
+    const cuuint64_t strides[3] = {bytes(x.ts, T), bytes(x.hs, heads), bytes(x.bs, B)};
+    const cuuint32_t box[4] = {64, C, 1, 1}, step[4] = {1, 1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, x.p, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool state_map(CUtensorMap *map, const void *states, long long rows, int DK, int DV) {
+    const EncodeTiledFn enc = get_encode_tiled();
+    if (!enc) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)DV, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)DV * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)DK}, step[2] = {1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(states), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool fetchable(const qgru_seq_tensor &x, int T, int B, int heads, int d) {
     const auto ok = [](long long s, int n) { return n <= 1 || (s > 0 && s % 8 == 0 && s < (1ll << 38)); };       // (a stride of 0 is not for TMA)
     return reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && d % 8 == 0 && ok(x.ts, T) && ok(x.bs, B) && ok(x.hs, heads);
 }
 
-}  // namespace
 
 // Whether the tensors can be fetched by TMA and written in vectors: rows and strides of a multiple of 16 bytes.
 bool walk_takes(const qgru_attention &a, bool reverse) {
     const auto dense = [](const float *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    if (reverse) return strides_ok(a.q, a.T, a.B, a.Hk, a.Dk) && strides_ok(a.dout, a.T, a.B, a.H, a.Dv) && dense(a.dstate) && dense(a.dstate0);
-    return strides_ok(a.q, a.T, a.B, a.Hk, a.Dk) && strides_ok(a.k, a.T, a.B, a.Hk, a.Dk) && strides_ok(a.v, a.T, a.B, a.H, a.Dv) &&
-           strides_ok(a.out, a.T, a.B, a.H, a.Dv) && dense(a.state0) && dense(a.state);
+    if (reverse) return fetchable(a.q, a.T, a.B, a.Hk, a.Dk) && fetchable(a.dout, a.T, a.B, a.H, a.Dv) && dense(a.dstate) && dense(a.dstate0);
+    return fetchable(a.q, a.T, a.B, a.Hk, a.Dk) && fetchable(a.k, a.T, a.B, a.Hk, a.Dk) && fetchable(a.v, a.T, a.B, a.H, a.Dv) &&
+           fetchable(a.out, a.T, a.B, a.H, a.Dv) && dense(a.state0) && dense(a.state);
 }
 int walk(const qgru_attention &a, const Cut &c, bool reverse, void *states, char *seg, float *through, int *flag, int sms, cudaStream_t st) {
     using std::integral_constant;

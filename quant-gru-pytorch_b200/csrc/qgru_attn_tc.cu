@@ -19,30 +19,23 @@ namespace {
 using namespace tile;
 constexpr int THREADS = 256;
 
-// Rows t0 .. t0 + 127 of a tensor (zeros from `tokens` on and behind its columns) as a tile of D columns.  Vec: rows and strides
-// are multiples of 16 bytes; else element by element.
-template <int D, bool Vec, int N = THREADS>
+// Rows t0 .. t0 + 127 of a tensor (zeros from `tokens` on and behind its columns) as a tile of D columns, element by element.
+template <int D, int N = THREADS>
 __device__ __forceinline__ void load_rows(uint32_t tile, const qgru_seq_tensor &x, long long base, int t0, int tokens, int d, int tid) {
     const bf16 *p = static_cast<const bf16 *>(x.p) + base + (long long)t0 * x.ts;
     constexpr int PER_ROW = D / 8;
 #pragma unroll
     for (int i = 0; i < C * PER_ROW / N; ++i) {
         const int e = i * N + tid, r = e / PER_ROW, c = e % PER_ROW;
-        const uint32_t to = tile + (c >> 3) * PANEL + chunk_at(r, c & 7);
-        if constexpr (Vec) {
-            const bool on = r < tokens && c * 8 < d;
-            cp_async(to, on ? p + r * x.ts + c * 8 : p, on ? 16 : 0);
-        } else {
-            uint32_t w[4];
+        uint32_t w[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int d0 = c * 8 + 2 * j;
-                const uint32_t u0 = r < tokens && d0 < d ? __bfloat16_as_ushort(p[r * x.ts + d0]) : 0u;
-                const uint32_t u1 = r < tokens && d0 + 1 < d ? __bfloat16_as_ushort(p[r * x.ts + d0 + 1]) : 0u;
-                w[j] = u0 | u1 << 16;
-            }
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        for (int j = 0; j < 4; ++j) {
+            const int d0 = c * 8 + 2 * j;
+            const uint32_t u0 = r < tokens && d0 < d ? __bfloat16_as_ushort(p[r * x.ts + d0]) : 0u;
+            const uint32_t u1 = r < tokens && d0 + 1 < d ? __bfloat16_as_ushort(p[r * x.ts + d0 + 1]) : 0u;
+            w[j] = u0 | u1 << 16;
         }
+        sts16(tile + (c >> 3) * PANEL + chunk_at(r, c & 7), w[0], w[1], w[2], w[3]);
     }
 }
 // A state [DK][DV] as it is kept before each chunk (bf16, padded) as a tile.
@@ -59,7 +52,7 @@ struct Shared {                 // behind the tiles
     float f[C];                 // factors of a token
     long long g_sums[4];
     double sums[4];
-    uint64_t bar[4];
+    uint64_t bar[6];
     uint32_t tmem;
     int failed;
 };
@@ -79,7 +72,7 @@ __device__ __forceinline__ void sum_decays(Shared &s, long long g, int tid) {
 }
 __device__ __forceinline__ void begin(Shared &s, uint32_t columns, int tid) {
     if (tid == 0) {
-        for (int i = 0; i < 4; ++i) tc::mbar_init(&s.bar[i], 1);
+        for (int i = 0; i < 6; ++i) tc::mbar_init(&s.bar[i], 1);
         s.failed = 0;
         tc::fence_barrier_init();
     }
@@ -153,8 +146,8 @@ __global__ void __launch_bounds__(THREADS) k_states_tc(const __grid_constant__ q
     };
     const auto fetch = [&](int i) {
         const int t0 = chunk_of(i) * C, tokens = min(max(n - t0, 0), C);
-        load_rows<DK, false>(k_raw, p.k, kb, t0, tokens, a.Dk, tid);
-        load_rows<DV, false>(v_raw + (i & 1) * VT, p.v, vb, t0, tokens, a.Dv, tid);
+        load_rows<DK>(k_raw, p.k, kb, t0, tokens, a.Dk, tid);
+        load_rows<DV>(v_raw + (i & 1) * VT, p.v, vb, t0, tokens, a.Dv, tid);
     };
     if (Reverse) {                                 // those behind the sequence: nothing reads the state there
         c = max(c, p.chunks - used);
@@ -281,9 +274,9 @@ __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant
     const int hk = h / (a.H / a.Hk);
     const bool carried = chunk > 0 || a.state0;
     const bf16 *S = states + ((long long)chunk * heads + bh) * (DK * DV);
-    load_rows<DK, false>(q_t, a.q, at(a.q, b, hk), t0, tokens, a.Dk, tid);
-    load_rows<DK, false>(k_t, a.k, at(a.k, b, hk), t0, tokens, a.Dk, tid);
-    load_rows<DV, false>(v_t, a.v, at(a.v, b, h), t0, tokens, a.Dv, tid);
+    load_rows<DK>(q_t, a.q, at(a.q, b, hk), t0, tokens, a.Dk, tid);
+    load_rows<DK>(k_t, a.k, at(a.k, b, hk), t0, tokens, a.Dk, tid);
+    load_rows<DV>(v_t, a.v, at(a.v, b, h), t0, tokens, a.Dv, tid);
     const long long g = load_decay(a, b, h, t0, tokens, tid);
     begin(s, 256, tid);
     const uint32_t base = lane_base(s.tmem, warp);
@@ -391,6 +384,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant
 // ------------------------------------------------------------------------------------- gradients
 constexpr int GRAD_THREADS = 512;
 struct Gradients {
+    CUtensorMap q, k, v, o, S, dS;       // where TMA takes the tensors
     const bf16 *states, *dstates;
     const float *through;                // products of the two, THROUGH parts each
     float *dq_heads, *dk_heads;          // [T][B][H][Dk] where heads share q and k, else null
@@ -478,7 +472,7 @@ __device__ __forceinline__ void copy_out(uint32_t tile, const qgru_seq_tensor &x
     }
 }
 
-template <int DK, int DV, bool Vec>
+template <int DK, int DV, bool Tma>
 __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_constant__ qgru_attention a, const __grid_constant__ Gradients p) {
     extern __shared__ unsigned char raw[];
     unsigned char *tiles = tiles_of(raw);
@@ -526,20 +520,48 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
     const int hk = h / (a.H / a.Hk);
     const long long state = ((long long)chunk * heads + bh) * (DK * DV);
     const long long g = load_decay(a, b, h, t0, tokens, tid);
-    load_rows<DK, Vec, GRAD_THREADS>(q_t, a.q, at(a.q, b, hk), t0, tokens, a.Dk, tid);
-    load_rows<DK, Vec, GRAD_THREADS>(k_t, a.k, at(a.k, b, hk), t0, tokens, a.Dk, tid);
-    cp_commit();
-    load_rows<DV, Vec, GRAD_THREADS>(v_t, a.v, at(a.v, b, h), t0, tokens, a.Dv, tid);
-    load_rows<DV, Vec, GRAD_THREADS>(o_t, a.dout, at(a.dout, b, h), t0, tokens, a.Dv, tid);
-    cp_commit();
-    load_state<DK, DV, GRAD_THREADS>(S_t, p.states + state, tid);
-    load_state<DK, DV, GRAD_THREADS>(dS_t, p.dstates + state, tid);
-    cp_commit();
+    if constexpr (!Tma) {
+        load_rows<DK, GRAD_THREADS>(q_t, a.q, at(a.q, b, hk), t0, tokens, a.Dk, tid);
+        load_rows<DK, GRAD_THREADS>(k_t, a.k, at(a.k, b, hk), t0, tokens, a.Dk, tid);
+        load_rows<DV, GRAD_THREADS>(v_t, a.v, at(a.v, b, h), t0, tokens, a.Dv, tid);
+        load_rows<DV, GRAD_THREADS>(o_t, a.dout, at(a.dout, b, h), t0, tokens, a.Dv, tid);
+        load_state<DK, DV, GRAD_THREADS>(S_t, p.states + state, tid);
+        load_state<DK, DV, GRAD_THREADS>(dS_t, p.dstates + state, tid);
+        cp_commit();
+    }
     begin(s, 512, tid);
+    if constexpr (Tma) {
+        if (tid == 0) {
+            tc::mbar_expect_tx(&s.bar[4], 2 * KT + 2 * VT);
+            for (int i = 0; i < DK / 64; ++i) {
+                tma_load_4d(k_t + i * PANEL, &p.k, &s.bar[4], i * 64, t0, hk, b);
+                tma_load_4d(q_t + i * PANEL, &p.q, &s.bar[4], i * 64, t0, hk, b);
+            }
+            for (int i = 0; i < DV / 64; ++i) {
+                tma_load_4d(v_t + i * PANEL, &p.v, &s.bar[4], i * 64, t0, h, b);
+                tma_load_4d(o_t + i * PANEL, &p.o, &s.bar[4], i * 64, t0, h, b);
+            }
+            tc::mbar_expect_tx(&s.bar[5], 2 * ST);
+            for (int i = 0; i < DV / 64; ++i) {
+                tc::tma_load_2d(tiles + 2 * KT + 2 * VT + i * (DK * 128), &p.S, &s.bar[5], i * 64, (chunk * heads + bh) * DK);
+                tc::tma_load_2d(tiles + 2 * KT + 2 * VT + ST + i * (DK * 128), &p.dS, &s.bar[5], i * 64, (chunk * heads + bh) * DK);
+            }
+        }
+    }
     const uint32_t tm = s.tmem, base = lane_base(tm, warp);
     const Operand q{q_t, PANEL}, k{k_t, PANEL}, v{v_t, PANEL}, o{o_t, PANEL}, S{S_t, DK * 128}, dS{dS_t, DK * 128}, E{E_t, PANEL};
     sum_decays(s, g, tid);
-    cp_wait<1>();
+    if constexpr (Tma) {
+        await(s, 4, 0);
+        if (tokens < C) {               // what lies behind the sequence was fetched too
+            for (int e = tid; e < (C - tokens) * 8; e += GRAD_THREADS) {
+                const int r = tokens + e / 8, at16 = r * 128 + e % 8 * 16;
+                for (int i = 0; i < (2 * KT + 2 * VT) / PANEL; ++i) sts16(q_t + i * PANEL + at16, 0u, 0u, 0u, 0u);
+            }
+        }
+    } else {
+        cp_wait<0>();
+    }
     fence_async();
     __syncthreads();
     if (tid < 32) {
@@ -551,8 +573,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
     }
     // from the start of t's block of 32 to t
     if (tid < C) s.f[tid] = tid < 32 ? ex2(s.G[tid].x + s.G[tid].y) : ex2_diff(s.G[tid], s.G[(tid & ~31) - 1]);
-    cp_wait<0>();
-    fence_async();
+    if constexpr (Tma) await(s, 5, 0);
     __syncthreads();
     if (tid < 32) {
         const uint32_t leader = elect();
@@ -705,8 +726,6 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
 }
 
 // ------------------------------------------------------------------------------------- launches
-bool vec_ok(const qgru_seq_tensor &x, int d) { return d % 8 == 0 && (x.ts | x.bs | x.hs) % 8 == 0 && reinterpret_cast<uintptr_t>(x.p) % 16 == 0; }
-
 template <class F>
 int with_smem(F *kernel, int tiles, int *bytes) {
     *bytes = tiles + 1024 + (int)sizeof(Shared);
@@ -759,7 +778,7 @@ int forward(const qgru_attention &a, const Cut &c, int *flag, cudaStream_t st) {
     SEQ_CK(cudaGetLastError());
     return QGRU_OK;
 }
-template <int DK, int DV, bool Vec>
+template <int DK, int DV, bool Tma>
 int backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStream_t st) {
     char *ws = static_cast<char *>(a.workspace);
     bf16 *dstates = reinterpret_cast<bf16 *>(ws);
@@ -770,14 +789,24 @@ int backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStre
     ws += a256(c.through);
     if (const int rc = walk_takes(a, true) ? walk(a, c, true, dstates, seg, through, flag, sms, st) : run_states<DK, DV, true>(a, c, dstates, seg, through, flag, st)) return rc;
     if (c.chunks == 0) return QGRU_OK;
-    Gradients g{static_cast<const bf16 *>(a.states), dstates, through, nullptr, nullptr, flag};
+    Gradients g{};
+    g.states = static_cast<const bf16 *>(a.states);
+    g.dstates = dstates;
+    g.through = through;
+    g.flag = flag;
+    if (Tma) {
+        const long long rows = (long long)c.chunks * a.B * a.H * DK;
+        if (!head_map(&g.q, a.q, a.T, a.B, a.Hk, a.Dk) || !head_map(&g.k, a.k, a.T, a.B, a.Hk, a.Dk) || !head_map(&g.v, a.v, a.T, a.B, a.H, a.Dv) ||
+            !head_map(&g.o, a.dout, a.T, a.B, a.H, a.Dv) || !state_map(&g.S, a.states, rows, DK, DV) || !state_map(&g.dS, dstates, rows, DK, DV))
+            return seq::fail(QGRU_ERR_CUDA, "cuTensorMapEncodeTiled");
+    }
     if (a.H != a.Hk) {
         g.dq_heads = reinterpret_cast<float *>(ws);
         g.dk_heads = g.dq_heads + group_bytes(a) / 8;
     }
     int bytes = 0;
-    if (const int rc = with_smem(k_gradients_tc<DK, DV, Vec>, GRADIENTS_TILES<DK, DV>, &bytes)) return rc;
-    k_gradients_tc<DK, DV, Vec><<<c.chunks * a.B * a.H, GRAD_THREADS, bytes, st>>>(a, g);
+    if (const int rc = with_smem(k_gradients_tc<DK, DV, Tma>, GRADIENTS_TILES<DK, DV>, &bytes)) return rc;
+    k_gradients_tc<DK, DV, Tma><<<c.chunks * a.B * a.H, GRAD_THREADS, bytes, st>>>(a, g);
     SEQ_CK(cudaGetLastError());
     return g.dq_heads ? sum_groups(a, g.dq_heads, g.dk_heads, st) : QGRU_OK;
 }
@@ -813,9 +842,9 @@ int tc_forward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaSt
     return by_size(a, [&](auto dk, auto dv) -> int { return forward<dk.value, dv.value>(a, c, flag, st); });
 }
 int tc_backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStream_t st) {
-    const bool vec = vec_ok(a.q, a.Dk) && vec_ok(a.k, a.Dk) && vec_ok(a.v, a.Dv) && vec_ok(a.dout, a.Dv);
+    const bool tma = fetchable(a.q, a.T, a.B, a.Hk, a.Dk) && fetchable(a.k, a.T, a.B, a.Hk, a.Dk) && fetchable(a.v, a.T, a.B, a.H, a.Dv) && fetchable(a.dout, a.T, a.B, a.H, a.Dv);
     return by_size(a, [&](auto dk, auto dv) -> int {
-        return vec ? backward<dk.value, dv.value, true>(a, c, flag, sms, st) : backward<dk.value, dv.value, false>(a, c, flag, sms, st);
+        return tma ? backward<dk.value, dv.value, true>(a, c, flag, sms, st) : backward<dk.value, dv.value, false>(a, c, flag, sms, st);
     });
 }
 

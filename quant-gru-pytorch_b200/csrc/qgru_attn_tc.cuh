@@ -15,6 +15,11 @@ Cut tc_cut(const qgru_attention &a, int sms);
 // flag: where a kernel says that a wait of its own has run out
 int tc_forward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStream_t st);
 int tc_backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStream_t st);
+// Tensor maps of a tensor's heads ([B][heads][T][D], boxes of 128 tokens x 64 columns) and of kept states ([rows][DV], boxes of DK x 64);
+// fetchable: whether TMA takes a tensor (rows and strides multiples of 16 bytes, no stride of 0)
+bool head_map(CUtensorMap *map, const qgru_seq_tensor &x, int T, int B, int heads, int d);
+bool state_map(CUtensorMap *map, const void *states, long long rows, int DK, int DV);
+bool fetchable(const qgru_seq_tensor &x, int T, int B, int heads, int d);
 // A walk through the chunks (qgru_attn_fwd.cu): forward with the outputs, or from the end with the gradient of the states alone
 bool walk_takes(const qgru_attention &a, bool reverse);
 int walk(const qgru_attention &a, const Cut &c, bool reverse, void *states, char *seg, float *through, int *flag, int sms, cudaStream_t st);
@@ -199,6 +204,11 @@ __device__ __forceinline__ float ex2_diff(float2 t, float2 s) { return ex2((t.x 
 // 16-byte chunk c (of eight columns) of row r of a panel
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 
+__device__ __forceinline__ void tma_load_4d(uint32_t to, const CUtensorMap *map, uint64_t *bar, int x, int t, int h, int b) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(to),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(tc::smem_u32(bar)), "r"(x), "r"(t), "r"(h), "r"(b)
+                 : "memory");
+}
 __device__ __forceinline__ void cp_async(uint32_t to, const void *from, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
