@@ -58,6 +58,21 @@ variable_list once(variable_list grads) {
     return (*std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", (int)grads.size()))(std::move(grads));
 }
 
+// The node that adds to a leaf's gradient lives as long as any graph of the leaf, with the stream that it was made on.  Where that is
+// the default stream, a backward inside a capture on another one would have it wait for the captured work, which CUDA forbids and
+// autograd does not survive.  Refused before anything is recorded.
+void check_capture(std::initializer_list<const Tensor *> leaves) {
+    for (const Tensor *t : leaves) {
+        if (!t->defined() || !t->is_cuda() || !t->requires_grad() || !t->is_leaf()) continue;
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(c10::cuda::getCurrentCUDAStream(t->get_device()).stream(), &capture) != cudaSuccess || capture == cudaStreamCaptureStatusNone) return;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto made_on = node ? node->stream() : std::nullopt;
+        TORCH_CHECK(!made_on || *made_on != c10::cuda::getDefaultCUDAStream(t->get_device()).unwrap(),
+                    "a graph of the same leaves that was made on the default stream still lives: release it (its outputs and losses) before the backward pass is captured");
+    }
+}
+
 // ------------------------------------------------------------------------------------- linear attention
 struct Sizes {
     int64_t T, B, H, Hk, Dk, Dv;
@@ -218,6 +233,7 @@ std::tuple<Tensor, Tensor> linear_attention(const Tensor &q, const Tensor &k, co
     }
     const double s = scale ? *scale : 1.0 / std::sqrt((double)q.size(3));
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || decay.requires_grad() || (state0.defined() && state0.requires_grad()))) {
+        check_capture({&q, &k, &v, &log_decay, &state0});
         const variable_list r = LinearAttention::apply(q, k, v, decay, some(state0), some(n), s, batch_first);
         return {r[0], r[1]};
     }
@@ -246,8 +262,8 @@ Tensor linear_attention_step(const Tensor &q0, const Tensor &k0, const Tensor &v
     a.v = at(v);
     a.decay = at(decay);
     a.out = at(out);
+    state.unsafeGetTensorImpl()->bump_version();           // (raises where the state must not be written)
     check(qgru_attention_step(&a, bs, hs, stream_of(q)), "qgru_attention_step");
-    state.unsafeGetTensorImpl()->bump_version();
     return out;
 }
 
@@ -346,6 +362,7 @@ py::object rms_norm(const Tensor &x, const Tensor &weight, const std::optional<T
     const Tensor r = residual ? *residual : Tensor();
     check_norm(x, weight, r);
     if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (r.defined() && r.requires_grad()))) {
+        check_capture({&x, &weight, &r});
         const variable_list got = RmsNorm::apply(x, weight, some(r), eps);
         return got.size() == 1 ? py::cast(got[0]) : py::make_tuple(got[0], got[1]);
     }
@@ -355,9 +372,11 @@ py::object rms_norm(const Tensor &x, const Tensor &weight, const std::optional<T
 
 py::object rms_norm_q8(const Tensor &x, const Tensor &weight, const std::optional<Tensor> &residual, double eps, std::optional<double> scale, int64_t zero_point, int64_t bits,
                        bool is_unsigned) {
-    const at::NoGradGuard off;
     const Tensor r = residual ? *residual : Tensor();
     check_norm(x, weight, r);
+    TORCH_CHECK(!at::GradMode::is_enabled() || !r.defined() || !(x.requires_grad() || r.requires_grad()),
+                "rms_norm_q8 has no gradient, and the stream that it returns would end the residual's: call it under torch.no_grad()");
+    const at::NoGradGuard off;
     const Tensor x2 = rows_of(x), w = weight.contiguous(), r2 = r.defined() ? rows_of(r) : Tensor(), h = r.defined() ? at::empty(x.sizes(), x.options()) : Tensor();
     const Tensor q = at::empty(x.sizes(), x.options().dtype(scale && is_unsigned ? at::kByte : at::kChar));
     const Tensor scales = scale ? Tensor() : at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));

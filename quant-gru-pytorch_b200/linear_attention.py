@@ -11,7 +11,9 @@ For every sequence and head, with the state S [Dk, Dv]
 
 Tensors are [T, B, heads, D] as the GRU's are [T, B, H] ([B, T, heads, D] with ``batch_first``) with any strides whose last
 is 1, float32 or bfloat16; states are float32.  Arguments are checked, memory is allocated and the library is called in
-csrc/qgru_seq_torch.cc.  Everything runs on the current stream of the tensors' device, waits for nothing and may be captured into a graph.
+csrc/qgru_seq_torch.cc.  Everything runs on the current stream of the tensors' device, waits for nothing and may be captured into a
+graph; where a backward pass is, no graph of the same leaves made on the default stream may still live (of q, k, v, log_decay and
+initial_state themselves it is refused).
 """
 import math
 
@@ -48,7 +50,9 @@ class LinearAttention(nn.Module):
 
     def __init__(self, input_size, num_heads, key_size=64, value_size=64, num_key_heads=None, batch_first=False, eps=1e-6):
         super().__init__()
-        num_key_heads = num_key_heads or num_heads
+        num_key_heads = num_heads if num_key_heads is None else num_key_heads
+        if min(input_size, num_heads, num_key_heads, key_size, value_size) < 1:
+            raise ValueError("sizes and numbers of heads must be positive")
         if num_heads % num_key_heads:
             raise ValueError(f"{num_heads} heads cannot share {num_key_heads} heads of q and k")
         self.input_size, self.num_heads, self.num_key_heads = input_size, num_heads, num_key_heads

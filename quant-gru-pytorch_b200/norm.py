@@ -18,7 +18,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
 
 
 def rms_norm_q8(x, weight, residual=None, eps=1e-6, scale=None, zero_point=0, bits=8, unsigned=False):
-    """The norm's output in 8 bits, without a gradient.
+    """The norm's output in 8 bits, without a gradient (refused where the residual's stream has one).
 
     With ``scale=None`` every row has a scale of its own: returns (q int8, scales [...] float32[, h]) with q * scale the
     norm, |q| <= 127 (a row of zeros: 0 and 0; a row with infinities or NaN: 0 and NaN).  With a scale (and zero point, width

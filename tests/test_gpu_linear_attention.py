@@ -476,3 +476,39 @@ def test_offsets_beyond_32_bits(dtype, cuda_device):
     want, bound = want_of(*[t[-2:][None] for t in tokens], last[-2:].clone(), None)
     out = la.linear_attention_step(*tokens, last)
     hold({"out": out[-2:][None], "state": last[-2:]}, want, bound)
+
+
+def test_a_capture_beside_a_living_graph_is_refused(cuda_device):
+    q, k, v, g, state, _ = make(cuda_device, 30, 2, 2, 64, 64, BF)
+    leaves = [t.requires_grad_() for t in (q, k, v, g, state)]
+    for only in range(5):
+        use = [t if i == only else t.detach() for i, t in enumerate(leaves)]
+        alive = la.linear_attention(*use)                       # on the default stream
+        side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            something = torch.zeros(8, device=cuda_device)
+            with pytest.raises(RuntimeError, match="still lives"):
+                la.linear_attention(*use)
+            with torch.no_grad():
+                out, _ = la.linear_attention(*use)              # no gradient, nothing to refuse
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, alive[0]) and not something.any()
+        del alive, graph
+
+
+def test_a_state_that_must_not_be_written_is_left_alone(cuda_device):
+    q, k, v, g, _, _ = make(cuda_device, 1, 2, 2, 64, 64, BF)
+    with torch.inference_mode():
+        state = torch.ones(2, 2, 64, 64, device=cuda_device)
+    with pytest.raises(RuntimeError, match="[Ii]nference"):
+        la.linear_attention_step(q[0], k[0], v[0], g[0], state)
+    assert bool((state == 1).all())
+    with torch.inference_mode():
+        la.linear_attention_step(q[0], k[0], v[0], g[0], state)
+
+
+@pytest.mark.parametrize("sizes", [(0, 2), (8, 0), (8, 4, 64, 64, 0), (8, 4, 0), (8, 4, 64, -1), (8, 4, 64, 64, 3)])
+def test_layer_sizes(sizes):
+    with pytest.raises(ValueError):
+        la.LinearAttention(*sizes)

@@ -253,3 +253,30 @@ def test_refusals(cuda_device):
             bad()
     with pytest.raises(RuntimeError, match="columns"):
         norm.rms_norm(torch.ones(1, 16385, device=cuda_device), torch.ones(16385, device=cuda_device))
+
+
+def test_a_capture_beside_a_living_graph_is_refused(cuda_device):
+    x, r, w = make(cuda_device, 30, 512, BF)
+    leaves = [t.requires_grad_() for t in (x, w, r)]
+    for only in range(3):
+        use = [t if i == only else t.detach() for i, t in enumerate(leaves)]
+        alive = norm.rms_norm(*use)                             # on the default stream
+        side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            something = torch.zeros(8, device=cuda_device)
+            with pytest.raises(RuntimeError, match="still lives"):
+                norm.rms_norm(*use)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert not something.any()
+        del alive, graph
+
+
+def test_eight_bits_do_not_cut_a_stream_that_has_a_gradient(cuda_device):
+    x, r, w = make(cuda_device, 3, 512, BF)
+    for a, b in ((x.detach().requires_grad_(), r), (x, r.detach().requires_grad_())):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            norm.rms_norm_q8(a, w, b)
+        with torch.no_grad():
+            norm.rms_norm_q8(a, w, b)
+    norm.rms_norm_q8(x, w.detach().requires_grad_(), r)         # a layer's weight alone has no part in the stream
