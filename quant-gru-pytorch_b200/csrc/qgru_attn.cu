@@ -207,6 +207,8 @@ struct Pass {                      // a state pass
 
 // grid: (B H, tiles of the state, segments).  Order of chunks: forward, or from the last one back (Reverse), where the weight of a
 // token is scale 2^G_t instead of 2^(G_C - G_t).
+// S' = 2^G_C S + (w k)^T v: a 64 x 64 tile of the state in registers, one product a chunk.  Every tile of the state reads k or v anew, and
+// the chunks follow one another: a chunk's latency bounds it (32 x 200 tokens of 8 heads of 64, fp32: 25 us, 6 us a chunk).
 template <class T, bool Reverse>
 __global__ void __launch_bounds__(THREADS) k_states(const __grid_constant__ qgru_attention a, const Pass p) {
     __shared__ alignas(16) float K[TILE], V[TILE];
@@ -268,7 +270,8 @@ __global__ void __launch_bounds__(THREADS) k_states(const __grid_constant__ qgru
     }
 }
 
-// The segments' own sums become the states that they start from.  A thread per element; eight segments' sums are in flight.
+// The segments' own sums become the states that they start from.  A thread per element; eight segments' sums are in flight.  Memory's
+// latency bounds it: a state of 4 heads of 128 x 128 over 37 segments, 10 MB, in 6 us.
 __global__ void __launch_bounds__(128) k_scan_segments(float *seg_state, const float *seg_log, const float *first, int segments, long long size, int per_head) {
     constexpr int AHEAD = 8;
     const long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x;
@@ -292,7 +295,9 @@ __global__ void __launch_bounds__(128) k_scan_segments(float *seg_state, const f
     }
 }
 
-// grid: chunks x B H, the heads of one chunk beside each other (their tokens lie together)
+// grid: chunks x B H, the heads of one chunk beside each other (their tokens lie together).  out = 2^G_t q S + P v, 64 columns of the
+// output at a time over 64 of the head's; the tiles pass through shared memory one after another, so a CTA waits for each: 37 x 127
+// tokens of 5 heads of 40 x 72, fp32, ragged: 25 us.  Up to 64 x 64 of fp32 the kernels further down fetch all tiles at once instead.
 template <class T>
 __global__ void __launch_bounds__(THREADS) k_outputs(const __grid_constant__ qgru_attention a, const float *states) {
     extern __shared__ float4 smem4[];
@@ -351,6 +356,7 @@ __global__ void __launch_bounds__(THREADS) k_outputs(const __grid_constant__ qgr
 }
 
 // grid: chunks x B H.  dq, dk: where the type's elements go, or fp32 sums of every head [T][B][H][Dk] (heads that share q and k).
+// Nine products of 64 x 64 tiles for each pair of them, tiles one after another: shared memory and its barriers bound it.
 template <class T>
 __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ qgru_attention a, const float *states, const float *dstates, float *dq_heads,
                                                        float *dk_heads) {
@@ -502,8 +508,10 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
 }
 
 // ------------------------------------------------------------------------------------- fp32, head sizes up to 64
-// Every chunk's tiles are fetched at once, asynchronously, into a tile each; then nothing waits for memory.  Sixteen warps, 16 x 16 sums a
-// warp.  32 x 200 tokens of 8 heads of 64: gradients 118 us tile after tile, with eight warps, three CTAs an SM.
+// Every chunk's tiles are fetched at once, asynchronously, into a tile each; then nothing waits for memory.  What bounds these is the
+// issue of mma.sync and of the operands' splits (two tf32 values for each, three products, rounded to nearest every eight K).
+// 32 x 200 ragged tokens of 8 heads of 64: outputs 32 us; gradients 85 us so, with sixteen warps, 16 x 16 sums a warp, and 118 us tile
+// after tile, with eight warps, three CTAs an SM.
 constexpr int ALL = 512, NT2 = 2;
 
 __device__ __forceinline__ void cp_float4(float *to, const float *from, bool on) {
@@ -706,7 +714,8 @@ __global__ void __launch_bounds__(ALL, 1) k_gradients_small(const __grid_constan
     }
 }
 
-// dq and dk of heads that share q and k: the sum over each group, one rounding.  V neighbouring elements a thread.
+// dq and dk of heads that share q and k: the sum over each group, one rounding.  V neighbouring elements a thread.  Bytes bound it: 6400
+// tokens, 8 heads of 64 summed in pairs, fp32, 39 MB in 9.5 us (4.1 TB/s, the sums come out of L2).
 template <class T, int V>
 __global__ void k_sum_groups(const __grid_constant__ qgru_attention a, const float *dq, const float *dk) {
     const int g = a.H / a.Hk, per_head = a.Dk / V;
@@ -820,7 +829,8 @@ int backward(const qgru_attention &a, const Cut &c, cudaStream_t st) {
 
 // ------------------------------------------------------------------------------------ single tokens
 // One CTA per (row, head, 128 columns of the state): a lane has V neighbouring columns of a state row, W lanes a row and 256 / W rows at
-// a time, U of them in flight.  Bytes bound it: the state, read and written once.
+// a time, U of them in flight.  Bytes bound it: the state, read and written once.  256 rows of 16 states of 128 x 128, 541 MB: 83 us, 6.5
+// TB/s.  One row of 4 states of 64 x 64: 2.8 us, the launch.
 template <class T, int V>
 __global__ void __launch_bounds__(256) k_step(const __grid_constant__ qgru_attention a, long long state_bs, long long state_hs, int W) {
     constexpr int U = 8;

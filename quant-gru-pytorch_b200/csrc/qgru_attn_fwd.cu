@@ -10,7 +10,12 @@
 //   X  a warp issues the products, one fetches tiles by TMA, two sum the decays up
 // In the order of the products the chunk's part of the state comes first, since the next chunk's outputs wait for it.
 //
-// What is rounded to bf16 on the way: P alone, once, as the output is in the end.
+// What is rounded to bf16 on the way: P alone, once, as the output is in the end; the state counts with 16 bits where it is a factor.
+//
+// What bounds it: the roles' instructions, not the bytes.  64 x 1000 tokens of 16 heads of 64, 524 MB: 172 to 180 us, 3 TB/s (2.9 us a
+// chunk and SM, the tensor pipe busy for 18 % of it).  The roles share one instruction cache, so their loops stay rolled: unrolled, with
+// 1.7 times the misses, 274 us.  A sixth warpgroup, P taken by two: 190.  16 x 1000 tokens of 8 heads of 128: 70 us with the outputs, 46
+// from the end without.  One phrase of 24 tokens, 4 heads of 64: 9 us, the latency of the roles one after another.
 #include <algorithm>
 #include <type_traits>
 

@@ -115,7 +115,8 @@ constexpr int STATES_TILES = DK / 64 * PANEL + 2 * (DV / 64) * PANEL + 3 * (DK /
 
 // grid (B H, segments).  S' = 2^G_C S + (w k)^T v: lane i of tensor memory is row i of the state, whose fp32 sums stay in
 // registers, half a row a thread.  While the products of a chunk run, the next one's tokens are read and the state before this one
-// leaves.  With DK = 64 lanes 64 .. 127 repeat the first 64 (M is 128) and are not read.
+// leaves.  With DK = 64 lanes 64 .. 127 repeat the first 64 (M is 128) and are not read.  One chunk's chain of load, split, product and
+// conversion bounds it, eight in turn: 16 x 1000 tokens of 8 heads of 60, 61 us.
 template <int DK, int DV, bool Reverse>
 __global__ void __launch_bounds__(THREADS) k_states_tc(const __grid_constant__ qgru_attention a, const __grid_constant__ Pass p) {
     extern __shared__ unsigned char raw[];
@@ -251,7 +252,8 @@ template <int DK, int DV>
 constexpr int OUTPUTS_TILES = 2 * (DK / 64) * PANEL + DV / 64 * PANEL;
 
 // grid: chunks x B H, the heads of one chunk beside each other.  Two threads a token, each half of the pairs' weights and half of the
-// output's columns.  The state lies where k was once q k^T is there.
+// output's columns.  The state lies where k was once q k^T is there.  Two CTAs an SM cover each other's waits; the element loads of what
+// TMA does not take bound it: 16 x 1000 tokens of 8 heads of 60, 117 us (64, by TMA, in k_walk: 34 with the states).
 template <int DK, int DV>
 __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant__ qgru_attention a, const bf16 *states, int *flag) {
     extern __shared__ unsigned char raw[];
@@ -438,9 +440,6 @@ __device__ __forceinline__ float scale_sums(uint32_t taddr, float w, uint32_t ti
     return dot ? dot_row(tile, row, c0, v) : 0.f;
 }
 
-// grid: chunks x B H.  Pairs lie as [s][t] here, lane s of tensor memory.  Four blocks of 128 columns of it:
-//   0  (k q^T), then P^T in bf16     1  (v dout^T), then dv     2  dk     3  dq
-// Four threads a row, a quarter of the columns each.  P^T is the operand of dv from tensor memory, E^T that of dk (K in its columns) and of dq (K in its rows) from shared memory.
 // A row's Cols values from column c0 on, as bf16, into a tile; and the tile's rows below `rows` into a tensor, whole lines at a time.
 template <int Cols>
 __device__ __forceinline__ void put_row(uint32_t tile, int row, int c0, const float (&v)[Cols]) {
@@ -472,6 +471,13 @@ __device__ __forceinline__ void copy_out(uint32_t tile, const qgru_seq_tensor &x
     }
 }
 
+// grid: chunks x B H.  Pairs lie as [s][t] here, lane s of tensor memory.  Four blocks of 128 columns of it:
+//   0  (k q^T), then P^T in bf16     1  (v dout^T), then dv     2  dk     3  dq
+// Four threads a row, a quarter of the columns each.  P^T is the operand of dv from tensor memory, E^T that of dk (K in its columns) and
+// of dq (K in its rows) from shared memory.
+// One CTA an SM, whose products, loads and conversions between tensor memory and operands follow one another: that chain bounds it.  16 x
+// 1000 tokens of 8 heads of 128: 105 us with 512 threads and tiles by TMA, 108 where the threads load them, 155 with 256 threads; bytes alone
+// would take 43 (285 MB).  A second CTA an SM has no room: 224 KB of operands.
 template <int DK, int DV, bool Tma>
 __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_constant__ qgru_attention a, const __grid_constant__ Gradients p) {
     extern __shared__ unsigned char raw[];
