@@ -89,8 +89,13 @@ __device__ __forceinline__ void await(Shared &s, int bar, uint32_t parity) {
 __device__ __forceinline__ void end(Shared &s, uint32_t columns, int *flag, int tid) {
     tc::tc_fence_before_sync();
     __syncthreads();
+    if (s.failed) {            // copies and products may be under way: a millisecond is far more than they take
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000ll) {
+        }
+        if (tid == 0) *flag = 1;
+    }
     if (tid < 32) tc::tmem_dealloc(s.tmem, columns);
-    if (tid == 0 && s.failed) *flag = 1;
 }
 __device__ __forceinline__ unsigned char *tiles_of(unsigned char *raw) {
     return reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -385,15 +390,19 @@ __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant
 
 // ------------------------------------------------------------------------------------- gradients
 constexpr int GRAD_THREADS = 512;
+struct Item {
+    int index, b, h, t0, all, tokens;
+};
 struct Gradients {
-    CUtensorMap q, k, v, o, S, dS;       // where TMA takes the tensors
+    CUtensorMap q, k, v, o, S, dS, dq, dk, dv;   // where TMA takes the tensors
     const bf16 *states, *dstates;
     const float *through;                // products of the two, THROUGH parts each
     float *dq_heads, *dk_heads;          // [T][B][H][Dk] where heads share q and k, else null
+    int items;                           // chunks of all heads
     int *flag;
 };
 template <int DK, int DV>
-constexpr int GRADIENTS_TILES = 2 * (DK / 64) * PANEL + 2 * (DV / 64) * PANEL + 2 * DK * DV * 2 + 2 * PANEL;
+constexpr int GRADIENTS_TILES = 2 * (DK / 64) * PANEL + 2 * (DV / 64) * PANEL + 2 * DK * DV * 2 + 2 * PANEL + (DV == 64 ? 2 * (DK / 64) * PANEL : 0);
 
 // Sum over the lanes of a warp for each of 32 columns: lane i gets column i's.
 __device__ __forceinline__ float sum_columns(float (&m)[32], int lane) {
@@ -449,7 +458,7 @@ __device__ __forceinline__ void put_row(uint32_t tile, int row, int c0, const fl
         sts16(tile + (c >> 3) * PANEL + chunk_at(row, c & 7), pack(v[i], v[i + 1]), pack(v[i + 2], v[i + 3]), pack(v[i + 4], v[i + 5]), pack(v[i + 6], v[i + 7]));
     }
 }
-template <int D>
+template <int D, bool Zeros>
 __device__ __forceinline__ void copy_out(uint32_t tile, const qgru_seq_tensor &x, long long base, int t0, int rows, int d, int tid) {
     bf16 *p = static_cast<bf16 *>(x.p) + base + (long long)t0 * x.ts;
     const bool vec = d % 8 == 0 && (x.ts | x.bs | x.hs) % 8 == 0 && reinterpret_cast<uintptr_t>(x.p) % 16 == 0;
@@ -458,7 +467,7 @@ __device__ __forceinline__ void copy_out(uint32_t tile, const qgru_seq_tensor &x
     for (int i = 0; i < C * PER_ROW / GRAD_THREADS; ++i) {
         const int e = i * GRAD_THREADS + tid, r = e / PER_ROW, c = e % PER_ROW;
         if (r >= rows || c * 8 >= d) continue;
-        const uint4 v = lds16(tile + (c >> 3) * PANEL + chunk_at(r, c & 7));
+        const uint4 v = Zeros ? make_uint4(0u, 0u, 0u, 0u) : lds16(tile + (c >> 3) * PANEL + chunk_at(r, c & 7));
         bf16 *to = p + (long long)r * x.ts + c * 8;
         if (vec) {
             *reinterpret_cast<uint4 *>(to) = v;
@@ -471,7 +480,7 @@ __device__ __forceinline__ void copy_out(uint32_t tile, const qgru_seq_tensor &x
     }
 }
 
-// grid: chunks x B H.  Pairs lie as [s][t] here, lane s of tensor memory.  Four blocks of 128 columns of it:
+// A CTA an SM, which takes chunk after chunk of all heads.  Pairs lie as [s][t] here, lane s of tensor memory.  Four blocks of 128 columns of it:
 //   0  (k q^T), then P^T in bf16     1  (v dout^T), then dv     2  dk     3  dq
 // Four threads a row, a quarter of the columns each.  P^T is the operand of dv from tensor memory, E^T that of dk (K in its columns) and
 // of dq (K in its rows) from shared memory.
@@ -485,17 +494,18 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
     Shared &s = *reinterpret_cast<Shared *>(tiles + GRADIENTS_TILES<DK, DV>);
     constexpr int KT = DK / 64 * PANEL, VT = DV / 64 * PANEL, ST = DK * DV * 2, KQ = DK / 4, VQ = DV / 4;
     const uint32_t q_t = tc::smem_u32(tiles), k_t = q_t + KT, v_t = k_t + KT, o_t = v_t + VT, S_t = o_t + VT, dS_t = S_t + ST, E_t = dS_t + ST;
+    // where dq and dk become rows of bf16: tiles of their own, or where these have no room those of the states, which have been used by then
+    const uint32_t dq_t = DV == 64 ? E_t + 2 * PANEL : S_t, dk_t = DV == 64 ? dq_t + KT : dS_t;
     // once v has been used, its tile holds sums by token
     float *t_sums = reinterpret_cast<float *>(tiles + 2 * KT);          // [4][128] over s of a block's lanes, for each t
     float *s_sums = t_sums + 4 * C, *q_dots = s_sums + 4 * C, *k_dots = q_dots + 4 * C;     // [4][128] each
     double *totals = reinterpret_cast<double *>(k_dots + 4 * C);        // [4]
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, heads = a.B * a.H, chunk = blockIdx.x / heads, bh = blockIdx.x % heads, b = bh / a.H, h = bh % a.H;
-    const int t0 = chunk * C, all = min(a.T - t0, C), tokens = min(max(valid_tokens(a, b) - t0, 0), C);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, heads = a.B * a.H, share = a.H / a.Hk;
     const int block = warp & 3, row = block * 32 + lane, part = warp >> 2;
-    const auto put_heads = [&](float *sums, const float (&v)[KQ]) {        // heads that share q and k: fp32, added up afterwards
-        if (row >= all) return;
+    const auto put_heads = [&](float *sums, const Item &x, const float (&v)[KQ]) {        // heads that share q and k: fp32, added up afterwards
+        if (row >= x.all) return;
         const int c0 = part * KQ;
-        float *to = sums + (((long long)(t0 + row) * a.B + b) * a.H + h) * a.Dk + c0;
+        float *to = sums + (((long long)(x.t0 + row) * a.B + x.b) * a.H + x.h) * a.Dk + c0;
 #pragma unroll
         for (int i = 0; i < KQ; i += 4) {
             if (a.Dk % 4 == 0) {
@@ -507,227 +517,280 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
             }
         }
     };
-    const long long gb = at(a.ddecay, b, h) + (long long)t0 * a.ddecay.ts;
-    if (tokens == 0) {
-        for (int e = tid; e < C * (DK + DV) / 8; e += GRAD_THREADS) sts16(q_t + e * 16, 0u, 0u, 0u, 0u);      // q's, k's and v's tiles, or more
-        __syncthreads();
-        if (p.dq_heads) {
-            const float z[KQ] = {};
-            put_heads(p.dq_heads, z);
-            put_heads(p.dk_heads, z);
-        } else {
-            copy_out<DK>(q_t, a.dq, at(a.dq, b, h), t0, all, a.Dk, tid);
-            copy_out<DK>(q_t, a.dk, at(a.dk, b, h), t0, all, a.Dk, tid);
+    // The CTA's next chunk with tokens; those before it, behind the ends of their sequences, get zeros.
+    const auto next_of = [&](long long index) {
+        Item x{};
+        for (; index < p.items; index += gridDim.x) {
+            x.index = (int)index;
+            x.b = x.index % heads / a.H;
+            x.h = x.index % heads % a.H;
+            x.t0 = x.index / heads * C;
+            x.all = min(a.T - x.t0, C);
+            x.tokens = min(max(valid_tokens(a, x.b) - x.t0, 0), C);
+            if (x.tokens) return x;
+            if (p.dq_heads) {
+                const float z[KQ] = {};
+                put_heads(p.dq_heads, x, z);
+                put_heads(p.dk_heads, x, z);
+            } else {
+                copy_out<DK, true>(0, a.dq, at(a.dq, x.b, x.h), x.t0, x.all, a.Dk, tid);
+                copy_out<DK, true>(0, a.dk, at(a.dk, x.b, x.h), x.t0, x.all, a.Dk, tid);
+            }
+            copy_out<DV, true>(0, a.dv, at(a.dv, x.b, x.h), x.t0, x.all, a.Dv, tid);
+            if (tid < x.all) seq::store_f(a.ddecay.p, at(a.ddecay, x.b, x.h) + (long long)(x.t0 + tid) * a.ddecay.ts, a.decay_bf16, 0.f);
         }
-        copy_out<DV>(q_t, a.dv, at(a.dv, b, h), t0, all, a.Dv, tid);
-        if (tid < all) seq::store_f(a.ddecay.p, gb + tid * a.ddecay.ts, a.decay_bf16, 0.f);
-        return;
-    }
-    const int hk = h / (a.H / a.Hk);
-    const long long state = ((long long)chunk * heads + bh) * (DK * DV);
-    const long long g = load_decay(a, b, h, t0, tokens, tid);
-    if constexpr (!Tma) {
-        load_rows<DK, GRAD_THREADS>(q_t, a.q, at(a.q, b, hk), t0, tokens, a.Dk, tid);
-        load_rows<DK, GRAD_THREADS>(k_t, a.k, at(a.k, b, hk), t0, tokens, a.Dk, tid);
-        load_rows<DV, GRAD_THREADS>(v_t, a.v, at(a.v, b, h), t0, tokens, a.Dv, tid);
-        load_rows<DV, GRAD_THREADS>(o_t, a.dout, at(a.dout, b, h), t0, tokens, a.Dv, tid);
-        load_state<DK, DV, GRAD_THREADS>(S_t, p.states + state, tid);
-        load_state<DK, DV, GRAD_THREADS>(dS_t, p.dstates + state, tid);
-        cp_commit();
-    }
+        return x;                       // (no tokens)
+    };
+    // Tiles by TMA, by one thread: keys and queries; values and the output's gradient; the states.
+    const auto fetch_qk = [&](const Item &x) {
+        tc::mbar_expect_tx(&s.bar[4], 2 * KT + 2 * VT);
+        for (int i = 0; i < DK / 64; ++i) {
+            tma_load_4d(k_t + i * PANEL, &p.k, &s.bar[4], i * 64, x.t0, x.h / share, x.b);
+            tma_load_4d(q_t + i * PANEL, &p.q, &s.bar[4], i * 64, x.t0, x.h / share, x.b);
+        }
+    };
+    const auto fetch_vo = [&](const Item &x) {
+        for (int i = 0; i < DV / 64; ++i) {
+            tma_load_4d(v_t + i * PANEL, &p.v, &s.bar[4], i * 64, x.t0, x.h, x.b);
+            tma_load_4d(o_t + i * PANEL, &p.o, &s.bar[4], i * 64, x.t0, x.h, x.b);
+        }
+    };
+    const auto fetch_states = [&](const Item &x) {
+        tc::mbar_expect_tx(&s.bar[5], 2 * ST);
+        for (int i = 0; i < DV / 64; ++i) {
+            tc::tma_load_2d(tiles + 2 * KT + 2 * VT + i * (DK * 128), &p.S, &s.bar[5], i * 64, x.index * DK);
+            tc::tma_load_2d(tiles + 2 * KT + 2 * VT + ST + i * (DK * 128), &p.dS, &s.bar[5], i * 64, x.index * DK);
+        }
+    };
+    Item x = next_of(blockIdx.x);
+    const auto decay_of = [&](const Item &x) {
+        return tid < x.tokens ? seq::load_f(a.decay.p, at(a.decay, x.b, x.h) + (long long)(x.t0 + tid) * a.decay.ts, a.decay_bf16) : 0.f;
+    };
+    float decay = decay_of(x);
     begin(s, 512, tid);
     if constexpr (Tma) {
-        if (tid == 0) {
-            tc::mbar_expect_tx(&s.bar[4], 2 * KT + 2 * VT);
-            for (int i = 0; i < DK / 64; ++i) {
-                tma_load_4d(k_t + i * PANEL, &p.k, &s.bar[4], i * 64, t0, hk, b);
-                tma_load_4d(q_t + i * PANEL, &p.q, &s.bar[4], i * 64, t0, hk, b);
-            }
-            for (int i = 0; i < DV / 64; ++i) {
-                tma_load_4d(v_t + i * PANEL, &p.v, &s.bar[4], i * 64, t0, h, b);
-                tma_load_4d(o_t + i * PANEL, &p.o, &s.bar[4], i * 64, t0, h, b);
-            }
-            tc::mbar_expect_tx(&s.bar[5], 2 * ST);
-            for (int i = 0; i < DV / 64; ++i) {
-                tc::tma_load_2d(tiles + 2 * KT + 2 * VT + i * (DK * 128), &p.S, &s.bar[5], i * 64, (chunk * heads + bh) * DK);
-                tc::tma_load_2d(tiles + 2 * KT + 2 * VT + ST + i * (DK * 128), &p.dS, &s.bar[5], i * 64, (chunk * heads + bh) * DK);
-            }
+        if (tid == 0 && x.tokens) {
+            fetch_qk(x);
+            fetch_vo(x);
+            fetch_states(x);
         }
     }
     const uint32_t tm = s.tmem, base = lane_base(tm, warp);
     const Operand q{q_t, PANEL}, k{k_t, PANEL}, v{v_t, PANEL}, o{o_t, PANEL}, S{S_t, DK * 128}, dS{dS_t, DK * 128}, E{E_t, PANEL};
-    sum_decays(s, g, tid);
-    if constexpr (Tma) {
-        await(s, 4, 0);
-        if (tokens < C) {               // what lies behind the sequence was fetched too
-            for (int e = tid; e < (C - tokens) * 8; e += GRAD_THREADS) {
-                const int r = tokens + e / 8, at16 = r * 128 + e % 8 * 16;
-                for (int i = 0; i < (2 * KT + 2 * VT) / PANEL; ++i) sts16(q_t + i * PANEL + at16, 0u, 0u, 0u, 0u);
-            }
+    for (uint32_t turn = 0; x.tokens; turn ^= 1) {
+        const int b = x.b, h = x.h, hk = h / share, t0 = x.t0, all = x.all, tokens = x.tokens;
+        if constexpr (!Tma) {
+            load_rows<DK, GRAD_THREADS>(q_t, a.q, at(a.q, b, hk), t0, tokens, a.Dk, tid);
+            load_rows<DK, GRAD_THREADS>(k_t, a.k, at(a.k, b, hk), t0, tokens, a.Dk, tid);
+            load_rows<DV, GRAD_THREADS>(v_t, a.v, at(a.v, b, h), t0, tokens, a.Dv, tid);
+            load_rows<DV, GRAD_THREADS>(o_t, a.dout, at(a.dout, b, h), t0, tokens, a.Dv, tid);
+            load_state<DK, DV, GRAD_THREADS>(S_t, p.states + (long long)x.index * (DK * DV), tid);
+            load_state<DK, DV, GRAD_THREADS>(dS_t, p.dstates + (long long)x.index * (DK * DV), tid);
+            cp_commit();
         }
-    } else {
-        cp_wait<0>();
-    }
-    fence_async();
-    __syncthreads();
-    if (tid < 32) {
-        const uint32_t leader = elect();
-        tc::tc_fence_after_sync();
-        product<false, false, C, DK>(leader, tm, k, q, false);
-        product<false, false, C, DV>(leader, tm + 128, v, o, false);
-        commit(leader, &s.bar[0]);
-    }
-    // from the start of t's block of 32 to t
-    if (tid < C) s.f[tid] = tid < 32 ? ex2(s.G[tid].x + s.G[tid].y) : ex2_diff(s.G[tid], s.G[(tid & ~31) - 1]);
-    if constexpr (Tma) await(s, 5, 0);
-    __syncthreads();
-    if (tid < 32) {
-        const uint32_t leader = elect();
-        tc::tc_fence_after_sync();
-        product<false, false, DK, DV>(leader, tm + 256, v, dS, false);
-        product<false, false, DK, DV>(leader, tm + 384, o, S, false);
-        commit(leader, &s.bar[1]);
-    }
-    await(s, 0, 0);
-    await(s, 1, 0);
-    const float2 G = s.G[row], last = s.G[C - 1];
-    // the pairs: blocks of 32 x 32, t from s on
-    uint32_t P[16];
-    float s_sum = 0.f;
-    if (part < block) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) P[i] = 0u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + i), 0u, 0u, 0u, 0u);
-    } else {
-        float m[32];
-        float2 sum = both(0.f);
-        const float2 r = both(a.scale * (part > block ? ex2_diff(s.G[part * 32 - 1], G) : 1.f));
-#pragma unroll
-        for (int t0 = 0; t0 < 32; t0 += 16) {
-            float2 x[8], y[8];
-            int32_t u[2][16];
-            tc::tmem_ld16(base + part * 32 + t0, u[0]);
-            tc::tmem_ld16(base + 128 + part * 32 + t0, u[1]);
-            tc::tmem_ld_wait();
-            uint32_t e[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = make_float2(__int_as_float(u[0][2 * i]), __int_as_float(u[0][2 * i + 1]));
-                y[i] = make_float2(__int_as_float(u[1][2 * i]), __int_as_float(u[1][2 * i + 1]));
-                const int t = t0 + 2 * i;
-                float2 w;
-                if (part > block) {
-                    w = __fmul2_rn(r, *reinterpret_cast<const float2 *>(&s.f[part * 32 + t]));
-                } else {
-                    const float4 g2 = *reinterpret_cast<const float4 *>(&s.G[part * 32 + t]);
-                    w = __fmul2_rn(r, make_float2(ex2_diff(make_float2(g2.x, g2.y), G), ex2_diff(make_float2(g2.z, g2.w), G)));
-                    // (not by a factor of 0: what it would hide may be infinite)
-                    if (t < lane) x[i].x = y[i].x = 0.f, w.x = 0.f;
-                    if (t + 1 < lane) x[i].y = y[i].y = 0.f, w.y = 0.f;
+        sum_decays(s, tid < C ? decay_units(decay) : 0, tid);
+        if constexpr (Tma) {
+            await(s, 4, turn);
+            if (tokens < C) {               // what lies behind the sequence was fetched too
+                for (int e = tid; e < (C - tokens) * 8; e += GRAD_THREADS) {
+                    const int r = tokens + e / 8, at16 = r * 128 + e % 8 * 16;
+                    for (int i = 0; i < (2 * KT + 2 * VT) / PANEL; ++i) sts16(q_t + i * PANEL + at16, 0u, 0u, 0u, 0u);
                 }
-                const float2 pv = __fmul2_rn(w, x[i]);
-                float2 mv = __fmul2_rn(pv, y[i]);
-                if (part == block) {            // a pair of a token with itself moves with no decay
-                    if (t == lane) mv.x = 0.f;
-                    if (t + 1 == lane) mv.y = 0.f;
-                }
-                sum = __fadd2_rn(sum, mv);
-                m[t] = mv.x;
-                m[t + 1] = mv.y;
-                P[t / 2] = pack(pv);
-                e[i] = pack(__fmul2_rn(w, y[i]));
             }
-            sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + t0 / 8), e[0], e[1], e[2], e[3]);
-            sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + t0 / 8 + 1), e[4], e[5], e[6], e[7]);
+        } else {
+            cp_wait<0>();
         }
-        s_sum = sum.x + sum.y;
-        t_sums[block * C + part * 32 + lane] = sum_columns(m, lane);
-    }
-    s_sums[part * C + row] = s_sum;
-    const float to_end = ex2_diff(last, G), from_start = a.scale * ex2(G.x + G.y);
-    k_dots[part * C + row] = scale_sums<KQ>(base + 256 + part * KQ, to_end, k_t, row, part * KQ, true);
-    q_dots[part * C + row] = scale_sums<KQ>(base + 384 + part * KQ, from_start, q_t, row, part * KQ, true);
-    fence_async();
-    tc::tmem_st_wait();
-    tc::tc_fence_before_sync();
-    __syncthreads();                                  // the pairs' sums have been read, E^T and the scaled sums are there
-    if (tid < 32) {
-        const uint32_t leader = elect();
-        tc::tc_fence_after_sync();
-        product<false, true, DV, DK>(leader, tm + 128, k, dS, false);
-        commit(leader, &s.bar[2]);
-        product<false, true, DK, C>(leader, tm + 256, E, q, true);
-        product<true, true, DK, C>(leader, tm + 384, E, k, true);
-        commit(leader, &s.bar[3]);
-    }
-    tc::tc_fence_after_sync();
-    tmem_store(base + part * 16, P);
-    // the decays' gradient: from each token on, every pair across it, and what passes from the state before the chunk to that behind it
-    double d = 0.0, own = 0.0;
-    if (tid < C) {
-        float t_sum = 0.f;
-        for (int w = 0; w <= tid >> 5; ++w) t_sum += t_sums[w * C + tid];
-        own = (double)t_sum;
-        double kd = 0.0;
-        for (int w = 0; w < 4; ++w) {
-            own += (double)q_dots[w * C + tid] - (double)s_sums[w * C + tid];
-            kd += (double)k_dots[w * C + tid];
+        fence_async();
+        __syncthreads();
+        if (tid < 32) {
+            const uint32_t leader = elect();
+            tc::tc_fence_after_sync();
+            product<false, false, C, DK>(leader, tm, k, q, false);
+            product<false, false, C, DV>(leader, tm + 128, v, o, false);
+            commit(leader, &s.bar[0]);
         }
-        d = running_sum<C>(kd - own, s.sums, tid) - (kd - own);
-    }
-    double total = own;
-    for (int i = 16; i; i >>= 1) total += __shfl_xor_sync(0xffffffffu, total, i);
-    if (lane == 0 && tid < C) totals[warp] = total;
-    tc::tmem_st_wait();
-    await(s, 2, 0);
-    scale_sums<VQ>(base + 128 + part * VQ, to_end, 0, 0, 0, false);
-    tc::tmem_st_wait();
-    tc::tc_fence_before_sync();
-    __syncthreads();
-    if (tid < 32) {
-        const uint32_t leader = elect();
+        // from the start of t's block of 32 to t
+        if (tid < C) s.f[tid] = tid < 32 ? ex2(s.G[tid].x + s.G[tid].y) : ex2_diff(s.G[tid], s.G[(tid & ~31) - 1]);
+        if constexpr (Tma) {
+            await(s, 5, turn);
+            if (tid == 0) stores_read<0>();               // E's tile was the last chunk's dv
+        }
+        __syncthreads();
+        if (tid < 32) {
+            const uint32_t leader = elect();
+            tc::tc_fence_after_sync();
+            product<false, false, DK, DV>(leader, tm + 256, v, dS, false);
+            product<false, false, DK, DV>(leader, tm + 384, o, S, false);
+            commit(leader, &s.bar[1]);
+        }
+        await(s, 0, turn);
+        await(s, 1, turn);
+        const float2 G = s.G[row], last = s.G[C - 1];
+        // the pairs: blocks of 32 x 32, t from s on
+        uint32_t P[16];
+        float s_sum = 0.f;
+        if (part < block) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) P[i] = 0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + i), 0u, 0u, 0u, 0u);
+        } else {
+            float m[32];
+            float2 sum = both(0.f);
+            const float2 r = both(a.scale * (part > block ? ex2_diff(s.G[part * 32 - 1], G) : 1.f));
+#pragma unroll
+            for (int t0 = 0; t0 < 32; t0 += 16) {
+                float2 x[8], y[8];
+                int32_t u[2][16];
+                tc::tmem_ld16(base + part * 32 + t0, u[0]);
+                tc::tmem_ld16(base + 128 + part * 32 + t0, u[1]);
+                tc::tmem_ld_wait();
+                uint32_t e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    x[i] = make_float2(__int_as_float(u[0][2 * i]), __int_as_float(u[0][2 * i + 1]));
+                    y[i] = make_float2(__int_as_float(u[1][2 * i]), __int_as_float(u[1][2 * i + 1]));
+                    const int t = t0 + 2 * i;
+                    float2 w;
+                    if (part > block) {
+                        w = __fmul2_rn(r, *reinterpret_cast<const float2 *>(&s.f[part * 32 + t]));
+                    } else {
+                        const float4 g2 = *reinterpret_cast<const float4 *>(&s.G[part * 32 + t]);
+                        w = __fmul2_rn(r, make_float2(ex2_diff(make_float2(g2.x, g2.y), G), ex2_diff(make_float2(g2.z, g2.w), G)));
+                        // (not by a factor of 0: what it would hide may be infinite)
+                        if (t < lane) x[i].x = y[i].x = 0.f, w.x = 0.f;
+                        if (t + 1 < lane) x[i].y = y[i].y = 0.f, w.y = 0.f;
+                    }
+                    const float2 pv = __fmul2_rn(w, x[i]);
+                    float2 mv = __fmul2_rn(pv, y[i]);
+                    if (part == block) {            // a pair of a token with itself moves with no decay
+                        if (t == lane) mv.x = 0.f;
+                        if (t + 1 == lane) mv.y = 0.f;
+                    }
+                    sum = __fadd2_rn(sum, mv);
+                    m[t] = mv.x;
+                    m[t + 1] = mv.y;
+                    P[t / 2] = pack(pv);
+                    e[i] = pack(__fmul2_rn(w, y[i]));
+                }
+                sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + t0 / 8), e[0], e[1], e[2], e[3]);
+                sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + t0 / 8 + 1), e[4], e[5], e[6], e[7]);
+            }
+            s_sum = sum.x + sum.y;
+            t_sums[block * C + part * 32 + lane] = sum_columns(m, lane);
+        }
+        s_sums[part * C + row] = s_sum;
+        const float to_end = ex2_diff(last, G), from_start = a.scale * ex2(G.x + G.y);
+        k_dots[part * C + row] = scale_sums<KQ>(base + 256 + part * KQ, to_end, k_t, row, part * KQ, true);
+        q_dots[part * C + row] = scale_sums<KQ>(base + 384 + part * KQ, from_start, q_t, row, part * KQ, true);
+        fence_async();
+        tc::tmem_st_wait();
+        tc::tc_fence_before_sync();
+        __syncthreads();                                  // the pairs' sums have been read, E^T and the scaled sums are there
+        if (tid < 32) {
+            const uint32_t leader = elect();
+            tc::tc_fence_after_sync();
+            product<false, true, DV, DK>(leader, tm + 128, k, dS, false);
+            commit(leader, &s.bar[2]);
+            product<false, true, DK, C>(leader, tm + 256, E, q, true);
+            product<true, true, DK, C>(leader, tm + 384, E, k, true);
+            commit(leader, &s.bar[3]);
+        }
         tc::tc_fence_after_sync();
-        product_ts<true, DV, C>(leader, tm + 128, tm, o, true);
-        commit(leader, &s.bar[2]);
-    }
-    if (tid < all) {
-        double x = d;
-        for (int w = 0; w < tid >> 5; ++w) x += s.sums[w];
-        double through = 0.0;
-        for (int w = 0; w < THROUGH; ++w) through += (double)p.through[((long long)chunk * heads + bh) * THROUGH + w];
-        x += totals[0] + totals[1] + totals[2] + totals[3] + through * (double)exp2_of(last);
-        seq::store_f(a.ddecay.p, gb + tid * a.ddecay.ts, a.decay_bf16, tid < tokens ? (float)x : 0.f);
-    }
-    // Out by way of the tiles of q, k and E, which nothing reads any more: a thread's part of a row on its own would be a store of 16 bytes
-    // in each of 32 lines.
-    const bool live = row < tokens;
-    await(s, 3, 0);
-    {
-        float x[KQ];
-        tmem_load(base + 384 + part * KQ, x);
+        tmem_store(base + part * 16, P);
+        // the decays' gradient: from each token on, every pair across it, and what passes from the state before the chunk to that behind it
+        double d = 0.0, own = 0.0;
+        if (tid < C) {
+            float t_sum = 0.f;
+            for (int w = 0; w <= tid >> 5; ++w) t_sum += t_sums[w * C + tid];
+            own = (double)t_sum;
+            double kd = 0.0;
+            for (int w = 0; w < 4; ++w) {
+                own += (double)q_dots[w * C + tid] - (double)s_sums[w * C + tid];
+                kd += (double)k_dots[w * C + tid];
+            }
+            d = running_sum<C>(kd - own, s.sums, tid) - (kd - own);
+        }
+        double total = own;
+        for (int i = 16; i; i >>= 1) total += __shfl_xor_sync(0xffffffffu, total, i);
+        if (lane == 0 && tid < C) totals[warp] = total;
+        tc::tmem_st_wait();
+        await(s, 2, 0);
+        scale_sums<VQ>(base + 128 + part * VQ, to_end, 0, 0, 0, false);
+        tc::tmem_st_wait();
+        tc::tc_fence_before_sync();
+        __syncthreads();
+        if (tid < 32) {
+            const uint32_t leader = elect();
+            tc::tc_fence_after_sync();
+            product_ts<true, DV, C>(leader, tm + 128, tm, o, true);
+            commit(leader, &s.bar[2]);
+        }
+        if (tid < all) {
+            double sum = d;
+            for (int w = 0; w < tid >> 5; ++w) sum += s.sums[w];
+            double through = 0.0;
+            for (int w = 0; w < THROUGH; ++w) through += (double)p.through[(long long)x.index * THROUGH + w];
+            sum += totals[0] + totals[1] + totals[2] + totals[3] + through * (double)exp2_of(last);
+            seq::store_f(a.ddecay.p, at(a.ddecay, b, h) + (long long)(t0 + tid) * a.ddecay.ts, a.decay_bf16, tid < tokens ? (float)sum : 0.f);
+        }
+        // The next chunk's tiles come as soon as nothing reads the ones that they replace.
+        const Item next = next_of((long long)x.index + gridDim.x);
+        decay = decay_of(next);
+        const bool live = row < tokens;
+        await(s, 3, turn);
+        if constexpr (Tma) {
+            if (tid == 0 && next.tokens) fetch_qk(next);
+        }
+        // Out by way of tiles: a thread's part of a row on its own would be a store of 16 bytes in each of 32 lines.
+        {
+            float r[KQ];
+            tmem_load(base + 384 + part * KQ, r);
 #pragma unroll
-        for (int i = 0; i < KQ; ++i) x[i] = live ? x[i] : 0.f;
-        p.dq_heads ? put_heads(p.dq_heads, x) : put_row(q_t, row, part * KQ, x);
-        tmem_load(base + 256 + part * KQ, x);
+            for (int i = 0; i < KQ; ++i) r[i] = live ? r[i] : 0.f;
+            p.dq_heads ? put_heads(p.dq_heads, x, r) : put_row(dq_t, row, part * KQ, r);
+            tmem_load(base + 256 + part * KQ, r);
 #pragma unroll
-        for (int i = 0; i < KQ; ++i) x[i] = live ? x[i] : 0.f;
-        p.dk_heads ? put_heads(p.dk_heads, x) : put_row(k_t, row, part * KQ, x);
-    }
-    await(s, 2, 1);
-    {
-        float x[VQ];
-        tmem_load(base + 128 + part * VQ, x);
+            for (int i = 0; i < KQ; ++i) r[i] = live ? r[i] : 0.f;
+            p.dk_heads ? put_heads(p.dk_heads, x, r) : put_row(dk_t, row, part * KQ, r);
+        }
+        await(s, 2, 1);
+        {
+            float r[VQ];
+            tmem_load(base + 128 + part * VQ, r);
 #pragma unroll
-        for (int i = 0; i < VQ; ++i) x[i] = live ? x[i] : 0.f;
-        put_row(E_t, row, part * VQ, x);
+            for (int i = 0; i < VQ; ++i) r[i] = live ? r[i] : 0.f;
+            put_row(E_t, row, part * VQ, r);
+        }
+        fence_async();                                    // (the sums in v's tile come before what TMA writes there)
+        tc::tc_fence_before_sync();
+        if (__syncthreads_or(s.failed)) break;
+        if constexpr (Tma) {
+            if (tid == 0) {
+                if (next.tokens) fetch_vo(next);
+                for (int i = 0; i < DK / 64 && !p.dq_heads; ++i) {
+                    tma_store_4d(&p.dq, dq_t + i * PANEL, i * 64, t0, h, b);
+                    tma_store_4d(&p.dk, dk_t + i * PANEL, i * 64, t0, h, b);
+                }
+                stores_commit();
+                for (int i = 0; i < DV / 64; ++i) tma_store_4d(&p.dv, E_t + i * PANEL, i * 64, t0, h, b);
+                stores_commit();
+                if (next.tokens) {
+                    if (DV == 128) stores_read<1>();      // dq's and dk's tiles are the states'
+                    fetch_states(next);
+                }
+            }
+        } else {
+            if (!p.dq_heads) {
+                copy_out<DK, false>(dq_t, a.dq, at(a.dq, b, h), t0, all, a.Dk, tid);
+                copy_out<DK, false>(dk_t, a.dk, at(a.dk, b, h), t0, all, a.Dk, tid);
+            }
+            copy_out<DV, false>(E_t, a.dv, at(a.dv, b, h), t0, all, a.Dv, tid);
+            __syncthreads();
+        }
+        x = next;
     }
-    __syncthreads();
-    if (!p.dq_heads) {
-        copy_out<DK>(q_t, a.dq, at(a.dq, b, h), t0, all, a.Dk, tid);
-        copy_out<DK>(k_t, a.dk, at(a.dk, b, h), t0, all, a.Dk, tid);
-    }
-    copy_out<DV>(E_t, a.dv, at(a.dv, b, h), t0, all, a.Dv, tid);
+    if (Tma && tid == 0) stores_read<0>();
     end(s, 512, p.flag, tid);
 }
 
@@ -800,10 +863,13 @@ int backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStre
     g.dstates = dstates;
     g.through = through;
     g.flag = flag;
+    g.items = c.chunks * a.B * a.H;
     if (Tma) {
         const long long rows = (long long)c.chunks * a.B * a.H * DK;
         if (!head_map(&g.q, a.q, a.T, a.B, a.Hk, a.Dk) || !head_map(&g.k, a.k, a.T, a.B, a.Hk, a.Dk) || !head_map(&g.v, a.v, a.T, a.B, a.H, a.Dv) ||
-            !head_map(&g.o, a.dout, a.T, a.B, a.H, a.Dv) || !state_map(&g.S, a.states, rows, DK, DV) || !state_map(&g.dS, dstates, rows, DK, DV))
+            !head_map(&g.o, a.dout, a.T, a.B, a.H, a.Dv) || !state_map(&g.S, a.states, rows, DK, DV) || !state_map(&g.dS, dstates, rows, DK, DV) ||
+            !head_map(&g.dv, a.dv, a.T, a.B, a.H, a.Dv) ||
+            (a.H == a.Hk && (!head_map(&g.dq, a.dq, a.T, a.B, a.H, a.Dk) || !head_map(&g.dk, a.dk, a.T, a.B, a.H, a.Dk))))
             return seq::fail(QGRU_ERR_CUDA, "cuTensorMapEncodeTiled");
     }
     if (a.H != a.Hk) {
@@ -812,7 +878,7 @@ int backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStre
     }
     int bytes = 0;
     if (const int rc = with_smem(k_gradients_tc<DK, DV, Tma>, GRADIENTS_TILES<DK, DV>, &bytes)) return rc;
-    k_gradients_tc<DK, DV, Tma><<<c.chunks * a.B * a.H, GRAD_THREADS, bytes, st>>>(a, g);
+    k_gradients_tc<DK, DV, Tma><<<std::min(g.items, sms), GRAD_THREADS, bytes, st>>>(a, g);
     SEQ_CK(cudaGetLastError());
     return g.dq_heads ? sum_groups(a, g.dq_heads, g.dk_heads, st) : QGRU_OK;
 }
@@ -848,7 +914,8 @@ int tc_forward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaSt
     return by_size(a, [&](auto dk, auto dv) -> int { return forward<dk.value, dv.value>(a, c, flag, st); });
 }
 int tc_backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStream_t st) {
-    const bool tma = fetchable(a.q, a.T, a.B, a.Hk, a.Dk) && fetchable(a.k, a.T, a.B, a.Hk, a.Dk) && fetchable(a.v, a.T, a.B, a.H, a.Dv) && fetchable(a.dout, a.T, a.B, a.H, a.Dv);
+    const bool tma = fetchable(a.q, a.T, a.B, a.Hk, a.Dk) && fetchable(a.k, a.T, a.B, a.Hk, a.Dk) && fetchable(a.v, a.T, a.B, a.H, a.Dv) && fetchable(a.dout, a.T, a.B, a.H, a.Dv) &&
+                     fetchable(a.dv, a.T, a.B, a.H, a.Dv) && (a.H != a.Hk || (fetchable(a.dq, a.T, a.B, a.H, a.Dk) && fetchable(a.dk, a.T, a.B, a.H, a.Dk)));
     return by_size(a, [&](auto dk, auto dv) -> int {
         return tma ? backward<dk.value, dv.value, true>(a, c, flag, sms, st) : backward<dk.value, dv.value, false>(a, c, flag, sms, st);
     });

@@ -209,6 +209,14 @@ __device__ __forceinline__ void tma_load_4d(uint32_t to, const CUtensorMap *map,
                  "l"(reinterpret_cast<uint64_t>(map)), "r"(tc::smem_u32(bar)), "r"(x), "r"(t), "r"(h), "r"(b)
                  : "memory");
 }
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap *map, uint32_t from, int x, int t, int h, int b) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(from),
+                 "r"(x), "r"(t), "r"(h), "r"(b)
+                 : "memory");
+}
+__device__ __forceinline__ void stores_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int Left>
+__device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(Left) : "memory"); }       // their tiles are free
 __device__ __forceinline__ void cp_async(uint32_t to, const void *from, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
