@@ -563,18 +563,30 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
         }
     };
     Item x = next_of(blockIdx.x);
+    // The decays of a chunk are the second four warps': read early, summed up while the first four sum up the last chunk's gradient.
+    const int token = tid - C;
+    const bool decays = tid >= C && tid < 2 * C;
     const auto decay_of = [&](const Item &x) {
-        return tid < x.tokens ? seq::load_f(a.decay.p, at(a.decay, x.b, x.h) + (long long)(x.t0 + tid) * a.decay.ts, a.decay_bf16) : 0.f;
+        return decays && token < x.tokens ? seq::load_f(a.decay.p, at(a.decay, x.b, x.h) + (long long)(x.t0 + token) * a.decay.ts, a.decay_bf16) : 0.f;
     };
-    float decay = decay_of(x);
+    const auto put_decays = [&](long long g) {
+        if (!decays) return;
+        for (int w = 0; w < token >> 5; ++w) g += s.g_sums[w];
+        s.G[token] = two_floats(g);
+    };
+    long long g = 0;
+    {
+        const float decay = decay_of(x);
+        if (decays) g = running_sum<C>(decay_units(decay), s.g_sums, token);
+    }
     begin(s, 512, tid);
     if constexpr (Tma) {
         if (tid == 0 && x.tokens) {
             fetch_qk(x);
             fetch_vo(x);
-            fetch_states(x);
         }
     }
+    put_decays(g);
     const uint32_t tm = s.tmem, base = lane_base(tm, warp);
     const Operand q{q_t, PANEL}, k{k_t, PANEL}, v{v_t, PANEL}, o{o_t, PANEL}, S{S_t, DK * 128}, dS{dS_t, DK * 128}, E{E_t, PANEL};
     for (uint32_t turn = 0; x.tokens; turn ^= 1) {
@@ -588,7 +600,6 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
             load_state<DK, DV, GRAD_THREADS>(dS_t, p.dstates + (long long)x.index * (DK * DV), tid);
             cp_commit();
         }
-        sum_decays(s, tid < C ? decay_units(decay) : 0, tid);
         if constexpr (Tma) {
             await(s, 4, turn);
             if (tokens < C) {               // what lies behind the sequence was fetched too
@@ -609,26 +620,31 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
             product<false, false, C, DV>(leader, tm + 128, v, o, false);
             commit(leader, &s.bar[0]);
         }
+        if constexpr (Tma) {
+            if (tid == 0) {
+                stores_read();             // the tiles of the states and of E were the last chunk's outputs
+                fetch_states(x);
+            }
+        }
         // from the start of t's block of 32 to t
         if (tid < C) s.f[tid] = tid < 32 ? ex2(s.G[tid].x + s.G[tid].y) : ex2_diff(s.G[tid], s.G[(tid & ~31) - 1]);
-        if constexpr (Tma) {
-            await(s, 5, turn);
-            if (tid == 0) stores_read<0>();               // E's tile was the last chunk's dv
-        }
+        const Item next = next_of((long long)x.index + gridDim.x);
+        const float decay = decay_of(next);
         __syncthreads();
-        if (tid < 32) {
+        if (warp == 3) {                      // (no pairs of its own)
             const uint32_t leader = elect();
+            if constexpr (Tma) await(s, 5, turn);
             tc::tc_fence_after_sync();
             product<false, false, DK, DV>(leader, tm + 256, v, dS, false);
             product<false, false, DK, DV>(leader, tm + 384, o, S, false);
             commit(leader, &s.bar[1]);
+            __syncwarp();
         }
         await(s, 0, turn);
-        await(s, 1, turn);
         const float2 G = s.G[row], last = s.G[C - 1];
         // the pairs: blocks of 32 x 32, t from s on
         uint32_t P[16];
-        float s_sum = 0.f;
+        float s_sum = 0.f, t_sum = 0.f;
         if (part < block) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) P[i] = 0u;
@@ -677,8 +693,10 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
                 sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + t0 / 8 + 1), e[4], e[5], e[6], e[7]);
             }
             s_sum = sum.x + sum.y;
-            t_sums[block * C + part * 32 + lane] = sum_columns(m, lane);
+            t_sum = sum_columns(m, lane);
         }
+        await(s, 1, turn);
+        if (part >= block) t_sums[block * C + part * 32 + lane] = t_sum;
         s_sums[part * C + row] = s_sum;
         const float to_end = ex2_diff(last, G), from_start = a.scale * ex2(G.x + G.y);
         k_dots[part * C + row] = scale_sums<KQ>(base + 256 + part * KQ, to_end, k_t, row, part * KQ, true);
@@ -710,6 +728,8 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
                 kd += (double)k_dots[w * C + tid];
             }
             d = running_sum<C>(kd - own, s.sums, tid) - (kd - own);
+        } else if (decays) {
+            g = running_sum<C>(decay_units(decay), s.g_sums, token);
         }
         double total = own;
         for (int i = 16; i; i >>= 1) total += __shfl_xor_sync(0xffffffffu, total, i);
@@ -726,6 +746,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
             product_ts<true, DV, C>(leader, tm + 128, tm, o, true);
             commit(leader, &s.bar[2]);
         }
+        put_decays(g);                        // (every thread has read the last chunk's)
         if (tid < all) {
             double sum = d;
             for (int w = 0; w < tid >> 5; ++w) sum += s.sums[w];
@@ -735,8 +756,6 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
             seq::store_f(a.ddecay.p, at(a.ddecay, b, h) + (long long)(t0 + tid) * a.ddecay.ts, a.decay_bf16, tid < tokens ? (float)sum : 0.f);
         }
         // The next chunk's tiles come as soon as nothing reads the ones that they replace.
-        const Item next = next_of((long long)x.index + gridDim.x);
-        decay = decay_of(next);
         const bool live = row < tokens;
         await(s, 3, turn);
         if constexpr (Tma) {
@@ -772,13 +791,8 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
                     tma_store_4d(&p.dq, dq_t + i * PANEL, i * 64, t0, h, b);
                     tma_store_4d(&p.dk, dk_t + i * PANEL, i * 64, t0, h, b);
                 }
-                stores_commit();
                 for (int i = 0; i < DV / 64; ++i) tma_store_4d(&p.dv, E_t + i * PANEL, i * 64, t0, h, b);
                 stores_commit();
-                if (next.tokens) {
-                    if (DV == 128) stores_read<1>();      // dq's and dk's tiles are the states'
-                    fetch_states(next);
-                }
             }
         } else {
             if (!p.dq_heads) {
@@ -790,7 +804,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
         }
         x = next;
     }
-    if (Tma && tid == 0) stores_read<0>();
+    if (Tma && tid == 0) stores_read();
     end(s, 512, p.flag, tid);
 }
 

@@ -215,8 +215,7 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap *map, uint32_t fr
                  : "memory");
 }
 __device__ __forceinline__ void stores_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-template <int Left>
-__device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(Left) : "memory"); }       // their tiles are free
+__device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }       // their tiles are free
 __device__ __forceinline__ void cp_async(uint32_t to, const void *from, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
