@@ -484,9 +484,11 @@ __device__ __forceinline__ void copy_out(uint32_t tile, const qgru_seq_tensor &x
 //   0  (k q^T), then P^T in bf16     1  (v dout^T), then dv     2  dk     3  dq
 // Four threads a row, a quarter of the columns each.  P^T is the operand of dv from tensor memory, E^T that of dk (K in its columns) and
 // of dq (K in its rows) from shared memory.
-// One CTA an SM, whose products, loads and conversions between tensor memory and operands follow one another: that chain bounds it.  16 x
-// 1000 tokens of 8 heads of 128: 105 us with 512 threads and tiles by TMA, 108 where the threads load them, 155 with 256 threads; bytes alone
-// would take 43 (285 MB).  A second CTA an SM has no room: 224 KB of operands.
+// The next chunk's tiles are fetched while this one's results leave (both by TMA), its decays are summed up beside this one's gradient
+// of them, and the products of the states run beside the pairs.  What bounds it is the chain of products, pairs and conversions between
+// tensor memory and operands, and what of the loads it does not cover: 224 KB of operands leave no room for a second CTA or for tiles
+// fetched earlier.  16 x 1000 tokens of 8 heads of 128: 90 us; 105 with a CTA a chunk and its tiles by TMA, 108 where the threads load
+// them, 155 with 256 threads.  Bytes alone would take 43 (285 MB).  Heads of 64: 62 us.
 template <int DK, int DV, bool Tma>
 __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_constant__ qgru_attention a, const __grid_constant__ Gradients p) {
     extern __shared__ unsigned char raw[];
