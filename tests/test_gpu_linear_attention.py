@@ -512,3 +512,23 @@ def test_a_state_that_must_not_be_written_is_left_alone(cuda_device):
 def test_layer_sizes(sizes):
     with pytest.raises(ValueError):
         la.LinearAttention(*sizes)
+
+
+@pytest.mark.parametrize("case", [
+    dict(H=8, Dk=64, Dv=64), dict(H=8, Dk=128, Dv=64, Hk=4), dict(H=8, Dk=64, Dv=128), dict(H=8, Dk=128, Dv=128, batch_first=True, fused=True),
+    dict(H=8, Dk=60, Dv=60), dict(H=8, Dk=100, Dv=128, Hk=2),
+], ids=lambda c: "-".join(f"{k}{v}" for k, v in c.items()))
+def test_more_chunks_than_multiprocessors(case, cuda_device):
+    T, B = 200, 45                     # 720 chunks, of which some are whole, some short, some behind the end of their sequence
+    lengths = [(0, 1, 127, 128, 129, 200, 63, 128, 200)[b % 9] for b in range(B)]
+    q, k, v, g, state, n = make(cuda_device, T, B, dtype=BF, decay=BF, lengths=lengths, **case)
+    bf = case.get("batch_first", False)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, g, state)]
+    out, last = la.linear_attention(*leaves, lengths=n, batch_first=bf)
+    dout, dstate = torch.randn_like(out), torch.randn_like(last)
+    grads = torch.autograd.grad((out, last), leaves, (dout, dstate), retain_graph=True)
+    want, bound = want_of(q, k, v, g, state, n, bf, dout=dout, dstate=dstate)
+    hold({"out": out, "state": last, **dict(zip(("dq", "dk", "dv", "dg", "dstate0"), grads))}, want, bound)
+    for _ in range(20):
+        again = torch.autograd.grad((out, last), leaves, (dout, dstate), retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(grads, again))
