@@ -236,7 +236,9 @@ struct Roles {
         };
         each([&](const Item<Reverse> &w, int chunk, int i) {
             const At<L::NS> st(i);
-            if (!wait(s, s.k_empty[st.buf], st.free)) return false;
+            // (k is there after the v that was in this stage before it: K waits for v of short chunks alone, and a phase of v_full that is
+            // two ahead of the barrier's would look like one that is over)
+            if (!wait(s, s.k_empty[st.buf], st.free) || !wait(s, s.v_full[st.buf], st.free)) return false;
             load(k_tile(st.buf), &p.k, &s.k_full[st.buf], DK / 64, chunk * C, w.h / p.share, w.b);
             if constexpr (Outputs) {
                 if (!wait(s, s.q_empty[st.buf], st.free)) return false;

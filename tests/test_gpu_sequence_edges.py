@@ -1,0 +1,35 @@
+"""Sequence operators where a value that does not count, an order of arrival or a caller's mode could reach a result."""
+import importlib
+
+import pytest
+import torch
+
+from __graft_entry__ import PKG_NAME
+from tests import seq_reference as ref
+from tests.test_gpu_linear_attention import hold, make, want_of
+
+la = importlib.import_module(PKG_NAME + ".linear_attention")
+norm = importlib.import_module(PKG_NAME + ".norm")
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.mark.parametrize("Dk,Dv", [(128, 64), (96, 40), (128, 128), (64, 64)])
+def test_short_chunks_behind_whole_ones(Dk, Dv, cuda_device):
+    """Many chunks a CTA whose keys come out of L2 (shared by all heads) and whose values do not: whatever arrives first, the rows behind
+    a sequence are cleared in the chunk that they belong to."""
+    T, B, H = 500, 90, 8
+    lengths = [(1, 129, 500, 0, 257, 385, 500, 130)[b % 8] for b in range(B)]
+    q, k, v, g, state, n = make(cuda_device, T, B, H, Dk, Dv, BF, Hk=1, lengths=lengths, decay=BF)
+    past = torch.arange(T, device=cuda_device)[:, None] >= n[None, :]
+    want = la.linear_attention(*[torch.where(past[(...,) + (None,) * (t.dim() - 2)], 0.0, t) for t in (q, k, v, g)], state, n)
+    for t in (q, k, g):
+        t[past] = float("nan")
+    v[past] = float("inf")
+    for _ in range(20):
+        got = la.linear_attention(q, k, v, g, state, n)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    part = slice(0, 8)
+    clean = [torch.where(past[:, part][(...,) + (None,) * (t.dim() - 2)], 0.0, t[:, part]) for t in (q, k, v, g)]
+    exact, bound = want_of(*clean, state[part], n[part])
+    hold({"out": want[0][:, part], "state": want[1][part]}, exact, bound)
