@@ -153,6 +153,13 @@ struct Four {
 #pragma unroll
         for (int i = 0; i < 4; ++i) *reinterpret_cast<float4 *>(to + idx((tid >> 4) + 16 * i, (tid & 15) * 4)) = v[i];
     }
+    // whether one of them is infinite or NaN
+    __device__ __forceinline__ bool odd() const {
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x = fmaf(v[i].x, 0.f, fmaf(v[i].y, 0.f, fmaf(v[i].z, 0.f, fmaf(v[i].w, 0.f, x))));
+        return !(x == 0.f);
+    }
 };
 template <class T>
 __device__ __forceinline__ void load_tile(float *to, const qgru_seq_tensor &x, long long base, int t0, int tokens, int d0, int d, int tid) {
@@ -337,11 +344,12 @@ __global__ void __launch_bounds__(THREADS) k_outputs(const __grid_constant__ qgr
             __syncthreads();
         }
         each(c, tid, [&](int t, int, float &x) { x *= a.scale * exp2_of(G[t]); });
-        load_tile<T>(Y, a.v, vb, t0, tokens, j, a.Dv, tid);
-        // A later token's infinity or NaN is none of an earlier one's business, and zero times it is NaN.
-        int odd = 0;
-        for (int e = tid; e < TILE; e += THREADS) odd |= !isfinite(Y[e]);
-        if (__syncthreads_or(odd)) {
+        Four v4;
+        v4.load<T>(a.v, vb, t0, tokens, j, a.Dv, tid);
+        v4.store(Y, tid);
+        // A later token's infinity or NaN is none of an earlier one's business, and zero times it is NaN.  (Each thread looks at what it
+        // has loaded itself: the tile is not whole before the barrier.)
+        if (__syncthreads_or(v4.odd())) {
             each(c, tid, [&](int t, int n, float &x) {
                 for (int s = 0; s <= t; ++s) x = fmaf(P[idx(t, s)], Y[idx(s, n)], x);
             });

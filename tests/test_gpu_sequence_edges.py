@@ -33,3 +33,20 @@ def test_short_chunks_behind_whole_ones(Dk, Dv, cuda_device):
     clean = [torch.where(past[:, part][(...,) + (None,) * (t.dim() - 2)], 0.0, t[:, part]) for t in (q, k, v, g)]
     exact, bound = want_of(*clean, state[part], n[part])
     hold({"out": want[0][:, part], "state": want[1][part]}, exact, bound)
+
+
+@pytest.mark.parametrize("dtype,Dk,Dv", [(F32, 128, 128), (BF, 200, 256), (F32, 72, 40), (F32, 64, 64), (BF, 128, 128), (BF, 60, 60)], ids=str)
+def test_one_infinite_value_at_each_token_of_a_chunk(dtype, Dk, Dv, cuda_device):
+    """Sequence b has a single infinity, at token b of its last chunk: no earlier output knows of it."""
+    C = 128 if dtype == BF and Dk <= 128 else 64
+    T = 2 * C
+    q, k, v, g, state, _ = make(cuda_device, T, C, 1, Dk, Dv, dtype, seed=5)
+    want, bound = want_of(q, k, v, g, state, None)
+    at = torch.arange(C, device=cuda_device)
+    v[C + at, at, 0, (7 * at) % Dv] = float("inf")
+    before = torch.arange(T, device=cuda_device)[:, None] < C + at[None, :]
+    for _ in range(20):
+        out = la.linear_attention(q, k, v, g, state)[0]
+        assert torch.isfinite(out[before]).all()
+        hold({"out": out[before]}, {"out": want["out"][before]}, {"out": bound["out"][before]})
+        assert not torch.isfinite(out[C + at, at, 0, (7 * at) % Dv]).any()
