@@ -5,12 +5,12 @@
 // different chunks at the same time and hand them on through barriers in shared memory:
 //   K  takes k times the decays to the chunk's end apart into three bf16 parts (24 bits), 64 tokens at a time
 //   S  keeps the state in fp32 registers: S' = 2^G_C S + (w k)^T v, and puts it, as two bf16 parts (16 bits), beside q
-//   P  weighs the pairs of tokens: q k^T out of tensor memory, times 2^(G_t - G_s), into it again as bf16, the operand of P v
+//   P  weighs the pairs of tokens: q k^T out of tensor memory, times 2^(G_t - G_s), into it again as two bf16 parts, the operand of P v
 //   O  out = 2^G_t q S + P v: out of tensor memory, into the output
 //   X  a warp issues the products, one fetches tiles by TMA, two sum the decays up
 // In the order of the products the chunk's part of the state comes first, since the next chunk's outputs wait for it.
 //
-// What is rounded to bf16 on the way: P alone, once, as the output is in the end; the state counts with 16 bits where it is a factor.
+// What is rounded on the way: P, and the state where it is a factor, to 16 bits (two bf16 parts each); the output once, to bf16, in the end.
 //
 // What bounds it: the roles' instructions, not the bytes.  64 x 1000 tokens of 16 heads of 64, 524 MB: 172 to 180 us, 3 TB/s (2.9 us a
 // chunk and SM, the tensor pipe busy for 18 % of it).  The roles share one instruction cache, so their loops stay rolled: unrolled, with
@@ -334,7 +334,7 @@ struct Roles {
                         float2 x = __fmul2_rn(unpack(in[q]), both(f));
 #pragma unroll
                         for (int t = 0; t < 3; ++t) {
-                            o[t][q] = pack(x);
+                            o[t][q] = t < 2 ? pack_part(x) : pack(x);
                             if (t < 2) x = rest(x, o[t][q]);
                         }
                     }
@@ -456,17 +456,17 @@ struct Roles {
 #pragma unroll 1
             for (int s0 = 0; s0 < C; s0 += 16) {
                 const int sb = s0 >> 5;
-                uint32_t P[8];
+                uint32_t P[16];
                 if (sb > warp) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) P[j] = 0u;
+                    for (int j = 0; j < 16; ++j) P[j] = 0u;
                 } else {
                     float2 x[8];
                     tmem_load(from + s0, x);
                     if (sb < warp) {
                         const float2 r = both(a.scale * ex2_diff(G, g.G(s0 | 31)));
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) P[j] = pack(__fmul2_rn(x[j], __fmul2_rn(r, *reinterpret_cast<const float2 *>(&g.to_block[s0 + 2 * j]))));
+                        for (int j = 0; j < 8; ++j) x[j] = __fmul2_rn(x[j], __fmul2_rn(r, *reinterpret_cast<const float2 *>(&g.to_block[s0 + 2 * j])));
                     } else {
                         const int last = lane - (s0 & 31);
                         const float2 minus = both(-1.f);
@@ -475,11 +475,16 @@ struct Roles {
                             const float2 d = __fadd2_rn(__ffma2_rn(*reinterpret_cast<const float2 *>(&g.hi[s0 + 2 * j]), minus, both(G.x)),
                                                         __ffma2_rn(*reinterpret_cast<const float2 *>(&g.lo[s0 + 2 * j]), minus, both(G.y)));
                             const float2 v = __fmul2_rn(x[j], __fmul2_rn(both(a.scale), make_float2(ex2(d.x), ex2(d.y))));
-                            P[j] = pack(2 * j <= last ? v.x : 0.f, 2 * j + 1 <= last ? v.y : 0.f);
+                            x[j] = make_float2(2 * j <= last ? v.x : 0.f, 2 * j + 1 <= last ? v.y : 0.f);
                         }
                     }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        P[j] = pack_part(x[j]);
+                        P[8 + j] = pack(rest(x[j], P[j]));
+                    }
                 }
-                tmem_st8(from + s0 / 2, P);       // columns that this warp has read already
+                tmem_st16(from + s0, P);
             }
             tc::tmem_st_wait();
             tc::tc_fence_before_sync();

@@ -305,42 +305,48 @@ __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant
         cp_commit();
     }
     const float2 G = s.G[row];
-    uint32_t P[32];
-    {
-        float x[64];
-        tmem_load(base + half * 64, x);
 #pragma unroll
-        for (int jb = 0; jb < 2; ++jb) {
-            const int sb = half * 2 + jb;               // block of s
+    for (int jb = 0; jb < 2; ++jb) {
+        const int sb = half * 2 + jb;                   // block of s
+        uint32_t P[32];                                 // of each sixteen columns the large parts, then the small ones, in their place
+        if (sb > block) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) P[i] = 0u;
+        } else {
+            float x[32];
+            tmem_load(base + sb * 32, x);
             if (sb < block) {
                 const float r = a.scale * ex2_diff(G, s.G[sb * 32 + 31]);
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) P[jb * 16 + i / 2] = pack(x[jb * 32 + i] * (r * s.f[sb * 32 + i]), x[jb * 32 + i + 1] * (r * s.f[sb * 32 + i + 1]));
-            } else if (sb == block) {
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float w0 = a.scale * ex2_diff(G, s.G[sb * 32 + i]), w1 = a.scale * ex2_diff(G, s.G[sb * 32 + i + 1]);
-                    P[jb * 16 + i / 2] = pack(i <= lane ? x[jb * 32 + i] * w0 : 0.f, i + 1 <= lane ? x[jb * 32 + i + 1] * w1 : 0.f);
-                }
+                for (int i = 0; i < 32; ++i) x[i] *= r * s.f[sb * 32 + i];
             } else {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) P[jb * 16 + i] = 0u;
+                for (int i = 0; i < 32; ++i) {
+                    const float w = a.scale * ex2_diff(G, s.G[sb * 32 + i]);
+                    x[i] = i <= lane ? x[i] * w : 0.f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+                const int at = (i & 16) + (i & 15) / 2;
+                const float2 v = make_float2(x[i], x[i + 1]);
+                P[at] = pack_part(v);
+                P[at + 8] = pack(rest(v, P[at]));
             }
         }
+        tmem_store(base + sb * 32, P);
     }
+    tc::tmem_st_wait();
     cp_wait<0>();
     fence_async();
     tc::tc_fence_before_sync();
-    __syncthreads();                                    // every sum of q k^T has been read, the state is there
+    __syncthreads();                                    // the pairs' weights and the state are there
     if (carried && tid < 32) {
         const uint32_t leader = elect();
         tc::tc_fence_after_sync();
         product<false, true, DV, DK>(leader, s.tmem + 128, Operand{q_t, PANEL}, Operand{k_t, DK * 128}, false);
         commit(leader, &s.bar[1]);
     }
-    tc::tc_fence_after_sync();
-    tmem_store(base + half * 32, P);
-    tc::tmem_st_wait();
     if (carried) {
         await(s, 1, 0);
         tmem_load(base + 128 + c0, o);
@@ -481,7 +487,7 @@ __device__ __forceinline__ void copy_out(uint32_t tile, const qgru_seq_tensor &x
 }
 
 // A CTA an SM, which takes chunk after chunk of all heads.  Pairs lie as [s][t] here, lane s of tensor memory.  Four blocks of 128 columns of it:
-//   0  (k q^T), then P^T in bf16     1  (v dout^T), then dv     2  dk     3  dq
+//   0  (k q^T), then P^T in two bf16 parts     1  (v dout^T), then dv     2  dk     3  dq
 // Four threads a row, a quarter of the columns each.  P^T is the operand of dv from tensor memory, E^T that of dk (K in its columns) and
 // of dq (K in its rows) from shared memory.
 // The next chunk's tiles are fetched while this one's results leave (both by TMA), its decays are summed up beside this one's gradient
@@ -645,11 +651,10 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
         await(s, 0, turn);
         const float2 G = s.G[row], last = s.G[C - 1];
         // the pairs: blocks of 32 x 32, t from s on
-        uint32_t P[16];
         float s_sum = 0.f, t_sum = 0.f;
         if (part < block) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) P[i] = 0u;
+            const uint32_t zeros[32] = {};
+            tmem_store(base + part * 32, zeros);
 #pragma unroll
             for (int i = 0; i < 4; ++i) sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + i), 0u, 0u, 0u, 0u);
         } else {
@@ -663,7 +668,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
                 tc::tmem_ld16(base + part * 32 + t0, u[0]);
                 tc::tmem_ld16(base + 128 + part * 32 + t0, u[1]);
                 tc::tmem_ld_wait();
-                uint32_t e[8];
+                uint32_t e[8], P[16];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     x[i] = make_float2(__int_as_float(u[0][2 * i]), __int_as_float(u[0][2 * i + 1]));
@@ -688,9 +693,11 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
                     sum = __fadd2_rn(sum, mv);
                     m[t] = mv.x;
                     m[t + 1] = mv.y;
-                    P[t / 2] = pack(pv);
+                    P[i] = pack_part(pv);
+                    P[8 + i] = pack(rest(pv, P[i]));
                     e[i] = pack(__fmul2_rn(w, y[i]));
                 }
+                tmem_st16(base + part * 32 + t0, P);          // (in the place of k q^T, which no other warp reads)
                 sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + t0 / 8), e[0], e[1], e[2], e[3]);
                 sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + t0 / 8 + 1), e[4], e[5], e[6], e[7]);
             }
@@ -716,8 +723,6 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
             product<true, true, DK, C>(leader, tm + 384, E, k, true);
             commit(leader, &s.bar[3]);
         }
-        tc::tc_fence_after_sync();
-        tmem_store(base + part * 16, P);
         // the decays' gradient: from each token on, every pair across it, and what passes from the state before the chunk to that behind it
         double d = 0.0, own = 0.0;
         if (tid < C) {
@@ -736,7 +741,6 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
         double total = own;
         for (int i = 16; i; i >>= 1) total += __shfl_xor_sync(0xffffffffu, total, i);
         if (lane == 0 && tid < C) totals[warp] = total;
-        tc::tmem_st_wait();
         await(s, 2, 0);
         scale_sums<VQ>(base + 128 + part * VQ, to_end, 0, 0, 0, false);
         tc::tmem_st_wait();

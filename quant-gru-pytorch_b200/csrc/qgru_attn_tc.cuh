@@ -121,14 +121,19 @@ __device__ __forceinline__ void product(uint32_t leader, uint32_t d, const Opera
         more = 1;
     }
 }
+// A as two parts: of each sixteen columns the first eight hold sixteen K of the large part, the others those of the small one, where their
+// sixteen fp32 values were before.
 template <bool BRows, int N, int K>
 __device__ __forceinline__ void product_ts(uint32_t leader, uint32_t d, uint32_t a, const Operand &b, bool add) {
     uint32_t b0 = desc_lo<BRows>(b), more = add;
 #pragma unroll 1
     for (int p = 0; p < K / 64; ++p) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mma_ts(leader, d, a + j * 8, b0 + desc_step<BRows>(b, j), idesc(N, false, BRows), j ? 1u : more);
-        a += 32;
+        for (int j = 0; j < 4; ++j) {
+            mma_ts(leader, d, a + j * 16 + 8, b0 + desc_step<BRows>(b, j), idesc(N, false, BRows), j ? 1u : more);
+            mma_ts(leader, d, a + j * 16, b0 + desc_step<BRows>(b, j), idesc(N, false, BRows), 1u);
+        }
+        a += 64;
         b0 += desc_step<BRows>(b, 4);
         more = 1;
     }
@@ -139,11 +144,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
                  "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
                  "r"(v[14]), "r"(v[15])
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
-                 "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
 // Cols / 16 groups of sixteen columns
@@ -183,6 +183,12 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 __device__ __forceinline__ float low(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float high(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 __device__ __forceinline__ uint32_t pack(float2 x) { return pack(x.x, x.y); }
+// The first of several parts: the largest finite value for an infinity, so that what is left of it is the infinity and not NaN
+__device__ __forceinline__ uint32_t pack_part(float2 x) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(x.y), "f"(x.x));
+    return r;
+}
 __device__ __forceinline__ float2 unpack(uint32_t x) { return make_float2(low(x), high(x)); }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 // Eight values, packed, times eight of a state's
@@ -192,7 +198,7 @@ __device__ __forceinline__ float2 dot8(const uint4 &u, const float2 *s, float2 s
     sum = __ffma2_rn(unpack(u.z), s[2], sum);
     return __ffma2_rn(unpack(u.w), s[3], sum);
 }
-// x minus what its rounding to bf16 keeps (exact)
+// x minus what its first part keeps (exact)
 __device__ __forceinline__ float2 rest(float2 x, uint32_t packed) { return __ffma2_rn(unpack(packed), make_float2(-1.f, -1.f), x); }
 __device__ __forceinline__ float ex2(float x) {
     float r;
