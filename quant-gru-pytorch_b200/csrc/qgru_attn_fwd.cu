@@ -80,7 +80,7 @@ struct Args {
     CUtensorMap q, k, v;                    // [B][heads][T][D]
     const float *first;                     // the state it starts from, or null
     float *last;                            // where the last one goes, or null
-    bf16 *states;                           // before each chunk in the pass's order, [chunks][B H][DK][DV], or null
+    bf16 *states;                           // before each chunk in the pass's order, [chunks][B H][2 parts][DV / 8][DK][8], or null
     const bf16 *other;                      // from the end: the forward's states, and where their products with these go
     float *through;
     float *seg_state, *seg_log;
@@ -372,13 +372,16 @@ struct Roles {
             double all = 0.0;
             for (int c = w.begin; c < w.stop; ++c, ++i) {
                 const At<SLOTS> at(i);
-                uint4 *keep = p.states && !p.own_sums ? reinterpret_cast<uint4 *>(p.states + ((long long)Item<Reverse>::chunk(p, c) * a.B * a.H + w.bh) * (DK * DV) + row * DV + c0) : nullptr;
+                uint4 *keep = p.states && !p.own_sums ? reinterpret_cast<uint4 *>(p.states + ((long long)Item<Reverse>::chunk(p, c) * a.B * a.H + w.bh) * (2 * DK * DV) + (c0 * DK + row * 8)) : nullptr;
                 if (Reverse && !p.own_sums) {
                     const long long head = (long long)Item<Reverse>::chunk(p, c) * a.B * a.H + w.bh;
-                    const uint4 *o = reinterpret_cast<const uint4 *>(p.other + head * (DK * DV) + row * DV + c0);
+                    const uint4 *o = reinterpret_cast<const uint4 *>(p.other + head * (2 * DK * DV) + (c0 * DK + row * 8));
                     float2 x = both(0.f);
 #pragma unroll
-                    for (int j = 0; j < N; j += 8) x = dot8(o[j / 8], &S[j / 2], x);
+                    for (int j = 0; j < N; j += 8) {
+                        x = dot8(o[DK * DV / 8 + j / 8 * DK], &S[j / 2], x);
+                        x = dot8(o[j / 8 * DK], &S[j / 2], x);
+                    }
                     float sum = x.x + x.y;
                     for (int e = 16; e; e >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, e);
                     if ((tid & 31) == 0) {
@@ -390,13 +393,17 @@ struct Roles {
                     if (i && !wait_warp(s, s.q_empty[At<L::NS>(i - 1).buf], At<L::NS>(i - 1).full)) return;      // q S of the chunk before is done
 #pragma unroll
                 for (int j = 0; j < N; j += 8) {
+                    if (!Outputs && !keep) break;
                     uint32_t hi[4], lo[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        hi[e] = pack(S[j / 2 + e]);
-                        if (Outputs) lo[e] = pack(rest(S[j / 2 + e], hi[e]));
+                        hi[e] = pack_part(S[j / 2 + e]);
+                        lo[e] = pack(rest(S[j / 2 + e], hi[e]));
                     }
-                    if (keep) keep[j / 8] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if (keep) {
+                        keep[j / 8 * DK] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        keep[DK * DV / 8 + j / 8 * DK] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
                     if constexpr (Outputs) {
                         const uint32_t off = (uint32_t)((c0 + j) >> 6) * (DK * 128) + chunk_at(row, ((c0 + j) >> 3) & 7);
                         sts16(state(0) + off, hi[0], hi[1], hi[2], hi[3]);
@@ -704,14 +711,6 @@ bool head_map(CUtensorMap *map, const qgru_seq_tensor &x, int T, int B, int head
                CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool state_map(CUtensorMap *map, const void *states, long long rows, int DK, int DV) {
-    const EncodeTiledFn enc = get_encode_tiled();
-    if (!enc) return false;
-    const cuuint64_t dims[2] = {(cuuint64_t)DV, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)DV * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)DK}, step[2] = {1, 1};
-    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(states), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
 bool fetchable(const qgru_seq_tensor &x, int T, int B, int heads, int d) {
     const auto ok = [](long long s, int n) { return n <= 1 || (s > 0 && s % 8 == 0 && s < (1ll << 38)); };       // (a stride of 0 is not for TMA)
     return reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && d % 8 == 0 && ok(x.ts, T) && ok(x.bs, B) && ok(x.hs, heads);

@@ -1,10 +1,9 @@
 // qgru_attn_tc.cu - linear attention on the tensor cores: the gradients, and the state pass and outputs of tensors that TMA does not take
 // (rows or strides that are no multiple of 16 bytes, strides of 0).  bf16, head sizes up to 128 (padded to 64 or 128), chunks of 128 tokens.
 //
-// Outputs and gradients take every chunk by itself, from the states that a pass over the chunks has left.  Rounded to bf16 on the way
-// are the weights of the pairs of tokens (P, E), and the state before a chunk and its gradient behind it where they are factors of a
-// product.  Each is one rounding of a factor, the size of the one that the results get in the end.  The states themselves are fp32:
-// their products take k scaled by the decays as three bf16 parts (24 bits).
+// Outputs and gradients take every chunk by itself, from the states that a pass over the chunks has left.  Rounded to 16 bits (two
+// bf16 parts, 2^-16 of the value) on the way are the weights of the pairs of tokens (P, E), and the state before a chunk and its gradient
+// behind it where they are factors of a product.  The states themselves are fp32: their products take k scaled by the decays as three bf16 parts (24 bits).
 #include <algorithm>
 #include <type_traits>
 
@@ -38,14 +37,11 @@ __device__ __forceinline__ void load_rows(uint32_t tile, const qgru_seq_tensor &
         sts16(tile + (c >> 3) * PANEL + chunk_at(r, c & 7), w[0], w[1], w[2], w[3]);
     }
 }
-// A state [DK][DV] as it is kept before each chunk (bf16, padded) as a tile.
-template <int DK, int DV, int N = THREADS>
-__device__ __forceinline__ void load_state(uint32_t tile, const bf16 *S, int tid) {
+// `Bytes` of a state as it is kept before each chunk.
+template <int Bytes, int N = THREADS>
+__device__ __forceinline__ void load_state(uint32_t to, const bf16 *S, int tid) {
 #pragma unroll
-    for (int i = 0; i < DK * DV / 8 / N; ++i) {
-        const int e = i * N + tid, r = e / (DV / 8), c = e % (DV / 8);
-        cp_async(tile + (c >> 3) * (DK * 128) + chunk_at(r, c & 7), S + e * 8, 16);
-    }
+    for (int i = 0; i < Bytes / 16 / N; ++i) cp_async(to + (i * N + tid) * 16, S + (i * N + tid) * 8, 16);
 }
 struct Shared {                 // behind the tiles
     float2 G[C];                // running sums of the decays, base 2
@@ -107,7 +103,7 @@ struct Pass {
     int k_share;
     const float *first;
     float *last;
-    bf16 *states;                  // before each chunk in the pass's order, [chunks][B H][DK][DV]
+    bf16 *states;                  // before each chunk in the pass's order, [chunks][B H][2 parts][DV / 8][DK][8]
     bool own_sums;                 // instead: each segment's sum, from zero
     const bf16 *other;             // from the end: the forward's states, and where their products with these go
     float *through;
@@ -146,9 +142,19 @@ __global__ void __launch_bounds__(THREADS) k_states_tc(const __grid_constant__ q
     const auto chunk_of = [&](int i) { return Reverse ? p.chunks - 1 - i : i; };
     const auto leave = [&](int chunk) {            // the state before the chunk
         if (own_sums || !mine) return;
-        uint4 *to = reinterpret_cast<uint4 *>(p.states + ((long long)chunk * gridDim.x + bh) * (DK * DV) + row * DV + c0);
+        uint4 *to = reinterpret_cast<uint4 *>(p.states + ((long long)chunk * gridDim.x + bh) * (2 * DK * DV) + (c0 * DK + row * 8));
 #pragma unroll
-        for (int i = 0; i < HALF; i += 8) to[i / 8] = make_uint4(pack(S[i], S[i + 1]), pack(S[i + 2], S[i + 3]), pack(S[i + 4], S[i + 5]), pack(S[i + 6], S[i + 7]));
+        for (int i = 0; i < HALF; i += 8) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 x = make_float2(S[i + 2 * j], S[i + 2 * j + 1]);
+                hi[j] = pack_part(x);
+                lo[j] = pack(rest(x, hi[j]));
+            }
+            to[i / 8 * DK] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            to[DK * DV / 8 + i / 8 * DK] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
     };
     const auto fetch = [&](int i) {
         const int t0 = chunk_of(i) * C, tokens = min(max(n - t0, 0), C);
@@ -183,12 +189,11 @@ __global__ void __launch_bounds__(THREADS) k_states_tc(const __grid_constant__ q
             uint32_t o[3][4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                float x0 = low(in[j]) * w, x1 = high(in[j]) * w;
+                float2 x = make_float2(low(in[j]) * w, high(in[j]) * w);
 #pragma unroll
                 for (int t = 0; t < 3; ++t) {
-                    o[t][j] = pack(x0, x1);
-                    x0 -= low(o[t][j]);
-                    x1 -= high(o[t][j]);
+                    o[t][j] = t < 2 ? pack_part(x) : pack(x);
+                    if (t < 2) x = rest(x, o[t][j]);
                 }
             }
 #pragma unroll
@@ -216,12 +221,13 @@ __global__ void __launch_bounds__(THREADS) k_states_tc(const __grid_constant__ q
             const long long head = (long long)chunk * gridDim.x + bh;
             float sum = 0.f;
             if (mine) {
-                const uint4 *o = reinterpret_cast<const uint4 *>(p.other + head * (DK * DV) + row * DV + c0);
+                const uint4 *o = reinterpret_cast<const uint4 *>(p.other + head * (2 * DK * DV) + (c0 * DK + row * 8));
                 float2 x = both(0.f);
 #pragma unroll
                 for (int i = 0; i < HALF; i += 8) {
                     const float2 u[4] = {make_float2(S[i], S[i + 1]), make_float2(S[i + 2], S[i + 3]), make_float2(S[i + 4], S[i + 5]), make_float2(S[i + 6], S[i + 7])};
-                    x = dot8(o[i / 8], u, x);
+                    x = dot8(o[DK * DV / 8 + i / 8 * DK], u, x);
+                    x = dot8(o[i / 8 * DK], u, x);
                 }
                 sum = x.x + x.y;
             }
@@ -280,7 +286,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant
     }
     const int hk = h / (a.H / a.Hk);
     const bool carried = chunk > 0 || a.state0;
-    const bf16 *S = states + ((long long)chunk * heads + bh) * (DK * DV);
+    const bf16 *S = states + ((long long)chunk * heads + bh) * (2 * DK * DV);
     load_rows<DK>(q_t, a.q, at(a.q, b, hk), t0, tokens, a.Dk, tid);
     load_rows<DK>(k_t, a.k, at(a.k, b, hk), t0, tokens, a.Dk, tid);
     load_rows<DV>(v_t, a.v, at(a.v, b, h), t0, tokens, a.Dv, tid);
@@ -301,7 +307,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant
     await(s, 0, 0);
     __syncthreads();
     if (carried) {
-        load_state<DK, DV>(k_t, S, tid);
+        load_state<DK * DV * 2>(k_t, S, tid);
         cp_commit();
     }
     const float2 G = s.G[row];
@@ -344,11 +350,24 @@ __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant
     if (carried && tid < 32) {
         const uint32_t leader = elect();
         tc::tc_fence_after_sync();
-        product<false, true, DV, DK>(leader, s.tmem + 128, Operand{q_t, PANEL}, Operand{k_t, DK * 128}, false);
+        product_state<true, DV, DK, DK>(leader, s.tmem + 128, Operand{q_t, PANEL}, k_t, false);
         commit(leader, &s.bar[1]);
     }
     if (carried) {
         await(s, 1, 0);
+        load_state<DK * DV * 2>(k_t, S + DK * DV, tid);      // its small part, where the large one was (no room for both beside a second CTA)
+        cp_commit();
+        cp_wait<0>();
+        fence_async();
+        tc::tc_fence_before_sync();
+        __syncthreads();
+        if (tid < 32) {
+            const uint32_t leader = elect();
+            tc::tc_fence_after_sync();
+            product_state<true, DV, DK, DK>(leader, s.tmem + 128, Operand{q_t, PANEL}, k_t, true);
+            commit(leader, &s.bar[3]);
+        }
+        await(s, 3, 0);
         tmem_load(base + 128 + c0, o);
         const float r = a.scale * ex2(G.x + G.y);
 #pragma unroll
@@ -400,15 +419,24 @@ struct Item {
     int index, b, h, t0, all, tokens;
 };
 struct Gradients {
-    CUtensorMap q, k, v, o, S, dS, dq, dk, dv;   // where TMA takes the tensors
+    CUtensorMap q, k, v, o, dq, dk, dv;  // where TMA takes the tensors
     const bf16 *states, *dstates;
     const float *through;                // products of the two, THROUGH parts each
     float *dq_heads, *dk_heads;          // [T][B][H][Dk] where heads share q and k, else null
     int items;                           // chunks of all heads
     int *flag;
 };
+// Shared memory: q, k, v, dout; the two parts of a state (X, Y: first that of the gradient behind the chunk, then the one before it); the
+// large part of E and the small one, which takes the place of X where a state is as large as it.
 template <int DK, int DV>
-constexpr int GRADIENTS_TILES = 2 * (DK / 64) * PANEL + 2 * (DV / 64) * PANEL + 2 * DK * DV * 2 + 2 * PANEL + (DV == 64 ? 2 * (DK / 64) * PANEL : 0);
+struct Tiles {
+    static constexpr int KT = DK / 64 * PANEL, VT = DV / 64 * PANEL, ST = DK * DV * 2, ET = 2 * PANEL;
+    static constexpr bool SHARED = ST >= ET;
+    static constexpr int K = KT, V = 2 * KT, O = V + VT, X = O + VT, Y = X + ST, E = Y + ST, E2 = SHARED ? X : E + ET, ALL = SHARED ? E + ET : E2 + ET;
+    // where the results become rows of bf16 when all products are done
+    static constexpr int DQ = DV == 128 ? X : E, DKEYS = DV == 128 ? Y : E2, DVALUES = DV == 128 ? E : X;
+    static_assert(DV == 128 ? KT <= ST && VT <= ET : KT <= ET && VT <= 2 * ST, "the results fit");
+};
 
 // Sum over the lanes of a warp for each of 32 columns: lane i gets column i's.
 __device__ __forceinline__ float sum_columns(float (&m)[32], int lane) {
@@ -487,23 +515,24 @@ __device__ __forceinline__ void copy_out(uint32_t tile, const qgru_seq_tensor &x
 }
 
 // A CTA an SM, which takes chunk after chunk of all heads.  Pairs lie as [s][t] here, lane s of tensor memory.  Four blocks of 128 columns of it:
-//   0  (k q^T), then P^T in two bf16 parts     1  (v dout^T), then dv     2  dk     3  dq
+//   0  k q^T, then P^T in two parts     1  v dout^T, then dq     2  dk     3  dv
 // Four threads a row, a quarter of the columns each.  P^T is the operand of dv from tensor memory, E^T that of dk (K in its columns) and
-// of dq (K in its rows) from shared memory.
-// The next chunk's tiles are fetched while this one's results leave (both by TMA), its decays are summed up beside this one's gradient
-// of them, and the products of the states run beside the pairs.  What bounds it is the chain of products, pairs and conversions between
-// tensor memory and operands, and what of the loads it does not cover: 224 KB of operands leave no room for a second CTA or for tiles
-// fetched earlier.  16 x 1000 tokens of 8 heads of 128: 90 us; 105 with a CTA a chunk and its tiles by TMA, 108 where the threads load
-// them, 155 with 256 threads.  Bytes alone would take 43 (285 MB).  Heads of 64: 62 us.
+// of dq (K in its rows) from shared memory.  P, E and the states are two bf16 parts each: 16 bits of a factor, so that a result is the
+// type's rounding of a sum that is nearly exact.  With one part, as much lost as by that rounding, the kernel took 92 us where it takes 100
+// (16 x 1000 tokens of 8 heads of 128; bytes alone would take 56, 363 MB).
+// The next chunk's tiles are fetched while this one's results leave (both by TMA), its decays are summed up beside this one's products,
+// those of the state's gradient run beside the pairs, and the state before the chunk comes after them into the same place.  What bounds
+// it is the chain of products, pairs and conversions between tensor memory and operands, and what of the loads it does not cover: 224 KB of
+// operands leave no room for a second CTA or for tiles fetched earlier.
 template <int DK, int DV, bool Tma>
 __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_constant__ qgru_attention a, const __grid_constant__ Gradients p) {
     extern __shared__ unsigned char raw[];
     unsigned char *tiles = tiles_of(raw);
-    Shared &s = *reinterpret_cast<Shared *>(tiles + GRADIENTS_TILES<DK, DV>);
-    constexpr int KT = DK / 64 * PANEL, VT = DV / 64 * PANEL, ST = DK * DV * 2, KQ = DK / 4, VQ = DV / 4;
-    const uint32_t q_t = tc::smem_u32(tiles), k_t = q_t + KT, v_t = k_t + KT, o_t = v_t + VT, S_t = o_t + VT, dS_t = S_t + ST, E_t = dS_t + ST;
-    // where dq and dk become rows of bf16: tiles of their own, or where these have no room those of the states, which have been used by then
-    const uint32_t dq_t = DV == 64 ? E_t + 2 * PANEL : S_t, dk_t = DV == 64 ? dq_t + KT : dS_t;
+    using L = Tiles<DK, DV>;
+    Shared &s = *reinterpret_cast<Shared *>(tiles + L::ALL);
+    constexpr int KT = L::KT, VT = L::VT, ST = L::ST, KQ = DK / 4, VQ = DV / 4;
+    const uint32_t q_t = tc::smem_u32(tiles), k_t = q_t + L::K, v_t = q_t + L::V, o_t = q_t + L::O, X_t = q_t + L::X, Y_t = q_t + L::Y, E_t = q_t + L::E, E2_t = q_t + L::E2;
+    const uint32_t dq_t = q_t + L::DQ, dk_t = q_t + L::DKEYS, dv_t = q_t + L::DVALUES;
     // once v has been used, its tile holds sums by token
     float *t_sums = reinterpret_cast<float *>(tiles + 2 * KT);          // [4][128] over s of a block's lanes, for each t
     float *s_sums = t_sums + 4 * C, *q_dots = s_sums + 4 * C, *k_dots = q_dots + 4 * C;     // [4][128] each
@@ -563,12 +592,10 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
             tma_load_4d(o_t + i * PANEL, &p.o, &s.bar[4], i * 64, x.t0, x.h, x.b);
         }
     };
-    const auto fetch_states = [&](const Item &x) {
+    // both parts of a state
+    const auto fetch_state = [&](const bf16 *states, const Item &x) {
         tc::mbar_expect_tx(&s.bar[5], 2 * ST);
-        for (int i = 0; i < DV / 64; ++i) {
-            tc::tma_load_2d(tiles + 2 * KT + 2 * VT + i * (DK * 128), &p.S, &s.bar[5], i * 64, x.index * DK);
-            tc::tma_load_2d(tiles + 2 * KT + 2 * VT + ST + i * (DK * 128), &p.dS, &s.bar[5], i * 64, x.index * DK);
-        }
+        bulk_load(X_t, states + (long long)x.index * (2 * DK * DV), 2 * ST, &s.bar[5]);
     };
     Item x = next_of(blockIdx.x);
     // The decays of a chunk are the second four warps': read early, summed up while the first four sum up the last chunk's gradient.
@@ -596,7 +623,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
     }
     put_decays(g);
     const uint32_t tm = s.tmem, base = lane_base(tm, warp);
-    const Operand q{q_t, PANEL}, k{k_t, PANEL}, v{v_t, PANEL}, o{o_t, PANEL}, S{S_t, DK * 128}, dS{dS_t, DK * 128}, E{E_t, PANEL};
+    const Operand q{q_t, PANEL}, k{k_t, PANEL}, v{v_t, PANEL}, o{o_t, PANEL}, E{E_t, PANEL}, E2{E2_t, PANEL};
     for (uint32_t turn = 0; x.tokens; turn ^= 1) {
         const int b = x.b, h = x.h, hk = h / share, t0 = x.t0, all = x.all, tokens = x.tokens;
         if constexpr (!Tma) {
@@ -604,8 +631,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
             load_rows<DK, GRAD_THREADS>(k_t, a.k, at(a.k, b, hk), t0, tokens, a.Dk, tid);
             load_rows<DV, GRAD_THREADS>(v_t, a.v, at(a.v, b, h), t0, tokens, a.Dv, tid);
             load_rows<DV, GRAD_THREADS>(o_t, a.dout, at(a.dout, b, h), t0, tokens, a.Dv, tid);
-            load_state<DK, DV, GRAD_THREADS>(S_t, p.states + (long long)x.index * (DK * DV), tid);
-            load_state<DK, DV, GRAD_THREADS>(dS_t, p.dstates + (long long)x.index * (DK * DV), tid);
+            load_state<2 * ST, GRAD_THREADS>(X_t, p.dstates + (long long)x.index * (2 * DK * DV), tid);
             cp_commit();
         }
         if constexpr (Tma) {
@@ -631,7 +657,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
         if constexpr (Tma) {
             if (tid == 0) {
                 stores_read();             // the tiles of the states and of E were the last chunk's outputs
-                fetch_states(x);
+                fetch_state(p.dstates, x);
             }
         }
         // from the start of t's block of 32 to t
@@ -641,19 +667,28 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
         __syncthreads();
         if (warp == 3) {                      // (no pairs of its own)
             const uint32_t leader = elect();
-            if constexpr (Tma) await(s, 5, turn);
+            if constexpr (Tma) await(s, 5, 0);
             tc::tc_fence_after_sync();
-            product<false, false, DK, DV>(leader, tm + 256, v, dS, false);
-            product<false, false, DK, DV>(leader, tm + 384, o, S, false);
+            product_state<false, DK, DV, DK>(leader, tm + 256, v, Y_t, false);
+            product_state<false, DK, DV, DK>(leader, tm + 256, v, X_t, true);
+            product_state<true, DV, DK, DK>(leader, tm + 384, k, Y_t, false);
+            product_state<true, DV, DK, DK>(leader, tm + 384, k, X_t, true);
             commit(leader, &s.bar[1]);
+            if constexpr (Tma) {
+                await(s, 1, turn);            // the state before the chunk in the same place
+                if (lane == 0) fetch_state(p.states, x);
+            }
             __syncwarp();
         }
         await(s, 0, turn);
         const float2 G = s.G[row], last = s.G[C - 1];
         // the pairs: blocks of 32 x 32, t from s on
         float s_sum = 0.f, t_sum = 0.f;
+        uint32_t small[16];                   // of E, until there is room for it
         if (part < block) {
             const uint32_t zeros[32] = {};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) small[i] = 0u;
             tmem_store(base + part * 32, zeros);
 #pragma unroll
             for (int i = 0; i < 4; ++i) sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + i), 0u, 0u, 0u, 0u);
@@ -695,7 +730,9 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
                     m[t + 1] = mv.y;
                     P[i] = pack_part(pv);
                     P[8 + i] = pack(rest(pv, P[i]));
-                    e[i] = pack(__fmul2_rn(w, y[i]));
+                    const float2 ev = __fmul2_rn(w, y[i]);
+                    e[i] = pack_part(ev);
+                    small[t / 2] = pack(rest(ev, e[i]));
                 }
                 tmem_st16(base + part * 32 + t0, P);          // (in the place of k q^T, which no other warp reads)
                 sts16(E_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + t0 / 8), e[0], e[1], e[2], e[3]);
@@ -704,62 +741,71 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
             s_sum = sum.x + sum.y;
             t_sum = sum_columns(m, lane);
         }
+        const auto put_small = [&] {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sts16(E2_t + (part >> 1) * PANEL + chunk_at(row, (part & 1) * 4 + i), small[4 * i], small[4 * i + 1], small[4 * i + 2], small[4 * i + 3]);
+        };
+        if constexpr (!L::SHARED) put_small();
         await(s, 1, turn);
+        if constexpr (!Tma) {
+            load_state<2 * ST, GRAD_THREADS>(X_t, p.states + (long long)x.index * (2 * DK * DV), tid);
+            cp_commit();
+        }
         if (part >= block) t_sums[block * C + part * 32 + lane] = t_sum;
         s_sums[part * C + row] = s_sum;
         const float to_end = ex2_diff(last, G), from_start = a.scale * ex2(G.x + G.y);
         k_dots[part * C + row] = scale_sums<KQ>(base + 256 + part * KQ, to_end, k_t, row, part * KQ, true);
-        q_dots[part * C + row] = scale_sums<KQ>(base + 384 + part * KQ, from_start, q_t, row, part * KQ, true);
+        scale_sums<VQ>(base + 384 + part * VQ, to_end, 0, 0, 0, false);
+        if constexpr (!Tma) cp_wait<0>();
         fence_async();
         tc::tmem_st_wait();
         tc::tc_fence_before_sync();
-        __syncthreads();                                  // the pairs' sums have been read, E^T and the scaled sums are there
+        __syncthreads();                                  // the pairs' sums have been read, P^T, E^T and the scaled sums are there
         if (tid < 32) {
             const uint32_t leader = elect();
+            if constexpr (Tma) await(s, 5, 1);
             tc::tc_fence_after_sync();
-            product<false, true, DV, DK>(leader, tm + 128, k, dS, false);
+            product_state<false, DK, DV, DK>(leader, tm + 128, o, Y_t, false);
+            product_state<false, DK, DV, DK>(leader, tm + 128, o, X_t, true);
             commit(leader, &s.bar[2]);
             product<false, true, DK, C>(leader, tm + 256, E, q, true);
-            product<true, true, DK, C>(leader, tm + 384, E, k, true);
-            commit(leader, &s.bar[3]);
+            product_ts<true, DV, C>(leader, tm + 384, tm, o, true);
         }
-        // the decays' gradient: from each token on, every pair across it, and what passes from the state before the chunk to that behind it
-        double d = 0.0, own = 0.0;
-        if (tid < C) {
-            float t_sum = 0.f;
-            for (int w = 0; w <= tid >> 5; ++w) t_sum += t_sums[w * C + tid];
-            own = (double)t_sum;
-            double kd = 0.0;
-            for (int w = 0; w < 4; ++w) {
-                own += (double)q_dots[w * C + tid] - (double)s_sums[w * C + tid];
-                kd += (double)k_dots[w * C + tid];
-            }
-            d = running_sum<C>(kd - own, s.sums, tid) - (kd - own);
-        } else if (decays) {
-            g = running_sum<C>(decay_units(decay), s.g_sums, token);
-        }
-        double total = own;
-        for (int i = 16; i; i >>= 1) total += __shfl_xor_sync(0xffffffffu, total, i);
-        if (lane == 0 && tid < C) totals[warp] = total;
-        await(s, 2, 0);
-        scale_sums<VQ>(base + 128 + part * VQ, to_end, 0, 0, 0, false);
+        if (decays) g = running_sum<C>(decay_units(decay), s.g_sums, token);
+        await(s, 2, turn);
+        q_dots[part * C + row] = scale_sums<KQ>(base + 128 + part * KQ, from_start, q_t, row, part * KQ, true);
+        if constexpr (L::SHARED) put_small();
+        fence_async();
         tc::tmem_st_wait();
         tc::tc_fence_before_sync();
         __syncthreads();
         if (tid < 32) {
             const uint32_t leader = elect();
             tc::tc_fence_after_sync();
-            product_ts<true, DV, C>(leader, tm + 128, tm, o, true);
-            commit(leader, &s.bar[2]);
+            product<true, true, DK, C>(leader, tm + 128, E2, k, true);
+            product<true, true, DK, C>(leader, tm + 128, E, k, true);
+            product<false, true, DK, C>(leader, tm + 256, E2, q, true);
+            commit(leader, &s.bar[3]);
         }
         put_decays(g);                        // (every thread has read the last chunk's)
-        if (tid < all) {
-            double sum = d;
+        // the decays' gradient: from each token on, every pair across it, and what passes from the state before the chunk to that behind it
+        if (tid < C) {
+            float t_sum = 0.f;
+            for (int w = 0; w <= tid >> 5; ++w) t_sum += t_sums[w * C + tid];
+            double own = (double)t_sum, kd = 0.0;
+            for (int w = 0; w < 4; ++w) {
+                own += (double)q_dots[w * C + tid] - (double)s_sums[w * C + tid];
+                kd += (double)k_dots[w * C + tid];
+            }
+            double sum = running_sum<C>(kd - own, s.sums, tid) - (kd - own);
+            for (int i = 16; i; i >>= 1) own += __shfl_xor_sync(0xffffffffu, own, i);
+            if (lane == 0) totals[warp] = own;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
             for (int w = 0; w < tid >> 5; ++w) sum += s.sums[w];
             double through = 0.0;
             for (int w = 0; w < THROUGH; ++w) through += (double)p.through[(long long)x.index * THROUGH + w];
             sum += totals[0] + totals[1] + totals[2] + totals[3] + through * (double)exp2_of(last);
-            seq::store_f(a.ddecay.p, at(a.ddecay, b, h) + (long long)(t0 + tid) * a.ddecay.ts, a.decay_bf16, tid < tokens ? (float)sum : 0.f);
+            if (tid < all) seq::store_f(a.ddecay.p, at(a.ddecay, b, h) + (long long)(t0 + tid) * a.ddecay.ts, a.decay_bf16, tid < tokens ? (float)sum : 0.f);
         }
         // The next chunk's tiles come as soon as nothing reads the ones that they replace.
         const bool live = row < tokens;
@@ -770,7 +816,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
         // Out by way of tiles: a thread's part of a row on its own would be a store of 16 bytes in each of 32 lines.
         {
             float r[KQ];
-            tmem_load(base + 384 + part * KQ, r);
+            tmem_load(base + 128 + part * KQ, r);
 #pragma unroll
             for (int i = 0; i < KQ; ++i) r[i] = live ? r[i] : 0.f;
             p.dq_heads ? put_heads(p.dq_heads, x, r) : put_row(dq_t, row, part * KQ, r);
@@ -779,13 +825,12 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
             for (int i = 0; i < KQ; ++i) r[i] = live ? r[i] : 0.f;
             p.dk_heads ? put_heads(p.dk_heads, x, r) : put_row(dk_t, row, part * KQ, r);
         }
-        await(s, 2, 1);
         {
             float r[VQ];
-            tmem_load(base + 128 + part * VQ, r);
+            tmem_load(base + 384 + part * VQ, r);
 #pragma unroll
             for (int i = 0; i < VQ; ++i) r[i] = live ? r[i] : 0.f;
-            put_row(E_t, row, part * VQ, r);
+            put_row(dv_t, row, part * VQ, r);
         }
         fence_async();                                    // (the sums in v's tile come before what TMA writes there)
         tc::tc_fence_before_sync();
@@ -797,7 +842,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
                     tma_store_4d(&p.dq, dq_t + i * PANEL, i * 64, t0, h, b);
                     tma_store_4d(&p.dk, dk_t + i * PANEL, i * 64, t0, h, b);
                 }
-                for (int i = 0; i < DV / 64; ++i) tma_store_4d(&p.dv, E_t + i * PANEL, i * 64, t0, h, b);
+                for (int i = 0; i < DV / 64; ++i) tma_store_4d(&p.dv, dv_t + i * PANEL, i * 64, t0, h, b);
                 stores_commit();
             }
         } else {
@@ -805,7 +850,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_cons
                 copy_out<DK, false>(dq_t, a.dq, at(a.dq, b, h), t0, all, a.Dk, tid);
                 copy_out<DK, false>(dk_t, a.dk, at(a.dk, b, h), t0, all, a.Dk, tid);
             }
-            copy_out<DV, false>(E_t, a.dv, at(a.dv, b, h), t0, all, a.Dv, tid);
+            copy_out<DV, false>(dv_t, a.dv, at(a.dv, b, h), t0, all, a.Dv, tid);
             __syncthreads();
         }
         x = next;
@@ -885,10 +930,8 @@ int backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStre
     g.flag = flag;
     g.items = c.chunks * a.B * a.H;
     if (Tma) {
-        const long long rows = (long long)c.chunks * a.B * a.H * DK;
         if (!head_map(&g.q, a.q, a.T, a.B, a.Hk, a.Dk) || !head_map(&g.k, a.k, a.T, a.B, a.Hk, a.Dk) || !head_map(&g.v, a.v, a.T, a.B, a.H, a.Dv) ||
-            !head_map(&g.o, a.dout, a.T, a.B, a.H, a.Dv) || !state_map(&g.S, a.states, rows, DK, DV) || !state_map(&g.dS, dstates, rows, DK, DV) ||
-            !head_map(&g.dv, a.dv, a.T, a.B, a.H, a.Dv) ||
+            !head_map(&g.o, a.dout, a.T, a.B, a.H, a.Dv) || !head_map(&g.dv, a.dv, a.T, a.B, a.H, a.Dv) ||
             (a.H == a.Hk && (!head_map(&g.dq, a.dq, a.T, a.B, a.H, a.Dk) || !head_map(&g.dk, a.dk, a.T, a.B, a.H, a.Dk))))
             return seq::fail(QGRU_ERR_CUDA, "cuTensorMapEncodeTiled");
     }
@@ -897,7 +940,7 @@ int backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStre
         g.dk_heads = g.dq_heads + group_bytes(a) / 8;
     }
     int bytes = 0;
-    if (const int rc = with_smem(k_gradients_tc<DK, DV, Tma>, GRADIENTS_TILES<DK, DV>, &bytes)) return rc;
+    if (const int rc = with_smem(k_gradients_tc<DK, DV, Tma>, Tiles<DK, DV>::ALL, &bytes)) return rc;
     k_gradients_tc<DK, DV, Tma><<<std::min(g.items, sms), GRAD_THREADS, bytes, st>>>(a, g);
     SEQ_CK(cudaGetLastError());
     return g.dq_heads ? sum_groups(a, g.dq_heads, g.dk_heads, st) : QGRU_OK;
@@ -924,7 +967,7 @@ Cut tc_cut(const qgru_attention &a, int sms) {
     c.segments = (int)std::max<long long>(1, std::min<long long>(c.chunks / 2, sms / units));
     c.per = std::max(1, (c.chunks + c.segments - 1) / c.segments);
     c.segments = std::max(1, (c.chunks + c.per - 1) / c.per);
-    c.states = sizeof(bf16) * (size_t)c.chunks * a.B * a.H * (a.Dk <= 64 ? 64 : 128) * (a.Dv <= 64 ? 64 : 128);
+    c.states = 2 * sizeof(bf16) * (size_t)c.chunks * a.B * a.H * (a.Dk <= 64 ? 64 : 128) * (a.Dv <= 64 ? 64 : 128);
     c.seg = c.segments > 1 ? sizeof(float) * c.segments * (state_elems(a) + (size_t)a.B * a.H) : 0;
     c.through = sizeof(float) * THROUGH * c.chunks * (size_t)a.B * a.H;
     return c;

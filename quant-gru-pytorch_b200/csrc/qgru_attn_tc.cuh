@@ -15,16 +15,16 @@ Cut tc_cut(const qgru_attention &a, int sms);
 // flag: where a kernel says that a wait of its own has run out
 int tc_forward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStream_t st);
 int tc_backward(const qgru_attention &a, const Cut &c, int *flag, int sms, cudaStream_t st);
-// Tensor maps of a tensor's heads ([B][heads][T][D], boxes of 128 tokens x 64 columns) and of kept states ([rows][DV], boxes of DK x 64);
-// fetchable: whether TMA takes a tensor (rows and strides multiples of 16 bytes, no stride of 0)
+// Tensor map of a tensor's heads ([B][heads][T][D], boxes of 128 tokens x 64 columns); fetchable: whether TMA takes a tensor (rows and strides multiples of 16 bytes, no stride of 0)
 bool head_map(CUtensorMap *map, const qgru_seq_tensor &x, int T, int B, int heads, int d);
-bool state_map(CUtensorMap *map, const void *states, long long rows, int DK, int DV);
 bool fetchable(const qgru_seq_tensor &x, int T, int B, int heads, int d);
 // A walk through the chunks (qgru_attn_fwd.cu): forward with the outputs, or from the end with the gradient of the states alone
 bool walk_takes(const qgru_attention &a, bool reverse);
 int walk(const qgru_attention &a, const Cut &c, bool reverse, void *states, char *seg, float *through, int *flag, int sms, cudaStream_t st);
-// The pass from the end meets every state's gradient in fp32: it multiplies it with the state, as bf16 as it was kept, and leaves the sum in
-// THROUGH parts a chunk and head (the sums of its warps).
+// The pass from the end meets every state's gradient in fp32: it multiplies it with the state, as it was kept, and leaves the sum in
+// THROUGH parts a chunk and head (the sums of its warps).  A state is kept as 32 bits, the two bf16 parts (16 of its bits) that the
+// products take it in: [chunk][B H][part][DV / 8][DK][8], so that the threads of a warp, a row each, read and write whole lines (row by row,
+// with 16 bytes of 32 lines an instruction, the passes took 86 and 66 us where they take 66 and 58, 16 x 1000 tokens of 8 heads of 128).
 constexpr int THROUGH = 8;
 
 namespace tile {
@@ -70,18 +70,19 @@ __device__ __forceinline__ uint32_t elect() {
         : "=r"(r));
     return r;
 }
+template <uint32_t B_HI = DESC_HI>
 __device__ __forceinline__ void mma(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t id, uint32_t accumulate) {
     asm volatile(
         "{\n"
         ".reg .pred p, e;\n"
         ".reg .b64 da, db;\n"
         "mov.b64 da, {%1, %5};\n"
-        "mov.b64 db, {%2, %5};\n"
+        "mov.b64 db, {%2, %7};\n"
         "setp.ne.b32 p, %4, 0;\n"
         "setp.ne.b32 e, %6, 0;\n"
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n"
         "}\n" ::"r"(d),
-        "r"(a_lo), "r"(b_lo), "r"(id), "r"(accumulate), "n"(DESC_HI), "r"(leader)
+        "r"(a_lo), "r"(b_lo), "r"(id), "r"(accumulate), "n"(DESC_HI), "r"(leader), "n"(B_HI)
         : "memory");
 }
 // A from tensor memory: lane i is row i, a column holds two neighbouring K, sixteen K are eight columns
@@ -118,6 +119,21 @@ __device__ __forceinline__ void product(uint32_t leader, uint32_t d, const Opera
         for (int j = 0; j < 4; ++j) mma(leader, d, a0 + desc_step<ARows>(a, j), b0 + desc_step<BRows>(b, j), idesc(N, ARows, BRows), j ? 1u : more);
         a0 += desc_step<ARows>(a, 4);
         b0 += desc_step<BRows>(b, 4);
+        more = 1;
+    }
+}
+// B a part of a state as it is kept, [columns / 8][Rows][8] without a swizzle: groups of eight rows are 128 bytes apart, neighbouring
+// eights of columns 16 Rows.  K in the columns (N in the rows), or the other way: the descriptor's leading distance is K's then, its stride N's.
+template <bool BRows, int N, int K, int Rows>
+__device__ __forceinline__ void product_state(uint32_t leader, uint32_t d, const Operand &a, uint32_t b, bool add) {
+    constexpr uint32_t HI = (uint32_t)(BRows ? Rows : 128 >> 4) | (1u << 14), STEP = BRows ? 256 >> 4 : 2 * Rows;
+    uint32_t a0 = desc_lo<false>(a), b0 = ((b & 0x3FFFFu) >> 4) | (uint32_t)(BRows ? 128 >> 4 : Rows) << 16, more = add;
+#pragma unroll 1
+    for (int p = 0; p < K / 64; ++p) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mma<HI>(leader, d, a0 + desc_step<false>(a, j), b0 + j * STEP, idesc(N, false, BRows), j ? 1u : more);
+        a0 += desc_step<false>(a, 4);
+        b0 += 4 * STEP;
         more = 1;
     }
 }
@@ -210,6 +226,9 @@ __device__ __forceinline__ float ex2_diff(float2 t, float2 s) { return ex2((t.x 
 // 16-byte chunk c (of eight columns) of row r of a panel
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 
+__device__ __forceinline__ void bulk_load(uint32_t to, const void *from, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes), "r"(tc::smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ void tma_load_4d(uint32_t to, const CUtensorMap *map, uint64_t *bar, int x, int t, int h, int b) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(to),
                  "l"(reinterpret_cast<uint64_t>(map)), "r"(tc::smem_u32(bar)), "r"(x), "r"(t), "r"(h), "r"(b)

@@ -34,7 +34,8 @@ def shared(x, heads):
 
 CASES = [dict(T=300, B=2, H=2, Dk=64, Dv=64), dict(T=300, B=2, H=2, Dk=128, Dv=64), dict(T=300, B=2, H=2, Dk=64, Dv=128), dict(T=300, B=2, H=2, Dk=128, Dv=128),
          dict(T=1000, B=1, H=2, Dk=128, Dv=128, fused=True), dict(T=260, B=3, H=4, Dk=64, Dv=64, Hk=2, lengths=[260, 129, 77]), dict(T=200, B=2, H=2, Dk=128, Dv=130),
-         dict(T=24, B=1, H=4, Dk=64, Dv=64), dict(T=128, B=2, H=2, Dk=60, Dv=60, h0=False)]
+         dict(T=24, B=1, H=4, Dk=64, Dv=64), dict(T=128, B=2, H=2, Dk=60, Dv=60, h0=False),
+         dict(T=300, B=2, H=2, Dk=60, Dv=60), dict(T=200, B=2, H=2, Dk=100, Dv=128, Hk=1), dict(T=200, B=2, H=2, Dk=33, Dv=17, lengths=[200, 130])]
 
 
 def check(got, want, d, types, Hk):
@@ -55,3 +56,22 @@ def test_outputs_are_nearly_their_types_roundings(case, decay, cuda_device):
     want = ref.attention(*args, state=state, lengths=n)
     d, types = limits(want, *args, state, n, *zeros)
     check({"out": out, "state": last}, want, d, types, Hk)
+
+
+@pytest.mark.parametrize("decay", [F32, BF], ids=["fp32_decays", "bf16_decays"])
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(f"{k}{v}" for k, v in c.items()))
+def test_gradients_are_nearly_their_types_roundings(case, decay, cuda_device):
+    q, k, v, g, state, n = make(cuda_device, dtype=BF, decay=decay, **case)
+    H, Hk = v.shape[2], q.shape[2]
+    names = ["dq", "dk", "dv", "dg"] + (["dstate0"] if state is not None else [])
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, g, state) if t is not None]
+    out, last = la.linear_attention(*leaves, lengths=n)
+    dout, dstate = torch.randn_like(out), torch.randn_like(last)
+    got = dict(zip(names, torch.autograd.grad((out, last), leaves, (dout, dstate))))
+    args = [x.repeat_interleave(H // Hk, 2) for x in (q, k)] + [v, g]
+    want = ref.attention(*args, state=state, lengths=n, dout=dout, dstate=dstate)
+    d, types = limits(want, *args, state, n, dout, dstate)
+    check(got, want, d, types, Hk)
+    with torch.no_grad():        # the form that keeps no states for a gradient
+        again = la.linear_attention(q, k, v, g, state, n)
+    assert torch.equal(again[0], out) and torch.equal(again[1], last)
