@@ -58,6 +58,11 @@ variable_list once(variable_list grads) {
     return (*std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", (int)grads.size()))(std::move(grads));
 }
 
+// There is no forward-mode derivative: results without one would be taken for constants.
+void check_tangents(std::initializer_list<const Tensor *> inputs) {
+    for (const Tensor *t : inputs) TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), "the sequence operators have no forward-mode derivative: an input has a tangent");
+}
+
 // The node that adds to a leaf's gradient lives as long as any graph of the leaf, with the stream that it was made on.  Where that is
 // the default stream, a backward inside a capture on another one would have it wait for the captured work, which CUDA forbids and
 // autograd does not survive.  Refused before anything is recorded.
@@ -232,6 +237,7 @@ std::tuple<Tensor, Tensor> linear_attention(const Tensor &q, const Tensor &k, co
         n = lengths->contiguous();
     }
     const double s = scale ? *scale : 1.0 / std::sqrt((double)q.size(3));
+    check_tangents({&q, &k, &v, &decay, &state0});
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || decay.requires_grad() || (state0.defined() && state0.requires_grad()))) {
         check_capture({&q, &k, &v, &log_decay, &state0});
         const variable_list r = LinearAttention::apply(q, k, v, decay, some(state0), some(n), s, batch_first);
@@ -245,6 +251,7 @@ Tensor linear_attention_step(const Tensor &q0, const Tensor &k0, const Tensor &v
     const Tensor decay = check_attention(q0, k0, v0, log_decay, 1);
     TORCH_CHECK(!at::GradMode::is_enabled() || !(q0.requires_grad() || k0.requires_grad() || v0.requires_grad() || decay.requires_grad() || state.requires_grad()),
                 "linear_attention_step has no gradient: call it under torch.no_grad(), or linear_attention with T = 1");
+    check_tangents({&q0, &k0, &v0, &decay, &state});
     const Sizes n{1, q0.size(0), v0.size(1), q0.size(1), q0.size(2), v0.size(2)};
     const std::vector<int64_t> want{n.B, n.H, n.Dk, n.Dv};
     TORCH_CHECK_VALUE(state.scalar_type() == at::kFloat && state.device() == q0.device() && state.sizes() == want, "state must be a float32 tensor of shape ", want, " on ",
@@ -361,6 +368,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
 py::object rms_norm(const Tensor &x, const Tensor &weight, const std::optional<Tensor> &residual, double eps) {
     const Tensor r = residual ? *residual : Tensor();
     check_norm(x, weight, r);
+    check_tangents({&x, &weight, &r});
     if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (r.defined() && r.requires_grad()))) {
         check_capture({&x, &weight, &r});
         const variable_list got = RmsNorm::apply(x, weight, some(r), eps);
@@ -376,6 +384,7 @@ py::object rms_norm_q8(const Tensor &x, const Tensor &weight, const std::optiona
     check_norm(x, weight, r);
     TORCH_CHECK(!at::GradMode::is_enabled() || !r.defined() || !(x.requires_grad() || r.requires_grad()),
                 "rms_norm_q8 has no gradient, and the stream that it returns would end the residual's: call it under torch.no_grad()");
+    if (r.defined()) check_tangents({&x, &r});
     const at::NoGradGuard off;
     const Tensor x2 = rows_of(x), w = weight.contiguous(), r2 = r.defined() ? rows_of(r) : Tensor(), h = r.defined() ? at::empty(x.sizes(), x.options()) : Tensor();
     const Tensor q = at::empty(x.sizes(), x.options().dtype(scale && is_unsigned ? at::kByte : at::kChar));

@@ -13,7 +13,7 @@ Tensors are [T, B, heads, D] as the GRU's are [T, B, H] ([B, T, heads, D] with `
 is 1, float32 or bfloat16; states are float32.  Arguments are checked, memory is allocated and the library is called in
 csrc/qgru_seq_torch.cc.  Everything runs on the current stream of the tensors' device, waits for nothing and may be captured into a
 graph; where a backward pass is, no graph of the same leaves made on the default stream may still live (of q, k, v, log_decay and
-initial_state themselves it is refused).
+initial_state themselves it is refused).  Gradients are of the first order and backward; inputs with a forward-mode tangent are refused.
 """
 import math
 

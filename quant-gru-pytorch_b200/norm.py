@@ -7,6 +7,7 @@
 
 Tensors are float32 or bfloat16 on the GPU, rows of up to 16384 features; arguments are checked, memory is allocated and the library
 is called in csrc/qgru_seq_torch.cc.  Everything runs on the current stream of the tensors' device and waits for nothing.
+Inputs with a forward-mode tangent are refused, by ``rms_norm_q8`` where the residual's stream has one.
 """
 from . import _cabi
 

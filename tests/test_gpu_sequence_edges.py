@@ -50,3 +50,33 @@ def test_one_infinite_value_at_each_token_of_a_chunk(dtype, Dk, Dv, cuda_device)
         assert torch.isfinite(out[before]).all()
         hold({"out": out[before]}, {"out": want["out"][before]}, {"out": bound["out"][before]})
         assert not torch.isfinite(out[C + at, at, 0, (7 * at) % Dv]).any()
+
+
+def test_inputs_with_a_tangent_are_refused(cuda_device):
+    import torch.autograd.forward_ad as fwd
+    q, k, v, g, state, _ = make(cuda_device, 20, 2, 2, 64, 64, F32)
+    x, w, r = torch.randn(3, 64, device=cuda_device), torch.ones(64, device=cuda_device), torch.randn(3, 64, device=cuda_device)
+    token = [t[0].clone() for t in (q, k, v, g)] + [state.clone()]
+    calls = [(la.linear_attention, [q, k, v, g, state]), (la.linear_attention, [q, k, v, g[0, 0].clone(), state]), (la.linear_attention_step, token), (norm.rms_norm, [x, w]),
+             (norm.rms_norm, [x, w, r])]
+    for call, args in calls:
+        for i in range(len(args)):
+            for grad in (False, True):
+                with fwd.dual_level(), torch.set_grad_enabled(grad):
+                    use = [fwd.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(args)]
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        call(*use)
+                    call(*[fwd.unpack_dual(t).primal for t in use])
+    before = token[4].clone()
+    for i in (0, 2):
+        with fwd.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+            use = [fwd.make_dual(t, t) if i == j else t for j, t in enumerate([x, w, r])]
+            norm.rms_norm_q8(*use)
+    with fwd.dual_level():
+        norm.rms_norm_q8(x, fwd.make_dual(w, w), r)            # a layer's weight alone has no part in the stream
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            la.linear_attention_step(*token[:4], fwd.make_dual(token[4], token[4]))
+    assert torch.equal(token[4], before)
+    layer = la.LinearAttention(64, 2, 32, 32).to(cuda_device)
+    with pytest.raises(Exception):
+        torch.func.jvp(lambda t: layer(t)[0], (torch.randn(5, 2, 64, device=cuda_device),), (torch.ones(5, 2, 64, device=cuda_device),))
