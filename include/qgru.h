@@ -589,10 +589,16 @@ QGRU_API int qgru_calibrate_from_histogram(const float *counts, int num_bins, fl
  * linear in its state, and the root-mean-square norm with the residual's addition that such layers stand
  * between.  These calls have no handle: they keep nothing, allocate nothing and wait for nothing; workspaces are the
  * caller's, and calls that do not share one may run at the same time.  They run on `device`, whatever the thread's current
- * device is.  A wait inside a kernel that runs out (each is bounded) leaves its results unfinished and is told once, by the next
- * of these calls that begins after the GPU got there (QGRU_ERR_TIMEOUT).
+ * device is.  What they do share is one word a device: a wait inside a kernel that runs out (each is bounded) leaves that kernel's results
+ * unfinished and sets it.  The next of these calls on the device that begins after the GPU got there, whichever it is, queues nothing and returns
+ * QGRU_ERR_TIMEOUT; so does, once, the next call of every other thread that had made one before.  (Whose results they were is not known:
+ * none of the device's that were not ready by then are to be used.)
+ * qgru_seq_check tells the same without a call: after a wait for the stream, of a replayed graph's kernels too.
+ * qgru_seq_test_expire, for tests of these reports: sets the word as a kernel does.
  * qgru_seq_last_error: why the calling thread's last of these calls failed. */
 QGRU_API const char *qgru_seq_last_error(void);
+QGRU_API int qgru_seq_check(int device);
+QGRU_API int qgru_seq_test_expire(int device);
 
 /* Element (t, b, h, d) of a tensor lies at p + t * ts + b * bs + h * hs + d (elements; decays have no d). */
 typedef struct qgru_seq_tensor {

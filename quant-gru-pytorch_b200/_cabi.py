@@ -162,6 +162,8 @@ SYMBOLS = {
     "qgru_calibrate_from_histogram": (C.c_int, [_F, C.c_int, C.c_float, C.c_float, C.c_int64, C.c_int,
                                                 C.c_int, C.c_float, C.POINTER(Op)]),
     "qgru_seq_last_error": (C.c_char_p, []),
+    "qgru_seq_check": (C.c_int, [C.c_int]),
+    "qgru_seq_test_expire": (C.c_int, [C.c_int]),
     "qgru_attention_sizes": (C.c_int, [C.POINTER(Attention)] + [C.POINTER(C.c_size_t)] * 3),
     "qgru_attention_forward": (C.c_int, [C.POINTER(Attention), _P]),
     "qgru_attention_backward": (C.c_int, [C.POINTER(Attention), _P]),
@@ -208,7 +210,6 @@ def check(status, where, handle=None):
         if status in (QGRU_ERR_BAD_ARG,):
             raise ValueError(f"{where}: {detail or 'bad argument'}")
         raise QgruError(status, where, detail)
-
 
 
 _seq = None

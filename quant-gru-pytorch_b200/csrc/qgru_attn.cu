@@ -1006,6 +1006,7 @@ static int attention_run(const qgru_attention *a, bool backward, void *stream) {
     if ((states && !a->states) || a->states_bytes < states) return seq::fail(QGRU_ERR_BAD_ARG, "states needs %zu bytes, got %zu", states, a->states_bytes);
     if ((ws && !a->workspace) || a->workspace_bytes < ws) return seq::fail(QGRU_ERR_BAD_ARG, "workspace needs %zu bytes, got %zu", ws, a->workspace_bytes);
     if ((reinterpret_cast<uintptr_t>(a->states) | reinterpret_cast<uintptr_t>(a->workspace)) % 256) return seq::fail(QGRU_ERR_BAD_ARG, "states and workspace must be aligned to 256 bytes");
+    if (const int rc = seq::check_expiry(a->device)) return rc;
     const seq::OnDevice on(a->device);
     SEQ_CK(on.error());
     attn::Cut c;
@@ -1028,6 +1029,7 @@ int qgru_attention_step(const qgru_attention *a, long long state_bs, long long s
     if (a->B == 0) return QGRU_OK;
     if (!a->q.p || !a->k.p || !a->v.p || !a->decay.p || !a->out.p || !a->state) return seq::fail(QGRU_ERR_BAD_ARG, "null tensor");
     if (a->T != 1 || a->lengths) return seq::fail(QGRU_ERR_BAD_ARG, "a step takes one token of every sequence");
+    if (const int rc = seq::check_expiry(a->device)) return rc;
     const seq::OnDevice on(a->device);
     SEQ_CK(on.error());
     cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -482,6 +482,7 @@ int qgru_norm_forward(const qgru_norm *n, void *stream) {
     if (n->q8 && !(n->q8_scale > 0.f) && !n->scales) return seq::fail(QGRU_ERR_BAD_ARG, "scales is null");
     if (n->q8 && n->q8_scale > 0.f && (n->q8_lo > n->q8_hi || n->q8_lo < -128 || n->q8_hi > 255 || n->q8_hi - n->q8_lo > 255 || (n->q8_lo < 0 && n->q8_hi > 127)))
         return seq::fail(QGRU_ERR_BAD_ARG, "%d .. %d is no range of 8 bits", n->q8_lo, n->q8_hi);
+    if (const int rc = seq::check_expiry(n->device)) return rc;
     const seq::OnDevice on(n->device);
     SEQ_CK(on.error());
     cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -502,6 +503,7 @@ size_t qgru_norm_workspace(int device, long long rows, int cols) {
 int qgru_norm_backward(const qgru_norm *n, const void *h, long long h_stride, const void *dy, long long dy_stride, const void *dh, long long dh_stride, void *dx,
                        long long dx_stride, void *dweight, void *workspace, size_t workspace_bytes, void *stream) {
     if (const int rc = norm::check(n)) return rc;
+    if (const int rc = seq::check_expiry(n->device)) return rc;
     const seq::OnDevice on(n->device);
     SEQ_CK(on.error());
     cudaStream_t st = static_cast<cudaStream_t>(stream);

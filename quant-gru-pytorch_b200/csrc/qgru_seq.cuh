@@ -14,8 +14,9 @@ namespace seq {
 int fail(int status, const char *fmt, ...);
 int cuda_fail(cudaError_t e, const char *where);
 
-// Where a kernel on the (current) device says that a bounded wait of its own has run out: a word of host memory, so that the next call
-// knows without waiting.  Returns QGRU_ERR_TIMEOUT, once, where an earlier call's has.
+// QGRU_ERR_TIMEOUT, once for each thread that makes these calls, where a wait inside a kernel of an earlier call on the device has run out.
+int check_expiry(int device);
+// Where a kernel on the (current) device says so: a word of host memory, so that the next call knows without waiting.
 int expiry_flag(int device, int **flag);
 
 // Work goes to the device that the caller names; the thread's current device is put back when the call ends.  (Set even where it

@@ -8,6 +8,7 @@ For every sequence and head, with the state S [Dk, Dv]
 ``linear_attention``       whole sequences (prompts, training); differentiable
 ``linear_attention_step``  one token of every sequence, the state updated in place (serving)
 ``LinearAttention``        a layer around them: norm with the residual's addition, projections, a gate for the decays
+``synchronize``            waits, and raises what went wrong inside a kernel
 
 Tensors are [T, B, heads, D] as the GRU's are [T, B, H] ([B, T, heads, D] with ``batch_first``) with any strides whose last
 is 1, float32 or bfloat16; states are float32.  Arguments are checked, memory is allocated and the library is called in
@@ -37,6 +38,17 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None):
     """One token of every sequence: q, k [B, Hk, Dk], v [B, H, Dv], log_decay [B, H] or [H].  state [B, H, Dk, Dv] float32, a
     head's state dense, is updated in place.  Returns out [B, H, Dv].  No gradient."""
     return (_cabi._seq or _cabi.seq()).linear_attention_step(q, k, v, log_decay, state, scale)
+
+
+def synchronize(device=None):
+    """Waits for the work on the current stream of `device` and raises what went wrong inside a kernel of these operators there (a bounded
+    wait that ran out: results are unfinished), replays of captured graphs included.  Without it the next call on the device raises it."""
+    device = torch.device("cuda" if device is None else device)
+    stream = torch.cuda.current_stream(device)
+    stream.synchronize()
+    status = _cabi.lib().qgru_seq_check(stream.device_index)
+    if status != _cabi.QGRU_OK:
+        raise _cabi.QgruError(status, "synchronize", _cabi.lib().qgru_seq_last_error().decode())
 
 
 class LinearAttention(nn.Module):

@@ -80,3 +80,90 @@ def test_inputs_with_a_tangent_are_refused(cuda_device):
     layer = la.LinearAttention(64, 2, 32, 32).to(cuda_device)
     with pytest.raises(Exception):
         torch.func.jvp(lambda t: layer(t)[0], (torch.randn(5, 2, 64, device=cuda_device),), (torch.ones(5, 2, 64, device=cuda_device),))
+
+
+_cabi = importlib.import_module(PKG_NAME + "._cabi")
+
+
+@pytest.fixture
+def expire(cuda_device):
+    """As a kernel leaves it whose wait has run out; nothing of it stays."""
+    def nothing_told():                  # (to this thread, nor to the one that runs backward passes)
+        leaf = torch.ones(1, 8, device=cuda_device, requires_grad=True)
+        for _ in range(3):
+            try:
+                norm.rms_norm(leaf, leaf[0]).sum().backward()
+            except RuntimeError as e:
+                assert "run out" in str(e)
+
+    nothing_told()
+    yield lambda: _cabi.check(_cabi.lib().qgru_seq_test_expire(0), "qgru_seq_test_expire")
+    nothing_told()
+
+
+def raises_expiry():
+    return pytest.raises(_cabi.QgruError, match="run out")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_whichever_call_comes_next_tells_that_a_wait_ran_out(dtype, expire, cuda_device):
+    q, k, v, g, state, _ = make(cuda_device, 20, 2, 2, 64, 64, dtype)
+    x, w, r = torch.randn(3, 64, device=cuda_device), torch.ones(64, device=cuda_device), torch.randn(3, 64, device=cuda_device)
+    wide = make(cuda_device, 20, 2, 2, 200, 64, dtype)[:5]
+    before = state.clone()
+    for call in (lambda: la.linear_attention(q, k, v, g, state), lambda: la.linear_attention(*wide), lambda: la.linear_attention_step(q[0], k[0], v[0], g[0], state),
+                 lambda: norm.rms_norm(x, w), lambda: norm.rms_norm(x, w, r), lambda: norm.rms_norm_q8(x, w), lambda: la.synchronize(), lambda: la.synchronize("cuda:0")):
+        expire()
+        with raises_expiry() as e:
+            call()
+        assert e.value.status == _cabi.QGRU_ERR_TIMEOUT
+        assert torch.equal(state, before)            # nothing was queued
+        call()                                       # told once
+        state.copy_(before)
+    leaf = q.detach().requires_grad_()
+    out, _ = la.linear_attention(leaf, k, v, g)
+    expire()
+    with pytest.raises(RuntimeError, match="run out"):          # (what a node throws is a RuntimeError when the engine hands it on)
+        torch.autograd.grad(out.sum(), leaf)
+
+
+def test_every_thread_is_told_of_a_wait_that_ran_out(expire, cuda_device):
+    """The one that finds it, and each that had work on the device; a thread whose first call comes later is not."""
+    import threading
+    q, k, v, g, state, _ = make(cuda_device, 20, 2, 2, 64, 64, BF)
+    begun, go, told = threading.Barrier(3), threading.Event(), []
+
+    def work(i):
+        la.linear_attention(q, k, v, g, state)
+        begun.wait()
+        go.wait()
+        for _ in range(3):
+            try:
+                la.linear_attention(q, k, v, g, state)
+            except _cabi.QgruError:
+                told.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    begun.wait()
+    expire()
+    with raises_expiry():
+        la.linear_attention(q, k, v, g, state)
+    go.set()
+    for t in threads:
+        t.join()
+    assert sorted(told) == [0, 1]
+    fresh = []
+
+    def late():
+        try:
+            la.linear_attention(q, k, v, g, state)
+            fresh.append("ran")
+        except _cabi.QgruError:
+            fresh.append("told")
+
+    t = threading.Thread(target=late)
+    t.start()
+    t.join()
+    assert fresh == ["ran"]
