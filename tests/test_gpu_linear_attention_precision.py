@@ -1,31 +1,15 @@
-"""Linear attention in bf16: nothing inside is coarser than 16 bits, so a result is its type's rounding of a sum that is nearly exact.
-
-A factor of a product on the tensor cores is one bf16 value or the sum of two or three.  Two parts: the first is off by 2^-8 of the factor
-at the most (half a step), the second by 2^-8 of what is left: 2^-16 of the factor.  So held are the pairs' weights (P, E), the
-state before a chunk and its gradient behind it, one of them in a product; k times its decays, three parts, is as good as
-fp32.  Sums are fp32, n terms one after the other: n 2^-24 of the sum of the terms' sizes.  With d = (2^-16 + n 2^-24) size a sum is off by d at the most;
-its rounding to the type is a nearest one, whose distance from the grid changes by no more than the sum does, so the result is off by
-|round(want) - want| + 2 d."""
+"""Linear attention: nothing inside is coarser than 16 bits (fp32 for fp32), so a result is its type's rounding of a sum that is nearly exact
+(tests/seq_terms.py says how near)."""
 import pytest
 import torch
 
 from tests import seq_reference as ref
+from tests import seq_terms as terms
+from tests.seq_terms import attention_limits
 from tests.test_gpu_linear_attention import BF, F32, la, make
+from tests.test_seq_limits import positive
 
 pytestmark = pytest.mark.gpu
-F = 2.0 ** -24
-
-
-def limits(want, q, k, v, g, state, n, dout, dstate):
-    """name -> how far it may be off, for time-first arguments with heads repeated."""
-    sizes = ref.attention(q.abs(), k.abs(), v.abs(), g, state.abs() if state is not None else None, n, None, dout.abs(), dstate.abs())
-    terms = q.shape[0] + 2 * max(q.shape[-1], v.shape[-1]) + 24
-    types = {"state": F32, "dstate0": F32, "dg": g.dtype}
-    d = {name: ((0 if types.get(name) == F32 and name != "dg" else 2.0 ** -16) + terms * F) * size for name, size in sizes.items()}
-    # the decays' gradient is a running sum of what cancels in a chunk
-    qdq, kdk = (q.double().abs() * sizes["dq"]).sum(-1), (k.double().abs() * sizes["dk"]).sum(-1)
-    d["dg"] = 2.0 ** -16 * sizes["dg"] + terms * F * (sizes["dg"] + (qdq + kdk).flip(0).cumsum(0).flip(0))
-    return d, {name: types.get(name, BF) for name in sizes}
 
 
 def shared(x, heads):
@@ -41,8 +25,8 @@ CASES = [dict(T=300, B=2, H=2, Dk=64, Dv=64), dict(T=300, B=2, H=2, Dk=128, Dv=6
 def check(got, want, d, types, Hk):
     for name, x in got.items():
         w, s = (shared(want[name], Hk), shared(d[name], Hk)) if name in ("dq", "dk") else (want[name], d[name])
-        off = (x.double() - w).abs() / ((w.to(types[name]).double() - w).abs() + 2 * s + 1e-30)
-        assert off.max() <= 1, f"{name}: {off.max():.2f} times the limit, at {[int(i) for i in (off == off.max()).nonzero()[0]]}"
+        off = terms.off_of(x, w, s, types[name])
+        assert off <= 1, f"{name}: {off:.2f} times the limit"
 
 
 @pytest.mark.parametrize("decay", [F32, BF], ids=["fp32_decays", "bf16_decays"])
@@ -52,9 +36,8 @@ def test_outputs_are_nearly_their_types_roundings(case, decay, cuda_device):
     H, Hk = v.shape[2], q.shape[2]
     out, last = la.linear_attention(q, k, v, g, state, n)
     args = [x.repeat_interleave(H // Hk, 2) for x in (q, k)] + [v, g]
-    zeros = torch.zeros_like(out), torch.zeros_like(last)
     want = ref.attention(*args, state=state, lengths=n)
-    d, types = limits(want, *args, state, n, *zeros)
+    d, types = attention_limits(want, *args, state, n)
     check({"out": out, "state": last}, want, d, types, Hk)
 
 
@@ -70,8 +53,41 @@ def test_gradients_are_nearly_their_types_roundings(case, decay, cuda_device):
     got = dict(zip(names, torch.autograd.grad((out, last), leaves, (dout, dstate))))
     args = [x.repeat_interleave(H // Hk, 2) for x in (q, k)] + [v, g]
     want = ref.attention(*args, state=state, lengths=n, dout=dout, dstate=dstate)
-    d, types = limits(want, *args, state, n, dout, dstate)
+    d, types = attention_limits(want, *args, state, n, dout, dstate)
     check(got, want, d, types, Hk)
     with torch.no_grad():        # the form that keeps no states for a gradient
         again = la.linear_attention(q, k, v, g, state, n)
     assert torch.equal(again[0], out) and torch.equal(again[1], last)
+
+
+@pytest.mark.parametrize("decay", [F32, BF], ids=["fp32_decays", "bf16_decays"])
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("Dk,Dv", [(64, 64), (64, 128), (128, 64), (128, 128), (60, 60), (33, 100), (200, 256)])
+def test_gradients_of_terms_that_do_not_cancel(Dk, Dv, dtype, decay, cuda_device):
+    """All positive: a limit is a part of the value itself, and no term of the decays' gradient can be missing."""
+    if dtype == F32 and decay == BF:
+        pytest.skip("decays are float32 or the type of q")
+    q, k, v, g, state, dout, dstate = (t.to(cuda_device) for t in positive(300, 1, 2, Dk, Dv, dtype))
+    g = g.to(decay)
+    leaves = [t.requires_grad_() for t in (q, k, v, g, state)]
+    out, last = la.linear_attention(*leaves)
+    got = dict(zip(("dq", "dk", "dv", "dg", "dstate0"), torch.autograd.grad((out, last), leaves, (dout, dstate))))
+    args = [t.detach() for t in leaves[:4]]
+    want = ref.attention(*args, state=state.detach(), dout=dout, dstate=dstate)
+    d, types = attention_limits(want, *args, state.detach(), None, dout, dstate)
+    check({"out": out.detach(), "state": last.detach(), **got}, want, d, types, 2)
+
+
+@pytest.mark.parametrize("T,D", terms.SHORT, ids=str)
+def test_states_of_a_few_tokens_have_24_bits(T, D, cuda_device):
+    """k times its decays, or q from the end, is three bf16 parts on the tensor cores, whichever kernel takes the size."""
+    q, k, v, _, _, _ = make(cuda_device, T, 4, 4, *D, BF, seed=T)
+    dout, g = torch.randn_like(v), -0.1 * torch.rand(T, 4, 4, device=cuda_device)
+    state = torch.zeros(4, 4, *D, device=cuda_device, requires_grad=True)
+    out, last = la.linear_attention(q, k, v, g, state)
+    dstate0, = torch.autograd.grad(out, state, dout)
+    want = ref.attention(q, k, v, g, dout=dout)
+    sizes = ref.attention(q.abs(), k.abs(), v.abs(), g, dout=dout.abs())
+    for name, x in (("state", last), ("dstate0", dstate0)):
+        off = ((x.double() - want[name]).abs() / terms.short_state_limit(sizes[name], T)).max()
+        assert off <= 1, f"{name}: {off:.2f} times the limit"
