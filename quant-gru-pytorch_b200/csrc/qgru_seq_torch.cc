@@ -50,6 +50,11 @@ Tensor readable(const Tensor &t) {
     }
     return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
+// A tensor saved for the backward, as it was: kernels go by its sizes and type.
+constexpr const char *HOOKED = "a saved-tensor hook has returned another type, shape or device than it was given";
+void check_saved(const Tensor &t, at::ScalarType type, at::IntArrayRef sizes, const Tensor &like) {
+    TORCH_CHECK(t.defined() && t.scalar_type() == type && t.sizes() == sizes && t.device() == like.device(), HOOKED);
+}
 // What a backward computes has no gradient of its own: whoever differentiates it is told.
 variable_list once(variable_list grads) {
     if (!at::GradMode::is_enabled()) return grads;
@@ -165,21 +170,32 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
         ctx->saved_data["batch_first"] = batch_first;
         ctx->saved_data["states"] = (int64_t)(states.defined() ? states.numel() : 0);
         ctx->saved_data["has_state"] = state0.defined();
+        ctx->saved_data["has_lengths"] = lengths.defined();
+        ctx->saved_data["shape"] = std::vector<int64_t>{q.size(0), q.size(1), q.size(2), q.size(3), v.size(2), v.size(3)};
+        ctx->saved_data["type"] = (int64_t)q.scalar_type();
+        ctx->saved_data["decay_type"] = (int64_t)decay.scalar_type();
         ctx->set_materialize_grads(false);
         return {out, state};
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         const variable_list saved = ctx->get_saved_variables();
         variable_list got(8);
+        if (!grads[0].defined() && !grads[1].defined()) return got;
         {
             const at::NoGradGuard off;
             const bool batch_first = ctx->saved_data["batch_first"].toBool();
-            const Tensor q = readable(saved[0]), k = readable(saved[1]), v = readable(saved[2]), &decay = saved[3], &lengths = saved[4];
+            const std::vector<int64_t> d = ctx->saved_data["shape"].toIntVector();
+            const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
+            const Tensor &like = grads[0].defined() ? grads[0] : grads[1], &decay = saved[3];
+            for (int i = 0; i < 2; ++i) check_saved(saved[i], type, {d[0], d[1], d[2], d[3]}, like);
+            check_saved(saved[2], type, {d[0], d[1], d[4], d[5]}, like);
+            check_saved(decay, (at::ScalarType)ctx->saved_data["decay_type"].toInt(), {d[0], d[1], d[4]}, like);
+            if (ctx->saved_data["has_lengths"].toBool()) check_saved(saved[4], at::kInt, {d[batch_first ? 0 : 1]}, like);
+            const Tensor q = readable(saved[0]), k = readable(saved[1]), v = readable(saved[2]), lengths = saved[4].defined() ? saved[4].contiguous() : Tensor();
             Tensor states = saved[5];
             const int64_t states_size = ctx->saved_data["states"].toInt();
             if (states_size) {
-                TORCH_CHECK(states.defined() && states.numel() == states_size && states.scalar_type() == at::kByte && states.device() == q.device(),
-                            "a saved-tensor hook has returned another type, shape or device than it was given");
+                check_saved(states, at::kByte, {states_size}, like);
                 if (!states.is_contiguous() || reinterpret_cast<uintptr_t>(states.data_ptr()) % 256) states = states.clone(at::MemoryFormat::Contiguous);
             }
             const Sizes n = sizes_of(q, v, batch_first);
@@ -332,6 +348,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
         auto [y, h, rstd] = norm_forward(x, weight, residual ? *residual : Tensor(), eps, true);
         ctx->save_for_backward({h.defined() ? h : x, weight, rstd});
         ctx->saved_data["residual"] = h.defined();
+        ctx->saved_data["weight_type"] = (int64_t)weight.scalar_type();
         ctx->set_materialize_grads(false);
         if (!h.defined()) return {y};
         return {y, h};
@@ -348,6 +365,9 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
         }
         {
             const at::NoGradGuard off;
+            check_saved(saved[0], dy.scalar_type(), dy.sizes(), dy);
+            check_saved(saved[1], (at::ScalarType)ctx->saved_data["weight_type"].toInt(), {dy.size(-1)}, dy);
+            check_saved(saved[2], at::kFloat, {dy.numel() / dy.size(-1)}, dy);
             const Tensor h2 = rows_of(saved[0]), weight = saved[1].contiguous(), rstd = saved[2].contiguous(), dy2 = rows_of(dy), dh2 = dh.defined() ? rows_of(dh) : Tensor();
             const Tensor dx = at::empty(saved[0].sizes(), saved[0].options()), dw = ctx->needs_input_grad(1) ? at::empty(weight.sizes(), weight.options()) : Tensor();
             qgru_norm n = norm_head(h2, weight);

@@ -167,3 +167,37 @@ def test_every_thread_is_told_of_a_wait_that_ran_out(expire, cuda_device):
     t.start()
     t.join()
     assert fresh == ["ran"]
+
+
+def hooked(change):
+    """One saved tensor after the other comes back changed; how many there are is in `count`."""
+    count = []
+
+    def pack(t):
+        count.append(t)
+        return len(count) - 1
+
+    return count, lambda only: torch.autograd.graph.saved_tensors_hooks(pack, lambda i: change(count[i]) if i == only else count[i])
+
+
+@pytest.mark.parametrize("change", [lambda t: t[..., :-1], lambda t: t.to(torch.float64), lambda t: t.cpu(), lambda t: t.flatten()[: t.numel() // 2], lambda t: t[None]],
+                         ids=["shorter", "double", "host", "half", "dimension"])
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_a_saved_tensor_that_comes_back_as_another_is_refused(dtype, change, cuda_device):
+    q, k, v, g, state, n = make(cuda_device, 150, 2, 2, 64, 64, dtype, lengths=[150, 40], decay=dtype)
+    x, r, w = torch.randn(6, 64, device=cuda_device).to(dtype), torch.randn(6, 64, device=cuda_device).to(dtype), torch.ones(64, device=cuda_device).to(dtype)
+    for call, args, saves in ((lambda *a: la.linear_attention(*a, lengths=n)[0], (q, k, v, g, state), 6), (lambda *a: norm.rms_norm(*a)[0], (x, w, r), 3), (norm.rms_norm, (x, w), 3)):
+        for only in range(saves):
+            leaves = [t.detach().requires_grad_() for t in args]
+            count, hooks = hooked(change)
+            with hooks(only):
+                out = call(*leaves)
+            assert len(count) == saves
+            with pytest.raises(RuntimeError, match="saved-tensor hook"):
+                torch.autograd.grad(out.float().sum(), leaves)
+    # lengths that come back in every second place of a larger tensor are still the lengths
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, g, state)]
+    want = torch.autograd.grad(la.linear_attention(*leaves, lengths=n)[0].float().sum(), leaves)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: torch.stack([t, t + 7], -1)[..., 0] if t.dtype == torch.int32 else t):
+        out = la.linear_attention(*leaves, lengths=n)[0]
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(out.float().sum(), leaves)))
