@@ -34,10 +34,13 @@ struct Sums {
     }
 };
 using Acc = Sums<4>;
-// x as two tf32 values (11 significant bits): the nearest one, and of the rest, which has twelve bits at the most, all but the last.  A NaN
-// whose bits run over in the first is one in the second.  (By hand: the conversion instruction is three times the work.)
+// x as two tf32 values (11 significant bits): the nearest one, and of the rest, which has twelve bits at the most, all but the last.  (By
+// hand: the conversion instruction is three times the work.)  The nearest one of the largest floats would be infinite, and an infinity less
+// itself is NaN: the first is finite always, the second may be the infinity or the NaN.  (The bound costs 7 %: 182 -> 194 us for the forward
+// and gradients of 32 x 200 tokens, 8 heads of 64.)
+constexpr float MOST = 0x1.ffdffep+127f;          // the largest that is rounded to a finite one
 __device__ __forceinline__ void two_tf32(float x, uint32_t &hi, uint32_t &lo) {
-    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    hi = (__float_as_uint(fminf(fmaxf(x, -MOST), MOST)) + 0x1000u) & 0xffffe000u;
     lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
@@ -319,6 +322,7 @@ __global__ void __launch_bounds__(THREADS) k_outputs(const __grid_constant__ qgr
         return;
     }
     const int hk = h / (a.H / a.Hk);
+    const bool carried = chunk > 0 || a.state0;
     const long long qb = at(a.q, b, hk), kb = at(a.k, b, hk), vb = at(a.v, b, h);
     const float *S = states + chunk * (long long)heads * a.Dk * a.Dv + (long long)bh * a.Dk * a.Dv;
     load_decays(G, g_sums, a, b, h, t0, tokens, tid);
@@ -336,7 +340,7 @@ __global__ void __launch_bounds__(THREADS) k_outputs(const __grid_constant__ qgr
     each(c, tid, [&](int t, int s, float &x) { P[idx(t, s)] = s <= t ? a.scale * exp2_diff(G[t], G[s]) * x : 0.f; });
     for (int j = 0; j < a.Dv; j += 64) {
         c.zero();
-        for (int d = 0; d < a.Dk; d += 64) {
+        for (int d = 0; d < a.Dk && carried; d += 64) {
             load_tile<T>(X, a.q, qb, t0, tokens, d, a.Dk, tid);
             load_state(Y, S, d, j, a, tid);
             __syncthreads();

@@ -30,7 +30,7 @@ def linear_attention(q, k, v, log_decay, initial_state=None, lengths=None, scale
     [T, B, H], or [H] for decays that stay the same, float32 or the type of q, at most 0; head sizes up to 256.
     initial_state [B, H, Dk, Dv] float32 (zeros without one).  lengths [B] int32 on the device: sequence b ends after
     lengths[b] tokens (clamped to 0 .. T); what lies behind does not count, its outputs and gradients are zeros.  scale: 1 / sqrt(Dk)
-    without one.  Returns (out like v, the states after the last tokens [B, H, Dk, Dv] float32)."""
+    without one.  An infinity or NaN of a token reaches no earlier output; what it reaches is infinite or NaN.  Returns (out like v, the states after the last tokens [B, H, Dk, Dv] float32)."""
     return (_cabi._seq or _cabi.seq()).linear_attention(q, k, v, log_decay, initial_state, lengths, scale, batch_first)
 
 

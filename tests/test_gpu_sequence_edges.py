@@ -201,3 +201,37 @@ def test_a_saved_tensor_that_comes_back_as_another_is_refused(dtype, change, cud
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: torch.stack([t, t + 7], -1)[..., 0] if t.dtype == torch.int32 else t):
         out = la.linear_attention(*leaves, lengths=n)[0]
     assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(out.float().sum(), leaves)))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("D", [8, 64, 128, 200])
+def test_the_largest_values_are_values(D, dtype, cuda_device):
+    """One factor of the largest finite value (or close to it), the others small: results are finite and as near as any."""
+    most = torch.finfo(dtype).max
+    for which in range(3):
+        q, k, v, g, state, _ = make(cuda_device, 70, 2, 1, D, D, dtype, memory=(4.0, 4.0), h0=False)
+        for i, t in enumerate((q, k, v)):
+            t.mul_(2.0 ** -12)
+            if i == which:
+                t[3::17, 0, 0, 0] = most
+                t[5::17, 1, 0, D - 1] = -most * (1 - 2.0 ** -12)
+        args = (q, k, v, g)
+        leaves = [t.detach().requires_grad_() for t in args]
+        out, last = la.linear_attention(*leaves)
+        want, bound = want_of(*args, None, None, dout=torch.full_like(out, 2.0 ** -30), dstate=torch.zeros_like(last))
+        grads = torch.autograd.grad(out, leaves[:3], torch.full_like(out, 2.0 ** -30))
+        hold({"out": out.detach(), "state": last.detach(), **dict(zip(("dq", "dk", "dv"), grads))}, want, bound)
+
+
+@pytest.mark.parametrize("which", range(3), ids="qkv")
+def test_infinities_of_a_single_token(which, cuda_device):
+    """fp32: the product's infinity, with its sign, and not NaN."""
+    for sign in (1.0, -1.0):
+        for shape in ((1, 1), (1, 40), (1, 100)):
+            q, k, v, g, _, _ = make(cuda_device, 1, 3, 2, *shape, F32, h0=False)
+            (q, k, v)[which][:] = sign * float("inf")
+            out, last = la.linear_attention(q, k, v, g)
+            want, _ = want_of(q, k, v, g, None, None)
+            assert torch.equal(out, want["out"].float()) and not out.isfinite().any() and not out.isnan().any()
+            if which:
+                assert torch.equal(last, want["state"].float())
