@@ -53,16 +53,18 @@ struct Slot {
     __device__ __forceinline__ float2 G(int t) const { return make_float2(hi[t], lo[t]); }
 };
 
-template <int DK, int DV, bool Outputs>
+template <int DK, int DV, bool Outputs, bool Reverse>
 struct Plan {
     static constexpr int KT = DK / 64 * PANEL, VT = DV / 64 * PANEL, STAGE = (Outputs ? 2 : 1) * KT + VT;
     static constexpr int PART = DK / 64 * PANEL / 2, PARTS = 3 * PART;            // 64 tokens
     static constexpr int STATE = DK * DV * 2, STATES = Outputs ? 2 * STATE : 0;
     static constexpr int NB = DK == 128 && (DV == 128 || !Outputs) ? 1 : 2;       // buffers of parts
-    static constexpr int ROOM = 213000 - NB * PARTS - STATES;
+    // from the end: a ring of pieces of the forward's states, each of so many eights of columns
+    static constexpr int PIECE = 16384, PIECES = 2 * STATE / PIECE, EIGHTS = PIECE / (DK * 16), RING = Reverse ? 2 * PIECE : 0;
+    static constexpr int ROOM = 213000 - NB * PARTS - STATES - RING;
     static constexpr int NS = ROOM / STAGE >= 3 ? 3 : ROOM / STAGE >= 2 ? 2 : 1;  // stages of tiles
     static constexpr int NQ = DV == 64 && NS > 1 ? 2 : 1;                         // buffers of q k^T
-    static constexpr int TILES = NS * STAGE + NB * PARTS + STATES;
+    static constexpr int TILES = NS * STAGE + NB * PARTS + STATES + RING;
     // columns of tensor memory
     static constexpr uint32_t INTER = NQ * 128, INTRA = INTER + DV, U = Outputs ? INTRA + DV : 0, COLUMNS = Outputs ? 512 : DV;
     static_assert(!Outputs || U + DV <= 512, "tensor memory");
@@ -71,7 +73,7 @@ struct Plan {
 
 struct Ctl {
     uint64_t k_full[3], k_empty[3], q_full[3], q_empty[3], v_full[3], v_empty[3], parts_full[2], parts_empty[2], pairs_full[2], p_full[2], g_full[SLOTS], g_empty[SLOTS];
-    uint64_t u_full, u_empty, s_full, o_empty;
+    uint64_t u_full, u_empty, s_full, o_empty, ring_full[2], ring_empty[2];
     uint32_t tmem;
     volatile int failed;
 };
@@ -149,7 +151,7 @@ struct At {
 };
 template <int DK, int DV, bool Outputs, bool Reverse>
 struct Roles {
-    using L = Plan<DK, DV, Outputs>;
+    using L = Plan<DK, DV, Outputs, Reverse>;
     const qgru_attention &a;
     const Args &p;
     Ctl &s;
@@ -162,6 +164,7 @@ struct Roles {
     __device__ __forceinline__ uint32_t q_tile(int st) const { return tiles + st * L::STAGE + L::KT + L::VT; }
     __device__ __forceinline__ uint32_t parts(int b) const { return tiles + L::NS * L::STAGE + b * L::PARTS; }
     __device__ __forceinline__ uint32_t state(int part) const { return tiles + L::NS * L::STAGE + L::NB * L::PARTS + part * L::STATE; }
+    __device__ __forceinline__ uint32_t ring(int b) const { return tiles + L::NS * L::STAGE + L::NB * L::PARTS + L::STATES + b * L::PIECE; }
     // f(item, its chunk in the pass's order, running number of the chunk) until it says that a wait has run out
     template <class F>
     __device__ __forceinline__ bool each(F f) const {
@@ -246,6 +249,19 @@ struct Roles {
             }
             if (!wait(s, s.v_empty[st.buf], st.free)) return false;
             load(v_tile(st.buf), &p.v, &s.v_full[st.buf], DV / 64, chunk * C, w.h, w.b);
+            return true;
+        });
+    }
+    // ---- From the end, a warp of P (which has nothing to weigh there): the forward's states, piece after piece
+    __device__ __forceinline__ void fetch_states() const {
+        each([&](const Item<Reverse> &w, int chunk, int i) {
+            const bf16 *from = p.other + ((long long)chunk * a.B * a.H + w.bh) * (2 * DK * DV);
+            for (int piece = 0; piece < L::PIECES; ++piece) {
+                const At<2> o(i * L::PIECES + piece);
+                if (!wait(s, s.ring_empty[o.buf], o.free)) return false;
+                tc::mbar_expect_tx(&s.ring_full[o.buf], L::PIECE);
+                bulk_load(ring(o.buf), from + piece * (L::PIECE / 2), L::PIECE, &s.ring_full[o.buf]);
+            }
             return true;
         });
     }
@@ -375,12 +391,17 @@ struct Roles {
                 uint4 *keep = p.states && !p.own_sums ? reinterpret_cast<uint4 *>(p.states + ((long long)Item<Reverse>::chunk(p, c) * a.B * a.H + w.bh) * (2 * DK * DV) + (c0 * DK + row * 8)) : nullptr;
                 if (Reverse && !p.own_sums) {
                     const long long head = (long long)Item<Reverse>::chunk(p, c) * a.B * a.H + w.bh;
-                    const uint4 *o = reinterpret_cast<const uint4 *>(p.other + head * (2 * DK * DV) + (c0 * DK + row * 8));
                     float2 x = both(0.f);
 #pragma unroll
-                    for (int j = 0; j < N; j += 8) {
-                        x = dot8(o[DK * DV / 8 + j / 8 * DK], &S[j / 2], x);
-                        x = dot8(o[j / 8 * DK], &S[j / 2], x);
+                    for (int e = 0; e < 2 * N / 8; ++e) {
+                        // eights of columns of the two parts; with 64 rows a piece holds both halves of them, the lanes' own and the others'
+                        const int part = e / (N / 8), j = e % (N / 8), at8 = part * (DV / 8) + (DK == 64 ? 0 : j), piece = at8 / L::EIGHTS;
+                        const bool first = at8 % L::EIGHTS == 0 && (DK != 64 || j == 0);
+                        const bool last = DK == 64 ? j == N / 8 - 1 && (part + 1) * (DV / 8) % L::EIGHTS == 0 : at8 % L::EIGHTS == L::EIGHTS - 1;
+                        const At<2> o(i * L::PIECES + piece);
+                        if (first && !wait_warp(s, s.ring_full[o.buf], o.full)) return;
+                        x = dot8(lds16(ring(o.buf) + (uint32_t)((part * (DV / 8) + c0 / 8 + j) % L::EIGHTS * DK + row) * 16), &S[j * 4], x);
+                        if (last) tc::mbar_arrive(&s.ring_empty[o.buf]);
                     }
                     float sum = x.x + x.y;
                     for (int e = 16; e; e >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, e);
@@ -580,7 +601,7 @@ struct Roles {
 
 template <int DK, int DV, bool Outputs, bool Reverse>
 __global__ void __launch_bounds__(THREADS, 1) k_walk(const __grid_constant__ qgru_attention a, const __grid_constant__ Args p) {
-    using L = Plan<DK, DV, Outputs>;
+    using L = Plan<DK, DV, Outputs, Reverse>;
     extern __shared__ unsigned char raw[];
     unsigned char *tiles = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     Slot *slots = reinterpret_cast<Slot *>(tiles + L::TILES);
@@ -602,6 +623,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_walk(const __grid_constant__ qgr
             tc::mbar_init(&s.parts_empty[i], 1);
             tc::mbar_init(&s.pairs_full[i], 1);
             tc::mbar_init(&s.p_full[i], WG);
+            tc::mbar_init(&s.ring_full[i], 1);
+            tc::mbar_init(&s.ring_empty[i], WG);
         }
         for (int i = 0; i < SLOTS; ++i) {
             tc::mbar_init(&s.g_full[i], 32);
@@ -642,6 +665,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_walk(const __grid_constant__ qgr
     } else if (wg == 3) {
         take_registers<G::P>();
         if constexpr (Outputs) r.weights();
+        if (Reverse && !p.own_sums && tid == 3 * WG) r.fetch_states();
+        __syncwarp();
     } else {
         take_registers<G::O>();
         if constexpr (Outputs) r.outputs();
@@ -661,7 +686,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_walk(const __grid_constant__ qgr
 template <int DK, int DV, bool Outputs, bool Reverse>
 int launch(const qgru_attention &a, const Args &p, int sms, cudaStream_t st) {
     const auto kernel = k_walk<DK, DV, Outputs, Reverse>;
-    constexpr int bytes = Plan<DK, DV, Outputs>::TILES + 1024 + SLOTS * (int)sizeof(Slot) + (int)sizeof(Ctl);
+    constexpr int bytes = Plan<DK, DV, Outputs, Reverse>::TILES + 1024 + SLOTS * (int)sizeof(Slot) + (int)sizeof(Ctl);
     static_assert(bytes <= 232448, "shared memory");
     SEQ_CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
     kernel<<<std::min(p.items, sms), THREADS, bytes, st>>>(a, p);

@@ -24,7 +24,8 @@ int walk(const qgru_attention &a, const Cut &c, bool reverse, void *states, char
 // The pass from the end meets every state's gradient in fp32: it multiplies it with the state, as it was kept, and leaves the sum in
 // THROUGH parts a chunk and head (the sums of its warps).  A state is kept as 32 bits, the two bf16 parts (16 of its bits) that the
 // products take it in: [chunk][B H][part][DV / 8][DK][8], so that the threads of a warp, a row each, read and write whole lines (row by row,
-// with 16 bytes of 32 lines an instruction, the passes took 86 and 66 us where they take 66 and 58, 16 x 1000 tokens of 8 heads of 128).
+// with 16 bytes of 32 lines an instruction, the two passes took 86 and 66 us where they take 65 and 58, and 46 with the
+// states on their way through shared memory; 16 x 1000 tokens of 8 heads of 128).
 constexpr int THROUGH = 8;
 
 namespace tile {
