@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(128) k_scan_segments(float *seg_state, const f
 
 // grid: chunks x B H, the heads of one chunk beside each other (their tokens lie together).  out = 2^G_t q S + P v, 64 columns of the
 // output at a time over 64 of the head's; the tiles pass through shared memory one after another, so a CTA waits for each: 37 x 127
-// tokens of 5 heads of 40 x 72, fp32, ragged: 25 us.  Up to 64 x 64 of fp32 the kernels further down fetch all tiles at once instead.
+// tokens of 5 heads of 40 x 72, fp32, ragged: 23 us.  Up to 64 x 64 of fp32 the kernels further down fetch all tiles at once instead.
 template <class T>
 __global__ void __launch_bounds__(THREADS) k_outputs(const __grid_constant__ qgru_attention a, const float *states) {
     extern __shared__ float4 smem4[];
@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(THREADS) k_gradients(const __grid_constant__ q
 // ------------------------------------------------------------------------------------- fp32, head sizes up to 64
 // Every chunk's tiles are fetched at once, asynchronously, into a tile each; then nothing waits for memory.  What bounds these is the
 // issue of mma.sync and of the operands' splits (two tf32 values for each, three products, rounded to nearest every eight K).
-// 32 x 200 ragged tokens of 8 heads of 64: outputs 32 us; gradients 85 us so, with sixteen warps, 16 x 16 sums a warp, and 118 us tile
+// 32 x 200 ragged tokens of 8 heads of 64: outputs 32 us; gradients 87 us so, with sixteen warps, 16 x 16 sums a warp, and 118 us tile
 // after tile, with eight warps, three CTAs an SM.
 constexpr int ALL = 512, NT2 = 2;
 

@@ -25,8 +25,8 @@ __device__ __forceinline__ int valid_tokens(const qgru_attention &a, int b) {
     return a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
 }
 
-// Decays are summed up in 64-bit integers, base 2, in units of 2^-38: exact sums (a token's own rounding is 2^-38, 128 of them make
-// 3e-10 of the decay) that depend on no order.  A decay below 2^-160 is zero to any fp32 sum and one above 2^128 infinite, so the
+// Decays are summed up in 64-bit integers, base 2, in units of 2^-38: exact sums (a token's own rounding is 2^-38, 128 of them make 5e-10)
+// that depend on no order.  A decay below 2^-160 is zero to any fp32 sum and one above 2^128 infinite, so the
 // clamps keep -inf, +inf and a chunk's sum in range (128 * 160 < 2^14.4, 2^52.4 units); a NaN is a value beyond all sums, which makes
 // every sum from it on NaN.
 constexpr float UNITS = 0x1p38f;
@@ -39,8 +39,9 @@ __device__ __forceinline__ long long decay_units(float x) {
     return __float2ll_rn(hi * UNITS) + __float2ll_rn(lo * UNITS);
 }
 __device__ __forceinline__ long long decay_units(const qgru_attention &a, long long at) { return decay_units(seq::load_f(a.decay.p, at, a.decay_bf16)); }
-// A running sum as two floats, so that the difference of two of them is as exact as the difference itself:
-// G_t - G_s = (hi_t - hi_s) + (lo_t - lo_s).
+// A running sum as two floats, so that the difference of two of them is as exact as a float of its size, however large the sums are:
+// G_t - G_s = (hi_t - hi_s) + (lo_t - lo_s), rounded once, 2^-24 of the difference.  (A difference of 20 is off by 1.2e-6 then, and so is
+// its power of two, which is 1e-6 itself.)
 __device__ __forceinline__ float2 two_floats(long long x) {
     if (x > NAN_UNITS / 2) return make_float2(__int_as_float(0x7fffffff), 0.f);
     const float hi = __ll2float_rn(x);
@@ -61,7 +62,7 @@ __device__ __forceinline__ T running_sum(T g, T *warp_sums, int tid) {
     return g;
 }
 
-// ---- kernels for every size and type (qgru_attn.cu): fp32 sums by multiply-adds
+// ---- kernels for every size and type (qgru_attn.cu): fp32, products by warp-level tensor instructions on two tf32 values an operand
 Cut generic_cut(const qgru_attention &a, int sms);
 int generic_forward(const qgru_attention &a, const Cut &c, cudaStream_t st);
 int generic_backward(const qgru_attention &a, const Cut &c, cudaStream_t st);

@@ -12,10 +12,12 @@
 //
 // What is rounded on the way: P, and the state where it is a factor, to 16 bits (two bf16 parts each); the output once, to bf16, in the end.
 //
-// What bounds it: the roles' instructions, not the bytes.  64 x 1000 tokens of 16 heads of 64, 524 MB: 172 to 180 us, 3 TB/s (2.9 us a
-// chunk and SM, the tensor pipe busy for 18 % of it).  The roles share one instruction cache, so their loops stay rolled: unrolled, with
-// 1.7 times the misses, 274 us.  A sixth warpgroup, P taken by two: 190.  16 x 1000 tokens of 8 heads of 128: 70 us with the outputs, 46
-// from the end without.  One phrase of 24 tokens, 4 heads of 64: 9 us, the latency of the roles one after another.
+// What bounds it: the products, one after the other, not the bytes.  64 x 1000 tokens of 16 heads of 64, 524 MB: 188 us, 2.8 TB/s, 5900
+// cycles a chunk and SM.  The warp that issues the products waits for no role: every operand is there when it comes to it (of a chunk's
+// 5900 cycles K works 3000, P 4300, O 1900, S 600).  Its 56 products take 100 cycles each, with five roles on the same shared and tensor
+// memory; alone they take 32 to 64.  P as one part would be eight products fewer, 175 us, and a rounding more in every output.  The roles
+// share one instruction cache, so their loops stay rolled.  16 x 1000 tokens of 8 heads of 128: 65 us with the outputs and kept states, 46
+// from the end without outputs.  One phrase of 24 tokens, 4 heads of 64: 9 us, the latency of the roles one after another.
 #include <algorithm>
 #include <type_traits>
 

@@ -117,7 +117,7 @@ constexpr int STATES_TILES = DK / 64 * PANEL + 2 * (DV / 64) * PANEL + 3 * (DK /
 // grid (B H, segments).  S' = 2^G_C S + (w k)^T v: lane i of tensor memory is row i of the state, whose fp32 sums stay in
 // registers, half a row a thread.  While the products of a chunk run, the next one's tokens are read and the state before this one
 // leaves.  With DK = 64 lanes 64 .. 127 repeat the first 64 (M is 128) and are not read.  One chunk's chain of load, split, product and
-// conversion bounds it, eight in turn: 16 x 1000 tokens of 8 heads of 60, 61 us.
+// conversion bounds it, eight in turn: 16 x 1000 tokens of 8 heads of 60, 63 us.
 template <int DK, int DV, bool Reverse>
 __global__ void __launch_bounds__(THREADS) k_states_tc(const __grid_constant__ qgru_attention a, const __grid_constant__ Pass p) {
     extern __shared__ unsigned char raw[];
@@ -264,7 +264,7 @@ constexpr int OUTPUTS_TILES = 2 * (DK / 64) * PANEL + DV / 64 * PANEL;
 
 // grid: chunks x B H, the heads of one chunk beside each other.  Two threads a token, each half of the pairs' weights and half of the
 // output's columns.  The state lies where k was once q k^T is there.  Two CTAs an SM cover each other's waits; the element loads of what
-// TMA does not take bound it: 16 x 1000 tokens of 8 heads of 60, 117 us (64, by TMA, in k_walk: 34 with the states).
+// TMA does not take bound it: 16 x 1000 tokens of 8 heads of 60, 119 us (64, by TMA, in k_walk: 34 with the states).
 template <int DK, int DV>
 __global__ void __launch_bounds__(THREADS, 2) k_outputs_tc(const __grid_constant__ qgru_attention a, const bf16 *states, int *flag) {
     extern __shared__ unsigned char raw[];
@@ -523,7 +523,7 @@ __device__ __forceinline__ void copy_out(uint32_t tile, const qgru_seq_tensor &x
 // The next chunk's tiles are fetched while this one's results leave (both by TMA), its decays are summed up beside this one's products,
 // those of the state's gradient run beside the pairs, and the state before the chunk comes after them into the same place.  What bounds
 // it is the chain of products, pairs and conversions between tensor memory and operands, and what of the loads it does not cover: 224 KB of
-// operands leave no room for a second CTA or for tiles fetched earlier.
+// operands leave no room for a second CTA or for tiles fetched earlier.  Heads of 64: 74 us; of 60, by the threads' own loads: 172.
 template <int DK, int DV, bool Tma>
 __global__ void __launch_bounds__(GRAD_THREADS) k_gradients_tc(const __grid_constant__ qgru_attention a, const __grid_constant__ Gradients p) {
     extern __shared__ unsigned char raw[];

@@ -5,8 +5,9 @@
 //
 // Bytes bound all of them: each tensor is read or written once, with a row in registers between its sum and its output.
 // TPR threads have a row, each E elements of it in vectors of V neighbours; a warp each up to 1024 columns, a CTA above.
-// 51200 x 1024 bf16 with residual, 420 MB: 67 us (6.3 TB/s).  In 8 bits with a scale a row, 367 MB: 76 us (4.8 TB/s), bound by the rounding's
-// instructions; 101 us with a conversion instruction for every element.  4096 x 8192: 42 us (6.4 TB/s).  One row: 3 us, the launch.
+// 51200 x 1024 bf16 with residual, 420 MB: 67 us (6.3 TB/s).  In 8 bits with a scale a row, 367 MB: 76 us (4.8 TB/s): the row's
+// phases (loads, sum, maximum, rounding, stores) follow one another; 101 us with a conversion instruction for every element.  4096 x
+// 8192: 41 us (6.5 TB/s).  One row: 3 us, the launch.
 #include <algorithm>
 #include <type_traits>
 
@@ -228,8 +229,8 @@ __device__ __forceinline__ void cp_async16(void *to, const void *from) {
 }
 
 // Rows in turn; a thread keeps the weights of its E columns and the sums of dw, which leave once a CTA.  Whole vectors of the next rows
-// (three of bf16, one of fp32) are on their way into shared memory, where each thread reads back what it has fetched itself;
-// single elements come straight from memory.  51200 x 1024 bf16 with the stream's gradient, 420 MB: 155 us with a warp a row and no row
+// (three of bf16, one of fp32; with sixteen elements a thread one and none) are on their way into shared memory, where each thread reads
+// back what it has fetched itself; single elements come straight from memory.  51200 x 1024 bf16 with the stream's gradient, 420 MB: 155 us with a warp a row and no row
 // ahead, 123 us with one row ahead in registers, 74 us so (5.7 TB/s).
 constexpr int AHEAD_BYTES = 192;                     // of shared memory a thread
 template <class T, class W, int V, int TPR, int E>
