@@ -179,9 +179,14 @@ struct Roles {
         return true;
     }
 
-    // ---- X, warp 0: products
+    // ---- X, warp 0: products.  Those that add to the same sums follow one another as they are issued; others need not, so the pairs of a chunk
+    // wait until P v of the chunk whose weights they overwrite is done.
     __device__ __forceinline__ bool pairs(uint32_t leader, int i) const {
         const At<L::NS> st(i);
+        if (i >= L::NQ) {
+            const At<L::NS> before(i - L::NQ);
+            if (!wait(s, s.v_empty[before.buf], before.full)) return false;
+        }
         if (!wait(s, s.k_full[st.buf], st.full) || !wait(s, s.q_full[st.buf], st.full)) return false;
         tc::tc_fence_after_sync();
         product<false, false, C, DK>(leader, s.tmem + (i % L::NQ) * 128, Operand{q_tile(st.buf), PANEL}, Operand{k_tile(st.buf), PANEL}, false);
