@@ -408,7 +408,10 @@ struct Roles {
                         const At<2> o(i * L::PIECES + piece);
                         if (first && !wait_warp(s, s.ring_full[o.buf], o.full)) return;
                         x = dot8(lds16(ring(o.buf) + (uint32_t)((part * (DV / 8) + c0 / 8 + j) % L::EIGHTS * DK + row) * 16), &S[j * 4], x);
-                        if (last) tc::mbar_arrive(&s.ring_empty[o.buf]);
+                        if (last) {
+                            fence_async();         // (ordinary reads, and the bulk copy that follows into the same place, are ordered by this alone)
+                            tc::mbar_arrive(&s.ring_empty[o.buf]);
+                        }
                     }
                     float sum = x.x + x.y;
                     for (int e = 16; e; e >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, e);

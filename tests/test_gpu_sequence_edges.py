@@ -235,3 +235,29 @@ def test_infinities_of_a_single_token(which, cuda_device):
             assert torch.equal(out, want["out"].float()) and not out.isfinite().any() and not out.isnan().any()
             if which:
                 assert torch.equal(last, want["state"].float())
+
+
+@pytest.mark.parametrize("case", [dict(Dk=64, Dv=64), dict(Dk=128, Dv=64), dict(Dk=64, Dv=128, Hk=4), dict(Dk=128, Dv=128), dict(Dk=128, Dv=128, Hk=2), dict(Dk=100, Dv=127)],
+                         ids=lambda c: "-".join(f"{k}{v}" for k, v in c.items()))
+def test_the_same_bits_beside_other_work(case, cuda_device):
+    """Many chunks a CTA while another stream keeps the memory and the multiprocessors busy: products and copies end in other orders, results do not."""
+    T, B = 700, 37
+    lengths = [min(T, (0, 1, 127, 128, 129, 200, 63, T, T, 385, 513)[b % 11]) for b in range(B)]
+    q, k, v, g, state, n = make(cuda_device, T, B, 8, dtype=BF, lengths=lengths, decay=BF, **case)
+    dout, dstate = torch.randn_like(v), torch.randn_like(state)
+
+    def run():
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, g, state)]
+        out, last = la.linear_attention(*leaves, lengths=n)
+        return [out.detach(), last.detach(), *torch.autograd.grad((out, last), leaves, (dout, dstate))]
+
+    other, a, b = torch.cuda.Stream(), torch.randn(2048, 2048, device=cuda_device), torch.empty(300_000_000, dtype=torch.uint8, device=cuda_device)
+    want = run()
+    for i in range(60):
+        with torch.cuda.stream(other):
+            if i % 3 == 0:
+                a @ a
+            elif i % 3 == 1:
+                b.fill_(i)
+        assert all(torch.equal(x, y) for x, y in zip(run(), want)), i
+    torch.cuda.synchronize()
